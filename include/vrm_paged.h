@@ -614,6 +614,45 @@ int vrm_paged_decode_tq_residual(
     int B, int H, int KH, int D, int PS, float scale, int bits, int qjl_dim, const float* signs,
     const float* jl, const float* angle_lut, vrm_stream_t stream);
 
+/* --------------------------------------------------------------------------
+ * A chunk of new tokens over a paged cache.  No counterpart in the reference,
+ * whose prompts run through the model's own attention before
+ * from_hf_cache stores them (core/paged_attention.py:716-805).
+ *
+ * The batch is ragged: sequence b's new tokens are rows cu_seqlens[b] ..
+ * cu_seqlens[b + 1] of N, and context_lens[b] counts its tokens in the cache,
+ * the new ones included: new token i of q_b is at position
+ * context_lens[b] - q_b + i.  Rows from cu_seqlens[B] on belong to no sequence
+ * and are neither read nor written.  All three arrays are int32 on the device.
+ * -------------------------------------------------------------------------- */
+
+/*
+ * out[n][h] = softmax(scale q[n][h] . K^T) V over the tokens t that row n sees:
+ * t < context_lens[b], in a page that is there, with causal != 0 t <= its own
+ * position, and with window > 0 t > its position - window.  A row that sees no
+ * token gives zeros (lse -inf).  Head h reads kv-head h / (H / KH).
+ *   query       [N][H][D] of q_dtype (VRM_SRC_*), with strides in elements
+ *               (last dim contiguous)
+ *   kv_pool, kv_scales, page_table as in vrm_paged_decode (any kv_dtype)
+ *   out         [N][H][D] of q_dtype
+ *   lse         [N][H] float32 or NULL: ln sum_t exp(scale q.k_t)
+ *   workspace   vrm_paged_chunk_workspace_bytes bytes, 16-byte aligned (may be
+ *               NULL where that is 0); written before it is read, so its
+ *               contents do not matter between calls
+ * Products are 16-bit matrix products where the query is bf16 or fp16 and the
+ * pool has the same type, int8 or fp8; float32 ones otherwise.  Sums and
+ * softmax statistics are float32.  Any D <= 256, any page size; int8 / fp8
+ * pools need D % 16 == 0 and PS % 4 == 0.
+ */
+size_t vrm_paged_chunk_workspace_bytes(int N, int B, int H, int KH, int D, int PS, int max_pp);
+int vrm_paged_chunk_attention(const void* query, int q_dtype, long long q_token_stride,
+                              long long q_head_stride, const void* kv_pool, const float* kv_scales,
+                              const int32_t* page_table, const int32_t* context_lens,
+                              const int32_t* cu_seqlens, void* out, float* lse, void* workspace,
+                              size_t workspace_bytes, int N, int B, int H, int KH, int D, int PS,
+                              int L, int P, int max_pp, int layer_idx, float scale, int causal,
+                              int window, int kv_dtype, vrm_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

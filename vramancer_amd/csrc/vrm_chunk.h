@@ -1,0 +1,208 @@
+// Attention of a ragged batch's new tokens over a paged cache: the call's
+// arguments, its work items, and what both kernels (16-bit matrix products,
+// float32 products) share.
+//
+// Rows.  The G = H / KH query heads of a kv-head read the same keys, so a
+// sequence's q_b new tokens make q_b G rows of one matrix per kv-head: row r
+// is head r % G of token r / G.  A tile is kRows of them.
+// Items.  A workgroup takes one item: a tile of one kv-head over a share of
+// the key blocks that its rows see.  A batch of few tiles is cut along the
+// keys (find_item) so that the GPU is full; the shares' (max, sum,
+// accumulator) go to the workspace and chunk_merge_kernel joins them.
+#pragma once
+#include <math.h>
+
+#include "vrm_common.h"
+
+namespace vrm {
+
+constexpr int kRows = 128;          // rows of a tile
+constexpr int kChunkThreads = 256;  // four wavefronts
+
+enum { kSrcF32 = 0, kSrcF16 = 1, kSrcBf16 = 2, kSrcI8 = 3, kSrcFp8 = 4 };  // element types of a pool
+
+struct ChunkArgs {
+  const void* q;
+  long long q_n, q_h;  // elements from a token's row to the next token's, and from a head's to the next
+  int q_type;          // VRM_SRC_*
+  const uint8_t* pool;
+  const float* scales;
+  PoolGeom g;
+  long long layer_off, s_layer_off;  // of the layer, in bytes and scale floats
+  const int32_t* table;
+  const int32_t* lens;
+  const int32_t* cu;
+  void* out;  // [N][H][D] of q_type
+  float* lse;
+  float* part;  // [items][kRows][dp]: accumulators of shares
+  float2* ml;   // [items][kRows]: their max (log2 units) and sum
+  int2* rec;    // [vtiles][KH]: first item and shares of a tile
+  int N, B, H, KH, G, D, PS, P, max_pp;
+  int dp;       // D as the kernel pads it
+  int vtiles;   // tiles when every sequence has one more than its rows fill
+  int items;    // items per kv-head that the grid (and the workspace) has room for
+  int ps_shift;      // log2 PS, or -1
+  int causal;
+  int window;        // tokens a row sees up to its own; 0: all
+  float sc;          // |scale| log2 e (1 for scale 0)
+  int q_sign;        // -1: the queries enter negated; 0: as zeros
+  int target;        // items wanted per kv-head; 0: one per tile
+  int min_blocks;    // key blocks an item has at least
+  int aligned;       // pool rows can be loaded 16 bytes at a time
+  int q_aligned;     // query rows too
+  int out_aligned;   // output rows can be stored 8 bytes at a time
+};
+
+__device__ __forceinline__ int clamp_int(int x, int lo, int hi) { return min(max(x, lo), hi); }
+
+struct Sequence {
+  int row0, q_len, ctx;
+};
+
+__device__ __forceinline__ Sequence load_sequence(const ChunkArgs& a, int b) {
+  Sequence s;
+  s.row0 = clamp_int(a.cu[b], 0, a.N);
+  s.q_len = max(clamp_int(a.cu[b + 1], 0, a.N) - s.row0, 0);
+  s.ctx = (int)min((long long)max(a.lens[b], 0), (long long)a.max_pp * a.PS);
+  return s;
+}
+
+// Tiles before those of sequence b when every sequence is given one more than
+// its rows fill: known from cu[b] alone, and at least as many as it needs.
+__device__ __forceinline__ int virtual_tile(const ChunkArgs& a, int row0, int b) {
+  return (int)((long long)row0 * a.G / kRows) + b;
+}
+
+__device__ __forceinline__ int tiles_of(const ChunkArgs& a, const Sequence& s) {
+  return (s.q_len * a.G + kRows - 1) / kRows;
+}
+
+// Key blocks of TN tokens that a tile of the sequence sees at most.
+template <int TN>
+__device__ __forceinline__ int blocks_of(const ChunkArgs& a, const Sequence& s) {
+  int span = s.ctx;
+  if (a.window) span = (int)min((long long)span, (long long)a.window + kRows / a.G + 1 + TN);
+  return (span + TN - 1) / TN;
+}
+
+// Inclusive prefix sum over the wavefront's lanes.
+__device__ __forceinline__ int wave_scan(int v) {
+  const int lane = __lane_id();
+#pragma unroll
+  for (int d = 1; d < kWave; d <<= 1) {
+    const int u = __shfl_up(v, d);
+    if (lane >= d) v += u;
+  }
+  return v;
+}
+
+struct Item {
+  int b, tile, share, shares;
+  int first;  // item index of the tile's share 0 (per kv-head)
+  Sequence s;
+};
+
+// Item idx of a kv-head: the shares of the first sequence's tiles (later tiles
+// first: under a causal mask they see more keys), then the next sequence's.
+// Shares have about (work of the kv-head) / target blocks, so that sequences
+// of any lengths fill the GPU evenly; every wavefront finds its item itself,
+// lane by lane over the sequences.
+template <int TN>
+__device__ __forceinline__ bool find_item(const ChunkArgs& a, int idx, Item& it) {
+  const int lane = __lane_id();
+  int share_blocks = 0x7fffffff;
+  if (a.target > 0) {
+    float work = 0.f;
+    for (int b0 = 0; b0 < a.B; b0 += kWave) {
+      const int b = b0 + lane;
+      if (b < a.B) {
+        const Sequence s = load_sequence(a, b);
+        work += (float)tiles_of(a, s) * (float)blocks_of<TN>(a, s);
+      }
+    }
+    work = group_sum<64>(work);
+    share_blocks = max(a.min_blocks, (int)fminf(ceilf(work / (float)a.target), 1e9f));
+  }
+  int before = 0;
+  for (int b0 = 0; b0 < a.B; b0 += kWave) {
+    const int b = b0 + lane;
+    Sequence s{0, 0, 0};
+    int tiles = 0, shares = 1;
+    if (b < a.B) {
+      s = load_sequence(a, b);
+      tiles = tiles_of(a, s);
+      const int blocks = blocks_of<TN>(a, s);
+      shares = max(1, (int)(((long long)blocks + share_blocks - 1) / share_blocks));
+    }
+    const int upto = wave_scan(tiles * shares);
+    const unsigned long long past = __ballot(before + upto > idx);
+    if (past) {
+      const int l = __ffsll(past) - 1;
+      it.b = b0 + l;
+      it.s.row0 = __builtin_amdgcn_readlane(s.row0, l);
+      it.s.q_len = __builtin_amdgcn_readlane(s.q_len, l);
+      it.s.ctx = __builtin_amdgcn_readlane(s.ctx, l);
+      it.shares = __builtin_amdgcn_readlane(shares, l);
+      const int nt = __builtin_amdgcn_readlane(tiles, l);
+      const int from = before + __builtin_amdgcn_readlane(upto, l) - nt * it.shares;
+      const int rem = idx - from;
+      it.tile = nt - 1 - rem / it.shares;
+      it.share = rem % it.shares;
+      it.first = idx - it.share;
+      return true;
+    }
+    before += __builtin_amdgcn_readlane(upto, kWave - 1);
+  }
+  return false;
+}
+
+// Key blocks [from, to) of an item: its share of those that the tile's rows see.
+template <int TN>
+__device__ __forceinline__ void item_blocks(const ChunkArgs& a, const Item& it, int& from, int& to) {
+  const int rows = it.s.q_len * a.G;
+  const int t0 = it.tile * kRows / a.G;                             // the tile's first token
+  const int t1 = (min(rows, (it.tile + 1) * kRows) - 1) / a.G;      // and its last
+  const int base = it.s.ctx - it.s.q_len;                           // position of token 0
+  const int hi = a.causal ? clamp_int(base + t1 + 1, 0, it.s.ctx) : it.s.ctx;
+  const int lo = a.window ? clamp_int(base + t0 - a.window + 1, 0, hi) : 0;
+  const int b0 = lo / TN, n = (hi + TN - 1) / TN - b0;
+  const int per = (n + it.shares - 1) / it.shares;
+  from = b0 + min(n, it.share * per);
+  to = b0 + min(n, (it.share + 1) * per);
+}
+
+// Share 0 leaves the merge the tile's first item and number of shares.
+__device__ __forceinline__ void put_record(const ChunkArgs& a, const Item& it, int kvh) {
+  const int vtile = virtual_tile(a, it.s.row0, it.b) + it.tile;
+  if (a.target > 0 && it.share == 0 && threadIdx.x == 0 && vtile < a.vtiles)
+    a.rec[(long long)vtile * a.KH + kvh] = make_int2(it.first, it.shares);
+}
+
+__device__ __forceinline__ int page_index(const ChunkArgs& a, int token) {
+  return a.ps_shift >= 0 ? token >> a.ps_shift : token / a.PS;
+}
+
+__device__ __forceinline__ float load_q(const ChunkArgs& a, long long at) {
+  if (a.q_type == VRM_SRC_F32) return static_cast<const float*>(a.q)[at];
+  const uint32_t h = static_cast<const uint16_t*>(a.q)[at];
+  return a.q_type == VRM_SRC_F16 ? f16_bits_to_f32(h) : bf16_bits_to_f32(h);
+}
+
+// 16 bytes of which the first `bytes` are there; the rest are zero.
+__device__ __forceinline__ uint4 load16(const uint8_t* p, int bytes, bool vec) {
+  if (vec && bytes >= 16) return *reinterpret_cast<const uint4*>(p);
+  uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    if (i < bytes) w[i / 4] |= (uint32_t)p[i] << (8 * (i % 4));
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// One launch of the attention kernel: float32 products (pool of kind kSrc*),
+// 16-bit products over float, int8 and fp8 pools.
+void launch_chunk_f32(const ChunkArgs& a, int kind, dim3 grid, hipStream_t st);
+void launch_chunk16_float(const ChunkArgs& a, dim3 grid, hipStream_t st);
+void launch_chunk16_i8(const ChunkArgs& a, dim3 grid, hipStream_t st);
+void launch_chunk16_fp8(const ChunkArgs& a, dim3 grid, hipStream_t st);
+
+}  // namespace vrm

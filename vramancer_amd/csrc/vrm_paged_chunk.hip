@@ -1,0 +1,246 @@
+// Attention of a ragged batch's new tokens over a paged cache: the entry
+// points, the choice of kernel and items, and the merge of items that share a
+// tile.  The kernels are in vrm_chunk16.h and vrm_paged_chunk_f32.hip.
+#include <math.h>
+
+#include "vrm_chunk.h"
+
+namespace vrm {
+namespace {
+
+// One wavefront per row: joins the shares' (max, sum, accumulator).
+__global__ void __launch_bounds__(256) chunk_merge_kernel(ChunkArgs a) {
+  const int vtile = blockIdx.x / a.KH, kvh = blockIdx.x % a.KH;
+  int lo = 0, hi = a.B - 1;  // the last sequence whose tiles start at or before vtile
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (virtual_tile(a, clamp_int(a.cu[mid], 0, a.N), mid) <= vtile)
+      lo = mid;
+    else
+      hi = mid - 1;
+  }
+  const Sequence s = load_sequence(a, lo);
+  const int tile = vtile - virtual_tile(a, s.row0, lo);
+  if (tile < 0 || tile >= tiles_of(a, s)) return;
+  const int2 r = a.rec[(long long)vtile * a.KH + kvh];
+  const int first = r.x, shares = r.y;
+  if (shares <= 1 || first < 0 || first + shares > a.items) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int rows = min(kRows, s.q_len * a.G - tile * kRows);
+  for (int j = 0; j < 4; ++j) {
+    const int row = blockIdx.y * 16 + wave * 4 + j;
+    if (row >= rows) return;
+    const auto slot = [&](int i) { return ((long long)(first + i) * a.KH + kvh) * kRows + row; };
+    float top = -INFINITY;
+    for (int i = lane; i < shares; i += kWave) top = fmaxf(top, a.ml[slot(i)].x);
+    top = group_max<64>(top);
+    float sum = 0.f;
+    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < shares; ++i) {
+      const float2 ml = a.ml[slot(i)];
+      const float w = ml.x == -INFINITY ? 0.f : exp2f(ml.x - top);
+      sum += w * ml.y;
+      const float* p = a.part + slot(i) * a.dp;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (lane + 64 * e < a.D) acc[e] += w * p[lane + 64 * e];
+    }
+    const int packed = tile * kRows + row;
+    const long long at = (long long)(s.row0 + packed / a.G) * a.H + kvh * a.G + packed % a.G;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int d = lane + 64 * e;
+      if (d >= a.D) break;
+      const float x = acc[e] * inv;
+      if (a.q_type == VRM_SRC_F32)
+        static_cast<float*>(a.out)[at * a.D + d] = x;
+      else if (a.q_type == VRM_SRC_F16)
+        static_cast<uint16_t*>(a.out)[at * a.D + d] = __builtin_bit_cast(unsigned short, (_Float16)x);
+      else
+        static_cast<uint16_t*>(a.out)[at * a.D + d] = __builtin_bit_cast(unsigned short, (__bf16)x);
+    }
+    if (a.lse && lane == 0) a.lse[at] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.69314718055994531f;
+  }
+}
+
+// Items of a call, from its sizes alone (lengths are on the device).
+struct ChunkPlan {
+  int target, min_blocks, vtiles, items, dp;
+  size_t rec_bytes, ml_bytes, bytes;
+};
+
+// Tiles that fill the GPU twice are left whole; fewer are cut into shares, at
+// least kMinBlocks blocks each, for about kWantedItems workgroups.
+constexpr int kWantedItems = 1024;
+constexpr int kMinBlocks = 4;
+
+bool plan_chunk(int N, int B, int H, int KH, int D, int PS, int max_pp, ChunkPlan& p) {
+  const long long G = H / KH;
+  const long long vtiles = N * G / kRows + B;
+  const long long blocks = ((long long)max_pp * PS + 31) / 32;  // at most, of 32 tokens
+  p.dp = D <= 64 ? 64 : D <= 96 ? 96 : D <= 128 ? 128 : 256;
+  p.min_blocks = kMinBlocks;
+  p.target = 0;
+  long long items = vtiles;
+  if (N * G / kRows * KH < kWantedItems && blocks > kMinBlocks) {
+    p.target = (kWantedItems + KH - 1) / KH;
+    const long long most = vtiles * ((blocks + kMinBlocks - 1) / kMinBlocks);
+    // sum of tiles * ceil(blocks / share): target + one per tile, and the
+    // rounding of the float sum that gives the share
+    items = vtiles + p.target + p.target / 256 + 2;
+    if (items > most) items = most;
+  }
+  if (items * KH > 0x7fffffffLL || N * G > 0x7fffffffLL) return false;
+  p.vtiles = (int)vtiles;
+  p.items = (int)items;
+  p.rec_bytes = p.ml_bytes = p.bytes = 0;
+  if (p.target) {
+    const int dp = p.dp == 96 ? 128 : p.dp;  // the float32 kernel pads 96 to 128
+    p.rec_bytes = ((size_t)vtiles * KH * sizeof(int2) + 255) / 256 * 256;
+    p.ml_bytes = (size_t)items * KH * kRows * sizeof(float2);
+    p.bytes = p.rec_bytes + p.ml_bytes + (size_t)items * KH * kRows * dp * sizeof(float);
+  }
+  return true;
+}
+
+bool bad_sizes(int N, int B, int H, int KH, int D, int PS, int max_pp) {
+  return N < 0 || B < 0 || H <= 0 || KH <= 0 || H % KH || D <= 0 || PS <= 0 || max_pp < 0;
+}
+
+}  // namespace
+}  // namespace vrm
+
+using namespace vrm;
+
+extern "C" size_t vrm_paged_chunk_workspace_bytes(int N, int B, int H, int KH, int D, int PS, int max_pp) {
+  ChunkPlan p;
+  if (bad_sizes(N, B, H, KH, D, PS, max_pp) || D > 256 || !plan_chunk(N, B, H, KH, D, PS, max_pp, p)) return 0;
+  return p.bytes;
+}
+
+extern "C" int vrm_paged_chunk_attention(const void* query, int q_dtype, long long q_token_stride,
+                                         long long q_head_stride, const void* kv_pool, const float* kv_scales,
+                                         const int32_t* page_table, const int32_t* context_lens,
+                                         const int32_t* cu_seqlens, void* out, float* lse, void* workspace,
+                                         size_t workspace_bytes, int N, int B, int H, int KH, int D, int PS, int L,
+                                         int P, int max_pp, int layer_idx, float scale, int causal, int window,
+                                         int kv_dtype, vrm_stream_t stream) {
+  const char* who = "vrm_paged_chunk_attention";
+  if (bad_sizes(N, B, H, KH, D, PS, max_pp) || L <= 0 || P <= 0 || window < 0) {
+    set_error("%s: bad sizes (N=%d B=%d H=%d KH=%d D=%d PS=%d L=%d P=%d max_pp=%d window=%d; H a multiple of KH)", who,
+              N, B, H, KH, D, PS, L, P, max_pp, window);
+    return VRM_ERR_ARG;
+  }
+  if (layer_idx < 0 || layer_idx >= L) {
+    set_error("%s: layer_idx %d outside [0, %d)", who, layer_idx, L);
+    return VRM_ERR_ARG;
+  }
+  if (!isfinite(scale)) {
+    set_error("%s: scale is not finite", who);
+    return VRM_ERR_ARG;
+  }
+  if (q_dtype != VRM_SRC_F32 && q_dtype != VRM_SRC_F16 && q_dtype != VRM_SRC_BF16) {
+    set_error("%s: unknown query dtype %d", who, q_dtype);
+    return VRM_ERR_ARG;
+  }
+  int kind;
+  long long row;
+  switch (kv_dtype) {
+    case VRM_KV_F32: kind = kSrcF32, row = 4LL * D; break;
+    case VRM_KV_F16: kind = kSrcF16, row = 2LL * D; break;
+    case VRM_KV_BF16: kind = kSrcBf16, row = 2LL * D; break;
+    case VRM_KV_I8:
+    case VRM_KV_I8_INLINE: kind = kSrcI8, row = D; break;
+    case VRM_KV_FP8E4M3:
+    case VRM_KV_FP8E4M3_INLINE: kind = kSrcFp8, row = D; break;
+    default: set_error("%s: unknown kv_dtype %d", who, kv_dtype); return VRM_ERR_ARG;
+  }
+  if (D > 256) {
+    set_error("%s: head_dim %d above 256", who, D);
+    return VRM_ERR_UNSUPPORTED;
+  }
+  if (kind >= kSrcI8 && (D % 16 || PS % 4)) {
+    set_error("%s: head_dim %d / page_size %d unsupported over a quantized pool (multiples of 16 / 4)", who, D, PS);
+    return VRM_ERR_UNSUPPORTED;
+  }
+  ChunkPlan p;
+  if (!plan_chunk(N, B, H, KH, D, PS, max_pp, p)) {
+    set_error("%s: too many rows (N=%d H=%d B=%d)", who, N, H, B);
+    return VRM_ERR_UNSUPPORTED;
+  }
+  if (N == 0 || B == 0) {
+    clear_error();
+    return VRM_OK;
+  }
+  if (!query || !kv_pool || !context_lens || !cu_seqlens || !out || (max_pp > 0 && !page_table)) {
+    set_error("%s: null pointer argument", who);
+    return VRM_ERR_ARG;
+  }
+  if ((kind >= kSrcI8) != (kv_scales != nullptr)) {
+    set_error("%s: kv_scales is for int8 and fp8 pools, and they need it", who);
+    return VRM_ERR_ARG;
+  }
+  if (kind >= kSrcI8) {
+    const int rc = check_pool_scales(kv_dtype, kv_pool, kv_scales, KH, PS, D, L, P, who);
+    if (rc) return rc;
+  }
+  const uintptr_t q_at = reinterpret_cast<uintptr_t>(query);
+  if (p.bytes && (!workspace || workspace_bytes < p.bytes || reinterpret_cast<uintptr_t>(workspace) % 16)) {
+    set_error("%s: workspace of %zu bytes, 16-byte aligned, needed (got %zu)", who, p.bytes, workspace_bytes);
+    return VRM_ERR_WORKSPACE;
+  }
+
+  ChunkArgs a{};
+  a.q = query;
+  a.q_n = q_token_stride;
+  a.q_h = q_head_stride;
+  a.q_type = q_dtype;
+  a.pool = static_cast<const uint8_t*>(kv_pool);
+  a.scales = kv_scales;
+  a.g = pool_geom(kv_dtype, KH, PS, D, row, P, L);
+  a.layer_off = (long long)layer_idx * a.g.layer;
+  a.s_layer_off = (long long)layer_idx * a.g.s_layer;
+  a.table = page_table;
+  a.lens = context_lens;
+  a.cu = cu_seqlens;
+  a.out = out;
+  a.lse = lse;
+  a.N = N, a.B = B, a.H = H, a.KH = KH, a.G = H / KH, a.D = D, a.PS = PS, a.P = P, a.max_pp = max_pp;
+  a.ps_shift = (PS & (PS - 1)) ? -1 : __builtin_ctz(PS);
+  a.causal = causal != 0;
+  a.window = window;
+  a.sc = scale == 0.f ? 1.f : fabsf(scale) * 1.44269504088896341f;
+  a.q_sign = scale == 0.f ? 0 : scale < 0.f ? -1 : 1;
+  a.target = p.target;
+  a.min_blocks = p.min_blocks;
+  a.vtiles = p.vtiles;
+  a.items = p.items;
+  a.aligned = row % 16 == 0 && reinterpret_cast<uintptr_t>(kv_pool) % 16 == 0;
+  a.q_aligned = q_at % 16 == 0 && q_token_stride % 8 == 0 && q_head_stride % 8 == 0;
+  a.out_aligned = D % 4 == 0 && reinterpret_cast<uintptr_t>(out) % 8 == 0;
+  // 16-bit products where queries and keys have one 16-bit type (codes have any)
+  const bool wide = q_dtype == VRM_SRC_F32 || kind == kSrcF32 || (q_dtype == VRM_SRC_F16 && kind == kSrcBf16) ||
+                    (q_dtype == VRM_SRC_BF16 && kind == kSrcF16);
+  a.dp = wide && p.dp == 96 ? 128 : p.dp;
+  char* ws = static_cast<char*>(workspace);
+  if (p.target) {
+    a.rec = reinterpret_cast<int2*>(ws);
+    a.ml = reinterpret_cast<float2*>(ws + p.rec_bytes);
+    a.part = reinterpret_cast<float*>(ws + p.rec_bytes + p.ml_bytes);
+  }
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  const dim3 grid((unsigned)p.items * (unsigned)KH);
+  if (wide)
+    launch_chunk_f32(a, kind, grid, st);
+  else if (kind == kSrcI8)
+    launch_chunk16_i8(a, grid, st);
+  else if (kind == kSrcFp8)
+    launch_chunk16_fp8(a, grid, st);
+  else
+    launch_chunk16_float(a, grid, st);
+  const int rc = launch_status(who);
+  if (rc || !p.target) return rc;
+  hipLaunchKernelGGL(chunk_merge_kernel, dim3((unsigned)p.vtiles * (unsigned)KH, kRows / 16), dim3(256), 0, st, a);
+  return launch_status(who);
+}

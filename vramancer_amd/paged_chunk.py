@@ -1,0 +1,164 @@
+"""A chunk of new tokens over the paged KV cache: its attention.
+
+The decode attends one token per sequence.  Prompts, chunks of prompts,
+drafted tokens to verify and batches that mix them with decoding requests have
+several; ``paged_attention_chunk`` attends them straight from the pages.  The
+reference has no counterpart: its prompts run through the model's own
+attention, and ``from_hf_cache`` stores the result
+(core/paged_attention.py:716-805).
+
+A batch is ragged and described by three int32 device tensors:
+
+* ``cu_seqlens`` [B + 1]: sequence b's new tokens are rows ``cu_seqlens[b] ..
+  cu_seqlens[b + 1]`` of the N given.  Rows from ``cu_seqlens[B]`` on belong to
+  no sequence: they are neither read nor written, so that N can stay fixed
+  while a captured graph is replayed over smaller batches;
+* ``context_lens`` [B]: tokens in the cache, the new ones included, so that new
+  token i of q is at position ``context_lens[b] - q + i``;
+* ``page_table`` [B, max_pages] as the decode takes it.
+
+Everything else is decided on the device; no call reads a tensor back.
+"""
+from __future__ import annotations
+
+import contextlib
+import functools
+import math
+from typing import Any, Optional
+
+import torch
+
+from . import _lib, kv_quant
+
+__all__ = ["paged_attention_chunk", "chunk_workspace"]
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(N: int, B: int, H: int, KH: int, D: int, PS: int, max_pp: int) -> int:
+    return _lib.load().vrm_paged_chunk_workspace_bytes(N, B, H, KH, D, PS, max_pp)
+
+
+def chunk_workspace(num_tokens: int, batch: int, num_heads: int, num_kv_heads: int, head_dim: int,
+                    max_pages_per_seq: int, device: Any, page_size: int = 16):
+    """The workspace a ``paged_attention_chunk`` call of these sizes needs,
+    for callers that keep one (``workspace=``)."""
+    nbytes = _workspace_bytes(num_tokens, batch, num_heads, num_kv_heads, head_dim, page_size, max_pages_per_seq)
+    return torch.empty(nbytes, dtype=torch.uint8, device=device)
+
+
+def on_device(t):
+    """Makes t's device the current one for a launch on its stream, where it
+    is not."""
+    if torch.cuda.current_device() == t.get_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(t.get_device())
+
+
+def check_pool(kv_pool, kv_scales, D: int):
+    """(pool, scales, kv_dtype code) of a pool as the C ABI takes it."""
+    if kv_pool.dim() != 6:
+        raise RuntimeError(f"kv_pool must be [P, L, 2, KH, PS, D], got shape {tuple(kv_pool.shape)}")
+    P, L, two, KH, PS, Dp = kv_pool.shape
+    if two != 2 or Dp != D:
+        raise RuntimeError(f"kv_pool shape {tuple(kv_pool.shape)} does not match head_dim {D}")
+    code = _lib.kv_dtype_code(kv_pool.dtype)
+    if code not in (_lib.VRM_KV_I8, _lib.VRM_KV_FP8E4M3):
+        if kv_scales is not None:
+            raise RuntimeError("kv_scales is only meaningful for int8 / float8_e4m3fn pools")
+        if not kv_pool.is_contiguous():
+            raise RuntimeError("a float kv_pool must be contiguous")
+        return code
+    want = (P, L, 2, KH, PS) if code == _lib.VRM_KV_I8 else (P, L, 2, KH)
+    if kv_scales is None or tuple(kv_scales.shape) != want or kv_scales.dtype != torch.float32:
+        raise RuntimeError(f"{kv_pool.dtype} pool needs float32 kv_scales of shape {want}")
+    code = kv_quant.pool_dtype_code(kv_pool, kv_scales)
+    if code is None:
+        raise RuntimeError("kv_pool and kv_scales must be dense arrays or the two views allocate_pool returns")
+    return code
+
+
+def check_batch(page_table, context_lens, cu_seqlens):
+    """(page_table, context_lens, cu_seqlens, B) as contiguous int32 tensors."""
+    if page_table.dim() != 2 or context_lens.dim() != 1 or page_table.shape[0] != context_lens.shape[0]:
+        raise RuntimeError(f"page_table must be [B, max_pages] and context_lens [B], got {tuple(page_table.shape)} and "
+                           f"{tuple(context_lens.shape)}")
+    B = context_lens.shape[0]
+    if tuple(cu_seqlens.shape) != (B + 1,):
+        raise RuntimeError(f"cu_seqlens must be [B + 1 = {B + 1}], got {tuple(cu_seqlens.shape)}")
+    out = []
+    for t in (page_table, context_lens, cu_seqlens):
+        if t.dtype != torch.int32:
+            if t.dtype not in (torch.int64, torch.int16, torch.int8, torch.uint8):
+                raise RuntimeError(f"page_table, context_lens and cu_seqlens must be integers, got {t.dtype}")
+            t = t.to(torch.int32)
+        out.append(t.contiguous())
+    return out[0], out[1], out[2], B
+
+
+def paged_attention_chunk(
+    query: Any,         # [N, H, D] float32 / float16 / bfloat16, last dim contiguous
+    kv_pool: Any,       # [P, L, 2, KH, PS, D] float32 / float16 / bfloat16 / int8 / float8_e4m3fn
+    page_table: Any,    # [B, max_pages]
+    context_lens: Any,  # [B], the new tokens included
+    cu_seqlens: Any,    # [B + 1]
+    layer_idx: int,
+    scale: Optional[float] = None,
+    kv_scales: Any = None,
+    causal: bool = True,
+    window: Optional[int] = None,
+    out: Any = None,
+    lse: Any = None,
+    workspace: Any = None,
+) -> Any:
+    """Attention of each sequence's new tokens over its pages; the new tokens'
+    keys and values are in the cache already.
+
+    Row n attends the tokens of its sequence up to its own position (all of
+    them with ``causal=False``), the last ``window`` of those when given.
+    Tokens of absent pages (entries < 0 or >= P) are skipped; a row that sees
+    nothing gives zeros.  ``scale`` defaults to 1 / sqrt(D).  Returns [N, H, D]
+    in the query's dtype (``out`` when given; rows past ``cu_seqlens[B]`` are
+    left as they were, undefined in an output allocated here).  ``lse``
+    optionally takes ln sum exp of the scaled scores, [N, H] float32, for
+    ``combine_attention``.
+
+    Calls may run at once on several streams if they share neither output nor
+    ``workspace``; results do not depend on what a workspace held before, and
+    are the same from call to call.
+    """
+    _lib.require_cuda(query, kv_pool, page_table, context_lens, cu_seqlens, kv_scales, out, lse, workspace)
+    if query.dim() != 3:
+        raise RuntimeError(f"query must be [N, H, D], got shape {tuple(query.shape)}")
+    N, H, D = query.shape
+    q_code = _lib.src_dtype_code(query.dtype)
+    code = check_pool(kv_pool, kv_scales, D)
+    P, L, _, KH, PS, _ = kv_pool.shape
+    page_table, context_lens, cu_seqlens, B = check_batch(page_table, context_lens, cu_seqlens)
+    if window is not None and not 0 < window < 1 << 31:
+        raise RuntimeError(f"window must be a positive number of tokens, got {window}")
+    if query.stride(2) != 1 and D > 1:
+        query = query.contiguous()
+    if out is None:
+        out = torch.empty((N, H, D), dtype=query.dtype, device=query.device)
+    elif tuple(out.shape) != (N, H, D) or out.dtype != query.dtype or not out.is_contiguous():
+        raise RuntimeError(f"out must be a contiguous {query.dtype} [{N}, {H}, {D}] tensor, got {out.dtype} "
+                           f"{tuple(out.shape)}")
+    if lse is not None and (tuple(lse.shape) != (N, H) or lse.dtype != torch.float32 or not lse.is_contiguous()):
+        raise RuntimeError(f"lse must be a contiguous float32 [{N}, {H}] tensor")
+    max_pp = page_table.shape[1]
+    need = _workspace_bytes(N, B, H, KH, D, PS, max_pp) if H % KH == 0 else 0
+    if workspace is None:
+        if need:
+            workspace = torch.empty(need, dtype=torch.uint8, device=query.device)
+    elif not workspace.is_contiguous():
+        raise RuntimeError("workspace must be contiguous")
+    ws_bytes = workspace.numel() * workspace.element_size() if workspace is not None else 0
+    with on_device(query):
+        rc = _lib.load().vrm_paged_chunk_attention(
+            _lib.ptr(query), q_code, query.stride(0), query.stride(1), _lib.ptr(kv_pool), _lib.ptr(kv_scales),
+            _lib.ptr(page_table), _lib.ptr(context_lens), _lib.ptr(cu_seqlens), _lib.ptr(out), _lib.ptr(lse),
+            _lib.ptr(workspace), ws_bytes, N, B, H, KH, D, PS, L, P, max_pp, int(layer_idx),
+            1.0 / math.sqrt(D) if scale is None else float(scale), int(bool(causal)), window or 0, code,
+            _lib.stream_of(query))
+    _lib.check(rc, "paged_attention_chunk")
+    return out
