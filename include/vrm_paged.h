@@ -653,6 +653,53 @@ int vrm_paged_chunk_attention(const void* query, int q_dtype, long long q_token_
                               int L, int P, int max_pp, int layer_idx, float scale, int causal,
                               int window, int kv_dtype, vrm_stream_t stream);
 
+/*
+ * RMS norm of every query and key head, then the rotation of its first
+ * rotary_dim dims by position, in float32 and rounded once:
+ *   x' = weight x / sqrt(mean(x^2) + eps)         (where the weight is given)
+ *   (a, b) -> (a cos - b sin, b cos + a sin)      (where cos_sin is given)
+ * over the pairs (d, d + rotary_dim / 2), or (2 d, 2 d + 1) with interleaved.
+ *   query, key   [N][H][D], [N][KH][D] of src_dtype, strides in elements; H or
+ *                KH may be 0
+ *   cos_sin      [max_positions][rotary_dim] float32: rotary_dim / 2 cosines,
+ *                then as many sines; NULL for no rotation
+ *   positions    [N] integers of position_bytes (4 or 8); a position outside
+ *                [0, max_positions) gives a row of NaN
+ *   q_weight, k_weight  [D] of weight_dtype, or NULL for no norm
+ *   query_out, key_out  dense, of src_dtype; may be the inputs if those are dense
+ */
+int vrm_qk_norm_rope(const void* query, long long q_token_stride, long long q_head_stride,
+                     const void* key, long long k_token_stride, long long k_head_stride,
+                     int src_dtype, const float* cos_sin, int rotary_dim, int max_positions,
+                     const void* positions, int position_bytes, const void* q_weight,
+                     const void* k_weight, int weight_dtype, float eps, int interleaved,
+                     void* query_out, void* key_out, int N, int H, int KH, int D,
+                     vrm_stream_t stream);
+
+/*
+ * The same over a ragged batch (above), the keys and the values going into
+ * their pages: new token i of sequence b to position context_lens[b] - q_b + i.
+ * Float pools take the rows rounded to nearest even; int8 pools the codes and
+ * per-token scales of vrm_kv_quant_append.  An fp8 page's scale is the largest
+ * of its scale so far (0 if its first new slot is 0) and amax / 448 over its
+ * new tokens; earlier codes are re-encoded once when it grows.
+ * positions (NULL: the tokens' own) rotate only.  Keys and values whose page
+ * is absent, whose position is negative or past the table, are dropped (the
+ * query row of a position outside the rotation table is NaN).  Sequences of one
+ * call must not write the same slots, in an fp8 pool not the same page.  H may
+ * be 0 (query NULL: only keys and values).
+ */
+int vrm_rope_append(const void* query, long long q_token_stride, long long q_head_stride,
+                    const void* key, long long k_token_stride, long long k_head_stride,
+                    const void* value, long long v_token_stride, long long v_head_stride,
+                    int src_dtype, const float* cos_sin, int rotary_dim, int max_positions,
+                    const void* positions, int position_bytes, const void* q_weight,
+                    const void* k_weight, int weight_dtype, float eps, int interleaved,
+                    void* query_out, void* kv_pool, float* kv_scales, int kv_dtype,
+                    const int32_t* page_table, const int32_t* context_lens,
+                    const int32_t* cu_seqlens, int N, int B, int H, int KH, int D, int PS, int L,
+                    int P, int max_pp, int layer_idx, vrm_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -108,3 +108,33 @@ def attend(q, vals, table, lens, cu, layer, scale=None, causal=True, window=None
             reach[rows, h] = p @ vz.abs()
             lse[rows, h] = torch.logsumexp(s, -1)
     return out, lse, reach
+
+
+def rope_angles(top, rot, base=10000.0):
+    """[top, rot] float32 as rope_table computes it, from its definition."""
+    freq = torch.tensor([base ** (-2 * i / rot) for i in range(rot // 2)], dtype=torch.float64)
+    a = torch.arange(top, dtype=torch.float64)[:, None] * freq
+    return torch.cat([a.cos(), a.sin()], 1).float()
+
+
+def norm_rope(x, w, table, positions, eps, interleaved):
+    """(y, size): float64 norm and rotation of [N, heads, D] rows, and the
+    magnitude that each element's float32 rounding errors go by."""
+    y = x.double()
+    if w is not None:
+        y = y / (y.pow(2).mean(-1, keepdim=True) + eps).sqrt() * w.double()
+    size = y.abs().clone()
+    out = y.clone()
+    if table is not None:
+        rot = table.shape[1]
+        half = rot // 2
+        a = torch.arange(half) * (2 if interleaved else 1)
+        b = a + (1 if interleaved else half)
+        known = (positions >= 0) & (positions < table.shape[0])
+        cs = table[positions.clamp(0, table.shape[0] - 1).long()].double()[:, None]
+        c, s = cs[..., :half], cs[..., half:]
+        out[..., a] = y[..., a] * c - y[..., b] * s
+        out[..., b] = y[..., b] * c + y[..., a] * s
+        size[..., a] = size[..., b] = y[..., a].abs() + y[..., b].abs()
+        out[~known] = math.nan
+    return out, size

@@ -84,6 +84,10 @@ SIGNATURES = {
     "vrm_attn_combine": (_i, [_p, _p, _p, _p, _ll, _i, _p, _p, _p]),
     "vrm_pack_bits": (_i, [_p, _ll, _i, _i, _p, _p]),
     "vrm_unpack_bits": (_i, [_p, _ll, _i, _i, _p, _p]),
+    "vrm_qk_norm_rope": (_i, [_p, _ll, _ll, _p, _ll, _ll, _i, _p, _i, _i, _p, _i, _p, _p, _i, _f, _i, _p, _p] + [_i] * 4
+                         + [_p]),
+    "vrm_rope_append": (_i, [_p, _ll, _ll, _p, _ll, _ll, _p, _ll, _ll, _i, _p, _i, _i, _p, _i, _p, _p, _i, _f, _i, _p,
+                             _p, _p, _i, _p, _p, _p] + [_i] * 10 + [_p]),
     "vrm_paged_chunk_workspace_bytes": (_sz, [_i] * 7),
     "vrm_paged_chunk_attention": (_i, [_p, _i, _ll, _ll] + [_p] * 8 + [_sz] + [_i] * 10 + [_f, _i, _i, _i, _p]),
 }

@@ -53,8 +53,6 @@ struct ChunkArgs {
   int out_aligned;   // output rows can be stored 8 bytes at a time
 };
 
-__device__ __forceinline__ int clamp_int(int x, int lo, int hi) { return min(max(x, lo), hi); }
-
 struct Sequence {
   int row0, q_len, ctx;
 };

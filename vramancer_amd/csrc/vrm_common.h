@@ -106,6 +106,8 @@ __device__ __forceinline__ float strided_sum(float v) {
   return v;
 }
 
+__device__ __forceinline__ int clamp_int(int x, int lo, int hi) { return min(max(x, lo), hi); }
+
 __device__ __forceinline__ float bf16_bits_to_f32(uint32_t h) { return __uint_as_float(h << 16); }
 
 __device__ __forceinline__ float f16_bits_to_f32(uint32_t h) {

@@ -1,10 +1,12 @@
-"""A chunk of new tokens over the paged KV cache: its attention.
+"""A chunk of new tokens over the paged KV cache: how it enters its pages and
+attends them.
 
 The decode attends one token per sequence.  Prompts, chunks of prompts,
 drafted tokens to verify and batches that mix them with decoding requests have
-several; ``paged_attention_chunk`` attends them straight from the pages.  The
-reference has no counterpart: its prompts run through the model's own
-attention, and ``from_hf_cache`` stores the result
+several.  ``rope_append`` norms and rotates their queries and keys and writes
+keys and values into the pages in one pass; ``paged_attention_chunk`` attends
+them straight from the pages.  The reference has no counterpart: its prompts
+run through the model's own attention, and ``from_hf_cache`` stores the result
 (core/paged_attention.py:716-805).
 
 A batch is ragged and described by three int32 device tensors:
@@ -21,7 +23,6 @@ Everything else is decided on the device; no call reads a tensor back.
 """
 from __future__ import annotations
 
-import contextlib
 import functools
 import math
 from typing import Any, Optional
@@ -29,8 +30,9 @@ from typing import Any, Optional
 import torch
 
 from . import _lib, kv_quant
+from .rope import check_heads, check_out, check_positions, check_table, check_weights, on_device
 
-__all__ = ["paged_attention_chunk", "chunk_workspace"]
+__all__ = ["rope_append", "paged_attention_chunk", "chunk_workspace"]
 
 
 @functools.lru_cache(maxsize=256)
@@ -44,14 +46,6 @@ def chunk_workspace(num_tokens: int, batch: int, num_heads: int, num_kv_heads: i
     for callers that keep one (``workspace=``)."""
     nbytes = _workspace_bytes(num_tokens, batch, num_heads, num_kv_heads, head_dim, page_size, max_pages_per_seq)
     return torch.empty(nbytes, dtype=torch.uint8, device=device)
-
-
-def on_device(t):
-    """Makes t's device the current one for a launch on its stream, where it
-    is not."""
-    if torch.cuda.current_device() == t.get_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(t.get_device())
 
 
 def check_pool(kv_pool, kv_scales, D: int):
@@ -93,6 +87,74 @@ def check_batch(page_table, context_lens, cu_seqlens):
             t = t.to(torch.int32)
         out.append(t.contiguous())
     return out[0], out[1], out[2], B
+
+
+def rope_append(
+    query: Any,         # [N, H, D] float32 / float16 / bfloat16, or None: only keys and values
+    key: Any,           # [N, KH, D]
+    value: Any,         # [N, KH, D]
+    kv_pool: Any,       # [P, L, 2, KH, PS, D] float32 / float16 / bfloat16 / int8 / float8_e4m3fn
+    page_table: Any,    # [B, max_pages]
+    context_lens: Any,  # [B], the new tokens included
+    cu_seqlens: Any,    # [B + 1]
+    layer_idx: int,
+    cos_sin: Any = None,  # [max_positions, rotary_dim] float32 (rope.rope_table), or None: no rotation
+    kv_scales: Any = None,
+    positions: Any = None,  # [N] int32 / int64; default: the tokens' own
+    q_weight: Any = None,
+    k_weight: Any = None,
+    eps: float = 1e-6,
+    interleaved: bool = False,
+    query_out: Any = None,
+) -> Any:
+    """Norms and rotates the new tokens' queries and keys as
+    ``rope.qk_norm_rope`` does, writes keys and values into their pages, and
+    returns the queries, [N, H, D] in their dtype (``None`` without queries).
+
+    Keys go from float32 straight to the pool's type: rounded to nearest even,
+    or to ``kv_quant``'s int8 codes and per-token scales.  An fp8 page's scale
+    becomes the larger of its own (0 if it is entered at slot 0) and
+    amax / 448 over its new tokens, and codes already in it are re-encoded once
+    when it grows.
+
+    ``positions`` change the rotation only, not the places.  Keys and values
+    for absent pages (entries < 0 or >= P), negative positions or positions
+    outside the rotation table are dropped; in the last case the query row is
+    NaN.  Rows from ``cu_seqlens[B]`` on are left as they were.  Sequences of
+    one call must not write the same slots, nor, in an fp8 pool, the same page.
+    """
+    _lib.require_cuda(key, query, value, kv_pool, page_table, context_lens, cu_seqlens, cos_sin, kv_scales, positions,
+                      q_weight, k_weight, query_out)
+    key = check_heads("key", key, None, None, None)
+    N, KH, D = key.shape
+    value = check_heads("value", value, N, D, key.dtype)
+    src = _lib.src_dtype_code(key.dtype)
+    code = check_pool(kv_pool, kv_scales, D)
+    P, L, _, pool_heads, PS, _ = kv_pool.shape
+    if KH != pool_heads or value.shape[1] != KH:
+        raise RuntimeError(f"key and value must have the pool's {pool_heads} heads, got {KH} and {value.shape[1]}")
+    H = 0
+    if query is not None:
+        query = check_heads("query", query, N, D, key.dtype)
+        H = query.shape[1]
+        query_out = check_out("query_out", query_out, query)
+    elif query_out is not None:
+        raise RuntimeError("query_out without a query")
+    page_table, context_lens, cu_seqlens, B = check_batch(page_table, context_lens, cu_seqlens)
+    rot, top = check_table(cos_sin, D)
+    if positions is not None:
+        positions = check_positions(positions, N)
+    q_weight, k_weight, w_code = check_weights(q_weight, k_weight, D)
+    with on_device(key):
+        rc = _lib.load().vrm_rope_append(
+            _lib.ptr(query), query.stride(0) if H else 0, query.stride(1) if H else 0, _lib.ptr(key), key.stride(0),
+            key.stride(1), _lib.ptr(value), value.stride(0), value.stride(1), src, _lib.ptr(cos_sin), rot, top,
+            _lib.ptr(positions), positions.element_size() if positions is not None else 4, _lib.ptr(q_weight),
+            _lib.ptr(k_weight), w_code, float(eps), int(bool(interleaved)), _lib.ptr(query_out), _lib.ptr(kv_pool),
+            _lib.ptr(kv_scales), code, _lib.ptr(page_table), _lib.ptr(context_lens), _lib.ptr(cu_seqlens), N, B, H, KH,
+            D, PS, L, P, page_table.shape[1], int(layer_idx), _lib.stream_of(key))
+    _lib.check(rc, "rope_append")
+    return query_out
 
 
 def paged_attention_chunk(
