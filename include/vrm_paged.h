@@ -644,7 +644,8 @@ int vrm_paged_decode_tq_residual(
  * softmax statistics are float32.  Any D <= 256, any page size; int8 / fp8
  * pools need D % 16 == 0 and PS % 4 == 0.
  */
-size_t vrm_paged_chunk_workspace_bytes(int N, int B, int H, int KH, int D, int PS, int max_pp);
+size_t vrm_paged_chunk_workspace_bytes(int N, int B, int H, int KH, int D, int PS, int max_pp,
+                                       int q_dtype, int kv_dtype);
 int vrm_paged_chunk_attention(const void* query, int q_dtype, long long q_token_stride,
                               long long q_head_stride, const void* kv_pool, const float* kv_scales,
                               const int32_t* page_table, const int32_t* context_lens,

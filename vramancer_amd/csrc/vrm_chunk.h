@@ -4,7 +4,7 @@
 //
 // Rows.  The G = H / KH query heads of a kv-head read the same keys, so a
 // sequence's q_b new tokens make q_b G rows of one matrix per kv-head: row r
-// is head r % G of token r / G.  A tile is kRows of them.
+// is head r % G of token r / G.  A tile is tile_rows of them.
 // Items.  A workgroup takes one item: a tile of one kv-head over a share of
 // the key blocks that its rows see.  A batch of few tiles is cut along the
 // keys (find_item) so that the GPU is full; the shares' (max, sum,
@@ -16,8 +16,8 @@
 
 namespace vrm {
 
-constexpr int kRows = 128;          // rows of a tile
-constexpr int kChunkThreads = 256;  // four wavefronts
+constexpr int kChunkThreads = 256;  // four wavefronts: tiles of 128 rows
+constexpr int kLargeThreads = 512;  // eight: tiles of 256
 
 enum { kSrcF32 = 0, kSrcF16 = 1, kSrcBf16 = 2, kSrcI8 = 3, kSrcFp8 = 4 };  // element types of a pool
 
@@ -34,11 +34,12 @@ struct ChunkArgs {
   const int32_t* cu;
   void* out;  // [N][H][D] of q_type
   float* lse;
-  float* part;  // [items][kRows][dp]: accumulators of shares
-  float2* ml;   // [items][kRows]: their max (log2 units) and sum
+  float* part;  // [items][tile_rows][dp]: accumulators of shares
+  float2* ml;   // [items][tile_rows]: their max (log2 units) and sum
   int2* rec;    // [vtiles][KH]: first item and shares of a tile
   int N, B, H, KH, G, D, PS, P, max_pp;
   int dp;       // D as the kernel pads it
+  int tile_rows, tile_shift;  // 128 or 256, and its logarithm
   int vtiles;   // tiles when every sequence has one more than its rows fill
   int items;    // items per kv-head that the grid (and the workspace) has room for
   int ps_shift;      // log2 PS, or -1
@@ -54,32 +55,36 @@ struct ChunkArgs {
 };
 
 struct Sequence {
-  int row0, q_len, ctx;
+  int row0, q_len;
+  int ctx;   // tokens that the page table has room for
+  int base;  // position of its first new token
 };
 
 __device__ __forceinline__ Sequence load_sequence(const ChunkArgs& a, int b) {
   Sequence s;
   s.row0 = clamp_int(a.cu[b], 0, a.N);
   s.q_len = max(clamp_int(a.cu[b + 1], 0, a.N) - s.row0, 0);
-  s.ctx = (int)min((long long)max(a.lens[b], 0), (long long)a.max_pp * a.PS);
+  const int len = max(a.lens[b], 0);
+  s.ctx = (int)min((long long)len, (long long)a.max_pp * a.PS);
+  s.base = len - s.q_len;
   return s;
 }
 
 // Tiles before those of sequence b when every sequence is given one more than
 // its rows fill: known from cu[b] alone, and at least as many as it needs.
 __device__ __forceinline__ int virtual_tile(const ChunkArgs& a, int row0, int b) {
-  return (int)((long long)row0 * a.G / kRows) + b;
+  return (int)(((long long)row0 * a.G) >> a.tile_shift) + b;
 }
 
 __device__ __forceinline__ int tiles_of(const ChunkArgs& a, const Sequence& s) {
-  return (s.q_len * a.G + kRows - 1) / kRows;
+  return (s.q_len * a.G + a.tile_rows - 1) >> a.tile_shift;
 }
 
 // Key blocks of TN tokens that a tile of the sequence sees at most.
 template <int TN>
 __device__ __forceinline__ int blocks_of(const ChunkArgs& a, const Sequence& s) {
   int span = s.ctx;
-  if (a.window) span = (int)min((long long)span, (long long)a.window + kRows / a.G + 1 + TN);
+  if (a.window) span = (int)min((long long)span, (long long)a.window + a.tile_rows / a.G + 1 + TN);
   return (span + TN - 1) / TN;
 }
 
@@ -99,6 +104,27 @@ struct Item {
   int first;  // item index of the tile's share 0 (per kv-head)
   Sequence s;
 };
+
+// What a wavefront's 32 rows from row0 of the tile are: lane's row (its column
+// of the score tiles), its token and head, and the positions of the first and
+// last row.
+struct RowGroup {
+  int row, tok, head, pos, first_pos, last_pos;
+  bool real;
+};
+__device__ __forceinline__ RowGroup row_group(const ChunkArgs& a, const Item& it, int kvh, int rows, int row0) {
+  RowGroup g;
+  g.row = row0 + (__lane_id() & 31);
+  const int packed = it.tile * a.tile_rows + g.row;
+  g.tok = packed / a.G;
+  g.head = kvh * a.G + packed - g.tok * a.G;
+  g.real = g.row < rows;
+  const int base = it.s.base;
+  g.pos = base + g.tok;
+  g.first_pos = base + (it.tile * a.tile_rows + row0) / a.G;
+  g.last_pos = base + (it.tile * a.tile_rows + min(rows, row0 + 32) - 1) / a.G;
+  return g;
+}
 
 // Item idx of a kv-head: the shares of the first sequence's tiles (later tiles
 // first: under a causal mask they see more keys), then the next sequence's.
@@ -124,7 +150,7 @@ __device__ __forceinline__ bool find_item(const ChunkArgs& a, int idx, Item& it)
   int before = 0;
   for (int b0 = 0; b0 < a.B; b0 += kWave) {
     const int b = b0 + lane;
-    Sequence s{0, 0, 0};
+    Sequence s{0, 0, 0, 0};
     int tiles = 0, shares = 1;
     if (b < a.B) {
       s = load_sequence(a, b);
@@ -140,6 +166,7 @@ __device__ __forceinline__ bool find_item(const ChunkArgs& a, int idx, Item& it)
       it.s.row0 = __builtin_amdgcn_readlane(s.row0, l);
       it.s.q_len = __builtin_amdgcn_readlane(s.q_len, l);
       it.s.ctx = __builtin_amdgcn_readlane(s.ctx, l);
+      it.s.base = __builtin_amdgcn_readlane(s.base, l);
       it.shares = __builtin_amdgcn_readlane(shares, l);
       const int nt = __builtin_amdgcn_readlane(tiles, l);
       const int from = before + __builtin_amdgcn_readlane(upto, l) - nt * it.shares;
@@ -158,9 +185,9 @@ __device__ __forceinline__ bool find_item(const ChunkArgs& a, int idx, Item& it)
 template <int TN>
 __device__ __forceinline__ void item_blocks(const ChunkArgs& a, const Item& it, int& from, int& to) {
   const int rows = it.s.q_len * a.G;
-  const int t0 = it.tile * kRows / a.G;                             // the tile's first token
-  const int t1 = (min(rows, (it.tile + 1) * kRows) - 1) / a.G;      // and its last
-  const int base = it.s.ctx - it.s.q_len;                           // position of token 0
+  const int t0 = it.tile * a.tile_rows / a.G;                             // the tile's first token
+  const int t1 = (min(rows, (it.tile + 1) * a.tile_rows) - 1) / a.G;      // and its last
+  const int base = it.s.base;
   const int hi = a.causal ? clamp_int(base + t1 + 1, 0, it.s.ctx) : it.s.ctx;
   const int lo = a.window ? clamp_int(base + t0 - a.window + 1, 0, hi) : 0;
   const int b0 = lo / TN, n = (hi + TN - 1) / TN - b0;
@@ -189,11 +216,13 @@ __device__ __forceinline__ float load_q(const ChunkArgs& a, long long at) {
 // 16 bytes of which the first `bytes` are there; the rest are zero.
 __device__ __forceinline__ uint4 load16(const uint8_t* p, int bytes, bool vec) {
   if (vec && bytes >= 16) return *reinterpret_cast<const uint4*>(p);
-  uint32_t w[4] = {0, 0, 0, 0};
-#pragma unroll
-  for (int i = 0; i < 16; ++i)
-    if (i < bytes) w[i / 4] |= (uint32_t)p[i] << (8 * (i % 4));
-  return make_uint4(w[0], w[1], w[2], w[3]);
+  unsigned long long lo = 0, hi = 0;
+#pragma unroll 1
+  for (int i = min(bytes, 16) - 1; i >= 0; --i) {
+    hi = hi << 8 | lo >> 56;
+    lo = lo << 8 | p[i];
+  }
+  return make_uint4((uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32));
 }
 
 // One launch of the attention kernel: float32 products (pool of kind kSrc*),

@@ -71,6 +71,15 @@ __device__ __forceinline__ uint2 codes4(uint32_t w) {
   }
 }
 
+// Bytes of a dword whose tokens (bits 0 .. 3) are there.
+__device__ __forceinline__ uint32_t keep_bytes(uint32_t bits) {
+  return ((bits & 1) * 0xffu) | ((bits >> 1 & 1) * 0xff00u) | ((bits >> 2 & 1) * 0xff0000u) |
+         ((bits >> 3 & 1) * 0xff000000u);
+}
+
+constexpr int max3(int x, int y, int z) { return x > y ? (x > z ? x : z) : (y > z ? y : z); }
+
+// Sizes of a block of 64 tokens in LDS.
 template <int KIND, int DP>
 struct ChunkTile {
   static constexpr bool kQuant = KIND >= kSrcI8;
@@ -80,350 +89,103 @@ struct ChunkTile {
   // do the transposed reads' four tokens of 64 bytes.
   static constexpr int kKStride = DP * 2 + 16;
   static constexpr int kVStride = DP * 2 + (DP * 2 % 128 == 0 ? 64 : 0);
+  static constexpr int kKBytes = kTokens * kKStride;
   static constexpr int kVBytes = kQuant ? kTokens * DP * 2 : kTokens * kVStride;
-  static constexpr int kMerge = 2 * (DP / 32 * 16 + 2) * 64 * 4;  // two wavefronts' partials
-  static constexpr int kTile = kTokens * kKStride + kVBytes;
-  static constexpr int kBytes = kTile > kMerge ? kTile : kMerge;
-  static constexpr int kPerRow = kQuant ? DP / 16 : DP / 8;          // 16-byte pieces of a K row
-  static constexpr int kAll = kTokens * kPerRow;                     // of K (and of V)
-  static constexpr int kPieces = (kAll + kChunkThreads - 1) / kChunkThreads;  // per thread
-  static constexpr bool kRagged = kAll % kChunkThreads != 0;
+  static constexpr int kBytes = kKBytes + kVBytes;
+  static constexpr int kPerRow = kQuant ? DP / 16 : DP / 8;  // 16-byte pieces of a K row
+  // 32 rows' accumulators, maxima and sums of a wavefront, for the merge of
+  // wavefronts that shared rows (two at a time)
+  static constexpr int kPartial = (DP / 32 * 16 + 2) * 64 * 4;
+  // a wavefront's own 32 tokens of V (few_rows, float pools)
+  static constexpr int kOwnV = kQuant ? 0 : 32 * kVStride;
 };
 
-template <typename T, int KIND, int DP>
-__global__ void __launch_bounds__(kChunkThreads, DP <= 128 ? 2 : 1) chunk_attn_kernel(ChunkArgs a) {
-  using Tile = ChunkTile<KIND, DP>;
-  constexpr bool QUANT = Tile::kQuant;
-  constexpr int TN = Tile::kTokens, NB = DP / 32, KK = DP / 16, NP = Tile::kPieces;
-  using PT = std::conditional_t<QUANT, Bf16, T>;  // type of the second product
-  constexpr bool SPLIT_P = QUANT && std::is_same_v<T, F16>;
-
-  __shared__ __align__(16) uint8_t tile_lds[Tile::kBytes];
-  __shared__ float scale_lds[2][TN];
-  __shared__ long long place_lds[4][TN];  // a token's K row from the layer's start, -1: not there
-  __shared__ unsigned long long there_lds[4];
-  uint8_t* const k_lds = tile_lds;
-  uint8_t* const v_lds = tile_lds + TN * Tile::kKStride;
-
-  const int kvh = blockIdx.x % a.KH;
-  Item it;
-  if (!find_item<TN>(a, blockIdx.x / a.KH, it)) return;
-  int from, to;
-  item_blocks<TN>(a, it, from, to);
-  put_record(a, it, kvh);
-
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int col = lane & 31, half = lane >> 5;
-
-  // Rows of the tile over wavefronts: 32 each; few rows leave two wavefronts
-  // to a row group, one for each half of a block's tokens.
-  const int rows = min(kRows, it.s.q_len * a.G - it.tile * kRows);
-  const bool halves = rows <= 64;
-  const int group = halves ? wave >> 1 : wave;
-  const bool active = group * 32 < rows;
-  const int row = group * 32 + col;                    // of the tile
-  const int tok = (it.tile * kRows + row) / a.G;       // the row's token
-  const int head = kvh * a.G + (it.tile * kRows + row) % a.G;
-  const int base = it.s.ctx - it.s.q_len;
-  const bool real = row < rows;
-  const int pos = base + tok;
-  const int first_pos = base + (it.tile * kRows + group * 32) / a.G;
-  const int last_pos = base + (it.tile * kRows + min(rows, group * 32 + 32) - 1) / a.G;
-
-  typename T::v8 q[KK];
-  {
-    const uint16_t* src = static_cast<const uint16_t*>(a.q) + (long long)(it.s.row0 + (real ? tok : 0)) * a.q_n +
-                          (long long)(real ? head : 0) * a.q_h;
-    const uint32_t flip = a.q_sign < 0 ? 0x80008000u : 0u;
+// Rows of a group as the operand of the first product: lane (col, half) holds
+// dims dim(kk) .. + 7 of its row for step kk.
+template <typename T, int KK, typename Dim>
+__device__ __forceinline__ void load_rows(const ChunkArgs& a, const Item& it, const RowGroup& g, Dim dim,
+                                          typename T::v8 (&q)[KK]) {
+  const uint16_t* src = static_cast<const uint16_t*>(a.q);
+  if (g.real) src += (long long)(it.s.row0 + g.tok) * a.q_n + (long long)g.head * a.q_h;
+  const uint32_t flip = a.q_sign < 0 ? 0x80008000u : 0u;
 #pragma unroll
-    for (int kk = 0; kk < KK; ++kk) {
-      const int d = kk * 16 + half * 8;
-      uint4 x = make_uint4(0, 0, 0, 0);
-      if (real && active && a.q_sign)
-        x = load16(reinterpret_cast<const uint8_t*>(src + d), (a.D - d) * 2, a.q_aligned);
-      q[kk] = __builtin_bit_cast(typename T::v8, make_uint4(x.x ^ flip, x.y ^ flip, x.z ^ flip, x.w ^ flip));
-    }
+  for (int kk = 0; kk < KK; ++kk) {
+    const int d = dim(kk);
+    uint4 x = make_uint4(0, 0, 0, 0);
+    if (g.real && a.q_sign) x = load16(reinterpret_cast<const uint8_t*>(src + d), (a.D - d) * 2, a.q_aligned);
+    q[kk] = __builtin_bit_cast(typename T::v8, make_uint4(x.x ^ flip, x.y ^ flip, x.z ^ flip, x.w ^ flip));
   }
+}
 
-  f32x16 o[NB];
+// Where 32 tokens of a score tile from t0 on lie for lane half `half`:
+// register i is token t0 + 8 (i / 4) + 4 half + i % 4.
+__device__ __forceinline__ bool needs_mask(const ChunkArgs& a, const RowGroup& g, int t0, uint32_t there) {
+  return there != ~0u || (a.causal && t0 + 31 > g.first_pos) || (a.window && t0 <= g.last_pos - a.window);
+}
+__device__ __forceinline__ void mask_scores(const ChunkArgs& a, const Item& it, const RowGroup& g, int t0, uint32_t there,
+                                            int half, f32x16& s) {
+  const int hi = (a.causal ? min(g.pos, it.s.ctx - 1) : it.s.ctx - 1) - t0 - 4 * half;
+  const int lo = a.window ? g.pos - a.window - t0 - 4 * half : -0x40000000;
+  const uint32_t bits = there >> (4 * half);
 #pragma unroll
-  for (int n = 0; n < NB; ++n) o[n] = f32x16{};
-  float m = -INFINITY, l = 0.f;
-
-  // --- staging -------------------------------------------------------------
-  const uint8_t* const k_base = a.pool + a.layer_off + (long long)kvh * a.g.head;
-  const uint8_t* const v_base = k_base + a.g.kv;
-  const int row_bytes = QUANT ? a.D : 2 * a.D;
-  const int32_t* const table = a.table + (long long)it.b * a.max_pp;
-
-  const auto page_of = [&](int block) {  // wavefront 0: the page of token `lane` of a block
-    const int t = block * TN + lane;
-    return block < to && t < it.s.ctx ? table[page_index(a, t)] : -1;
-  };
-  const auto put_places = [&](int block, int page) {
-    const int t = block * TN + lane;
-    const bool there = page >= 0 && page < a.P;
-    const int slot = t - page_index(a, t) * a.PS;
-    place_lds[block & 3][lane] = there ? (long long)page * a.g.page + (long long)slot * row_bytes : -1;
-    const unsigned long long mask = __ballot(there);
-    if (lane == 0) there_lds[block & 3] = mask;
-  };
-  uint4 kr[NP], vr[NP];
-  float ksc = 0.f, vsc = 0.f;
-  const auto load_tile = [&](int block) {
-#pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      const int c = tid + i * kChunkThreads;
-      kr[i] = vr[i] = make_uint4(0, 0, 0, 0);
-      if (Tile::kRagged && c >= Tile::kAll) continue;
-      const int t = c / Tile::kPerRow, w = c % Tile::kPerRow;
-      const long long at = place_lds[block & 3][t];
-      if (at >= 0) kr[i] = load16(k_base + at + w * 16, row_bytes - w * 16, a.aligned);
-      if constexpr (!QUANT) {
-        if (at >= 0) vr[i] = load16(v_base + at + w * 16, row_bytes - w * 16, a.aligned);
-      } else {  // V: four tokens' codes of a dim in a dword, 4 D bytes for the four tokens
-        const int t4 = c / (DP / 4) * 4, w4 = c % (DP / 4);
-        const long long at4 = place_lds[block & 3][t4];
-        if (at4 >= 0 && w4 * 4 < a.D) vr[i] = load16(v_base + at4 + w4 * 16, 16, a.aligned);
-      }
-    }
-  };
-  const auto load_scales = [&](int block, int page) {  // wavefront 0, quantized pools
-    ksc = vsc = 0.f;
-    if (page >= 0 && page < a.P) {
-      const int t = block * TN + lane;
-      const float* s = a.scales + a.s_layer_off + (long long)page * a.g.s_page + (long long)kvh * a.g.s_head +
-                       (KIND == kSrcI8 ? t - page_index(a, t) * a.PS : 0);
-      ksc = s[0];
-      vsc = s[a.g.s_kv];
-    }
-  };
-  const auto put_tile = [&](int block) {
-    const unsigned long long there = there_lds[block & 3];
-#pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      const int c = tid + i * kChunkThreads;
-      if (Tile::kRagged && c >= Tile::kAll) continue;
-      const int t = c / Tile::kPerRow, w = c % Tile::kPerRow;
-      if constexpr (!QUANT) {
-        *reinterpret_cast<uint4*>(k_lds + t * Tile::kKStride + w * 16) = kr[i];
-        *reinterpret_cast<uint4*>(v_lds + t * Tile::kVStride + w * 16) = vr[i];
-      } else {
-        const uint2 k0 = codes4<T, KIND>(kr[i].x), k1 = codes4<T, KIND>(kr[i].y);
-        const uint2 k2 = codes4<T, KIND>(kr[i].z), k3 = codes4<T, KIND>(kr[i].w);
-        uint4* dst = reinterpret_cast<uint4*>(k_lds + t * Tile::kKStride + w * 32);
-        dst[0] = make_uint4(k0.x, k0.y, k1.x, k1.y);
-        dst[1] = make_uint4(k2.x, k2.y, k3.x, k3.y);
-        // V^T: [16-token step][lane half][dim][8 tokens]
-        const int quad = c / (DP / 4), w4 = c % (DP / 4);
-        const uint32_t bits = (uint32_t)(there >> (4 * quad)) & 15u;
-        const uint32_t keep = ((bits & 1) * 0xffu) | ((bits >> 1 & 1) * 0xff00u) | ((bits >> 2 & 1) * 0xff0000u) |
-                              ((bits >> 3) * 0xff000000u);
-        const int nd = a.D >> 4;
-        int d0 = w4 * 4 / nd, d1 = w4 * 4 % nd;
-        uint8_t* vt = v_lds + ((quad >> 2) * 2 + (quad & 1)) * DP * 16 + (quad >> 1 & 1) * 8;
-        const uint32_t words[4] = {vr[i].x, vr[i].y, vr[i].z, vr[i].w};
-        if (w4 * 4 < a.D) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            *reinterpret_cast<uint2*>(vt + (d0 + 16 * d1) * 16) = codes4<Bf16, KIND>(words[j] & keep);
-            if (++d1 == nd) d1 = 0, ++d0;
-          }
-        }
-      }
-    }
-    if (QUANT && wave == 0) {
-      scale_lds[0][lane] = ksc;
-      scale_lds[1][lane] = vsc;
-    }
-  };
-
-  // --- one block's NS x 32 tokens from sub st0 -----------------------------
-  const auto compute = [&](int block, auto ns, int st0) {
-    constexpr int NS = decltype(ns)::value;
-    const int t0 = block * TN + st0 * 32;
-    if (a.causal && t0 > last_pos) return;
-    if (a.window && t0 + NS * 32 - 1 <= first_pos - a.window) return;
-    f32x16 s[NS];
-#pragma unroll
-    for (int u = 0; u < NS; ++u) {
-      s[u] = f32x16{};
-#pragma unroll
-      for (int kk = 0; kk < KK; ++kk) {
-        const uint4 x = *reinterpret_cast<const uint4*>(k_lds + ((st0 + u) * 32 + col) * Tile::kKStride +
-                                                        (kk * 16 + half * 8) * 2);
-        s[u] = T::mfma(__builtin_bit_cast(typename T::v8, x), q[kk], s[u]);
-      }
-    }
-    if constexpr (QUANT) {
-#pragma unroll
-      for (int u = 0; u < NS; ++u)
-#pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-          const float4 x = *reinterpret_cast<const float4*>(&scale_lds[0][(st0 + u) * 32 + 2 * i + 4 * half]);
-          s[u][i] *= x.x, s[u][i + 1] *= x.y, s[u][i + 2] *= x.z, s[u][i + 3] *= x.w;
-        }
-    }
-    const unsigned long long there = there_lds[block & 3];
-    const bool mask = there != ~0ull || (a.causal && t0 + NS * 32 - 1 > first_pos) ||
-                      (a.window && t0 <= last_pos - a.window);
-    if (mask) {
-      const int hi = (a.causal ? min(pos, it.s.ctx - 1) : it.s.ctx - 1) - t0 - 4 * half;
-      const int lo = a.window ? pos - a.window - t0 - 4 * half : -0x40000000;
-#pragma unroll
-      for (int u = 0; u < NS; ++u) {
-        const uint32_t bits = (uint32_t)(there >> (32 * (st0 + u))) >> (4 * half);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int t = 8 * (i / 4) + i % 4;
-          const bool ok = 32 * u + t <= hi && 32 * u + t > lo && (bits >> t & 1);
-          s[u][i] = ok ? s[u][i] : -INFINITY;
-        }
-      }
-    }
-    float top = s[0][0];
-#pragma unroll
-    for (int u = 0; u < NS; ++u)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) top = fmaxf(top, s[u][i]);
-    top = xor_max<32>(top) * a.sc;
-    // The maximum moves only when it would leave weights above 2^8: the
-    // accumulators are rescaled a few times per row, not per block.
-    if (__any(top > m + 8.f)) {
-      const float next = fmaxf(m, top);
-      const float f = next == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - next);
-#pragma unroll
-      for (int n = 0; n < NB; ++n)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) o[n][i] *= f;
-      l *= f;
-      m = next;
-    }
-    const float ref = m == -INFINITY ? 0.f : m;
-#pragma unroll
-    for (int u = 0; u < NS; ++u)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        s[u][i] = __builtin_amdgcn_exp2f(fmaf(s[u][i], a.sc, -ref));
-        l += s[u][i];
-      }
-#pragma unroll
-    for (int u = 0; u < NS; ++u)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        f32x8 p;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) p[i] = s[u][8 * e + i];
-        if constexpr (QUANT) {
-          const float* vs = &scale_lds[1][(st0 + u) * 32 + 16 * e + 4 * half];
-          const float4 x = *reinterpret_cast<const float4*>(vs), y = *reinterpret_cast<const float4*>(vs + 8);
-          p[0] *= x.x, p[1] *= x.y, p[2] *= x.z, p[3] *= x.w;
-          p[4] *= y.x, p[5] *= y.y, p[6] *= y.z, p[7] *= y.w;
-        }
-        const auto pb = __builtin_convertvector(p, typename PT::v8);
-        typename PT::v8 low;
-        if constexpr (SPLIT_P) low = __builtin_convertvector(p - __builtin_convertvector(pb, f32x8), typename PT::v8);
-        const int step = (st0 + u) * 2 + e;  // of 16 tokens
-#pragma unroll
-        for (int n = 0; n < NB; ++n) {
-          typename PT::v8 v;
-          if constexpr (QUANT) {
-            v = __builtin_bit_cast(typename PT::v8, *reinterpret_cast<const uint4*>(
-                                                        v_lds + ((step * 2 + half) * DP + n * 32 + col) * 16));
-          } else {
-            typedef __attribute__((address_space(3))) s16x4* lds_t;
-            const uint8_t* x = v_lds + (step * 16 + 4 * half + ((lane & 15) >> 2)) * Tile::kVStride +
-                               (n * 32 + (lane & 16) + (lane & 3) * 4) * 2;
-            const s16x4 r0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t)x);
-            const s16x4 r1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t)(x + 8 * Tile::kVStride));
-            typedef short s16x8 __attribute__((ext_vector_type(8)));
-            v = __builtin_bit_cast(typename PT::v8, __builtin_shufflevector(r0, r1, 0, 1, 2, 3, 4, 5, 6, 7));
-          }
-          o[n] = PT::mfma(v, pb, o[n]);
-          if constexpr (SPLIT_P) o[n] = PT::mfma(v, low, o[n]);
-        }
-      }
-  };
-
-  // --- the item's blocks ---------------------------------------------------
-  int page1 = -1, page2 = -1;  // wavefront 0: pages of the next block and the one after
-  if (wave == 0) {
-    const int page0 = page_of(from);
-    page1 = page_of(from + 1);
-    page2 = page_of(from + 2);
-    put_places(from, page0);
-    put_places(from + 1, page1);
-    if (QUANT) load_scales(from, page0);
+  for (int i = 0; i < 16; ++i) {
+    const int t = 8 * (i / 4) + i % 4;
+    s[i] = t <= hi && t > lo && (bits >> t & 1) ? s[i] : -INFINITY;
   }
-  __syncthreads();
-  if (from < to) load_tile(from);
-  for (int block = from; block < to; ++block) {
-    __syncthreads();  // the block before is computed
-    put_tile(block);
-    if (wave == 0) put_places(block + 2, page2);
-    __syncthreads();
-    if (block + 1 < to) load_tile(block + 1);
-    if (wave == 0) {
-      if (QUANT) load_scales(block + 1, page1);
-      page1 = page2;
-      page2 = page_of(block + 3);
-    }
-    if (active) {
-      if (halves)
-        compute(block, std::integral_constant<int, 1>{}, wave & 1);
-      else
-        compute(block, std::integral_constant<int, 2>{}, 0);
-    }
-  }
+}
 
-  // --- results -------------------------------------------------------------
-  l = xor_add<32>(l);
-  if (halves) {  // the two halves of a row group, joined in LDS
-    __syncthreads();
-    float* x = reinterpret_cast<float*>(tile_lds) + group * (NB * 16 + 2) * 64 + lane;
-    if (active && (wave & 1)) {
+__device__ __forceinline__ float top_of(const f32x16& s) {
+  float top = s[0];
 #pragma unroll
-      for (int n = 0; n < NB; ++n)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) x[(n * 16 + i) * 64] = o[n][i];
-      x[NB * 16 * 64] = m;
-      x[(NB * 16 + 1) * 64] = l;
-    }
-    __syncthreads();
-    if (!active || (wave & 1)) return;
-    const float m2 = x[NB * 16 * 64], l2 = x[(NB * 16 + 1) * 64];
-    const float both = fmaxf(m, m2);
-    const float f1 = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - both);
-    const float f2 = m2 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m2 - both);
+  for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
+  return top;
+}
+
+// The running maximum moves only when it would leave weights above 2^8: the
+// accumulators are rescaled a few times per row, not per block.
+template <int NB>
+__device__ __forceinline__ void raise_max(float top, float& m, float& l, f32x16 (&o)[NB]) {
+  if (__any(top > m + 8.f)) {
+    const float next = fmaxf(m, top);
+    const float f = next == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - next);
 #pragma unroll
     for (int n = 0; n < NB; ++n)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) o[n][i] = o[n][i] * f1 + x[(n * 16 + i) * 64] * f2;
-    l = l * f1 + l2 * f2;
-    m = both;
+      for (int i = 0; i < 16; ++i) o[n][i] *= f;
+    l *= f;
+    m = next;
   }
-  if (!active || !real) return;
+}
+
+// A group's results: to the output, or to the workspace as a share's partial.
+// Lane (col, half) holds dims dim(n, 2 i + 4 half) .. + 3 of its row in
+// registers i .. i + 3 of block n.
+template <typename T, int DP, typename Dim>
+__device__ __forceinline__ void put_rows(const ChunkArgs& a, const Item& it, const RowGroup& g, float m, float l,
+                                         const f32x16 (&o)[DP / 32], Dim dim) {
+  constexpr int NB = DP / 32;
+  const int half = __lane_id() >> 5;
+  if (!g.real) return;
   if (it.shares > 1) {
-    const long long slot = (long long)blockIdx.x * kRows + row;
+    const long long slot = (long long)blockIdx.x * a.tile_rows + g.row;
     float* dst = a.part + slot * DP;
 #pragma unroll
     for (int n = 0; n < NB; ++n)
 #pragma unroll
       for (int i = 0; i < 16; i += 4)
-        *reinterpret_cast<float4*>(dst + n * 32 + 2 * i + 4 * half) =
+        *reinterpret_cast<float4*>(dst + dim(n, 2 * i + 4 * half)) =
             make_float4(o[n][i], o[n][i + 1], o[n][i + 2], o[n][i + 3]);
     if (half == 0) a.ml[slot] = make_float2(m, l);
     return;
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  const long long at = (long long)(it.s.row0 + tok) * a.H + head;
+  const long long at = (long long)(it.s.row0 + g.tok) * a.H + g.head;
   uint16_t* dst = static_cast<uint16_t*>(a.out) + at * a.D;
 #pragma unroll
   for (int n = 0; n < NB; ++n)
 #pragma unroll
     for (int i = 0; i < 16; i += 4) {
-      const int d = n * 32 + 2 * i + 4 * half;
+      const int d = dim(n, 2 * i + 4 * half);
       const f32x2 x = {o[n][i] * inv, o[n][i + 1] * inv}, y = {o[n][i + 2] * inv, o[n][i + 3] * inv};
       const uint2 w = make_uint2(__builtin_bit_cast(uint32_t, __builtin_convertvector(x, typename T::v2)),
                                  __builtin_bit_cast(uint32_t, __builtin_convertvector(y, typename T::v2)));
@@ -439,8 +201,684 @@ __global__ void __launch_bounds__(kChunkThreads, DP <= 128 ? 2 : 1) chunk_attn_k
   if (a.lse && half == 0) a.lse[at] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * 0.69314718055994531f;
 }
 
+// Joins the partials of wavefronts FROM .. into those before them through LDS
+// (kPartial bytes each).  Every wavefront of the workgroup calls it.
+template <int NB>
+__device__ __forceinline__ void join(float* lds, bool give, bool take, int slot, float& m, float& l, f32x16 (&o)[NB]) {
+  float* x = lds + slot * (NB * 16 + 2) * 64 + (threadIdx.x & 63);
+  __syncthreads();
+  if (give) {
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[(n * 16 + i) * 64] = o[n][i];
+    x[NB * 16 * 64] = m;
+    x[(NB * 16 + 1) * 64] = l;
+  }
+  __syncthreads();
+  if (take) {
+    const float m2 = x[NB * 16 * 64], l2 = x[(NB * 16 + 1) * 64];
+    const float both = fmaxf(m, m2);
+    const float f1 = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - both);
+    const float f2 = m2 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m2 - both);
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[n][i] = o[n][i] * f1 + x[(n * 16 + i) * 64] * f2;
+    l = l * f1 + l2 * f2;
+    m = both;
+  }
+}
+
+// V's operand for 16 tokens (tokens 4 half .. + 3 and 8 + 4 half .. + 3 of
+// them) and dims 32 n .. + 31, from row-major LDS.
+template <typename V8>
+__device__ __forceinline__ V8 read_v(const uint8_t* v_lds, int stride, int token0, int n) {
+  typedef __attribute__((address_space(3))) s16x4* lds_t;
+  const int lane = __lane_id();
+  const uint8_t* x =
+      v_lds + (token0 + 4 * (lane >> 5) + ((lane & 15) >> 2)) * stride + (n * 32 + (lane & 16) + (lane & 3) * 4) * 2;
+  const s16x4 r0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t)x);
+  const s16x4 r1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t)(x + 8 * stride));
+  return __builtin_bit_cast(V8, __builtin_shufflevector(r0, r1, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+// Gathers blocks of 64 tokens through the page table, WAVES wavefronts of them
+// a run of consecutive tokens each: global memory to registers (load),
+// registers to LDS (put).  A run within one page (page sizes that are
+// multiples of the run's length) has one address per wavefront and no
+// bookkeeping per lane; other page sizes, and runs with tokens that are not
+// there, look up every row.
+template <typename T, int KIND, int DP, int WAVES>
+struct Stage {
+  using Tile = ChunkTile<KIND, DP>;
+  static constexpr bool QUANT = Tile::kQuant;
+  static constexpr int TN = Tile::kTokens, RUN = TN / WAVES;
+  static constexpr int kRun = RUN * Tile::kPerRow;  // 16-byte pieces of a run's K (and V)
+  static constexpr int NP = (kRun + 63) / 64;       // per lane
+  static constexpr bool kRagged = kRun % 64 != 0;
+  static constexpr int kRing = 8;
+  struct Shared {
+    long long place[kRing][TN];  // a token's K row from the layer's start, -1: not there
+    unsigned long long there[kRing];
+    float scale[kRing][2][QUANT ? TN : 1];
+  };
+
+  const ChunkArgs& a;
+  Shared& sh;
+  const uint8_t *k_base, *v_base;
+  const float* s_base;
+  const int32_t* table;
+  int ctx, to, row_bytes, lane, wave;
+  bool one_page;  // a run lies in one page, its rows can be loaded 16 bytes at a time
+  uint4 kr[NP], vr[NP];
+  int next_page;  // wavefront 0: page of token `lane` of block `paged`
+  int paged;
+  float ks, vs;   // wavefront 0: scales of token `lane` of block paged - 1
+
+  __device__ __forceinline__ Stage(const ChunkArgs& args, const Item& it, int kvh, int blocks_end, Shared& shared)
+      : a(args), sh(shared), ctx(it.s.ctx), to(blocks_end) {
+    k_base = a.pool + a.layer_off + (long long)kvh * a.g.head;
+    v_base = k_base + a.g.kv;
+    s_base = QUANT ? a.scales + a.s_layer_off + (long long)kvh * a.g.s_head : nullptr;
+    row_bytes = QUANT ? a.D : 2 * a.D;
+    table = a.table + (long long)it.b * a.max_pp;
+    lane = threadIdx.x & 63;
+    wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    one_page = a.PS % RUN == 0 && a.aligned && a.D == DP;
+  }
+
+  // Wavefront 0.
+  __device__ __forceinline__ int page_of(int block) const {
+    const int t = block * TN + lane;
+    return block < to && t < ctx ? table[page_index(a, t)] : -1;
+  }
+  __device__ __forceinline__ void put_places(int block, int page) {
+    const int t = block * TN + lane;
+    const bool there = page >= 0 && page < a.P;
+    const int slot = t - page_index(a, t) * a.PS;
+    sh.place[block % kRing][lane] = there ? (long long)page * a.g.page + (long long)slot * row_bytes : -1;
+    const unsigned long long mask = __ballot(there);
+    if (lane == 0) sh.there[block % kRing] = mask;
+    if constexpr (QUANT) {
+      ks = vs = 0.f;
+      if (there) {
+        const float* s = s_base + (long long)page * a.g.s_page + (KIND == kSrcI8 ? slot : 0);
+        ks = s[0];
+        vs = s[a.g.s_kv];
+      }
+    }
+  }
+  __device__ __forceinline__ void put_scales(int block) {
+    if constexpr (QUANT) {
+      sh.scale[block % kRing][0][lane] = ks;
+      sh.scale[block % kRing][1][lane] = vs;
+    }
+  }
+  // Places of the first two blocks, and the page of the third.
+  __device__ __forceinline__ void begin(int from) {
+    if (wave == 0) {
+      const int p0 = page_of(from), p1 = page_of(from + 1);
+      next_page = page_of(from + 2);
+      put_places(from, p0);
+      put_scales(from);
+      put_places(from + 1, p1);
+    }
+    paged = from + 2;
+  }
+  // Places of the block after those known, the page of the next one, and the
+  // scales of the one before (loaded a call ago).
+  __device__ __forceinline__ void more_places() {
+    if (wave == 0) {
+      put_scales(paged - 1);
+      put_places(paged, next_page);
+      next_page = page_of(paged + 1);
+    }
+    ++paged;
+  }
+
+  // Tokens of the wavefront's run of a block that are there, a bit each.
+  __device__ __forceinline__ uint32_t run_there(int block) const {
+    const unsigned long long there = sh.there[block % kRing];
+    return (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(there >> (RUN * wave))) & ((1u << RUN) - 1);
+  }
+
+  __device__ __forceinline__ void load(int block) {
+    if (one_page && run_there(block) == (1u << RUN) - 1) {
+      const long long at = sh.place[block % kRing][RUN * wave];
+      const long long run = (long long)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)at) |
+                            (long long)__builtin_amdgcn_readfirstlane((uint32_t)(at >> 32)) << 32;
+      const uint8_t *k = k_base + run, *v = v_base + run;
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        const uint32_t off = (lane + 64 * i) * 16;
+        if (kRagged && lane + 64 * i >= kRun) break;
+        kr[i] = *reinterpret_cast<const uint4*>(k + off);
+        vr[i] = *reinterpret_cast<const uint4*>(v + off);
+      }
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const int c = lane + 64 * i;
+      kr[i] = vr[i] = make_uint4(0, 0, 0, 0);
+      if (kRagged && c >= kRun) break;
+      const int t = RUN * wave + c / Tile::kPerRow, w = c % Tile::kPerRow;
+      const long long at = sh.place[block % kRing][t];
+      if (at >= 0) kr[i] = load16(k_base + at + w * 16, row_bytes - w * 16, a.aligned);
+      if constexpr (!QUANT) {
+        if (at >= 0) vr[i] = load16(v_base + at + w * 16, row_bytes - w * 16, a.aligned);
+      } else {  // V: four tokens' codes of a dim in a dword, 4 D bytes for the four tokens
+        const int t4 = RUN * wave + c / (DP / 4) * 4, w4 = c % (DP / 4);
+        const long long at4 = sh.place[block % kRing][t4];
+        if (at4 >= 0 && w4 * 4 < a.D) vr[i] = load16(v_base + at4 + w4 * 16, 16, a.aligned);
+      }
+    }
+  }
+
+  __device__ __forceinline__ void put(int block, uint8_t* k_lds, uint8_t* v_lds) {
+    const uint32_t there = QUANT ? run_there(block) : 0;
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const int c = lane + 64 * i;
+      if (kRagged && c >= kRun) break;
+      const int t = RUN * wave + c / Tile::kPerRow, w = c % Tile::kPerRow;
+      if constexpr (!QUANT) {
+        *reinterpret_cast<uint4*>(k_lds + t * Tile::kKStride + w * 16) = kr[i];
+        *reinterpret_cast<uint4*>(v_lds + t * Tile::kVStride + w * 16) = vr[i];
+      } else {
+        const uint2 k0 = codes4<T, KIND>(kr[i].x), k1 = codes4<T, KIND>(kr[i].y);
+        const uint2 k2 = codes4<T, KIND>(kr[i].z), k3 = codes4<T, KIND>(kr[i].w);
+        uint4* dst = reinterpret_cast<uint4*>(k_lds + t * Tile::kKStride + w * 32);
+        dst[0] = make_uint4(k0.x, k0.y, k1.x, k1.y);
+        dst[1] = make_uint4(k2.x, k2.y, k3.x, k3.y);
+        // V^T: [16-token step][lane half][dim][8 tokens]
+        const int quad = RUN / 4 * wave + c / (DP / 4), w4 = c % (DP / 4);
+        const uint32_t keep = keep_bytes(there >> (c / (DP / 4) * 4));
+        uint8_t* vt = v_lds + ((quad >> 2) * 2 + (quad & 1)) * DP * 16 + (quad >> 1 & 1) * 8;
+        const uint32_t words[4] = {vr[i].x, vr[i].y, vr[i].z, vr[i].w};
+        if (DP % 64 == 0 && a.D == DP) {  // four dims 16 apart
+          uint8_t* v0 = vt + (w4 * 4 / (DP / 16) + 16 * (w4 * 4 % (DP / 16))) * 16;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) *reinterpret_cast<uint2*>(v0 + j * 256) = codes4<Bf16, KIND>(words[j] & keep);
+        } else if (w4 * 4 < a.D) {
+          const int nd = a.D >> 4;
+          int d0 = w4 * 4 / nd, d1 = w4 * 4 % nd;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            *reinterpret_cast<uint2*>(vt + (d0 + 16 * d1) * 16) = codes4<Bf16, KIND>(words[j] & keep);
+            if (++d1 == nd) d1 = 0, ++d0;
+          }
+        }
+      }
+    }
+  }
+};
+
+// Scores of 32 tokens times their K scales, and weights times their V scales.
+__device__ __forceinline__ void scale_scores(const float* ks, int half, f32x16& s) {
+#pragma unroll
+  for (int i = 0; i < 16; i += 4) {
+    const float4 x = *reinterpret_cast<const float4*>(ks + 2 * i + 4 * half);
+    s[i] *= x.x, s[i + 1] *= x.y, s[i + 2] *= x.z, s[i + 3] *= x.w;
+  }
+}
+__device__ __forceinline__ void scale_weights(const float* vs, int e, int half, f32x8& p) {
+  const float4 x = *reinterpret_cast<const float4*>(vs + 16 * e + 4 * half);
+  const float4 y = *reinterpret_cast<const float4*>(vs + 16 * e + 8 + 4 * half);
+  p[0] *= x.x, p[1] *= x.y, p[2] *= x.z, p[3] *= x.w;
+  p[4] *= y.x, p[5] *= y.y, p[6] *= y.z, p[7] *= y.w;
+}
+
+// A tile of at most 32 rows: every wavefront attends 32 tokens at a time of
+// its own, with no barrier, and they join at the end.  K comes from
+// memory in the layout of the matrix operand (a lane's 16-byte pieces of its
+// token's row), refilled as soon as the scores are taken; V of the quantized
+// pools too (its tiling puts a lane's four tokens of a dim in a dword), V of
+// float pools through the wavefront's own LDS.
+// Bound: memory.
+template <typename T, int KIND, int DP, int WAVES>
+__device__ __forceinline__ void few_rows(const ChunkArgs& a, const Item& it, int kvh, int rows, int from, int to,
+                                         uint8_t* lds, float (*own_scale)[2][32]) {
+  using Tile = ChunkTile<KIND, DP>;
+  using PT = std::conditional_t<KIND >= kSrcI8, Bf16, T>;
+  constexpr bool QUANT = Tile::kQuant;
+  constexpr bool SPLIT_P = QUANT && std::is_same_v<T, F16>;
+  constexpr int NB = DP / 32, KK = DP / 16, KP = QUANT ? DP / 32 : DP / 16;
+  const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const RowGroup g = row_group(a, it, kvh, rows, 0);
+
+  typename T::v8 q[KK];
+  load_rows<T, KK>(a, it, g, [&](int kk) { return QUANT ? (kk >> 1) * 32 + half * 16 + (kk & 1) * 8 : kk * 16 + half * 8; },
+                   q);
+  f32x16 o[NB];
+#pragma unroll
+  for (int n = 0; n < NB; ++n) o[n] = f32x16{};
+  float m = -INFINITY, l = 0.f;
+
+  const uint8_t* const k_base = a.pool + a.layer_off + (long long)kvh * a.g.head;
+  const uint8_t* const v_base = k_base + a.g.kv;
+  const float* const s_base = QUANT ? a.scales + a.s_layer_off + (long long)kvh * a.g.s_head : nullptr;
+  const int32_t* const table = a.table + (long long)it.b * a.max_pp;
+  const int row_bytes = QUANT ? a.D : 2 * a.D;
+  const int nd = a.D >> 4;
+  const bool whole = a.D == DP;  // a lane's dims of V are consecutive dwords
+  uint8_t* const own_v = lds + wave * Tile::kOwnV;
+
+  const auto page_of = [&](int sub) {
+    const int t = sub * 32 + col;
+    return sub < 2 * to && t < it.s.ctx ? table[page_index(a, t)] : -1;
+  };
+  const auto place_of = [&](int sub, int page) {
+    const int t = sub * 32 + col;
+    return page >= 0 && page < a.P ? (long long)page * a.g.page + (long long)(t - page_index(a, t) * a.PS) * row_bytes : -1;
+  };
+  uint4 kr[KP], vr[QUANT ? 1 : KP];
+  uint32_t vw[2][2][QUANT ? NB : 1];
+  float ks = 0.f, vs = 0.f;
+  const auto load_k = [&](long long at, int sub, int page) {
+#pragma unroll
+    for (int p = 0; p < KP; ++p) {
+      const int d = QUANT ? p * 32 + half * 16 : (p * 16 + half * 8) * 2;  // bytes into the row
+      kr[p] = at >= 0 ? load16(k_base + at + d, row_bytes - d, a.aligned) : make_uint4(0, 0, 0, 0);
+    }
+    if constexpr (QUANT) {
+      ks = vs = 0.f;
+      if (at >= 0) {
+        const int t = sub * 32 + col;
+        const float* s = s_base + (long long)page * a.g.s_page + (KIND == kSrcI8 ? t - page_index(a, t) * a.PS : 0);
+        ks = s[0];
+        vs = s[a.g.s_kv];
+      }
+    }
+  };
+  const auto load_v = [&](long long at) {
+    if constexpr (QUANT) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const long long quad = __shfl(at, 16 * e + 8 * j + 4 * half);  // place of the four tokens' first
+#pragma unroll
+          for (int n = 0; n < NB; ++n) {
+            const int c = whole ? NB * (col >> 4) + n : 2 * n + (col >> 4);
+            const uint8_t* p = v_base + quad + ((col & 15) * nd + c) * 4;
+            uint32_t w = 0;
+            if (quad >= 0 && c < nd)
+              w = a.aligned ? *reinterpret_cast<const uint32_t*>(p)
+                            : p[0] | (uint32_t)p[1] << 8 | (uint32_t)p[2] << 16 | (uint32_t)p[3] << 24;
+            vw[e][j][n] = w;
+          }
+        }
+    } else {
+#pragma unroll
+      for (int p = 0; p < KP; ++p) {
+        const int d = (p * 16 + half * 8) * 2;
+        vr[p] = at >= 0 ? load16(v_base + at + d, row_bytes - d, a.aligned) : make_uint4(0, 0, 0, 0);
+      }
+    }
+  };
+
+  int sub = 2 * from + wave;
+  int page = page_of(sub), page1 = page_of(sub + WAVES);
+  long long at = place_of(sub, page);
+  load_k(at, sub, page);
+  load_v(at);
+  for (; sub < 2 * to; sub += WAVES) {
+    const int t0 = sub * 32;
+    const uint32_t there = (uint32_t)__ballot(at >= 0);
+    f32x16 s{};
+#pragma unroll
+    for (int p = 0; p < KP; ++p) {
+      if constexpr (QUANT) {
+        const uint2 x0 = codes4<T, KIND>(kr[p].x), x1 = codes4<T, KIND>(kr[p].y);
+        const uint2 x2 = codes4<T, KIND>(kr[p].z), x3 = codes4<T, KIND>(kr[p].w);
+        s = T::mfma(__builtin_bit_cast(typename T::v8, make_uint4(x0.x, x0.y, x1.x, x1.y)), q[2 * p], s);
+        s = T::mfma(__builtin_bit_cast(typename T::v8, make_uint4(x2.x, x2.y, x3.x, x3.y)), q[2 * p + 1], s);
+      } else {
+        s = T::mfma(__builtin_bit_cast(typename T::v8, kr[p]), q[p], s);
+      }
+    }
+    if constexpr (QUANT) {
+      if (half == 0) {
+        own_scale[wave][0][col] = ks;
+        own_scale[wave][1][col] = vs;
+      }
+    }
+    // the next 32 tokens' K
+    const long long at1 = place_of(sub + WAVES, page1);
+    load_k(at1, sub + WAVES, page1);
+    page1 = page_of(sub + 2 * WAVES);
+    __syncwarp();
+    if constexpr (QUANT) scale_scores(own_scale[wave][0], half, s);
+    if (needs_mask(a, g, t0, there)) mask_scores(a, it, g, t0, there, half, s);
+    raise_max<NB>(xor_max<32>(top_of(s)) * a.sc, m, l, o);
+    const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], a.sc, -ref));
+      l += s[i];
+    }
+    if constexpr (!QUANT) {
+#pragma unroll
+      for (int p = 0; p < KP; ++p)
+        *reinterpret_cast<uint4*>(own_v + col * Tile::kVStride + (p * 16 + half * 8) * 2) = vr[p];
+      load_v(at1);
+      __syncwarp();
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      f32x8 p;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) p[i] = s[8 * e + i];
+      if constexpr (QUANT) scale_weights(own_scale[wave][1], e, half, p);
+      const auto pb = __builtin_convertvector(p, typename PT::v8);
+      typename PT::v8 low;
+      if constexpr (SPLIT_P) low = __builtin_convertvector(p - __builtin_convertvector(pb, f32x8), typename PT::v8);
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+        typename PT::v8 v;
+        if constexpr (QUANT) {
+          const uint32_t k0 = keep_bytes(there >> (16 * e + 4 * half));
+          const uint32_t k1 = keep_bytes(there >> (16 * e + 8 + 4 * half));
+          const uint2 x0 = codes4<Bf16, KIND>(vw[e][0][n] & k0), x1 = codes4<Bf16, KIND>(vw[e][1][n] & k1);
+          v = __builtin_bit_cast(typename PT::v8, make_uint4(x0.x, x0.y, x1.x, x1.y));
+        } else {
+          v = read_v<typename PT::v8>(own_v, Tile::kVStride, 16 * e, n);
+        }
+        o[n] = PT::mfma(v, pb, o[n]);
+        if constexpr (SPLIT_P) o[n] = PT::mfma(v, low, o[n]);
+      }
+    }
+    if constexpr (QUANT) load_v(at1);
+    __syncwarp();
+    at = at1;
+  }
+  l = xor_add<32>(l);
+#pragma unroll
+  for (int n = WAVES / 2; n >= 1; n /= 2)
+    join<NB>(reinterpret_cast<float*>(lds), wave >= n && wave < 2 * n, wave < n, wave & (n - 1), m, l, o);
+  if (wave == 0)
+    put_rows<T, DP>(a, it, g, m, l, o, [&](int n, int r) {
+      return QUANT && whole ? (r & 15) + 16 * (NB * (r >> 4) + n) : n * 32 + r;
+    });
+}
+
+// Tiles of 128 rows, 32 to a wavefront, two workgroups to a CU: one's
+// products run while the other's wavefronts are in their softmax.
+template <typename T, int KIND, int DP>
+__global__ void __launch_bounds__(kChunkThreads, DP <= 128 ? 2 : 1) chunk_attn_kernel(ChunkArgs a) {
+  using Tile = ChunkTile<KIND, DP>;
+  using Gather = Stage<T, KIND, DP, 4>;
+  using PT = std::conditional_t<KIND >= kSrcI8, Bf16, T>;  // type of the second product
+  constexpr bool QUANT = Tile::kQuant;
+  constexpr bool SPLIT_P = QUANT && std::is_same_v<T, F16>;
+  constexpr int TN = Tile::kTokens, NB = DP / 32, KK = DP / 16;
+  constexpr int kLds = max3(Tile::kBytes, 2 * Tile::kPartial, 4 * Tile::kOwnV);
+  __shared__ __align__(16) uint8_t lds[kLds];
+  __shared__ __align__(16) typename Gather::Shared shared;
+  __shared__ __align__(16) float own_scale[QUANT ? 4 : 1][2][32];
+  uint8_t* const k_lds = lds;
+  uint8_t* const v_lds = lds + Tile::kKBytes;
+
+  const int kvh = blockIdx.x % a.KH;
+  Item it;
+  if (!find_item<TN>(a, blockIdx.x / a.KH, it)) return;
+  int from, to;
+  item_blocks<TN>(a, it, from, to);
+  put_record(a, it, kvh);
+  const int rows = min(a.tile_rows, it.s.q_len * a.G - it.tile * a.tile_rows);
+  if (rows <= 32) {
+    few_rows<T, KIND, DP, 4>(a, it, kvh, rows, from, to, lds, own_scale);
+    return;
+  }
+
+  const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // up to 64 rows leave two wavefronts to a row group, one for each half of a
+  // block's tokens
+  const bool halves = rows <= 64;
+  const int group = halves ? wave >> 1 : wave;
+  const bool active = group * 32 < rows;
+  const RowGroup g = row_group(a, it, kvh, rows, group * 32);
+  typename T::v8 q[KK];
+  load_rows<T, KK>(a, it, g, [&](int kk) { return kk * 16 + half * 8; }, q);
+  f32x16 o[NB];
+#pragma unroll
+  for (int n = 0; n < NB; ++n) o[n] = f32x16{};
+  float m = -INFINITY, l = 0.f;
+
+  // NS x 32 tokens of a block from its 32-token part st0 on
+  const auto compute = [&](int block, auto ns, int st0) {
+    constexpr int NS = decltype(ns)::value;
+    const int t0 = block * TN + st0 * 32;
+    if (a.causal && t0 > g.last_pos) return;
+    if (a.window && t0 + NS * 32 - 1 <= g.first_pos - a.window) return;
+    const unsigned long long there = shared.there[block % Gather::kRing];
+    const auto* scale = shared.scale[block % Gather::kRing];
+    f32x16 s[NS];
+    float top = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < NS; ++u) {
+      s[u] = f32x16{};
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) {
+        const uint4 x = *reinterpret_cast<const uint4*>(k_lds + ((st0 + u) * 32 + col) * Tile::kKStride +
+                                                        (kk * 16 + half * 8) * 2);
+        s[u] = T::mfma(__builtin_bit_cast(typename T::v8, x), q[kk], s[u]);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < NS; ++u) {
+      if constexpr (QUANT) scale_scores(scale[0] + (st0 + u) * 32, half, s[u]);
+      const uint32_t bits = (uint32_t)(there >> (32 * (st0 + u)));
+      if (needs_mask(a, g, t0 + 32 * u, bits)) mask_scores(a, it, g, t0 + 32 * u, bits, half, s[u]);
+      top = fmaxf(top, top_of(s[u]));
+    }
+    raise_max<NB>(xor_max<32>(top) * a.sc, m, l, o);
+    const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int u = 0; u < NS; ++u)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        s[u][i] = __builtin_amdgcn_exp2f(fmaf(s[u][i], a.sc, -ref));
+        l += s[u][i];
+      }
+#pragma unroll
+    for (int u = 0; u < NS; ++u)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        f32x8 p;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) p[i] = s[u][8 * e + i];
+        if constexpr (QUANT) scale_weights(scale[1] + (st0 + u) * 32, e, half, p);
+        const auto pb = __builtin_convertvector(p, typename PT::v8);
+        typename PT::v8 low;
+        if constexpr (SPLIT_P) low = __builtin_convertvector(p - __builtin_convertvector(pb, f32x8), typename PT::v8);
+        const int step = (st0 + u) * 2 + e;  // of 16 tokens
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+          typename PT::v8 v;
+          if constexpr (QUANT)
+            v = __builtin_bit_cast(typename PT::v8, *reinterpret_cast<const uint4*>(
+                                                        v_lds + ((step * 2 + half) * DP + n * 32 + col) * 16));
+          else
+            v = read_v<typename PT::v8>(v_lds, Tile::kVStride, step * 16, n);
+          o[n] = PT::mfma(v, pb, o[n]);
+          if constexpr (SPLIT_P) o[n] = PT::mfma(v, low, o[n]);
+        }
+      }
+  };
+
+  Gather st(a, it, kvh, to, shared);
+  st.begin(from);
+  __syncthreads();
+  if (from < to) st.load(from);
+  for (int block = from; block < to; ++block) {
+    __syncthreads();  // the block before is computed
+    st.put(block, k_lds, v_lds);
+    st.more_places();
+    __syncthreads();
+    if (block + 1 < to) st.load(block + 1);
+    if (active) {
+      if (halves)
+        compute(block, std::integral_constant<int, 1>{}, wave & 1);
+      else
+        compute(block, std::integral_constant<int, 2>{}, 0);
+    }
+  }
+  l = xor_add<32>(l);
+  if (halves) join<NB>(reinterpret_cast<float*>(lds), active && (wave & 1), active && !(wave & 1), group, m, l, o);
+  if (!active || (halves && (wave & 1))) return;
+  put_rows<T, DP>(a, it, g, m, l, o, [](int n, int r) { return n * 32 + r; });
+}
+
+// Tiles of 256 rows, 32 to each of eight wavefronts, one workgroup to a CU.
+// A wavefront forms the scores of the next block while the weights of this
+// one are taken, and its SIMD's other wavefront fills what is left.  Three
+// blocks are in LDS, so that one barrier per block is enough, and a fourth in
+// registers.
+template <typename T, int KIND, int DP>
+__global__ void __launch_bounds__(kLargeThreads, 1) chunk_attn_large_kernel(ChunkArgs a) {
+  using Tile = ChunkTile<KIND, DP>;
+  using Gather = Stage<T, KIND, DP, 8>;
+  using PT = std::conditional_t<KIND >= kSrcI8, Bf16, T>;
+  constexpr bool QUANT = Tile::kQuant;
+  constexpr bool SPLIT_P = QUANT && std::is_same_v<T, F16>;
+  constexpr int TN = Tile::kTokens, NB = DP / 32, KK = DP / 16;
+  constexpr int kLds = max3(3 * Tile::kBytes, 4 * Tile::kPartial, 8 * Tile::kOwnV);
+  __shared__ __align__(16) uint8_t lds[kLds];
+  __shared__ __align__(16) typename Gather::Shared shared;
+  __shared__ __align__(16) float own_scale[QUANT ? 8 : 1][2][32];
+
+  const int kvh = blockIdx.x % a.KH;
+  Item it;
+  if (!find_item<TN>(a, blockIdx.x / a.KH, it)) return;
+  int from, to;
+  item_blocks<TN>(a, it, from, to);
+  put_record(a, it, kvh);
+  const int rows = min(a.tile_rows, it.s.q_len * a.G - it.tile * a.tile_rows);
+  if (rows <= 32) {
+    few_rows<T, KIND, DP, 8>(a, it, kvh, rows, from, to, lds, own_scale);
+    return;
+  }
+
+  const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const bool active = wave * 32 < rows;
+  const RowGroup g = row_group(a, it, kvh, rows, wave * 32);
+  typename T::v8 q[KK];
+  load_rows<T, KK>(a, it, g, [&](int kk) { return kk * 16 + half * 8; }, q);
+  f32x16 o[NB];
+#pragma unroll
+  for (int n = 0; n < NB; ++n) o[n] = f32x16{};
+  float m = -INFINITY, l = 0.f;
+
+  Gather st(a, it, kvh, to, shared);
+  st.begin(from);
+  __syncthreads();
+  st.load(from);
+  st.more_places();
+  st.put(from, lds, lds + Tile::kKBytes);
+  st.load(from + 1);
+  st.put(from + 1, lds + Tile::kBytes, lds + Tile::kBytes + Tile::kKBytes);
+  __syncthreads();
+  st.load(from + 2);
+  st.more_places();
+  __syncthreads();
+
+  const auto scores = [&](const uint8_t* k_lds, f32x16 (&s)[2]) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      s[u] = f32x16{};
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) {
+        const uint4 x =
+            *reinterpret_cast<const uint4*>(k_lds + (u * 32 + col) * Tile::kKStride + (kk * 16 + half * 8) * 2);
+        s[u] = T::mfma(__builtin_bit_cast(typename T::v8, x), q[kk], s[u]);
+      }
+    }
+  };
+  // the weights of a block's scores `now` and their product with V, with the
+  // scores `next` of the block after it
+  const auto step = [&](int block, const uint8_t* v_lds, const uint8_t* next_k, f32x16 (&now)[2], f32x16 (&next)[2]) {
+    const unsigned long long there = shared.there[block % Gather::kRing];
+    const auto* scale = shared.scale[block % Gather::kRing];
+    float top = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      if constexpr (QUANT) scale_scores(scale[0] + u * 32, half, now[u]);
+      const uint32_t bits = (uint32_t)(there >> (32 * u));
+      const int t0 = block * TN + 32 * u;
+      if (needs_mask(a, g, t0, bits)) mask_scores(a, it, g, t0, bits, half, now[u]);
+      top = fmaxf(top, top_of(now[u]));
+    }
+    raise_max<NB>(xor_max<32>(top) * a.sc, m, l, o);
+    const float ref = m == -INFINITY ? 0.f : m;
+    scores(next_k, next);
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        now[u][i] = __builtin_amdgcn_exp2f(fmaf(now[u][i], a.sc, -ref));
+        l += now[u][i];
+      }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      f32x8 p;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) p[i] = now[e >> 1][8 * (e & 1) + i];
+      if constexpr (QUANT) scale_weights(scale[1] + (e >> 1) * 32, e & 1, half, p);
+      const auto pb = __builtin_convertvector(p, typename PT::v8);
+      typename PT::v8 low;
+      if constexpr (SPLIT_P) low = __builtin_convertvector(p - __builtin_convertvector(pb, f32x8), typename PT::v8);
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+        typename PT::v8 v;
+        if constexpr (QUANT)
+          v = __builtin_bit_cast(typename PT::v8,
+                                 *reinterpret_cast<const uint4*>(v_lds + ((e * 2 + half) * DP + n * 32 + col) * 16));
+        else
+          v = read_v<typename PT::v8>(v_lds, Tile::kVStride, e * 16, n);
+        o[n] = PT::mfma(v, pb, o[n]);
+        if constexpr (SPLIT_P) o[n] = PT::mfma(v, low, o[n]);
+      }
+    }
+  };
+
+  f32x16 s0[2], s1[2];
+  int slot = 0;  // of the block, of three
+  const auto turn = [&](int block, f32x16 (&now)[2], f32x16 (&next)[2]) {
+    const int slot1 = slot == 2 ? 0 : slot + 1, slot2 = slot == 0 ? 2 : slot - 1;
+    uint8_t* const k2 = lds + slot2 * Tile::kBytes;
+    st.put(block + 2, k2, k2 + Tile::kKBytes);
+    st.load(block + 3);
+    st.more_places();
+    if (active) step(block, lds + slot * Tile::kBytes + Tile::kKBytes, lds + slot1 * Tile::kBytes, now, next);
+    __syncthreads();
+    slot = slot1;
+  };
+  if (active) scores(lds, s0);
+  for (int block = from; block < to; block += 2) {
+    turn(block, s0, s1);
+    if (block + 1 < to) turn(block + 1, s1, s0);
+  }
+  if (!active) return;
+  put_rows<T, DP>(a, it, g, m, xor_add<32>(l), o, [](int n, int x) { return n * 32 + x; });
+}
+
 template <typename T, int KIND>
 void launch_chunk16_t(const ChunkArgs& a, dim3 grid, hipStream_t st) {
+  if (a.tile_rows == 256) {
+    if (a.dp == 64)
+      hipLaunchKernelGGL((chunk_attn_large_kernel<T, KIND, 64>), grid, dim3(kLargeThreads), 0, st, a);
+    else if (a.dp == 96)
+      hipLaunchKernelGGL((chunk_attn_large_kernel<T, KIND, 96>), grid, dim3(kLargeThreads), 0, st, a);
+    else
+      hipLaunchKernelGGL((chunk_attn_large_kernel<T, KIND, 128>), grid, dim3(kLargeThreads), 0, st, a);
+    return;
+  }
   if (a.dp == 64)
     hipLaunchKernelGGL((chunk_attn_kernel<T, KIND, 64>), grid, dim3(kChunkThreads), 0, st, a);
   else if (a.dp == 96)

@@ -8,9 +8,13 @@
 namespace vrm {
 namespace {
 
-// One wavefront per row: joins the shares' (max, sum, accumulator).
+// One wavefront per row: joins the shares' (max, sum, accumulator).  Lane i
+// weighs share i (64 at a time); the accumulators are then loaded eight
+// shares at once.
+constexpr int kMergeRows = 4;  // rows of a workgroup
 __global__ void __launch_bounds__(256) chunk_merge_kernel(ChunkArgs a) {
   const int vtile = blockIdx.x / a.KH, kvh = blockIdx.x % a.KH;
+  const int2 r = a.rec[(long long)vtile * a.KH + kvh];
   int lo = 0, hi = a.B - 1;  // the last sequence whose tiles start at or before vtile
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
@@ -22,84 +26,114 @@ __global__ void __launch_bounds__(256) chunk_merge_kernel(ChunkArgs a) {
   const Sequence s = load_sequence(a, lo);
   const int tile = vtile - virtual_tile(a, s.row0, lo);
   if (tile < 0 || tile >= tiles_of(a, s)) return;
-  const int2 r = a.rec[(long long)vtile * a.KH + kvh];
   const int first = r.x, shares = r.y;
   if (shares <= 1 || first < 0 || first + shares > a.items) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int rows = min(kRows, s.q_len * a.G - tile * kRows);
-  for (int j = 0; j < 4; ++j) {
-    const int row = blockIdx.y * 16 + wave * 4 + j;
-    if (row >= rows) return;
-    const auto slot = [&](int i) { return ((long long)(first + i) * a.KH + kvh) * kRows + row; };
-    float top = -INFINITY;
-    for (int i = lane; i < shares; i += kWave) top = fmaxf(top, a.ml[slot(i)].x);
-    top = group_max<64>(top);
-    float sum = 0.f;
-    float acc[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int i = 0; i < shares; ++i) {
-      const float2 ml = a.ml[slot(i)];
-      const float w = ml.x == -INFINITY ? 0.f : exp2f(ml.x - top);
-      sum += w * ml.y;
-      const float* p = a.part + slot(i) * a.dp;
+  const int row = blockIdx.y * kMergeRows + wave;
+  if (row >= min(a.tile_rows, s.q_len * a.G - tile * a.tile_rows)) return;
+  const long long slot0 = ((long long)first * a.KH + kvh) * a.tile_rows + row;
+  const long long next = (long long)a.KH * a.tile_rows;  // from a share's row to the next share's
+  float top = -INFINITY, sum = 0.f;
+  float acc[4] = {0.f, 0.f, 0.f, 0.f};
+  const float* const part = a.part + slot0 * a.dp + lane;
+  for (int i0 = 0; i0 < shares; i0 += kWave) {
+    const float2 ml = i0 + lane < shares ? a.ml[slot0 + (i0 + lane) * next] : make_float2(-INFINITY, 0.f);
+    const float higher = fmaxf(top, group_max<64>(ml.x));
+    const float f = top == -INFINITY ? 0.f : exp2f(top - higher);
+    const float w = ml.x == -INFINITY ? 0.f : exp2f(ml.x - higher);
+    top = higher;
+    sum = sum * f + group_sum<64>(w * ml.y);
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (lane + 64 * e < a.D) acc[e] += w * p[lane + 64 * e];
-    }
-    const int packed = tile * kRows + row;
-    const long long at = (long long)(s.row0 + packed / a.G) * a.H + kvh * a.G + packed % a.G;
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    for (int e = 0; e < 4; ++e) acc[e] *= f;
+    const int n = min(kWave, shares - i0);
+    for (int j0 = 0; j0 < n; j0 += 8) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int d = lane + 64 * e;
-      if (d >= a.D) break;
-      const float x = acc[e] * inv;
-      if (a.q_type == VRM_SRC_F32)
-        static_cast<float*>(a.out)[at * a.D + d] = x;
-      else if (a.q_type == VRM_SRC_F16)
-        static_cast<uint16_t*>(a.out)[at * a.D + d] = __builtin_bit_cast(unsigned short, (_Float16)x);
-      else
-        static_cast<uint16_t*>(a.out)[at * a.D + d] = __builtin_bit_cast(unsigned short, (__bf16)x);
+      for (int j = 0; j < 8; ++j) {
+        if (j0 + j >= n) break;
+        const float wj = __shfl(w, j0 + j);
+        const float* x = part + (i0 + j0 + j) * next * a.dp;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (64 * e < a.dp && lane + 64 * e < a.D) acc[e] += wj * x[64 * e];
+      }
     }
-    if (a.lse && lane == 0) a.lse[at] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.69314718055994531f;
   }
+  const int packed = tile * a.tile_rows + row;
+  const long long at = (long long)(s.row0 + packed / a.G) * a.H + kvh * a.G + packed % a.G;
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int d = lane + 64 * e;
+    if (d >= a.D) break;
+    const float x = acc[e] * inv;
+    if (a.q_type == VRM_SRC_F32)
+      static_cast<float*>(a.out)[at * a.D + d] = x;
+    else if (a.q_type == VRM_SRC_F16)
+      static_cast<uint16_t*>(a.out)[at * a.D + d] = __builtin_bit_cast(unsigned short, (_Float16)x);
+    else
+      static_cast<uint16_t*>(a.out)[at * a.D + d] = __builtin_bit_cast(unsigned short, (__bf16)x);
+  }
+  if (a.lse && lane == 0) a.lse[at] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.69314718055994531f;
 }
 
-// Items of a call, from its sizes alone (lengths are on the device).
+// Items of a call, from its sizes and types alone (lengths are on the device).
 struct ChunkPlan {
-  int target, min_blocks, vtiles, items, dp;
+  bool wide;  // float32 products
+  int kind;   // kSrc* of the pool
+  int target, min_blocks, tile_rows, vtiles, items, dp;
   size_t rec_bytes, ml_bytes, bytes;
 };
 
-// Tiles that fill the GPU twice are left whole; fewer are cut into shares, at
-// least kMinBlocks blocks each, for about kWantedItems workgroups.
-constexpr int kWantedItems = 1024;
+// Tiles that fill the GPU are left whole; fewer are cut into shares, at least
+// kMinBlocks blocks each, for about so many workgroups.
 constexpr int kMinBlocks = 4;
 
-bool plan_chunk(int N, int B, int H, int KH, int D, int PS, int max_pp, ChunkPlan& p) {
+int pool_kind(int kv_dtype) {
+  switch (kv_dtype) {
+    case VRM_KV_F32: return kSrcF32;
+    case VRM_KV_F16: return kSrcF16;
+    case VRM_KV_BF16: return kSrcBf16;
+    case VRM_KV_I8:
+    case VRM_KV_I8_INLINE: return kSrcI8;
+    case VRM_KV_FP8E4M3:
+    case VRM_KV_FP8E4M3_INLINE: return kSrcFp8;
+    default: return -1;
+  }
+}
+
+bool plan_chunk(int N, int B, int H, int KH, int D, int PS, int max_pp, int q_dtype, int kv_dtype, ChunkPlan& p) {
   const long long G = H / KH;
-  const long long vtiles = N * G / kRows + B;
-  const long long blocks = ((long long)max_pp * PS + 31) / 32;  // at most, of 32 tokens
-  p.dp = D <= 64 ? 64 : D <= 96 ? 96 : D <= 128 ? 128 : 256;
+  if (N * G > 0x7fff0000LL) return false;
+  p.kind = pool_kind(kv_dtype);
+  // 16-bit products where queries and keys have one 16-bit type (codes have any)
+  p.wide = q_dtype == VRM_SRC_F32 || p.kind == kSrcF32 || (q_dtype == VRM_SRC_F16 && p.kind == kSrcBf16) ||
+           (q_dtype == VRM_SRC_BF16 && p.kind == kSrcF16);
+  p.dp = D <= 64 ? 64 : D <= 96 && !p.wide ? 96 : D <= 128 ? 128 : 256;
+  const int block = p.wide ? 32 : 64;
+  const long long blocks = ((long long)max_pp * PS + block - 1) / block;  // of a sequence, at most
+  const bool large = !p.wide && D <= 128 && N * G >= 192LL * B;
+  p.tile_rows = large ? 256 : 128;
+  const int wanted = large ? 256 : 512;  // workgroups resident at once
+  const long long vtiles = N * G / p.tile_rows + B;
   p.min_blocks = kMinBlocks;
   p.target = 0;
   long long items = vtiles;
-  if (N * G / kRows * KH < kWantedItems && blocks > kMinBlocks) {
-    p.target = (kWantedItems + KH - 1) / KH;
+  if (N * G / p.tile_rows * KH < 2 * wanted && blocks > kMinBlocks) {
+    p.target = (wanted + KH - 1) / KH;
     const long long most = vtiles * ((blocks + kMinBlocks - 1) / kMinBlocks);
     // sum of tiles * ceil(blocks / share): target + one per tile, and the
     // rounding of the float sum that gives the share
     items = vtiles + p.target + p.target / 256 + 2;
     if (items > most) items = most;
   }
-  if (items * KH > 0x7fffffffLL || N * G > 0x7fffffffLL) return false;
+  if (items * KH > 0x7fffffffLL) return false;
   p.vtiles = (int)vtiles;
   p.items = (int)items;
   p.rec_bytes = p.ml_bytes = p.bytes = 0;
   if (p.target) {
-    const int dp = p.dp == 96 ? 128 : p.dp;  // the float32 kernel pads 96 to 128
     p.rec_bytes = ((size_t)vtiles * KH * sizeof(int2) + 255) / 256 * 256;
-    p.ml_bytes = (size_t)items * KH * kRows * sizeof(float2);
-    p.bytes = p.rec_bytes + p.ml_bytes + (size_t)items * KH * kRows * dp * sizeof(float);
+    p.ml_bytes = (size_t)items * KH * p.tile_rows * sizeof(float2);
+    p.bytes = p.rec_bytes + p.ml_bytes + (size_t)items * KH * p.tile_rows * p.dp * sizeof(float);
   }
   return true;
 }
@@ -113,9 +147,12 @@ bool bad_sizes(int N, int B, int H, int KH, int D, int PS, int max_pp) {
 
 using namespace vrm;
 
-extern "C" size_t vrm_paged_chunk_workspace_bytes(int N, int B, int H, int KH, int D, int PS, int max_pp) {
+extern "C" size_t vrm_paged_chunk_workspace_bytes(int N, int B, int H, int KH, int D, int PS, int max_pp, int q_dtype,
+                                                  int kv_dtype) {
   ChunkPlan p;
-  if (bad_sizes(N, B, H, KH, D, PS, max_pp) || D > 256 || !plan_chunk(N, B, H, KH, D, PS, max_pp, p)) return 0;
+  if (bad_sizes(N, B, H, KH, D, PS, max_pp) || D > 256 || pool_kind(kv_dtype) < 0 ||
+      !plan_chunk(N, B, H, KH, D, PS, max_pp, q_dtype, kv_dtype, p))
+    return 0;
   return p.bytes;
 }
 
@@ -144,18 +181,12 @@ extern "C" int vrm_paged_chunk_attention(const void* query, int q_dtype, long lo
     set_error("%s: unknown query dtype %d", who, q_dtype);
     return VRM_ERR_ARG;
   }
-  int kind;
-  long long row;
-  switch (kv_dtype) {
-    case VRM_KV_F32: kind = kSrcF32, row = 4LL * D; break;
-    case VRM_KV_F16: kind = kSrcF16, row = 2LL * D; break;
-    case VRM_KV_BF16: kind = kSrcBf16, row = 2LL * D; break;
-    case VRM_KV_I8:
-    case VRM_KV_I8_INLINE: kind = kSrcI8, row = D; break;
-    case VRM_KV_FP8E4M3:
-    case VRM_KV_FP8E4M3_INLINE: kind = kSrcFp8, row = D; break;
-    default: set_error("%s: unknown kv_dtype %d", who, kv_dtype); return VRM_ERR_ARG;
+  const int kind = pool_kind(kv_dtype);
+  if (kind < 0) {
+    set_error("%s: unknown kv_dtype %d", who, kv_dtype);
+    return VRM_ERR_ARG;
   }
+  const long long row = kind == kSrcF32 ? 4LL * D : kind < kSrcI8 ? 2LL * D : D;  // bytes of a token
   if (D > 256) {
     set_error("%s: head_dim %d above 256", who, D);
     return VRM_ERR_UNSUPPORTED;
@@ -165,7 +196,7 @@ extern "C" int vrm_paged_chunk_attention(const void* query, int q_dtype, long lo
     return VRM_ERR_UNSUPPORTED;
   }
   ChunkPlan p;
-  if (!plan_chunk(N, B, H, KH, D, PS, max_pp, p)) {
+  if (!plan_chunk(N, B, H, KH, D, PS, max_pp, q_dtype, kv_dtype, p)) {
     set_error("%s: too many rows (N=%d H=%d B=%d)", who, N, H, B);
     return VRM_ERR_UNSUPPORTED;
   }
@@ -219,10 +250,9 @@ extern "C" int vrm_paged_chunk_attention(const void* query, int q_dtype, long lo
   a.aligned = row % 16 == 0 && reinterpret_cast<uintptr_t>(kv_pool) % 16 == 0;
   a.q_aligned = q_at % 16 == 0 && q_token_stride % 8 == 0 && q_head_stride % 8 == 0;
   a.out_aligned = D % 4 == 0 && reinterpret_cast<uintptr_t>(out) % 8 == 0;
-  // 16-bit products where queries and keys have one 16-bit type (codes have any)
-  const bool wide = q_dtype == VRM_SRC_F32 || kind == kSrcF32 || (q_dtype == VRM_SRC_F16 && kind == kSrcBf16) ||
-                    (q_dtype == VRM_SRC_BF16 && kind == kSrcF16);
-  a.dp = wide && p.dp == 96 ? 128 : p.dp;
+  a.dp = p.dp;
+  a.tile_rows = p.tile_rows;
+  a.tile_shift = p.tile_rows == 256 ? 8 : 7;
   char* ws = static_cast<char*>(workspace);
   if (p.target) {
     a.rec = reinterpret_cast<int2*>(ws);
@@ -231,7 +261,7 @@ extern "C" int vrm_paged_chunk_attention(const void* query, int q_dtype, long lo
   }
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const dim3 grid((unsigned)p.items * (unsigned)KH);
-  if (wide)
+  if (p.wide)
     launch_chunk_f32(a, kind, grid, st);
   else if (kind == kSrcI8)
     launch_chunk16_i8(a, grid, st);
@@ -241,6 +271,6 @@ extern "C" int vrm_paged_chunk_attention(const void* query, int q_dtype, long lo
     launch_chunk16_float(a, grid, st);
   const int rc = launch_status(who);
   if (rc || !p.target) return rc;
-  hipLaunchKernelGGL(chunk_merge_kernel, dim3((unsigned)p.vtiles * (unsigned)KH, kRows / 16), dim3(256), 0, st, a);
+  hipLaunchKernelGGL(chunk_merge_kernel, dim3((unsigned)p.vtiles * (unsigned)KH, a.tile_rows / kMergeRows), dim3(256), 0, st, a);
   return launch_status(who);
 }

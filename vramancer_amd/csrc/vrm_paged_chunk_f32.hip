@@ -67,20 +67,14 @@ __global__ void __launch_bounds__(kChunkThreads, DP <= 128 ? 2 : 1) chunk_attn_f
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, half = lane >> 5;
-  const int rows = min(kRows, it.s.q_len * a.G - it.tile * kRows);
+  const int rows = min(a.tile_rows, it.s.q_len * a.G - it.tile * a.tile_rows);
   const bool active = wave * 32 < rows;
-  const int row = wave * 32 + col;
-  const int tok = (it.tile * kRows + row) / a.G;
-  const int head = kvh * a.G + (it.tile * kRows + row) % a.G;
-  const int base = it.s.ctx - it.s.q_len;
-  const bool real = row < rows;
-  const int pos = base + tok;
-  const int first_pos = base + (it.tile * kRows + wave * 32) / a.G;
-  const int last_pos = base + (it.tile * kRows + min(rows, wave * 32 + 32) - 1) / a.G;
+  const RowGroup g = row_group(a, it, kvh, rows, wave * 32);
+  const bool real = g.real;
 
   float q[DP / 2];
   {
-    const long long at = (long long)(it.s.row0 + (real ? tok : 0)) * a.q_n + (long long)(real ? head : 0) * a.q_h;
+    const long long at = (long long)(it.s.row0 + (real ? g.tok : 0)) * a.q_n + (long long)(real ? g.head : 0) * a.q_h;
 #pragma unroll
     for (int j = 0; j < DP / 2; ++j) {
       const int d = j / 4 * 8 + half * 4 + j % 4;
@@ -182,8 +176,8 @@ __global__ void __launch_bounds__(kChunkThreads, DP <= 128 ? 2 : 1) chunk_attn_f
 
   const auto compute = [&](int block) {
     const int t0 = block * TN;
-    if (a.causal && t0 > last_pos) return;
-    if (a.window && t0 + TN - 1 <= first_pos - a.window) return;
+    if (a.causal && t0 > g.last_pos) return;
+    if (a.window && t0 + TN - 1 <= g.first_pos - a.window) return;
     f32x16 s{};
 #pragma unroll
     for (int j = 0; j < DP / 8; ++j) {
@@ -198,9 +192,9 @@ __global__ void __launch_bounds__(kChunkThreads, DP <= 128 ? 2 : 1) chunk_attn_f
       for (int i = 0; i < 16; ++i) s[i] *= scale_lds[0][i / 4 * 8 + 4 * half + i % 4];
     }
     const uint32_t there = there_lds[block & 3];
-    if (there != ~0u || (a.causal && t0 + TN - 1 > first_pos) || (a.window && t0 <= last_pos - a.window)) {
-      const int hi = (a.causal ? min(pos, it.s.ctx - 1) : it.s.ctx - 1) - t0 - 4 * half;
-      const int lo = a.window ? pos - a.window - t0 - 4 * half : -0x40000000;
+    if (there != ~0u || (a.causal && t0 + TN - 1 > g.first_pos) || (a.window && t0 <= g.last_pos - a.window)) {
+      const int hi = (a.causal ? min(g.pos, it.s.ctx - 1) : it.s.ctx - 1) - t0 - 4 * half;
+      const int lo = a.window ? g.pos - a.window - t0 - 4 * half : -0x40000000;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const int t = 8 * (i / 4) + i % 4;
@@ -266,7 +260,7 @@ __global__ void __launch_bounds__(kChunkThreads, DP <= 128 ? 2 : 1) chunk_attn_f
   l = xor_add<32>(l);
   if (!active || !real) return;
   if (it.shares > 1) {
-    const long long slot = (long long)blockIdx.x * kRows + row;
+    const long long slot = (long long)blockIdx.x * a.tile_rows + g.row;
     float* dst = a.part + slot * DP;
 #pragma unroll
     for (int n = 0; n < NB; ++n)
@@ -277,7 +271,7 @@ __global__ void __launch_bounds__(kChunkThreads, DP <= 128 ? 2 : 1) chunk_attn_f
     if (half == 0) a.ml[slot] = make_float2(m, l);
     return;
   }
-  const long long at = (long long)(it.s.row0 + tok) * a.H + head;
+  const long long at = (long long)(it.s.row0 + g.tok) * a.H + g.head;
 #pragma unroll
   for (int n = 0; n < NB; ++n)
 #pragma unroll

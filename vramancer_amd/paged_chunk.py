@@ -36,16 +36,19 @@ __all__ = ["rope_append", "paged_attention_chunk", "chunk_workspace"]
 
 
 @functools.lru_cache(maxsize=256)
-def _workspace_bytes(N: int, B: int, H: int, KH: int, D: int, PS: int, max_pp: int) -> int:
-    return _lib.load().vrm_paged_chunk_workspace_bytes(N, B, H, KH, D, PS, max_pp)
+def _workspace_bytes(N: int, B: int, H: int, KH: int, D: int, PS: int, max_pp: int, q_code: int, kv_code: int) -> int:
+    return _lib.load().vrm_paged_chunk_workspace_bytes(N, B, H, KH, D, PS, max_pp, q_code, kv_code)
 
 
-def chunk_workspace(num_tokens: int, batch: int, num_heads: int, num_kv_heads: int, head_dim: int,
-                    max_pages_per_seq: int, device: Any, page_size: int = 16):
-    """The workspace a ``paged_attention_chunk`` call of these sizes needs,
-    for callers that keep one (``workspace=``)."""
-    nbytes = _workspace_bytes(num_tokens, batch, num_heads, num_kv_heads, head_dim, page_size, max_pages_per_seq)
-    return torch.empty(nbytes, dtype=torch.uint8, device=device)
+def chunk_workspace(query, kv_pool, batch: int, max_pages_per_seq: int):
+    """The workspace that a ``paged_attention_chunk`` call needs for a query
+    and a pool of these shapes and types, for callers that keep one
+    (``workspace=``)."""
+    N, H, D = query.shape
+    KH, PS = kv_pool.shape[3], kv_pool.shape[4]
+    nbytes = _workspace_bytes(N, batch, H, KH, D, PS, max_pages_per_seq, _lib.src_dtype_code(query.dtype),
+                              _lib.kv_dtype_code(kv_pool.dtype))
+    return torch.empty(nbytes, dtype=torch.uint8, device=query.device)
 
 
 def check_pool(kv_pool, kv_scales, D: int):
@@ -208,7 +211,7 @@ def paged_attention_chunk(
     if lse is not None and (tuple(lse.shape) != (N, H) or lse.dtype != torch.float32 or not lse.is_contiguous()):
         raise RuntimeError(f"lse must be a contiguous float32 [{N}, {H}] tensor")
     max_pp = page_table.shape[1]
-    need = _workspace_bytes(N, B, H, KH, D, PS, max_pp) if H % KH == 0 else 0
+    need = _workspace_bytes(N, B, H, KH, D, PS, max_pp, q_code, code) if H % KH == 0 else 0
     if workspace is None:
         if need:
             workspace = torch.empty(need, dtype=torch.uint8, device=query.device)
