@@ -315,16 +315,26 @@ struct Stage {
       sh.scale[block % kRing][1][lane] = vs;
     }
   }
-  // Places of the first two blocks, and the page of the third.
+  // Places of the first three blocks, and the page of the fourth.
   __device__ __forceinline__ void begin(int from) {
     if (wave == 0) {
-      const int p0 = page_of(from), p1 = page_of(from + 1);
-      next_page = page_of(from + 2);
+      const int p0 = page_of(from), p1 = page_of(from + 1), p2 = page_of(from + 2);
+      next_page = page_of(from + 3);
       put_places(from, p0);
-      put_scales(from);
+      const float k0 = ks, v0 = vs;
       put_places(from + 1, p1);
+      const float k1 = ks, v1 = vs;
+      put_places(from + 2, p2);
+      if constexpr (QUANT) {
+        const float k2 = ks, v2 = vs;
+        ks = k0, vs = v0;
+        put_scales(from);
+        ks = k1, vs = v1;
+        put_scales(from + 1);
+        ks = k2, vs = v2;
+      }
     }
-    paged = from + 2;
+    paged = from + 3;
   }
   // Places of the block after those known, the page of the next one, and the
   // scales of the one before (loaded a call ago).
@@ -474,126 +484,144 @@ __device__ __forceinline__ void few_rows(const ChunkArgs& a, const Item& it, int
     const int t = sub * 32 + col;
     return page >= 0 && page < a.P ? (long long)page * a.g.page + (long long)(t - page_index(a, t) * a.PS) * row_bytes : -1;
   };
-  uint4 kr[KP], vr[QUANT ? 1 : KP];
-  uint32_t vw[2][2][QUANT ? NB : 1];
-  float ks = 0.f, vs = 0.f;
-  const auto load_k = [&](long long at, int sub, int page) {
+  // DEPTH x 32 tokens are under way per wavefront
+  constexpr int DEPTH = QUANT ? 2 : 1;
+  uint4 kr[DEPTH][KP], vr[DEPTH][QUANT ? 1 : KP];
+  uint32_t vw[DEPTH][2][2][QUANT ? NB : 1];
+  float ks[DEPTH], vs[DEPTH];
+  long long at[DEPTH];
+  int page[DEPTH];  // of the 32 tokens to be loaded next
+  const auto load_k = [&](int b, int sub) {
 #pragma unroll
     for (int p = 0; p < KP; ++p) {
       const int d = QUANT ? p * 32 + half * 16 : (p * 16 + half * 8) * 2;  // bytes into the row
-      kr[p] = at >= 0 ? load16(k_base + at + d, row_bytes - d, a.aligned) : make_uint4(0, 0, 0, 0);
+      kr[b][p] = at[b] >= 0 ? load16(k_base + at[b] + d, row_bytes - d, a.aligned) : make_uint4(0, 0, 0, 0);
     }
     if constexpr (QUANT) {
-      ks = vs = 0.f;
-      if (at >= 0) {
+      ks[b] = vs[b] = 0.f;
+      if (at[b] >= 0) {
         const int t = sub * 32 + col;
-        const float* s = s_base + (long long)page * a.g.s_page + (KIND == kSrcI8 ? t - page_index(a, t) * a.PS : 0);
-        ks = s[0];
-        vs = s[a.g.s_kv];
+        const float* s = s_base + (long long)page[b] * a.g.s_page + (KIND == kSrcI8 ? t - page_index(a, t) * a.PS : 0);
+        ks[b] = s[0];
+        vs[b] = s[a.g.s_kv];
       }
     }
   };
-  const auto load_v = [&](long long at) {
+  const auto load_v = [&](int b) {
     if constexpr (QUANT) {
 #pragma unroll
       for (int e = 0; e < 2; ++e)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          const long long quad = __shfl(at, 16 * e + 8 * j + 4 * half);  // place of the four tokens' first
+          const long long quad = __shfl(at[b], 16 * e + 8 * j + 4 * half);  // place of the four tokens' first
+          uint32_t(&w)[NB] = vw[b][e][j];
+          const uint8_t* p = v_base + quad + ((col & 15) * nd + (whole ? NB : 1) * (col >> 4)) * 4;
 #pragma unroll
-          for (int n = 0; n < NB; ++n) {
-            const int c = whole ? NB * (col >> 4) + n : 2 * n + (col >> 4);
-            const uint8_t* p = v_base + quad + ((col & 15) * nd + c) * 4;
-            uint32_t w = 0;
-            if (quad >= 0 && c < nd)
-              w = a.aligned ? *reinterpret_cast<const uint32_t*>(p)
-                            : p[0] | (uint32_t)p[1] << 8 | (uint32_t)p[2] << 16 | (uint32_t)p[3] << 24;
-            vw[e][j][n] = w;
+          for (int n = 0; n < NB; ++n) w[n] = 0;
+          if (quad < 0) continue;
+          if (whole && a.aligned) {
+            __builtin_memcpy(w, __builtin_assume_aligned(p, NB % 4 == 0 ? 16 : NB % 2 == 0 ? 8 : 4), 4 * NB);
+          } else {
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+              const uint8_t* x = p + (whole ? 4 * n : 8 * n);
+              if (whole || 2 * n + (col >> 4) < nd)
+                w[n] = x[0] | (uint32_t)x[1] << 8 | (uint32_t)x[2] << 16 | (uint32_t)x[3] << 24;
+            }
           }
         }
     } else {
 #pragma unroll
       for (int p = 0; p < KP; ++p) {
         const int d = (p * 16 + half * 8) * 2;
-        vr[p] = at >= 0 ? load16(v_base + at + d, row_bytes - d, a.aligned) : make_uint4(0, 0, 0, 0);
+        vr[b][p] = at[b] >= 0 ? load16(v_base + at[b] + d, row_bytes - d, a.aligned) : make_uint4(0, 0, 0, 0);
       }
     }
   };
 
   int sub = 2 * from + wave;
-  int page = page_of(sub), page1 = page_of(sub + WAVES);
-  long long at = place_of(sub, page);
-  load_k(at, sub, page);
-  load_v(at);
-  for (; sub < 2 * to; sub += WAVES) {
-    const int t0 = sub * 32;
-    const uint32_t there = (uint32_t)__ballot(at >= 0);
-    f32x16 s{};
 #pragma unroll
-    for (int p = 0; p < KP; ++p) {
+  for (int b = 0; b < DEPTH; ++b) page[b] = page_of(sub + b * WAVES);
+#pragma unroll
+  for (int b = 0; b < DEPTH; ++b) {
+    at[b] = place_of(sub + b * WAVES, page[b]);
+    load_k(b, sub + b * WAVES);
+    load_v(b);
+  }
+#pragma unroll
+  for (int b = 0; b < DEPTH; ++b) page[b] = page_of(sub + (DEPTH + b) * WAVES);
+  for (; sub < 2 * to; sub += DEPTH * WAVES) {
+#pragma unroll
+    for (int b = 0; b < DEPTH; ++b) {
+      const int now = sub + b * WAVES, next = now + DEPTH * WAVES, t0 = now * 32;
+      if (b > 0 && now >= 2 * to) break;
+      const uint32_t there = (uint32_t)__ballot(at[b] >= 0);
+      f32x16 s{};
+#pragma unroll
+      for (int p = 0; p < KP; ++p) {
+        if constexpr (QUANT) {
+          const uint2 x0 = codes4<T, KIND>(kr[b][p].x), x1 = codes4<T, KIND>(kr[b][p].y);
+          const uint2 x2 = codes4<T, KIND>(kr[b][p].z), x3 = codes4<T, KIND>(kr[b][p].w);
+          s = T::mfma(__builtin_bit_cast(typename T::v8, make_uint4(x0.x, x0.y, x1.x, x1.y)), q[2 * p], s);
+          s = T::mfma(__builtin_bit_cast(typename T::v8, make_uint4(x2.x, x2.y, x3.x, x3.y)), q[2 * p + 1], s);
+        } else {
+          s = T::mfma(__builtin_bit_cast(typename T::v8, kr[b][p]), q[p], s);
+        }
+      }
       if constexpr (QUANT) {
-        const uint2 x0 = codes4<T, KIND>(kr[p].x), x1 = codes4<T, KIND>(kr[p].y);
-        const uint2 x2 = codes4<T, KIND>(kr[p].z), x3 = codes4<T, KIND>(kr[p].w);
-        s = T::mfma(__builtin_bit_cast(typename T::v8, make_uint4(x0.x, x0.y, x1.x, x1.y)), q[2 * p], s);
-        s = T::mfma(__builtin_bit_cast(typename T::v8, make_uint4(x2.x, x2.y, x3.x, x3.y)), q[2 * p + 1], s);
-      } else {
-        s = T::mfma(__builtin_bit_cast(typename T::v8, kr[p]), q[p], s);
+        if (half == 0) {
+          own_scale[wave][0][col] = ks[b];
+          own_scale[wave][1][col] = vs[b];
+        }
       }
-    }
-    if constexpr (QUANT) {
-      if (half == 0) {
-        own_scale[wave][0][col] = ks;
-        own_scale[wave][1][col] = vs;
+      // this buffer's next K (its V still waits for the weights)
+      const long long at1 = place_of(next, page[b]);
+      at[b] = at1;
+      load_k(b, next);
+      __syncwarp();
+      if constexpr (QUANT) scale_scores(own_scale[wave][0], half, s);
+      if (needs_mask(a, g, t0, there)) mask_scores(a, it, g, t0, there, half, s);
+      raise_max<NB>(xor_max<32>(top_of(s)) * a.sc, m, l, o);
+      const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], a.sc, -ref));
+        l += s[i];
       }
-    }
-    // the next 32 tokens' K
-    const long long at1 = place_of(sub + WAVES, page1);
-    load_k(at1, sub + WAVES, page1);
-    page1 = page_of(sub + 2 * WAVES);
-    __syncwarp();
-    if constexpr (QUANT) scale_scores(own_scale[wave][0], half, s);
-    if (needs_mask(a, g, t0, there)) mask_scores(a, it, g, t0, there, half, s);
-    raise_max<NB>(xor_max<32>(top_of(s)) * a.sc, m, l, o);
-    const float ref = m == -INFINITY ? 0.f : m;
+      if constexpr (!QUANT) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], a.sc, -ref));
-      l += s[i];
-    }
-    if constexpr (!QUANT) {
+        for (int p = 0; p < KP; ++p)
+          *reinterpret_cast<uint4*>(own_v + col * Tile::kVStride + (p * 16 + half * 8) * 2) = vr[b][p];
+        load_v(b);
+        __syncwarp();
+      }
 #pragma unroll
-      for (int p = 0; p < KP; ++p)
-        *reinterpret_cast<uint4*>(own_v + col * Tile::kVStride + (p * 16 + half * 8) * 2) = vr[p];
-      load_v(at1);
+      for (int e = 0; e < 2; ++e) {
+        f32x8 p;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) p[i] = s[8 * e + i];
+        if constexpr (QUANT) scale_weights(own_scale[wave][1], e, half, p);
+        const auto pb = __builtin_convertvector(p, typename PT::v8);
+        typename PT::v8 low;
+        if constexpr (SPLIT_P) low = __builtin_convertvector(p - __builtin_convertvector(pb, f32x8), typename PT::v8);
+        const uint32_t k0 = keep_bytes(there >> (16 * e + 4 * half)), k1 = keep_bytes(there >> (16 * e + 8 + 4 * half));
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+          typename PT::v8 v;
+          if constexpr (QUANT) {
+            const uint2 x0 = codes4<Bf16, KIND>(vw[b][e][0][n] & k0), x1 = codes4<Bf16, KIND>(vw[b][e][1][n] & k1);
+            v = __builtin_bit_cast(typename PT::v8, make_uint4(x0.x, x0.y, x1.x, x1.y));
+          } else {
+            v = read_v<typename PT::v8>(own_v, Tile::kVStride, 16 * e, n);
+          }
+          o[n] = PT::mfma(v, pb, o[n]);
+          if constexpr (SPLIT_P) o[n] = PT::mfma(v, low, o[n]);
+        }
+      }
+      if constexpr (QUANT) load_v(b);
+      page[b] = page_of(next + DEPTH * WAVES);
       __syncwarp();
     }
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      f32x8 p;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) p[i] = s[8 * e + i];
-      if constexpr (QUANT) scale_weights(own_scale[wave][1], e, half, p);
-      const auto pb = __builtin_convertvector(p, typename PT::v8);
-      typename PT::v8 low;
-      if constexpr (SPLIT_P) low = __builtin_convertvector(p - __builtin_convertvector(pb, f32x8), typename PT::v8);
-#pragma unroll
-      for (int n = 0; n < NB; ++n) {
-        typename PT::v8 v;
-        if constexpr (QUANT) {
-          const uint32_t k0 = keep_bytes(there >> (16 * e + 4 * half));
-          const uint32_t k1 = keep_bytes(there >> (16 * e + 8 + 4 * half));
-          const uint2 x0 = codes4<Bf16, KIND>(vw[e][0][n] & k0), x1 = codes4<Bf16, KIND>(vw[e][1][n] & k1);
-          v = __builtin_bit_cast(typename PT::v8, make_uint4(x0.x, x0.y, x1.x, x1.y));
-        } else {
-          v = read_v<typename PT::v8>(own_v, Tile::kVStride, 16 * e, n);
-        }
-        o[n] = PT::mfma(v, pb, o[n]);
-        if constexpr (SPLIT_P) o[n] = PT::mfma(v, low, o[n]);
-      }
-    }
-    if constexpr (QUANT) load_v(at1);
-    __syncwarp();
-    at = at1;
   }
   l = xor_add<32>(l);
 #pragma unroll
@@ -778,12 +806,13 @@ __global__ void __launch_bounds__(kLargeThreads, 1) chunk_attn_large_kernel(Chun
   Gather st(a, it, kvh, to, shared);
   st.begin(from);
   __syncthreads();
-  st.load(from);
-  st.more_places();
-  st.put(from, lds, lds + Tile::kKBytes);
-  st.load(from + 1);
-  st.put(from + 1, lds + Tile::kBytes, lds + Tile::kBytes + Tile::kKBytes);
-  __syncthreads();
+  {
+    Gather second = st;
+    st.load(from);
+    second.load(from + 1);
+    st.put(from, lds, lds + Tile::kKBytes);
+    second.put(from + 1, lds + Tile::kBytes, lds + Tile::kBytes + Tile::kKBytes);
+  }
   st.load(from + 2);
   st.more_places();
   __syncthreads();

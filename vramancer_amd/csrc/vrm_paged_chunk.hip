@@ -8,29 +8,32 @@
 namespace vrm {
 namespace {
 
-// One wavefront per row: joins the shares' (max, sum, accumulator).  Lane i
-// weighs share i (64 at a time); the accumulators are then loaded eight
-// shares at once.
+// One wavefront per output row: joins the shares' (max, sum, accumulator).
+// Lane i weighs share i (64 at a time); the accumulators are then loaded
+// eight shares at once.
 constexpr int kMergeRows = 4;  // rows of a workgroup
-__global__ void __launch_bounds__(256) chunk_merge_kernel(ChunkArgs a) {
-  const int vtile = blockIdx.x / a.KH, kvh = blockIdx.x % a.KH;
-  const int2 r = a.rec[(long long)vtile * a.KH + kvh];
-  int lo = 0, hi = a.B - 1;  // the last sequence whose tiles start at or before vtile
+__global__ void __launch_bounds__(64 * kMergeRows) chunk_merge_kernel(ChunkArgs a) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const long long at = (long long)blockIdx.x * kMergeRows + wave;  // token * H + head
+  if (at >= (long long)a.N * a.H) return;
+  const int n = (int)(at / a.H), head = (int)(at % a.H), kvh = head / a.G;
+  int lo = 0, hi = a.B - 1;  // the last sequence that starts at or before row n
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (virtual_tile(a, clamp_int(a.cu[mid], 0, a.N), mid) <= vtile)
+    if (a.cu[mid] <= n)
       lo = mid;
     else
       hi = mid - 1;
   }
   const Sequence s = load_sequence(a, lo);
-  const int tile = vtile - virtual_tile(a, s.row0, lo);
-  if (tile < 0 || tile >= tiles_of(a, s)) return;
+  if (n < s.row0 || n >= s.row0 + s.q_len) return;
+  const int packed = (n - s.row0) * a.G + head - kvh * a.G;
+  const int row = packed & (a.tile_rows - 1);
+  const int vtile = virtual_tile(a, s.row0, lo) + (packed >> a.tile_shift);
+  if (vtile >= a.vtiles) return;
+  const int2 r = a.rec[(long long)vtile * a.KH + kvh];
   const int first = r.x, shares = r.y;
-  if (shares <= 1 || first < 0 || first + shares > a.items) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int row = blockIdx.y * kMergeRows + wave;
-  if (row >= min(a.tile_rows, s.q_len * a.G - tile * a.tile_rows)) return;
+  if (shares <= 1 || first < 0 || shares > a.items || first > a.items - shares) return;
   const long long slot0 = ((long long)first * a.KH + kvh) * a.tile_rows + row;
   const long long next = (long long)a.KH * a.tile_rows;  // from a share's row to the next share's
   float top = -INFINITY, sum = 0.f;
@@ -58,8 +61,6 @@ __global__ void __launch_bounds__(256) chunk_merge_kernel(ChunkArgs a) {
       }
     }
   }
-  const int packed = tile * a.tile_rows + row;
-  const long long at = (long long)(s.row0 + packed / a.G) * a.H + kvh * a.G + packed % a.G;
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
@@ -103,7 +104,7 @@ int pool_kind(int kv_dtype) {
 
 bool plan_chunk(int N, int B, int H, int KH, int D, int PS, int max_pp, int q_dtype, int kv_dtype, ChunkPlan& p) {
   const long long G = H / KH;
-  if (N * G > 0x7fff0000LL) return false;
+  if ((long long)N * H > 0x7fff0000LL) return false;
   p.kind = pool_kind(kv_dtype);
   // 16-bit products where queries and keys have one 16-bit type (codes have any)
   p.wide = q_dtype == VRM_SRC_F32 || p.kind == kSrcF32 || (q_dtype == VRM_SRC_F16 && p.kind == kSrcBf16) ||
@@ -271,6 +272,7 @@ extern "C" int vrm_paged_chunk_attention(const void* query, int q_dtype, long lo
     launch_chunk16_float(a, grid, st);
   const int rc = launch_status(who);
   if (rc || !p.target) return rc;
-  hipLaunchKernelGGL(chunk_merge_kernel, dim3((unsigned)p.vtiles * (unsigned)KH, a.tile_rows / kMergeRows), dim3(256), 0, st, a);
+  hipLaunchKernelGGL(chunk_merge_kernel, dim3((unsigned)(((long long)N * H + kMergeRows - 1) / kMergeRows)),
+                     dim3(64 * kMergeRows), 0, st, a);
   return launch_status(who);
 }
