@@ -794,8 +794,12 @@ __global__ void __launch_bounds__(kLargeThreads, 1) chunk_attn_large_kernel(Chun
 
   const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const bool active = wave * 32 < rows;
-  const RowGroup g = row_group(a, it, kvh, rows, wave * 32);
+  // up to 128 rows leave two wavefronts to a row group, one for each half of a
+  // block's tokens
+  const bool halves = rows <= 128;
+  const int group = halves ? wave >> 1 : wave;
+  const bool active = group * 32 < rows;
+  const RowGroup g = row_group(a, it, kvh, rows, group * 32);
   typename T::v8 q[KK];
   load_rows<T, KK>(a, it, g, [&](int kk) { return kk * 16 + half * 8; }, q);
   f32x16 o[NB];
@@ -817,84 +821,96 @@ __global__ void __launch_bounds__(kLargeThreads, 1) chunk_attn_large_kernel(Chun
   st.more_places();
   __syncthreads();
 
-  const auto scores = [&](const uint8_t* k_lds, f32x16 (&s)[2]) {
+  // NS x 32 tokens of each block from its 32-token part u0 on
+  const auto blocks = [&](auto ns, int u0) {
+    constexpr int NS = decltype(ns)::value;
+    const auto scores = [&](const uint8_t* k_lds, f32x16 (&s)[NS]) {
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      s[u] = f32x16{};
+      for (int u = 0; u < NS; ++u) {
+        s[u] = f32x16{};
 #pragma unroll
-      for (int kk = 0; kk < KK; ++kk) {
-        const uint4 x =
-            *reinterpret_cast<const uint4*>(k_lds + (u * 32 + col) * Tile::kKStride + (kk * 16 + half * 8) * 2);
-        s[u] = T::mfma(__builtin_bit_cast(typename T::v8, x), q[kk], s[u]);
+        for (int kk = 0; kk < KK; ++kk) {
+          const uint4 x = *reinterpret_cast<const uint4*>(k_lds + ((u0 + u) * 32 + col) * Tile::kKStride +
+                                                          (kk * 16 + half * 8) * 2);
+          s[u] = T::mfma(__builtin_bit_cast(typename T::v8, x), q[kk], s[u]);
+        }
       }
-    }
-  };
-  // the weights of a block's scores `now` and their product with V, with the
-  // scores `next` of the block after it
-  const auto step = [&](int block, const uint8_t* v_lds, const uint8_t* next_k, f32x16 (&now)[2], f32x16 (&next)[2]) {
-    const unsigned long long there = shared.there[block % Gather::kRing];
-    const auto* scale = shared.scale[block % Gather::kRing];
-    float top = -INFINITY;
+    };
+    // the weights of a block's scores `now` and their product with V, with the
+    // scores `next` of the block after it
+    const auto step = [&](int block, const uint8_t* v_lds, const uint8_t* next_k, f32x16 (&now)[NS],
+                          f32x16 (&next)[NS]) {
+      const unsigned long long there = shared.there[block % Gather::kRing];
+      const auto* scale = shared.scale[block % Gather::kRing];
+      float top = -INFINITY;
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      if constexpr (QUANT) scale_scores(scale[0] + u * 32, half, now[u]);
-      const uint32_t bits = (uint32_t)(there >> (32 * u));
-      const int t0 = block * TN + 32 * u;
-      if (needs_mask(a, g, t0, bits)) mask_scores(a, it, g, t0, bits, half, now[u]);
-      top = fmaxf(top, top_of(now[u]));
-    }
-    raise_max<NB>(xor_max<32>(top) * a.sc, m, l, o);
-    const float ref = m == -INFINITY ? 0.f : m;
-    scores(next_k, next);
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        now[u][i] = __builtin_amdgcn_exp2f(fmaf(now[u][i], a.sc, -ref));
-        l += now[u][i];
+      for (int u = 0; u < NS; ++u) {
+        if constexpr (QUANT) scale_scores(scale[0] + (u0 + u) * 32, half, now[u]);
+        const uint32_t bits = (uint32_t)(there >> (32 * (u0 + u)));
+        const int t0 = block * TN + 32 * (u0 + u);
+        if (needs_mask(a, g, t0, bits)) mask_scores(a, it, g, t0, bits, half, now[u]);
+        top = fmaxf(top, top_of(now[u]));
       }
+      raise_max<NB>(xor_max<32>(top) * a.sc, m, l, o);
+      const float ref = m == -INFINITY ? 0.f : m;
+      scores(next_k, next);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      f32x8 p;
+      for (int u = 0; u < NS; ++u)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) p[i] = now[e >> 1][8 * (e & 1) + i];
-      if constexpr (QUANT) scale_weights(scale[1] + (e >> 1) * 32, e & 1, half, p);
-      const auto pb = __builtin_convertvector(p, typename PT::v8);
-      typename PT::v8 low;
-      if constexpr (SPLIT_P) low = __builtin_convertvector(p - __builtin_convertvector(pb, f32x8), typename PT::v8);
+        for (int i = 0; i < 16; ++i) {
+          now[u][i] = __builtin_amdgcn_exp2f(fmaf(now[u][i], a.sc, -ref));
+          l += now[u][i];
+        }
 #pragma unroll
-      for (int n = 0; n < NB; ++n) {
-        typename PT::v8 v;
-        if constexpr (QUANT)
-          v = __builtin_bit_cast(typename PT::v8,
-                                 *reinterpret_cast<const uint4*>(v_lds + ((e * 2 + half) * DP + n * 32 + col) * 16));
-        else
-          v = read_v<typename PT::v8>(v_lds, Tile::kVStride, e * 16, n);
-        o[n] = PT::mfma(v, pb, o[n]);
-        if constexpr (SPLIT_P) o[n] = PT::mfma(v, low, o[n]);
+      for (int e = 0; e < 2 * NS; ++e) {
+        f32x8 p;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) p[i] = now[e >> 1][8 * (e & 1) + i];
+        if constexpr (QUANT) scale_weights(scale[1] + (u0 + (e >> 1)) * 32, e & 1, half, p);
+        const auto pb = __builtin_convertvector(p, typename PT::v8);
+        typename PT::v8 low;
+        if constexpr (SPLIT_P) low = __builtin_convertvector(p - __builtin_convertvector(pb, f32x8), typename PT::v8);
+        const int part = 2 * u0 + e;  // of 16 tokens
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+          typename PT::v8 v;
+          if constexpr (QUANT)
+            v = __builtin_bit_cast(typename PT::v8, *reinterpret_cast<const uint4*>(
+                                                        v_lds + ((part * 2 + half) * DP + n * 32 + col) * 16));
+          else
+            v = read_v<typename PT::v8>(v_lds, Tile::kVStride, part * 16, n);
+          o[n] = PT::mfma(v, pb, o[n]);
+          if constexpr (SPLIT_P) o[n] = PT::mfma(v, low, o[n]);
+        }
       }
-    }
-  };
+    };
 
-  f32x16 s0[2], s1[2];
-  int slot = 0;  // of the block, of three
-  const auto turn = [&](int block, f32x16 (&now)[2], f32x16 (&next)[2]) {
-    const int slot1 = slot == 2 ? 0 : slot + 1, slot2 = slot == 0 ? 2 : slot - 1;
-    uint8_t* const k2 = lds + slot2 * Tile::kBytes;
-    st.put(block + 2, k2, k2 + Tile::kKBytes);
-    st.load(block + 3);
-    st.more_places();
-    if (active) step(block, lds + slot * Tile::kBytes + Tile::kKBytes, lds + slot1 * Tile::kBytes, now, next);
-    __syncthreads();
-    slot = slot1;
+    f32x16 s0[NS], s1[NS];
+    int slot = 0;  // of the block, of three
+    const auto turn = [&](int block, f32x16 (&now)[NS], f32x16 (&next)[NS]) {
+      const int slot1 = slot == 2 ? 0 : slot + 1, slot2 = slot == 0 ? 2 : slot - 1;
+      uint8_t* const k2 = lds + slot2 * Tile::kBytes;
+      st.put(block + 2, k2, k2 + Tile::kKBytes);
+      st.load(block + 3);
+      st.more_places();
+      if (active) step(block, lds + slot * Tile::kBytes + Tile::kKBytes, lds + slot1 * Tile::kBytes, now, next);
+      __syncthreads();
+      slot = slot1;
+    };
+    if (active) scores(lds, s0);
+    for (int block = from; block < to; block += 2) {
+      turn(block, s0, s1);
+      if (block + 1 < to) turn(block + 1, s1, s0);
+    }
   };
-  if (active) scores(lds, s0);
-  for (int block = from; block < to; block += 2) {
-    turn(block, s0, s1);
-    if (block + 1 < to) turn(block + 1, s1, s0);
-  }
-  if (!active) return;
-  put_rows<T, DP>(a, it, g, m, xor_add<32>(l), o, [](int n, int x) { return n * 32 + x; });
+  if (halves)
+    blocks(std::integral_constant<int, 1>{}, wave & 1);
+  else
+    blocks(std::integral_constant<int, 2>{}, 0);
+  l = xor_add<32>(l);
+  if (halves) join<NB>(reinterpret_cast<float*>(lds), active && (wave & 1), active && !(wave & 1), group, m, l, o);
+  if (!active || (halves && (wave & 1))) return;
+  put_rows<T, DP>(a, it, g, m, l, o, [](int n, int x) { return n * 32 + x; });
 }
 
 template <typename T, int KIND>

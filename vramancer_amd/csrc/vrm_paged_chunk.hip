@@ -8,73 +8,93 @@
 namespace vrm {
 namespace {
 
-// One wavefront per output row: joins the shares' (max, sum, accumulator).
-// Lane i weighs share i (64 at a time); the accumulators are then loaded
-// eight shares at once.
-constexpr int kMergeRows = 4;  // rows of a workgroup
-__global__ void __launch_bounds__(64 * kMergeRows) chunk_merge_kernel(ChunkArgs a) {
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const long long at = (long long)blockIdx.x * kMergeRows + wave;  // token * H + head
-  if (at >= (long long)a.N * a.H) return;
-  const int n = (int)(at / a.H), head = (int)(at % a.H), kvh = head / a.G;
-  int lo = 0, hi = a.B - 1;  // the last sequence that starts at or before row n
+// Joins the shares of a tile's rows, half a wavefront to a row: (max, sum,
+// accumulator) of every share, 16 bytes of an accumulator to a lane, eight
+// shares' loads under way (what another XCD wrote takes about 2 us to come).
+constexpr int kMergeRows = 16;  // rows of a workgroup
+template <int DP>
+__global__ void __launch_bounds__(256) chunk_merge_kernel(ChunkArgs a) {
+  constexpr int VEC = DP <= 128 ? 1 : 2;  // 16-byte pieces of a lane
+  const int vtile = blockIdx.x / a.KH, kvh = blockIdx.x % a.KH;
+  const int2 r = a.rec[(long long)vtile * a.KH + kvh];
+  int lo = 0, hi = a.B - 1;  // the last sequence whose tiles start at or before vtile
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (a.cu[mid] <= n)
+    if (virtual_tile(a, clamp_int(a.cu[mid], 0, a.N), mid) <= vtile)
       lo = mid;
     else
       hi = mid - 1;
   }
   const Sequence s = load_sequence(a, lo);
-  if (n < s.row0 || n >= s.row0 + s.q_len) return;
-  const int packed = (n - s.row0) * a.G + head - kvh * a.G;
-  const int row = packed & (a.tile_rows - 1);
-  const int vtile = virtual_tile(a, s.row0, lo) + (packed >> a.tile_shift);
-  if (vtile >= a.vtiles) return;
-  const int2 r = a.rec[(long long)vtile * a.KH + kvh];
+  const int tile = vtile - virtual_tile(a, s.row0, lo);
+  if (tile < 0 || tile >= tiles_of(a, s)) return;
   const int first = r.x, shares = r.y;
   if (shares <= 1 || first < 0 || shares > a.items || first > a.items - shares) return;
-  const long long slot0 = ((long long)first * a.KH + kvh) * a.tile_rows + row;
-  const long long next = (long long)a.KH * a.tile_rows;  // from a share's row to the next share's
-  float top = -INFINITY, sum = 0.f;
-  float acc[4] = {0.f, 0.f, 0.f, 0.f};
-  const float* const part = a.part + slot0 * a.dp + lane;
-  for (int i0 = 0; i0 < shares; i0 += kWave) {
-    const float2 ml = i0 + lane < shares ? a.ml[slot0 + (i0 + lane) * next] : make_float2(-INFINITY, 0.f);
-    const float higher = fmaxf(top, group_max<64>(ml.x));
-    const float f = top == -INFINITY ? 0.f : exp2f(top - higher);
-    const float w = ml.x == -INFINITY ? 0.f : exp2f(ml.x - higher);
-    top = higher;
-    sum = sum * f + group_sum<64>(w * ml.y);
+  const int rows = min(a.tile_rows, s.q_len * a.G - tile * a.tile_rows);
+  const int l = threadIdx.x & 31;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) acc[e] *= f;
-    const int n = min(kWave, shares - i0);
-    for (int j0 = 0; j0 < n; j0 += 8) {
+  for (int turn = 0; turn < 2; ++turn) {
+    const int row = blockIdx.y * kMergeRows + turn * 8 + (threadIdx.x >> 5);
+    if (row >= rows) continue;
+    const long long slot0 = ((long long)first * a.KH + kvh) * a.tile_rows + row;
+    const long long next = (long long)a.KH * a.tile_rows;  // from a share's row to the next share's
+    const float* const part = a.part + slot0 * DP + 4 * l;
+    float top = -INFINITY, sum = 0.f;
+    float4 acc[VEC] = {};
+    for (int i0 = 0; i0 < shares; i0 += 8) {
+      float2 ml[8];
+      float4 x[8][VEC];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        if (j0 + j >= n) break;
-        const float wj = __shfl(w, j0 + j);
-        const float* x = part + (i0 + j0 + j) * next * a.dp;
+        const bool on = i0 + j < shares;
+        ml[j] = on ? a.ml[slot0 + (i0 + j) * next] : make_float2(-INFINITY, 0.f);
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (64 * e < a.dp && lane + 64 * e < a.D) acc[e] += wj * x[64 * e];
+        for (int v = 0; v < VEC; ++v)
+          x[j][v] = on && 4 * l + 128 * v < DP
+                        ? *reinterpret_cast<const float4*>(part + (i0 + j) * next * DP + 128 * v)
+                        : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+      float higher = top;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) higher = fmaxf(higher, ml[j].x);
+      const float f = top == -INFINITY ? 0.f : exp2f(top - higher);
+      top = higher;
+      sum *= f;
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) acc[v].x *= f, acc[v].y *= f, acc[v].z *= f, acc[v].w *= f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        // a share that saw nothing has no part (its maximum is -inf)
+        const float w = ml[j].x == -INFINITY ? 0.f : exp2f(ml[j].x - top);
+        sum += w * ml[j].y;
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+          acc[v].x += w * x[j][v].x, acc[v].y += w * x[j][v].y;
+          acc[v].z += w * x[j][v].z, acc[v].w += w * x[j][v].w;
+        }
       }
     }
-  }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const int packed = tile * a.tile_rows + row;
+    const int tok = packed / a.G;
+    const long long at = (long long)(s.row0 + tok) * a.H + kvh * a.G + packed - tok * a.G;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const int d = lane + 64 * e;
-    if (d >= a.D) break;
-    const float x = acc[e] * inv;
-    if (a.q_type == VRM_SRC_F32)
-      static_cast<float*>(a.out)[at * a.D + d] = x;
-    else if (a.q_type == VRM_SRC_F16)
-      static_cast<uint16_t*>(a.out)[at * a.D + d] = __builtin_bit_cast(unsigned short, (_Float16)x);
-    else
-      static_cast<uint16_t*>(a.out)[at * a.D + d] = __builtin_bit_cast(unsigned short, (__bf16)x);
+    for (int v = 0; v < VEC; ++v) {
+      const float y[4] = {acc[v].x * inv, acc[v].y * inv, acc[v].z * inv, acc[v].w * inv};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int d = 4 * l + 128 * v + e;
+        if (d >= a.D) break;
+        if (a.q_type == VRM_SRC_F32)
+          static_cast<float*>(a.out)[at * a.D + d] = y[e];
+        else if (a.q_type == VRM_SRC_F16)
+          static_cast<uint16_t*>(a.out)[at * a.D + d] = __builtin_bit_cast(unsigned short, (_Float16)y[e]);
+        else
+          static_cast<uint16_t*>(a.out)[at * a.D + d] = __builtin_bit_cast(unsigned short, (__bf16)y[e]);
+      }
+    }
+    if (a.lse && l == 0) a.lse[at] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.69314718055994531f;
   }
-  if (a.lse && lane == 0) a.lse[at] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.69314718055994531f;
 }
 
 // Items of a call, from its sizes and types alone (lengths are on the device).
@@ -87,7 +107,7 @@ struct ChunkPlan {
 
 // Tiles that fill the GPU are left whole; fewer are cut into shares, at least
 // kMinBlocks blocks each, for about so many workgroups.
-constexpr int kMinBlocks = 4;
+constexpr int kMinBlocks = 2;
 
 int pool_kind(int kv_dtype) {
   switch (kv_dtype) {
@@ -112,7 +132,7 @@ bool plan_chunk(int N, int B, int H, int KH, int D, int PS, int max_pp, int q_dt
   p.dp = D <= 64 ? 64 : D <= 96 && !p.wide ? 96 : D <= 128 ? 128 : 256;
   const int block = p.wide ? 32 : 64;
   const long long blocks = ((long long)max_pp * PS + block - 1) / block;  // of a sequence, at most
-  const bool large = !p.wide && D <= 128 && N * G >= 192LL * B;
+  const bool large = !p.wide && D <= 128 && N * G >= 64LL * B;
   p.tile_rows = large ? 256 : 128;
   const int wanted = large ? 256 : 512;  // workgroups resident at once
   const long long vtiles = N * G / p.tile_rows + B;
@@ -272,7 +292,14 @@ extern "C" int vrm_paged_chunk_attention(const void* query, int q_dtype, long lo
     launch_chunk16_float(a, grid, st);
   const int rc = launch_status(who);
   if (rc || !p.target) return rc;
-  hipLaunchKernelGGL(chunk_merge_kernel, dim3((unsigned)(((long long)N * H + kMergeRows - 1) / kMergeRows)),
-                     dim3(64 * kMergeRows), 0, st, a);
+  const dim3 merge((unsigned)p.vtiles * (unsigned)KH, a.tile_rows / kMergeRows);
+  if (a.dp == 64)
+    hipLaunchKernelGGL((chunk_merge_kernel<64>), merge, dim3(256), 0, st, a);
+  else if (a.dp == 96)
+    hipLaunchKernelGGL((chunk_merge_kernel<96>), merge, dim3(256), 0, st, a);
+  else if (a.dp == 128)
+    hipLaunchKernelGGL((chunk_merge_kernel<128>), merge, dim3(256), 0, st, a);
+  else
+    hipLaunchKernelGGL((chunk_merge_kernel<256>), merge, dim3(256), 0, st, a);
   return launch_status(who);
 }
