@@ -824,65 +824,120 @@ __global__ void __launch_bounds__(kLargeThreads, 1) chunk_attn_large_kernel(Chun
   // NS x 32 tokens of each block from its 32-token part u0 on
   const auto blocks = [&](auto ns, int u0) {
     constexpr int NS = decltype(ns)::value;
-    const auto scores = [&](const uint8_t* k_lds, f32x16 (&s)[NS]) {
+    constexpr int FIRST = NS * KK, SECOND = 2 * NS * NB, ALL = FIRST + SECOND;  // products of a step
+    constexpr int AHEAD = 4;  // operands under way from LDS
+    // operand of product i: K (16 dims of 32 tokens), then V (32 dims of 16 tokens)
+    const auto read_k = [&](const uint8_t* k_lds, int i) {
+      return *reinterpret_cast<const uint4*>(k_lds + ((u0 + i % NS) * 32 + col) * Tile::kKStride +
+                                             (i / NS * 16 + half * 8) * 2);
+    };
+    const auto read_operand = [&](const uint8_t* k_lds, const uint8_t* v_lds, int i) {
+      if (i < FIRST) return read_k(k_lds, i);
+      const int part = 2 * u0 + (i - FIRST) / NB, n = (i - FIRST) % NB;
+      if constexpr (QUANT)
+        return *reinterpret_cast<const uint4*>(v_lds + ((part * 2 + half) * DP + n * 32 + col) * 16);
+      else
+        return read_v<uint4>(v_lds, Tile::kVStride, part * 16, n);
+    };
+    const auto k_scale = [&](int block, f32x16 (&s)[NS]) {
+      if constexpr (QUANT) {
 #pragma unroll
-      for (int u = 0; u < NS; ++u) {
-        s[u] = f32x16{};
-#pragma unroll
-        for (int kk = 0; kk < KK; ++kk) {
-          const uint4 x = *reinterpret_cast<const uint4*>(k_lds + ((u0 + u) * 32 + col) * Tile::kKStride +
-                                                          (kk * 16 + half * 8) * 2);
-          s[u] = T::mfma(__builtin_bit_cast(typename T::v8, x), q[kk], s[u]);
-        }
+        for (int u = 0; u < NS; ++u)
+          scale_scores(shared.scale[block % Gather::kRing][0] + (u0 + u) * 32, half, s[u]);
       }
     };
-    // the weights of a block's scores `now` and their product with V, with the
-    // scores `next` of the block after it
+
+    float top = -INFINITY;  // of the scores `now` of the next step
+    // One block: the weights of its scores `now` and their product with V,
+    // and the scores `next` of the block after it.  Written slot by slot, a
+    // product each, with the operand four slots ahead and a share of the
+    // vector work; nothing crosses a slot's end.  (Left to the compiler, each
+    // product waited for the LDS read right before it.)
     const auto step = [&](int block, const uint8_t* v_lds, const uint8_t* next_k, f32x16 (&now)[NS],
                           f32x16 (&next)[NS]) {
       const unsigned long long there = shared.there[block % Gather::kRing];
-      const auto* scale = shared.scale[block % Gather::kRing];
-      float top = -INFINITY;
+      uint4 f[AHEAD];
 #pragma unroll
-      for (int u = 0; u < NS; ++u) {
-        if constexpr (QUANT) scale_scores(scale[0] + (u0 + u) * 32, half, now[u]);
-        const uint32_t bits = (uint32_t)(there >> (32 * (u0 + u)));
-        const int t0 = block * TN + 32 * (u0 + u);
-        if (needs_mask(a, g, t0, bits)) mask_scores(a, it, g, t0, bits, half, now[u]);
-        top = fmaxf(top, top_of(now[u]));
+      for (int i = 0; i < AHEAD; ++i) f[i] = read_operand(next_k, v_lds, i);
+      bool mask = false;
+#pragma unroll
+      for (int u = 0; u < NS; ++u)
+        mask |= needs_mask(a, g, block * TN + 32 * (u0 + u), (uint32_t)(there >> (32 * (u0 + u))));
+      if (mask) {
+        top = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < NS; ++u) {
+          mask_scores(a, it, g, block * TN + 32 * (u0 + u), (uint32_t)(there >> (32 * (u0 + u))), half, now[u]);
+          top = fmaxf(top, top_of(now[u]));
+        }
       }
       raise_max<NB>(xor_max<32>(top) * a.sc, m, l, o);
       const float ref = m == -INFINITY ? 0.f : m;
-      scores(next_k, next);
+      top = -INFINITY;
+      typename PT::v8 pb[2 * NS], low[2 * NS];
 #pragma unroll
-      for (int u = 0; u < NS; ++u)
+      for (int u = 0; u < NS; ++u) next[u] = f32x16{};
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          now[u][i] = __builtin_amdgcn_exp2f(fmaf(now[u][i], a.sc, -ref));
-          l += now[u][i];
+      for (int i = 0; i < ALL; ++i) {
+        const uint4 x = f[i % AHEAD];
+        if (i < FIRST) {
+          next[i % NS] = T::mfma(__builtin_bit_cast(typename T::v8, x), q[i / NS], next[i % NS]);
+        } else {
+          const int e = (i - FIRST) / NB, n = (i - FIRST) % NB;
+          o[n] = PT::mfma(__builtin_bit_cast(typename PT::v8, x), pb[e], o[n]);
+          if constexpr (SPLIT_P) o[n] = PT::mfma(__builtin_bit_cast(typename PT::v8, x), low[e], o[n]);
         }
+        if (i + AHEAD < ALL) f[i % AHEAD] = read_operand(next_k, v_lds, i + AHEAD);
+        // weights, the last of them ready for the last 16 tokens' products
+        constexpr int kUntil = FIRST + (2 * NS - 1) * NB;
+        const int c0 = (16 * NS * i + kUntil - 1) / kUntil, c1 = (16 * NS * (i + 1) + kUntil - 1) / kUntil;
 #pragma unroll
-      for (int e = 0; e < 2 * NS; ++e) {
-        f32x8 p;
+        for (int c = c0; c < (c1 < 16 * NS ? c1 : 16 * NS); ++c) {
+          const float y = __builtin_amdgcn_exp2f(fmaf(now[c / 16][c % 16], a.sc, -ref));
+          now[c / 16][c % 16] = y;
+          l += y;
+          if (c % 8 == 7) {
+            const int e = c / 8;
+            f32x8 p;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) p[i] = now[e >> 1][8 * (e & 1) + i];
-        if constexpr (QUANT) scale_weights(scale[1] + (u0 + (e >> 1)) * 32, e & 1, half, p);
-        const auto pb = __builtin_convertvector(p, typename PT::v8);
-        typename PT::v8 low;
-        if constexpr (SPLIT_P) low = __builtin_convertvector(p - __builtin_convertvector(pb, f32x8), typename PT::v8);
-        const int part = 2 * u0 + e;  // of 16 tokens
-#pragma unroll
-        for (int n = 0; n < NB; ++n) {
-          typename PT::v8 v;
-          if constexpr (QUANT)
-            v = __builtin_bit_cast(typename PT::v8, *reinterpret_cast<const uint4*>(
-                                                        v_lds + ((part * 2 + half) * DP + n * 32 + col) * 16));
-          else
-            v = read_v<typename PT::v8>(v_lds, Tile::kVStride, part * 16, n);
-          o[n] = PT::mfma(v, pb, o[n]);
-          if constexpr (SPLIT_P) o[n] = PT::mfma(v, low, o[n]);
+            for (int j = 0; j < 8; ++j) p[j] = now[e / 2][8 * (e % 2) + j];
+            if constexpr (QUANT)
+              scale_weights(shared.scale[block % Gather::kRing][1] + (u0 + e / 2) * 32, e % 2, half, p);
+            pb[e] = __builtin_convertvector(p, typename PT::v8);
+            if constexpr (SPLIT_P)
+              low[e] = __builtin_convertvector(p - __builtin_convertvector(pb[e], f32x8), typename PT::v8);
+          }
         }
+        // K scales and the maximum of the next scores, from two slots after they are whole
+        if (i >= FIRST + 2) {
+          constexpr int kSlots = SECOND - 2;
+          const int t0 = 4 * NS * (i - FIRST - 2) / kSlots, t1 = 4 * NS * (i - FIRST - 1) / kSlots;
+#pragma unroll
+          for (int t = t0; t < t1; ++t) {
+            f32x16& s = next[t / 4];
+            const int j = t % 4 * 4;
+            if constexpr (QUANT) {
+              const float4 y = *reinterpret_cast<const float4*>(
+                  shared.scale[(block + 1) % Gather::kRing][0] + (u0 + t / 4) * 32 + 2 * j + 4 * half);
+              s[j] *= y.x, s[j + 1] *= y.y, s[j + 2] *= y.z, s[j + 3] *= y.w;
+            }
+            top = fmaxf(fmaxf(top, s[j]), s[j + 1]);
+            top = fmaxf(fmaxf(top, s[j + 2]), s[j + 3]);
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
+    };
+    const auto first_scores = [&](f32x16 (&s)[NS]) {
+#pragma unroll
+      for (int u = 0; u < NS; ++u) s[u] = f32x16{};
+#pragma unroll
+      for (int i = 0; i < FIRST; ++i)
+        s[i % NS] = T::mfma(__builtin_bit_cast(typename T::v8, read_k(lds, i)), q[i / NS], s[i % NS]);
+      k_scale(from, s);
+#pragma unroll
+      for (int u = 0; u < NS; ++u) top = fmaxf(top, top_of(s[u]));
     };
 
     f32x16 s0[NS], s1[NS];
@@ -897,7 +952,7 @@ __global__ void __launch_bounds__(kLargeThreads, 1) chunk_attn_large_kernel(Chun
       __syncthreads();
       slot = slot1;
     };
-    if (active) scores(lds, s0);
+    if (active) first_scores(s0);
     for (int block = from; block < to; block += 2) {
       turn(block, s0, s1);
       if (block + 1 < to) turn(block + 1, s1, s0);
