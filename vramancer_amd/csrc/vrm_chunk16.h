@@ -764,9 +764,11 @@ __global__ void __launch_bounds__(kChunkThreads, DP <= 128 ? 2 : 1) chunk_attn_k
 
 // Tiles of 256 rows, 32 to each of eight wavefronts, one workgroup to a CU.
 // A wavefront forms the scores of the next block while the weights of this
-// one are taken, and its SIMD's other wavefront fills what is left.  Three
-// blocks are in LDS, so that one barrier per block is enough, and a fourth in
-// registers.
+// one are taken.  Its SIMD's other wavefront runs half a step behind: one
+// meets the block's barrier at the end of a step, the other between the
+// products of K and of V, so that one's masks, maxima and staging fall beside
+// the other's products.  Four blocks are in LDS (the wavefronts ahead write
+// block + 2 while those behind still read block - 1), a fifth in registers.
 template <typename T, int KIND, int DP>
 __global__ void __launch_bounds__(kLargeThreads, 1) chunk_attn_large_kernel(ChunkArgs a) {
   using Tile = ChunkTile<KIND, DP>;
@@ -775,7 +777,7 @@ __global__ void __launch_bounds__(kLargeThreads, 1) chunk_attn_large_kernel(Chun
   constexpr bool QUANT = Tile::kQuant;
   constexpr bool SPLIT_P = QUANT && std::is_same_v<T, F16>;
   constexpr int TN = Tile::kTokens, NB = DP / 32, KK = DP / 16;
-  constexpr int kLds = max3(3 * Tile::kBytes, 4 * Tile::kPartial, 8 * Tile::kOwnV);
+  constexpr int kLds = max3(4 * Tile::kBytes, 4 * Tile::kPartial, 8 * Tile::kOwnV);
   __shared__ __align__(16) uint8_t lds[kLds];
   __shared__ __align__(16) typename Gather::Shared shared;
   __shared__ __align__(16) float own_scale[QUANT ? 8 : 1][2][32];
@@ -799,6 +801,7 @@ __global__ void __launch_bounds__(kLargeThreads, 1) chunk_attn_large_kernel(Chun
   const bool halves = rows <= 128;
   const int group = halves ? wave >> 1 : wave;
   const bool active = group * 32 < rows;
+  const bool behind = wave >= 4;  // wavefronts w and w + 4 share a SIMD
   const RowGroup g = row_group(a, it, kvh, rows, group * 32);
   typename T::v8 q[KK];
   load_rows<T, KK>(a, it, g, [&](int kk) { return kk * 16 + half * 8; }, q);
@@ -880,6 +883,7 @@ __global__ void __launch_bounds__(kLargeThreads, 1) chunk_attn_large_kernel(Chun
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int i = 0; i < ALL; ++i) {
+        if (i == FIRST && behind) __syncthreads();
         const uint4 x = f[i % AHEAD];
         if (i < FIRST) {
           next[i % NS] = T::mfma(__builtin_bit_cast(typename T::v8, x), q[i / NS], next[i % NS]);
@@ -941,16 +945,13 @@ __global__ void __launch_bounds__(kLargeThreads, 1) chunk_attn_large_kernel(Chun
     };
 
     f32x16 s0[NS], s1[NS];
-    int slot = 0;  // of the block, of three
     const auto turn = [&](int block, f32x16 (&now)[NS], f32x16 (&next)[NS]) {
-      const int slot1 = slot == 2 ? 0 : slot + 1, slot2 = slot == 0 ? 2 : slot - 1;
-      uint8_t* const k2 = lds + slot2 * Tile::kBytes;
-      st.put(block + 2, k2, k2 + Tile::kKBytes);
+      const auto slot = [&](int ahead) { return lds + ((block - from + ahead) & 3) * Tile::kBytes; };
+      st.put(block + 2, slot(2), slot(2) + Tile::kKBytes);
       st.load(block + 3);
       st.more_places();
-      if (active) step(block, lds + slot * Tile::kBytes + Tile::kKBytes, lds + slot1 * Tile::kBytes, now, next);
-      __syncthreads();
-      slot = slot1;
+      if (active) step(block, slot(0) + Tile::kKBytes, slot(1), now, next);
+      if (!active || !behind) __syncthreads();
     };
     if (active) first_scores(s0);
     for (int block = from; block < to; block += 2) {
