@@ -243,12 +243,12 @@ __device__ __forceinline__ V8 read_v(const uint8_t* v_lds, int stride, int token
   return __builtin_bit_cast(V8, __builtin_shufflevector(r0, r1, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
-// Gathers blocks of 64 tokens through the page table, WAVES wavefronts of them
-// a run of consecutive tokens each: global memory to registers (load),
-// registers to LDS (put).  A run within one page (page sizes that are
-// multiples of the run's length) has one address per wavefront and no
-// bookkeeping per lane; other page sizes, and runs with tokens that are not
-// there, look up every row.
+// Gathers blocks of 64 tokens through the page table, a run of consecutive
+// tokens to each of WAVES wavefronts, which finds its own pages (a block
+// ahead): global memory to registers (load), registers to LDS (put).  A run
+// within one page (page sizes that are multiples of its length) has one
+// address; other page sizes, and runs with tokens that are not there, look up
+// every row.
 template <typename T, int KIND, int DP, int WAVES>
 struct Stage {
   using Tile = ChunkTile<KIND, DP>;
@@ -258,9 +258,9 @@ struct Stage {
   static constexpr int NP = (kRun + 63) / 64;       // per lane
   static constexpr bool kRagged = kRun % 64 != 0;
   static constexpr int kRing = 8;
+  using Bits = std::conditional_t<RUN == 8, uint8_t, uint16_t>;
   struct Shared {
-    long long place[kRing][TN];  // a token's K row from the layer's start, -1: not there
-    unsigned long long there[kRing];
+    unsigned long long there[kRing];  // tokens of a block that are there, a bit each
     float scale[kRing][2][QUANT ? TN : 1];
   };
 
@@ -270,11 +270,11 @@ struct Stage {
   const float* s_base;
   const int32_t* table;
   int ctx, to, row_bytes, lane, wave;
-  bool one_page;  // a run lies in one page, its rows can be loaded 16 bytes at a time
+  bool one_page;  // a run lies in one page and is contiguous there
   uint4 kr[NP], vr[NP];
-  int next_page;  // wavefront 0: page of token `lane` of block `paged`
-  int paged;
-  float ks, vs;   // wavefront 0: scales of token `lane` of block paged - 1
+  int page;       // lane i: of token i % RUN of the run to be loaded next, -1: none
+  uint32_t bits;  // tokens of the run in registers that are there
+  float ks, vs;   // lane i < RUN: their scales
 
   __device__ __forceinline__ Stage(const ChunkArgs& args, const Item& it, int kvh, int blocks_end, Shared& shared)
       : a(args), sh(shared), ctx(it.s.ctx), to(blocks_end) {
@@ -288,76 +288,30 @@ struct Stage {
     one_page = a.PS % RUN == 0 && a.aligned && a.D == DP;
   }
 
-  // Wavefront 0.
   __device__ __forceinline__ int page_of(int block) const {
-    const int t = block * TN + lane;
+    const int t = block * TN + RUN * wave + lane % RUN;
     return block < to && t < ctx ? table[page_index(a, t)] : -1;
   }
-  __device__ __forceinline__ void put_places(int block, int page) {
-    const int t = block * TN + lane;
+
+  // `page` is the block's; on return it is the next block's.
+  __device__ __forceinline__ void load(int block) {
+    const int run0 = block * TN + RUN * wave;
     const bool there = page >= 0 && page < a.P;
-    const int slot = t - page_index(a, t) * a.PS;
-    sh.place[block % kRing][lane] = there ? (long long)page * a.g.page + (long long)slot * row_bytes : -1;
-    const unsigned long long mask = __ballot(there);
-    if (lane == 0) sh.there[block % kRing] = mask;
+    bits = (uint32_t)__ballot(there) & ((1u << RUN) - 1);
+    if (lane == 0) reinterpret_cast<Bits*>(&sh.there[block % kRing])[wave] = (Bits)bits;
+    const int slot = run0 + lane % RUN - page_index(a, run0 + lane % RUN) * a.PS;
     if constexpr (QUANT) {
       ks = vs = 0.f;
-      if (there) {
+      if (there && lane < RUN) {
         const float* s = s_base + (long long)page * a.g.s_page + (KIND == kSrcI8 ? slot : 0);
         ks = s[0];
         vs = s[a.g.s_kv];
       }
     }
-  }
-  __device__ __forceinline__ void put_scales(int block) {
-    if constexpr (QUANT) {
-      sh.scale[block % kRing][0][lane] = ks;
-      sh.scale[block % kRing][1][lane] = vs;
-    }
-  }
-  // Places of the first three blocks, and the page of the fourth.
-  __device__ __forceinline__ void begin(int from) {
-    if (wave == 0) {
-      const int p0 = page_of(from), p1 = page_of(from + 1), p2 = page_of(from + 2);
-      next_page = page_of(from + 3);
-      put_places(from, p0);
-      const float k0 = ks, v0 = vs;
-      put_places(from + 1, p1);
-      const float k1 = ks, v1 = vs;
-      put_places(from + 2, p2);
-      if constexpr (QUANT) {
-        const float k2 = ks, v2 = vs;
-        ks = k0, vs = v0;
-        put_scales(from);
-        ks = k1, vs = v1;
-        put_scales(from + 1);
-        ks = k2, vs = v2;
-      }
-    }
-    paged = from + 3;
-  }
-  // Places of the block after those known, the page of the next one, and the
-  // scales of the one before (loaded a call ago).
-  __device__ __forceinline__ void more_places() {
-    if (wave == 0) {
-      put_scales(paged - 1);
-      put_places(paged, next_page);
-      next_page = page_of(paged + 1);
-    }
-    ++paged;
-  }
-
-  // Tokens of the wavefront's run of a block that are there, a bit each.
-  __device__ __forceinline__ uint32_t run_there(int block) const {
-    const unsigned long long there = sh.there[block % kRing];
-    return (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(there >> (RUN * wave))) & ((1u << RUN) - 1);
-  }
-
-  __device__ __forceinline__ void load(int block) {
-    if (one_page && run_there(block) == (1u << RUN) - 1) {
-      const long long at = sh.place[block % kRing][RUN * wave];
-      const long long run = (long long)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)at) |
-                            (long long)__builtin_amdgcn_readfirstlane((uint32_t)(at >> 32)) << 32;
+    if (one_page && bits == (1u << RUN) - 1) {
+      const long long run = (long long)__builtin_amdgcn_readfirstlane(page) * a.g.page +
+                            (long long)__builtin_amdgcn_readfirstlane(slot) * row_bytes;
+      page = page_of(block + 1);
       const uint8_t *k = k_base + run, *v = v_base + run;
 #pragma unroll
       for (int i = 0; i < NP; ++i) {
@@ -368,26 +322,32 @@ struct Stage {
       }
       return;
     }
+    const long long place = there ? (long long)page * a.g.page + (long long)slot * row_bytes : -1;
+    page = page_of(block + 1);
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
       const int c = lane + 64 * i;
       kr[i] = vr[i] = make_uint4(0, 0, 0, 0);
-      if (kRagged && c >= kRun) break;
-      const int t = RUN * wave + c / Tile::kPerRow, w = c % Tile::kPerRow;
-      const long long at = sh.place[block % kRing][t];
+      const int w = c % Tile::kPerRow;
+      const long long at = __shfl(place, c / Tile::kPerRow % RUN);
+      // V of the quantized pools: four tokens' codes of a dim in a dword
+      const int w4 = c % (DP / 4);
+      const long long at4 = QUANT ? __shfl(place, c / (DP / 4) * 4 % RUN) : 0;
+      if (kRagged && c >= kRun) continue;
       if (at >= 0) kr[i] = load16(k_base + at + w * 16, row_bytes - w * 16, a.aligned);
       if constexpr (!QUANT) {
         if (at >= 0) vr[i] = load16(v_base + at + w * 16, row_bytes - w * 16, a.aligned);
-      } else {  // V: four tokens' codes of a dim in a dword, 4 D bytes for the four tokens
-        const int t4 = RUN * wave + c / (DP / 4) * 4, w4 = c % (DP / 4);
-        const long long at4 = sh.place[block % kRing][t4];
+      } else {
         if (at4 >= 0 && w4 * 4 < a.D) vr[i] = load16(v_base + at4 + w4 * 16, 16, a.aligned);
       }
     }
   }
 
   __device__ __forceinline__ void put(int block, uint8_t* k_lds, uint8_t* v_lds) {
-    const uint32_t there = QUANT ? run_there(block) : 0;
+    if (QUANT && lane < RUN) {
+      sh.scale[block % kRing][0][RUN * wave + lane] = ks;
+      sh.scale[block % kRing][1][RUN * wave + lane] = vs;
+    }
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
       const int c = lane + 64 * i;
@@ -404,19 +364,23 @@ struct Stage {
         dst[1] = make_uint4(k2.x, k2.y, k3.x, k3.y);
         // V^T: [16-token step][lane half][dim][8 tokens]
         const int quad = RUN / 4 * wave + c / (DP / 4), w4 = c % (DP / 4);
-        const uint32_t keep = keep_bytes(there >> (c / (DP / 4) * 4));
         uint8_t* vt = v_lds + ((quad >> 2) * 2 + (quad & 1)) * DP * 16 + (quad >> 1 & 1) * 8;
-        const uint32_t words[4] = {vr[i].x, vr[i].y, vr[i].z, vr[i].w};
+        uint32_t words[4] = {vr[i].x, vr[i].y, vr[i].z, vr[i].w};
+        if (bits != (1u << RUN) - 1) {
+          const uint32_t keep = keep_bytes(bits >> (c / (DP / 4) * 4));
+#pragma unroll
+          for (int j = 0; j < 4; ++j) words[j] &= keep;
+        }
         if (DP % 64 == 0 && a.D == DP) {  // four dims 16 apart
           uint8_t* v0 = vt + (w4 * 4 / (DP / 16) + 16 * (w4 * 4 % (DP / 16))) * 16;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) *reinterpret_cast<uint2*>(v0 + j * 256) = codes4<Bf16, KIND>(words[j] & keep);
+          for (int j = 0; j < 4; ++j) *reinterpret_cast<uint2*>(v0 + j * 256) = codes4<Bf16, KIND>(words[j]);
         } else if (w4 * 4 < a.D) {
           const int nd = a.D >> 4;
           int d0 = w4 * 4 / nd, d1 = w4 * 4 % nd;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            *reinterpret_cast<uint2*>(vt + (d0 + 16 * d1) * 16) = codes4<Bf16, KIND>(words[j] & keep);
+            *reinterpret_cast<uint2*>(vt + (d0 + 16 * d1) * 16) = codes4<Bf16, KIND>(words[j]);
             if (++d1 == nd) d1 = 0, ++d0;
           }
         }
@@ -740,13 +704,11 @@ __global__ void __launch_bounds__(kChunkThreads, DP <= 128 ? 2 : 1) chunk_attn_k
   };
 
   Gather st(a, it, kvh, to, shared);
-  st.begin(from);
-  __syncthreads();
+  st.page = st.page_of(from);
   if (from < to) st.load(from);
   for (int block = from; block < to; ++block) {
     __syncthreads();  // the block before is computed
     st.put(block, k_lds, v_lds);
-    st.more_places();
     __syncthreads();
     if (block + 1 < to) st.load(block + 1);
     if (active) {
@@ -801,7 +763,6 @@ __global__ void __launch_bounds__(kLargeThreads, 1) chunk_attn_large_kernel(Chun
   const bool halves = rows <= 128;
   const int group = halves ? wave >> 1 : wave;
   const bool active = group * 32 < rows;
-  const bool behind = wave >= 4;  // wavefronts w and w + 4 share a SIMD
   const RowGroup g = row_group(a, it, kvh, rows, group * 32);
   typename T::v8 q[KK];
   load_rows<T, KK>(a, it, g, [&](int kk) { return kk * 16 + half * 8; }, q);
@@ -811,22 +772,23 @@ __global__ void __launch_bounds__(kLargeThreads, 1) chunk_attn_large_kernel(Chun
   float m = -INFINITY, l = 0.f;
 
   Gather st(a, it, kvh, to, shared);
-  st.begin(from);
-  __syncthreads();
   {
     Gather second = st;
+    st.page = st.page_of(from);
+    second.page = st.page_of(from + 1);
     st.load(from);
     second.load(from + 1);
     st.put(from, lds, lds + Tile::kKBytes);
     second.put(from + 1, lds + Tile::kBytes, lds + Tile::kBytes + Tile::kKBytes);
+    st.page = second.page;
   }
   st.load(from + 2);
-  st.more_places();
   __syncthreads();
 
   // NS x 32 tokens of each block from its 32-token part u0 on
-  const auto blocks = [&](auto ns, int u0) {
+  const auto blocks = [&](auto ns, auto behind, int u0) {
     constexpr int NS = decltype(ns)::value;
+    constexpr bool BEHIND = decltype(behind)::value;
     constexpr int FIRST = NS * KK, SECOND = 2 * NS * NB, ALL = FIRST + SECOND;  // products of a step
     constexpr int AHEAD = 4;  // operands under way from LDS
     // operand of product i: K (16 dims of 32 tokens), then V (32 dims of 16 tokens)
@@ -851,6 +813,7 @@ __global__ void __launch_bounds__(kLargeThreads, 1) chunk_attn_large_kernel(Chun
     };
 
     float top = -INFINITY;  // of the scores `now` of the next step
+    unsigned long long there = shared.there[from % Gather::kRing];  // of its block
     // One block: the weights of its scores `now` and their product with V,
     // and the scores `next` of the block after it.  Written slot by slot, a
     // product each, with the operand four slots ahead and a share of the
@@ -858,7 +821,6 @@ __global__ void __launch_bounds__(kLargeThreads, 1) chunk_attn_large_kernel(Chun
     // product waited for the LDS read right before it.)
     const auto step = [&](int block, const uint8_t* v_lds, const uint8_t* next_k, f32x16 (&now)[NS],
                           f32x16 (&next)[NS]) {
-      const unsigned long long there = shared.there[block % Gather::kRing];
       uint4 f[AHEAD];
 #pragma unroll
       for (int i = 0; i < AHEAD; ++i) f[i] = read_operand(next_k, v_lds, i);
@@ -883,7 +845,7 @@ __global__ void __launch_bounds__(kLargeThreads, 1) chunk_attn_large_kernel(Chun
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int i = 0; i < ALL; ++i) {
-        if (i == FIRST && behind) __syncthreads();
+        if (BEHIND && i == FIRST) __syncthreads();
         const uint4 x = f[i % AHEAD];
         if (i < FIRST) {
           next[i % NS] = T::mfma(__builtin_bit_cast(typename T::v8, x), q[i / NS], next[i % NS]);
@@ -913,6 +875,7 @@ __global__ void __launch_bounds__(kLargeThreads, 1) chunk_attn_large_kernel(Chun
               low[e] = __builtin_convertvector(p - __builtin_convertvector(pb[e], f32x8), typename PT::v8);
           }
         }
+        if (i == ALL - 4) there = shared.there[(block + 1) % Gather::kRing];
         // K scales and the maximum of the next scores, from two slots after they are whole
         if (i >= FIRST + 2) {
           constexpr int kSlots = SECOND - 2;
@@ -949,9 +912,8 @@ __global__ void __launch_bounds__(kLargeThreads, 1) chunk_attn_large_kernel(Chun
       const auto slot = [&](int ahead) { return lds + ((block - from + ahead) & 3) * Tile::kBytes; };
       st.put(block + 2, slot(2), slot(2) + Tile::kKBytes);
       st.load(block + 3);
-      st.more_places();
       if (active) step(block, slot(0) + Tile::kKBytes, slot(1), now, next);
-      if (!active || !behind) __syncthreads();
+      if (!BEHIND || !active) __syncthreads();
     };
     if (active) first_scores(s0);
     for (int block = from; block < to; block += 2) {
@@ -960,9 +922,11 @@ __global__ void __launch_bounds__(kLargeThreads, 1) chunk_attn_large_kernel(Chun
     }
   };
   if (halves)
-    blocks(std::integral_constant<int, 1>{}, wave & 1);
-  else
-    blocks(std::integral_constant<int, 2>{}, 0);
+    blocks(std::integral_constant<int, 1>{}, std::false_type{}, wave & 1);
+  else if (wave < 4)
+    blocks(std::integral_constant<int, 2>{}, std::false_type{}, 0);
+  else  // wavefronts w and w + 4 share a SIMD
+    blocks(std::integral_constant<int, 2>{}, std::true_type{}, 0);
   l = xor_add<32>(l);
   if (halves) join<NB>(reinterpret_cast<float*>(lds), active && (wave & 1), active && !(wave & 1), group, m, l, o);
   if (!active || (halves && (wave & 1))) return;
