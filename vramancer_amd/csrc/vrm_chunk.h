@@ -231,5 +231,6 @@ void launch_chunk_f32(const ChunkArgs& a, int kind, dim3 grid, hipStream_t st);
 void launch_chunk16_float(const ChunkArgs& a, dim3 grid, hipStream_t st);
 void launch_chunk16_i8(const ChunkArgs& a, dim3 grid, hipStream_t st);
 void launch_chunk16_fp8(const ChunkArgs& a, dim3 grid, hipStream_t st);
+void launch_chunk16_256(const ChunkArgs& a, int kind, dim3 grid, hipStream_t st);  // head dims above 128
 
 }  // namespace vrm

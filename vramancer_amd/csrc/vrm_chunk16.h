@@ -145,7 +145,7 @@ __device__ __forceinline__ float top_of(const f32x16& s) {
 // accumulators are rescaled a few times per row, not per block.
 template <int NB>
 __device__ __forceinline__ void raise_max(float top, float& m, float& l, f32x16 (&o)[NB]) {
-  if (__any(top > m + 8.f)) {
+  if (__builtin_expect(__any(top > m + 8.f), 0)) {
     const float next = fmaxf(m, top);
     const float f = next == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - next);
 #pragma unroll
@@ -269,7 +269,8 @@ struct Stage {
   const uint8_t *k_base, *v_base;
   const float* s_base;
   const int32_t* table;
-  int ctx, to, row_bytes, lane, wave;
+  int row_bytes, lane, wave;
+  int limit;      // tokens from here on are not there
   bool one_page;  // a run lies in one page and is contiguous there
   uint4 kr[NP], vr[NP];
   int page;       // lane i: of token i % RUN of the run to be loaded next, -1: none
@@ -277,7 +278,8 @@ struct Stage {
   float ks, vs;   // lane i < RUN: their scales
 
   __device__ __forceinline__ Stage(const ChunkArgs& args, const Item& it, int kvh, int blocks_end, Shared& shared)
-      : a(args), sh(shared), ctx(it.s.ctx), to(blocks_end) {
+      : a(args), sh(shared) {
+    const int ctx = it.s.ctx, to = blocks_end;
     k_base = a.pool + a.layer_off + (long long)kvh * a.g.head;
     v_base = k_base + a.g.kv;
     s_base = QUANT ? a.scales + a.s_layer_off + (long long)kvh * a.g.s_head : nullptr;
@@ -285,21 +287,25 @@ struct Stage {
     table = a.table + (long long)it.b * a.max_pp;
     lane = threadIdx.x & 63;
     wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    one_page = a.PS % RUN == 0 && a.aligned && a.D == DP;
+    one_page = a.ps_shift >= 0 && a.PS >= RUN && a.aligned && a.D == DP;
+    limit = min(ctx, to * TN);
   }
 
+  // Page of the lane's token of a block (any entry of the table for a token
+  // from `limit` on: load() drops those).
   __device__ __forceinline__ int page_of(int block) const {
-    const int t = block * TN + RUN * wave + lane % RUN;
-    return block < to && t < ctx ? table[page_index(a, t)] : -1;
+    const int t = min(block * TN + RUN * wave + lane % RUN, limit - 1);
+    return limit > 0 ? table[page_index(a, t)] : -1;
   }
 
   // `page` is the block's; on return it is the next block's.
   __device__ __forceinline__ void load(int block) {
-    const int run0 = block * TN + RUN * wave;
-    const bool there = page >= 0 && page < a.P;
+    const int run0 = block * TN + RUN * wave, t = run0 + lane % RUN;
+    const bool there = t < limit && page >= 0 && page < a.P;
     bits = (uint32_t)__ballot(there) & ((1u << RUN) - 1);
-    if (lane == 0) reinterpret_cast<Bits*>(&sh.there[block % kRing])[wave] = (Bits)bits;
-    const int slot = run0 + lane % RUN - page_index(a, run0 + lane % RUN) * a.PS;
+    reinterpret_cast<Bits*>(&sh.there[block % kRing])[wave] = (Bits)bits;  // (every lane the same)
+    const bool fast = one_page && bits == (1u << RUN) - 1;
+    const int slot = fast ? t & (a.PS - 1) : t - page_index(a, t) * a.PS;
     if constexpr (QUANT) {
       ks = vs = 0.f;
       if (there && lane < RUN) {
@@ -308,10 +314,9 @@ struct Stage {
         vs = s[a.g.s_kv];
       }
     }
-    if (one_page && bits == (1u << RUN) - 1) {
+    if (__builtin_expect(fast, 1)) {
       const long long run = (long long)__builtin_amdgcn_readfirstlane(page) * a.g.page +
-                            (long long)__builtin_amdgcn_readfirstlane(slot) * row_bytes;
-      page = page_of(block + 1);
+                            (long long)((run0 & (a.PS - 1)) * row_bytes);
       const uint8_t *k = k_base + run, *v = v_base + run;
 #pragma unroll
       for (int i = 0; i < NP; ++i) {
@@ -320,13 +325,16 @@ struct Stage {
         kr[i] = *reinterpret_cast<const uint4*>(k + off);
         vr[i] = *reinterpret_cast<const uint4*>(v + off);
       }
+      page = page_of(block + 1);
       return;
     }
     const long long place = there ? (long long)page * a.g.page + (long long)slot * row_bytes : -1;
     page = page_of(block + 1);
+    int first = lane;  // opaque: what follows from it stays here, in no register of the loop
+    asm("" : "+v"(first));
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
-      const int c = lane + 64 * i;
+      const int c = first + 64 * i;
       kr[i] = vr[i] = make_uint4(0, 0, 0, 0);
       const int w = c % Tile::kPerRow;
       const long long at = __shfl(place, c / Tile::kPerRow % RUN);
@@ -621,9 +629,11 @@ __global__ void __launch_bounds__(kChunkThreads, DP <= 128 ? 2 : 1) chunk_attn_k
   item_blocks<TN>(a, it, from, to);
   put_record(a, it, kvh);
   const int rows = min(a.tile_rows, it.s.q_len * a.G - it.tile * a.tile_rows);
-  if (rows <= 32) {
-    few_rows<T, KIND, DP, 4>(a, it, kvh, rows, from, to, lds, own_scale);
-    return;
+  if constexpr (DP <= 128) {  // (at 256 its operands would not fit the registers)
+    if (rows <= 32) {
+      few_rows<T, KIND, DP, 4>(a, it, kvh, rows, from, to, lds, own_scale);
+      return;
+    }
   }
 
   const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
@@ -813,7 +823,17 @@ __global__ void __launch_bounds__(kLargeThreads, 1) chunk_attn_large_kernel(Chun
     };
 
     float top = -INFINITY;  // of the scores `now` of the next step
-    unsigned long long there = shared.there[from % Gather::kRing];  // of its block
+    // of its block: tokens that are there; blocks [whole0, whole1) are seen
+    // whole by every row of the group, as far as they are there
+    uint32_t there[NS];
+    const auto read_there = [&](int block) {
+#pragma unroll
+      for (int u = 0; u < NS; ++u)
+        there[u] = __builtin_amdgcn_readfirstlane(
+            reinterpret_cast<const uint32_t*>(&shared.there[block % Gather::kRing])[u0 + u]);
+    };
+    const int whole0 = a.window ? (max(g.last_pos - a.window + 1, 0) + TN - 1) / TN : 0;
+    const int whole1 = a.causal ? (g.first_pos + 1) / TN : 0x7fffffff;
     // One block: the weights of its scores `now` and their product with V,
     // and the scores `next` of the block after it.  Written slot by slot, a
     // product each, with the operand four slots ahead and a share of the
@@ -824,15 +844,14 @@ __global__ void __launch_bounds__(kLargeThreads, 1) chunk_attn_large_kernel(Chun
       uint4 f[AHEAD];
 #pragma unroll
       for (int i = 0; i < AHEAD; ++i) f[i] = read_operand(next_k, v_lds, i);
-      bool mask = false;
+      bool mask = block < whole0 || block >= whole1;
 #pragma unroll
-      for (int u = 0; u < NS; ++u)
-        mask |= needs_mask(a, g, block * TN + 32 * (u0 + u), (uint32_t)(there >> (32 * (u0 + u))));
-      if (mask) {
+      for (int u = 0; u < NS; ++u) mask |= there[u] != ~0u;
+      if (__builtin_expect(mask, 0)) {
         top = -INFINITY;
 #pragma unroll
         for (int u = 0; u < NS; ++u) {
-          mask_scores(a, it, g, block * TN + 32 * (u0 + u), (uint32_t)(there >> (32 * (u0 + u))), half, now[u]);
+          mask_scores(a, it, g, block * TN + 32 * (u0 + u), there[u], half, now[u]);
           top = fmaxf(top, top_of(now[u]));
         }
       }
@@ -875,7 +894,7 @@ __global__ void __launch_bounds__(kLargeThreads, 1) chunk_attn_large_kernel(Chun
               low[e] = __builtin_convertvector(p - __builtin_convertvector(pb[e], f32x8), typename PT::v8);
           }
         }
-        if (i == ALL - 4) there = shared.there[(block + 1) % Gather::kRing];
+        if (i == ALL - 3) read_there(block + 1);
         // K scales and the maximum of the next scores, from two slots after they are whole
         if (i >= FIRST + 2) {
           constexpr int kSlots = SECOND - 2;
@@ -897,6 +916,7 @@ __global__ void __launch_bounds__(kLargeThreads, 1) chunk_attn_large_kernel(Chun
       }
     };
     const auto first_scores = [&](f32x16 (&s)[NS]) {
+      read_there(from);
 #pragma unroll
       for (int u = 0; u < NS; ++u) s[u] = f32x16{};
 #pragma unroll
@@ -948,10 +968,8 @@ void launch_chunk16_t(const ChunkArgs& a, dim3 grid, hipStream_t st) {
     hipLaunchKernelGGL((chunk_attn_kernel<T, KIND, 64>), grid, dim3(kChunkThreads), 0, st, a);
   else if (a.dp == 96)
     hipLaunchKernelGGL((chunk_attn_kernel<T, KIND, 96>), grid, dim3(kChunkThreads), 0, st, a);
-  else if (a.dp == 128)
-    hipLaunchKernelGGL((chunk_attn_kernel<T, KIND, 128>), grid, dim3(kChunkThreads), 0, st, a);
   else
-    hipLaunchKernelGGL((chunk_attn_kernel<T, KIND, 256>), grid, dim3(kChunkThreads), 0, st, a);
+    hipLaunchKernelGGL((chunk_attn_kernel<T, KIND, 128>), grid, dim3(kChunkThreads), 0, st, a);
 }
 
 }  // namespace

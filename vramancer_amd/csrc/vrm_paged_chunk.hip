@@ -284,6 +284,8 @@ extern "C" int vrm_paged_chunk_attention(const void* query, int q_dtype, long lo
   const dim3 grid((unsigned)p.items * (unsigned)KH);
   if (p.wide)
     launch_chunk_f32(a, kind, grid, st);
+  else if (p.dp == 256)
+    launch_chunk16_256(a, kind, grid, st);
   else if (kind == kSrcI8)
     launch_chunk16_i8(a, grid, st);
   else if (kind == kSrcFp8)
