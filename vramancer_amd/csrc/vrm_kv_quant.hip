@@ -115,40 +115,6 @@ __global__ void __launch_bounds__(64) quant_i8_kernel(QuantArgs a) {
 // 87 us (4.6 TB/s), fp8 350 -> 82.
 // ---------------------------------------------------------------------------
 
-// Codes of 8 elements, little end first.  v_cvt_pk_fp8_f32 gives
-// vrm_e4m3::encode's code for every float up to 464 in magnitude (all of them
-// compared) but not for NaN, whose codes are the only ones with seven low bits
-// set: those lanes take the general path.
-template <bool FP8>
-__device__ __forceinline__ void codes8(const float (&x)[8], float scale, uint32_t& lo, uint32_t& hi) {
-  bool slow = !fast_scale(scale);
-  if (!slow) {
-    const float y = __fdiv_rn(1.f, scale);
-    if constexpr (FP8) {
-      float q[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) q[i] = copysignf(div_by(x[i], scale, y), x[i]);  // -0 stays -0
-      int a = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);
-      a = __builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], a, true);
-      int b = __builtin_amdgcn_cvt_pk_fp8_f32(q[4], q[5], 0, false);
-      b = __builtin_amdgcn_cvt_pk_fp8_f32(q[6], q[7], b, true);
-      lo = (uint32_t)a;
-      hi = (uint32_t)b;
-      slow = ((((~lo & 0x7f7f7f7fu) - 0x01010101u) | ((~hi & 0x7f7f7f7fu) - 0x01010101u)) & 0x80808080u) != 0;
-    } else {
-      lo = int8_codes4(x, scale, y);
-      hi = int8_codes4(x + 4, scale, y);
-    }
-  }
-  if (slow) {
-    uint32_t c[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) c[i] = FP8 ? fp8_code(x[i], scale) : (uint8_t)int8_code(x[i], scale);
-    lo = pack4(c[0], c[1], c[2], c[3]);
-    hi = pack4(c[4], c[5], c[6], c[7]);
-  }
-}
-
 // First dims of a lane's two runs of four: 16-bit sources 8 c and 8 c + 4 (one
 // 16-byte load), 32-bit ones 4 c and D / 2 + 4 c (two loads, each contiguous
 // over the 16 lanes: 20 us against 33 us with adjacent ones at 512 pages).

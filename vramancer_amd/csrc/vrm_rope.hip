@@ -12,13 +12,17 @@
 // Bound: memory; each row is read and written once.  Rows (a token's query,
 // key or value head) go to groups of lanes: a lane holds two 8-element pieces
 // chosen so that both members of a pair are in it, a head of 128 takes 8
-// lanes, and the sum of squares three DPP steps.  Rows whose sizes or
-// alignment do not allow 16-byte accesses take a wavefront each.
-// Quantized pools: a workgroup takes the new tokens of one page, K or V and
-// kv-head: their rows are laid into LDS (16 tokens at a time) and leave as
-// whole dwords of codes, K token-major, V four tokens of a dim to a dword; an
-// fp8 page's scale needs its tokens' maximum first.
+// lanes, and the sum of squares three DPP steps.  A group takes up to
+// kRopeHeads heads of a token, whose cosines, sines and weights it loads once.
+// Rows whose sizes or alignment do not allow 16-byte accesses take a wavefront
+// each.
+// Quantized pools: a workgroup takes the new tokens of one page, K or V, and
+// two kv-heads: their rows are laid into LDS (16 tokens at a time) and leave
+// as whole dwords of codes, K token-major, V four tokens of a dim to a dword;
+// an fp8 page's scale needs its tokens' maximum first.
 #include <math.h>
+
+#include <type_traits>
 
 #include "vrm_kv_codes.h"
 
@@ -26,7 +30,9 @@ namespace vrm {
 namespace {
 
 constexpr int kRopeThreads = 256;
-constexpr int kRopeTokens = 16;  // rows in LDS at a time
+constexpr int kRopeTokens = 16;  // of a page in LDS at a time
+constexpr int kRopeHeads = 4;    // of a token to a group of lanes
+constexpr int kPageHeads = 2;    // of a page to a workgroup
 
 struct RopeArgs {
   const void *q, *k, *v;
@@ -48,8 +54,11 @@ struct RopeArgs {
   int kv_dtype, fp8;
   const int32_t *table, *lens, *cu;
   int B, PS, P, max_pp;
-  int heads;       // rows per token of the row workgroups: H, KH, KH as far as they take part
-  int row_blocks;  // workgroups of rows; page workgroups follow
+  int q_units, kv_units;  // groups' shares of a token's queries, and of its keys (and of its values)
+  int units;              // of a token: q_units, kv_units, kv_units as far as they take part
+  uint32_t units_mul;     // n / units = (t + ((n - t) >> 1)) >> units_shift, t = high half of n units_mul
+  int units_shift;
+  int row_blocks;         // workgroups of rows; page workgroups follow
 };
 
 template <int T>
@@ -146,6 +155,13 @@ __device__ __forceinline__ int page_at(const RopeArgs& a, int b, int pos) {
   return p >= 0 && p < a.P ? p : -1;
 }
 
+// n / units for n < 2^31 (Granlund and Montgomery 1994).
+__device__ __forceinline__ uint32_t div_units(const RopeArgs& a, uint32_t n) {
+  if (a.units == 1) return n;
+  const uint32_t t = __umulhi(n, a.units_mul);
+  return (t + ((n - t) >> 1)) >> a.units_shift;
+}
+
 // First dims of the two pieces of lane l (of D / 16) of a row, and whether
 // they are rotated: both members of every pair are in the lane.
 struct Pieces {
@@ -160,30 +176,52 @@ __device__ __forceinline__ Pieces pieces(const RopeArgs& a, int l) {
   return {d, d + 8, false};
 }
 
-// Norm (w != NULL) and rotation of one row held by LG lanes, lane l with the
-// pieces x, y; lanes l >= D / 16 hold zeros.
+// What a lane needs of the weights and of a position's angles.
+struct Lane {
+  Pieces p;
+  bool on;  // lanes l >= D / 16 hold zeros
+  float wx[8], wy[8], c[8], s[8];
+};
+__device__ __forceinline__ void load_weights(const RopeArgs& a, const void* w, Lane& n) {
+  if (!w || !n.on) return;
+  const auto both = [&](auto type) {
+    load8<decltype(type)::value>(w, n.p.a, n.wx);
+    load8<decltype(type)::value>(w, n.p.b, n.wy);
+  };
+  if (a.w_type == VRM_SRC_F32)
+    both(std::integral_constant<int, VRM_SRC_F32>{});
+  else if (a.w_type == VRM_SRC_F16)
+    both(std::integral_constant<int, VRM_SRC_F16>{});
+  else
+    both(std::integral_constant<int, VRM_SRC_BF16>{});
+}
+__device__ __forceinline__ void load_angles(const RopeArgs& a, long long angle, int l, Lane& n) {
+  if (!n.p.turn || !n.on) return;
+  load8<VRM_SRC_F32>(a.cos_sin, angle * a.rot + 8 * l, n.c);
+  load8<VRM_SRC_F32>(a.cos_sin, angle * a.rot + (a.rot >> 1) + 8 * l, n.s);
+}
+
+// Norm (w != NULL) and rotation of one row held by LG lanes, a lane with the
+// pieces x, y.
 template <int LG>
-__device__ __forceinline__ void norm_turn(const RopeArgs& a, const void* w, bool turn, long long angle, const Pieces& p,
-                                          int l, float (&x)[8], float (&y)[8]) {
-  const bool on = 16 * l < a.D;
-  if (w) {
+__device__ __forceinline__ void norm_turn(const RopeArgs& a, bool norm, bool turn, const Lane& n, float (&x)[8],
+                                          float (&y)[8]) {
+  if (norm) {
     float s = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) s += x[i] * x[i] + y[i] * y[i];
     s = group_sum<LG>(s);
     const float inv = 1.f / sqrtf(s / (float)a.D + a.eps);
-    if (on) {
+    if (n.on) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        x[i] *= inv * load1(w, p.a + i, a.w_type);
-        y[i] *= inv * load1(w, p.b + i, a.w_type);
+        x[i] *= inv * n.wx[i];
+        y[i] *= inv * n.wy[i];
       }
     }
   }
-  if (!turn || !p.turn || !on) return;
-  float c[8], s[8];
-  load8<VRM_SRC_F32>(a.cos_sin, angle * a.rot + 8 * l, c);
-  load8<VRM_SRC_F32>(a.cos_sin, angle * a.rot + (a.rot >> 1) + 8 * l, s);
+  if (!turn || !n.p.turn || !n.on) return;
+  const float *c = n.c, *s = n.s;
   if (a.interleaved) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -226,80 +264,105 @@ __device__ __forceinline__ float turned(const RopeArgs& a, bool turn, long long 
   return second ? y * c + x * s : x * c - y * s;
 }
 
-// What row hh of a token is: its source, weight, and where it goes.
-struct Row {
-  const void* src;
-  const void* w;
-  long long from;
-  int what;  // 0 query, 1 key, 2 value
-  int head;
-};
-__device__ __forceinline__ Row row_of(const RopeArgs& a, int n, int hh) {
-  if (hh < a.H) return {a.q, a.qw, n * a.q_n + hh * a.q_h, 0, hh};
-  hh -= a.H;
-  if (hh < a.KH) return {a.k, a.kw, n * a.k_n + hh * a.k_h, 1, hh};
-  hh -= a.KH;
-  return {a.v, nullptr, n * a.v_n + hh * a.v_h, 2, hh};
-}
-
-// One row of the row workgroups.  GROUP: lanes per row (64: the general path).
+// One unit of the row workgroups: up to kRopeHeads heads of a token, by LG
+// lanes (64: the general path, a row at a time).
 template <int T, int LG, bool GENERAL>
-__device__ void do_row(const RopeArgs& a, long long r, float* lds) {
-  const int n = (int)(r / a.heads), hh = (int)(r % a.heads);
+__device__ __forceinline__ void do_unit(const RopeArgs& a, uint32_t unit, float* lds) {
+  const int n = (int)div_units(a, unit);
+  int u = (int)(unit - (uint32_t)n * a.units);
   Token t;
   if (!locate(a, n, t)) return;
-  const Row row = row_of(a, n, hh);
+  const int what = u < a.q_units ? 0 : u < a.q_units + a.kv_units ? 1 : 2;  // query, key, value
+  u -= what == 0 ? 0 : what == 1 ? a.q_units : a.q_units + a.kv_units;
+  const int head0 = u * kRopeHeads, heads = min(kRopeHeads, (what == 0 ? a.H : a.KH) - head0);
   const bool ok = in_table(a, t);
-  // destination
+  // (three branches: selects between the argument struct's fields would copy
+  // it to scratch memory)
+  const void *src, *w = nullptr;
+  long long step, row;
+  if (what == 0) {
+    src = a.q, w = a.qw, step = a.q_h, row = a.q_n;
+  } else if (what == 1) {
+    src = a.k, w = a.kw, step = a.k_h, row = a.k_n;
+  } else {
+    src = a.v, step = a.v_h, row = a.v_n;
+  }
+  const long long from = n * row + head0 * step;
+  // destination of head0, in elements of `type`, and from a head to the next
   void* dst;
-  long long at;
-  int type;
-  if (row.what == 0) {
-    dst = a.q_out, at = ((long long)n * a.H + row.head) * a.D, type = T;
+  long long at, next = a.D;
+  int type = T;
+  if (what == 0) {
+    dst = a.q_out, at = ((long long)n * a.H + head0) * a.D;
   } else if (!a.pool) {
-    dst = a.k_out, at = ((long long)n * a.KH + row.head) * a.D, type = T;
+    dst = a.k_out, at = ((long long)n * a.KH + head0) * a.D;
   } else {
     const int page = page_at(a, t.b, t.pos);
     if (page < 0 || !ok) return;
-    const int size = a.kv_dtype == VRM_KV_F32 ? 4 : 2;
-    dst = a.pool + a.layer_off + (long long)page * a.g.page + (long long)row.head * a.g.head +
-          (row.what == 2 ? a.g.kv : 0) + (long long)(t.pos % a.PS) * a.D * size;
-    at = 0, type = a.kv_dtype;
+    type = a.kv_dtype;
+    dst = a.pool + a.layer_off + (long long)page * a.g.page + (what == 2 ? a.g.kv : 0);
+    next = (long long)a.PS * a.D;
+    at = head0 * next + (long long)(t.pos % a.PS) * a.D;
   }
-  const bool turn = a.cos_sin && row.what < 2 && ok;
+  const bool turn = a.cos_sin && what < 2 && ok;
   // a position outside the table has no rotation: such rows are made NaN
   const float spoil = ok ? 0.f : __uint_as_float(0x7fc00000u);
   if constexpr (GENERAL) {
     const int lane = threadIdx.x & 63;
-    for (int d = lane; d < a.D; d += kWave) lds[d] = load1(row.src, row.from + d, T);
-    __syncwarp();
-    norm_row(a, row.w, lds);
-    for (int d = lane; d < a.D; d += kWave) store1(dst, at + d, type, turned(a, turn, t.angle, lds, d) + spoil);
+    for (int h = 0; h < heads; ++h) {
+      for (int d = lane; d < a.D; d += kWave) lds[d] = load1(src, from + h * step + d, T);
+      __syncwarp();
+      norm_row(a, w, lds);
+      for (int d = lane; d < a.D; d += kWave)
+        store1(dst, at + h * next + d, type, turned(a, turn, t.angle, lds, d) + spoil);
+      __syncwarp();
+    }
   } else {
     const int l = threadIdx.x & (LG - 1);
-    const Pieces p = pieces(a, l);
-    float x[8] = {}, y[8] = {};
-    if (16 * l < a.D) {
-      load8<T>(row.src, row.from + p.a, x);
-      load8<T>(row.src, row.from + p.b, y);
-    }
-    norm_turn<LG>(a, row.w, turn, t.angle, p, l, x, y);
-    if (!ok)
+    Lane ln;
+    ln.p = pieces(a, l);
+    ln.on = 16 * l < a.D;
+    float x[kRopeHeads][8], y[kRopeHeads][8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = y[i] = spoil;
-    if (16 * l < a.D) {
-      store8(dst, at + p.a, type, x);
-      store8(dst, at + p.b, type, y);
+    for (int h = 0; h < kRopeHeads; ++h) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[h][i] = y[h][i] = 0.f;
+      if (ln.on && h < heads) {
+        load8<T>(src, from + h * step + ln.p.a, x[h]);
+        load8<T>(src, from + h * step + ln.p.b, y[h]);
+      }
+    }
+    load_weights(a, w, ln);
+    if (turn) load_angles(a, t.angle, l, ln);
+#pragma unroll
+    for (int h = 0; h < kRopeHeads; ++h) {
+      norm_turn<LG>(a, w, turn, ln, x[h], y[h]);
+      if (!ok)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[h][i] = y[h][i] = spoil;
+      if (ln.on && h < heads) {
+        store8(dst, at + h * next + ln.p.a, type, x[h]);
+        store8(dst, at + h * next + ln.p.b, type, y[h]);
+      }
     }
   }
 }
 
-// The new tokens of one page of a quantized pool, K or V, one kv-head.
+// The new tokens of one page of a quantized pool, K or V, kPageHeads kv-heads.
 // Sequence b owns virtual pages cu[b] / PS + 2 b .. of the launch: at least as
 // many as its tokens can touch, known without the lengths before it.
+constexpr int kPageRows = kRopeTokens * kPageHeads;
+struct PageShared {
+  float rows[kPageRows][256 + 4];
+  float max[kPageRows];               // of a row's magnitudes
+  float scale[kPageRows], inv[kPageRows];
+  int ok[kPageRows];                  // whether it is a new token
+};
+
 template <int T, int LG, bool GENERAL>
-__device__ void do_page(const RopeArgs& a, int block, float (*rows)[256 + 4], float* row_max, int* row_ok) {
-  const int vpage = block / (2 * a.KH), kv = block / a.KH % 2, head = block % a.KH;
+__device__ __forceinline__ void do_page(const RopeArgs& a, int block, PageShared& sh) {
+  const int pairs = (a.KH + kPageHeads - 1) / kPageHeads;
+  const int vpage = block / (2 * pairs), kv = block / pairs % 2, head0 = block % pairs * kPageHeads;
   const auto vfirst = [&](int b) { return clamp_int(a.cu[b], 0, a.N) / a.PS + 2 * b; };
   int lo = 0, hi = a.B - 1;
   while (lo < hi) {
@@ -313,95 +376,124 @@ __device__ void do_page(const RopeArgs& a, int block, float (*rows)[256 + 4], fl
   if (c1 <= c0 || j < 0) return;
   const int len = a.lens[lo], start = len - (c1 - c0), from = max(start, 0);
   const int pi = from / a.PS + j;
+  if (pi >= a.max_pp) return;
   const int page_pos = pi * a.PS;
-  if (pi >= a.max_pp || page_pos >= len) return;
+  if (page_pos >= len) return;
   const int pid = page_at(a, lo, page_pos);
   if (pid < 0) return;
-  const int s0 = max(from, page_pos) - page_pos, s1 = min(len, page_pos + a.PS) - page_pos;  // its new slots
+  const int s0 = max(from, page_pos) - page_pos, s1 = min(len - page_pos, a.PS);  // its new slots
   if (s0 >= s1) return;
-  uint8_t* dst = a.pool + a.layer_off + (long long)pid * a.g.page + (long long)head * a.g.head + (kv ? a.g.kv : 0);
-  float* sc = a.scales + a.s_layer_off + (long long)pid * a.g.s_page + (long long)head * a.g.s_head + (kv ? a.g.s_kv : 0);
+  const int heads = min(kPageHeads, a.KH - head0);
+  uint8_t* const dst0 = a.pool + a.layer_off + (long long)pid * a.g.page + (long long)head0 * a.g.head + (kv ? a.g.kv : 0);
+  float* const sc0 =
+      a.scales + a.s_layer_off + (long long)pid * a.g.s_page + (long long)head0 * a.g.s_head + (kv ? a.g.s_kv : 0);
   const int tid = threadIdx.x, lane = tid & 63;
   const int D = a.D;
+  const void *src, *w = nullptr;
+  long long src_n, src_h;
+  if (kv) {
+    src = a.v, src_n = a.v_n, src_h = a.v_h;
+  } else {
+    src = a.k, w = a.kw, src_n = a.k_n, src_h = a.k_h;
+  }
+  const bool turn = a.cos_sin && kv == 0;
 
-  // rows of slots c .. c + 15 into LDS, with their maxima; -1: not a new token
+  // rows of slots c .. c + 15 (row i: slot c + i % 16 of head i / 16) into LDS
   const auto fill = [&](int c) {
     constexpr int kLanes = GENERAL ? 64 : LG;
-    for (int i = tid / kLanes; i < kRopeTokens; i += kRopeThreads / kLanes) {
-      const int slot = c + i;
+    Lane ln;
+    if constexpr (!GENERAL) {
+      ln.p = pieces(a, tid & (LG - 1));
+      ln.on = 16 * (tid & (LG - 1)) < D;
+      load_weights(a, w, ln);
+    }
+    for (int i = tid / kLanes; i < kPageRows; i += kRopeThreads / kLanes) {
+      const int slot = c + i % kRopeTokens, h = i / kRopeTokens;
       const int n = c0 + page_pos + slot - start;
-      bool ok = slot >= s0 && slot < s1;
+      bool ok = slot >= s0 && slot < s1 && h < heads;
       Token t;
       t.b = lo, t.pos = page_pos + slot, t.angle = t.pos;
       if (ok && a.positions)
         t.angle =
             a.pos_bytes == 8 ? static_cast<const long long*>(a.positions)[n] : static_cast<const int32_t*>(a.positions)[n];
       ok = ok && in_table(a, t);
-      const Row row = row_of(a, ok ? n : c0, a.H + kv * a.KH + head);
-      const bool turn = a.cos_sin && kv == 0;
+      const long long at = n * src_n + (head0 + h) * src_h;
       float big = 0.f;
       if constexpr (GENERAL) {
-        for (int d = lane; d < D; d += kWave) rows[i][d] = ok ? load1(row.src, row.from + d, T) : 0.f;
+        float* const row = sh.rows[i];
+        for (int d = lane; d < D; d += kWave) row[d] = ok ? load1(src, at + d, T) : 0.f;
         __syncwarp();
-        if (ok) norm_row(a, row.w, rows[i]);
+        if (ok) norm_row(a, w, row);
         float z[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int d = lane + 64 * e;
-          z[e] = d < D ? turned(a, turn && ok, t.angle, rows[i], d) : 0.f;
+          z[e] = d < D ? turned(a, turn && ok, t.angle, row, d) : 0.f;
           big = fmaxf(big, fabsf(z[e]));
         }
         __syncwarp();
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if (lane + 64 * e < D) rows[i][lane + 64 * e] = z[e];
+          if (lane + 64 * e < D) row[lane + 64 * e] = z[e];
         big = group_max<64>(big);
       } else {
-        const int l = tid & (LG - 1);
-        const Pieces p = pieces(a, l);
         float x[8] = {}, y[8] = {};
-        if (ok && 16 * l < D) {
-          load8<T>(row.src, row.from + p.a, x);
-          load8<T>(row.src, row.from + p.b, y);
+        if (ok && ln.on) {
+          load8<T>(src, at + ln.p.a, x);
+          load8<T>(src, at + ln.p.b, y);
         }
-        norm_turn<LG>(a, row.w, turn && ok, t.angle, p, l, x, y);
-        if (16 * l < D) {
+        if (turn && ok) load_angles(a, t.angle, tid & (LG - 1), ln);
+        norm_turn<LG>(a, w, turn && ok, ln, x, y);
+        if (ln.on) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            big = fmaxf(big, fmaxf(fabsf(x[e]), fabsf(y[e])));
-            rows[i][p.a + e] = x[e];
-            rows[i][p.b + e] = y[e];
-          }
+          for (int e = 0; e < 8; ++e) big = fmaxf(big, fmaxf(fabsf(x[e]), fabsf(y[e])));
+          float4* const fx = reinterpret_cast<float4*>(&sh.rows[i][ln.p.a]);
+          float4* const fy = reinterpret_cast<float4*>(&sh.rows[i][ln.p.b]);
+          fx[0] = make_float4(x[0], x[1], x[2], x[3]), fx[1] = make_float4(x[4], x[5], x[6], x[7]);
+          fy[0] = make_float4(y[0], y[1], y[2], y[3]), fy[1] = make_float4(y[4], y[5], y[6], y[7]);
         }
         big = group_max<LG>(big);
       }
       if (tid % kLanes == 0) {
-        row_max[i] = big;
-        row_ok[i] = ok;
+        sh.max[i] = big;
+        sh.ok[i] = ok;
+        if (!a.fp8) {
+          const float s = __fdiv_rn(big, 127.f);
+          sh.scale[i] = s;
+          sh.inv[i] = __fdiv_rn(1.f, s);
+        }
       }
     }
   };
 
   const int c_first = s0 / kRopeTokens * kRopeTokens;
   const bool once = c_first + kRopeTokens >= s1;
-  float scale = 0.f;
+  float scale[kPageHeads] = {}, inv[kPageHeads] = {};
   if (a.fp8) {
-    const float old = s0 > 0 ? *sc : 0.f;
-    float big = 0.f;
+    float old[kPageHeads], big[kPageHeads] = {};
+#pragma unroll
+    for (int h = 0; h < kPageHeads; ++h) old[h] = h < heads && s0 > 0 ? sc0[h * a.g.s_head] : 0.f;
     for (int c = c_first; c < s1; c += kRopeTokens) {
       __syncthreads();
       fill(c);
       __syncthreads();
-      big = fmaxf(big, group_max<16>(row_max[lane & 15]));
+#pragma unroll
+      for (int h = 0; h < kPageHeads; ++h) big[h] = fmaxf(big[h], group_max<16>(sh.max[h * kRopeTokens + (lane & 15)]));
     }
-    scale = fmaxf(old, __fdiv_rn(big, 448.f));
-    __syncthreads();  // every thread has the old scale
-    if (tid == 0) *sc = scale;
-    if (s0 > 0 && scale > old) {  // the page's earlier codes against the new scale
-      for (int i = tid; i < s0 * D; i += kRopeThreads) {
-        const int t = i / D, d = i % D;
-        uint8_t* p = dst + (kv ? (((t >> 2) * 16 + (d & 15)) * (D >> 4) + (d >> 4)) * 4 + (t & 3) : t * D + d);
-        *p = fp8_code(e4m3fn_to_f32(*p) * old, scale);
+    __syncthreads();  // every thread has the old scales
+#pragma unroll
+    for (int h = 0; h < kPageHeads; ++h) {
+      scale[h] = fmaxf(old[h], __fdiv_rn(big[h], 448.f));
+      inv[h] = __fdiv_rn(1.f, scale[h]);
+      if (h >= heads) break;
+      if (tid == 0) sc0[h * a.g.s_head] = scale[h];
+      if (s0 > 0 && scale[h] > old[h]) {  // the page's earlier codes against the new scale
+        uint8_t* const dst = dst0 + h * a.g.head;
+        for (int i = tid; i < s0 * D; i += kRopeThreads) {
+          const int t = i / D, d = i % D;
+          uint8_t* p = dst + (kv ? (((t >> 2) * 16 + (d & 15)) * (D >> 4) + (d >> 4)) * 4 + (t & 3) : t * D + d);
+          *p = fp8_code(e4m3fn_to_f32(*p) * old[h], scale[h]);
+        }
       }
     }
   }
@@ -411,30 +503,64 @@ __device__ void do_page(const RopeArgs& a, int block, float (*rows)[256 + 4], fl
       fill(c);
       __syncthreads();
     }
-    const auto code = [&](int i, int d) -> uint32_t {
-      if (a.fp8) return fp8_code(rows[i][d], scale);
-      return (uint8_t)int8_code(rows[i][d], __fdiv_rn(row_max[i], 127.f));
-    };
-    if (!a.fp8 && tid < kRopeTokens && row_ok[tid]) sc[c + tid] = __fdiv_rn(row_max[tid], 127.f);
-    for (int i = tid; i < kRopeTokens * D / 4; i += kRopeThreads) {
-      if (kv == 0) {
-        const int t = i / (D / 4), d = i % (D / 4) * 4;
-        if (!row_ok[t]) continue;
-        *reinterpret_cast<uint32_t*>(dst + (long long)(c + t) * D + d) =
-            pack4(code(t, d), code(t, d + 1), code(t, d + 2), code(t, d + 3));
-      } else {
-        const int t = i / D * 4, w = i % D;
-        const int d = w / (D >> 4) + 16 * (w % (D >> 4));
-        uint8_t* p = dst + (long long)(c + t) * D + w * 4;
-        const int have = row_ok[t] | row_ok[t + 1] << 1 | row_ok[t + 2] << 2 | row_ok[t + 3] << 3;
-        if (!have) continue;
-        const uint32_t word = pack4(code(t, d), code(t + 1, d), code(t + 2, d), code(t + 3, d));
-        if (have == 15) {
-          *reinterpret_cast<uint32_t*>(p) = word;
-        } else {
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (have >> e & 1) p[e] = (uint8_t)(word >> (8 * e));
+    for (int h = 0; h < kPageHeads; ++h) {
+      if (h >= heads) break;
+      const int r0 = h * kRopeTokens;
+      uint8_t* const dst = dst0 + h * a.g.head + (long long)c * D;
+      float* const sc = sc0 + h * a.g.s_head;
+      if (!a.fp8 && tid < kRopeTokens && sh.ok[r0 + tid]) sc[c + tid] = sh.scale[r0 + tid];
+      // four codes of (row, dim) .. with their scales
+      const auto codes = [&](const float (&x)[4], const float (&s)[4], const float (&y)[4]) -> uint32_t {
+        const bool quick = fast_scale(s[0]) && fast_scale(s[1]) && fast_scale(s[2]) && fast_scale(s[3]);
+        if (quick) {
+          float q[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) q[e] = div_by(x[e], s[e], y[e]);
+          if (a.fp8) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) q[e] = copysignf(q[e], x[e]);  // -0 stays -0
+            int k = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);
+            k = __builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], k, true);
+            // a NaN's code (seven low bits set): the general path
+            if (((~(uint32_t)k & 0x7f7f7f7fu) - 0x01010101u & 0x80808080u) == 0) return (uint32_t)k;
+          } else {
+            uint32_t k[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              k[e] = __float_as_uint(__fadd_rn(fminf(fmaxf(q[e], -127.f), 127.f), 12582912.f)) & 0xffu;
+            return pack4(k[0], k[1], k[2], k[3]);
+          }
+        }
+        uint32_t k[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) k[e] = a.fp8 ? fp8_code(x[e], s[e]) : (uint8_t)int8_code(x[e], s[e]);
+        return pack4(k[0], k[1], k[2], k[3]);
+      };
+      for (int i = tid; i < kRopeTokens * D / 4; i += kRopeThreads) {
+        if (kv == 0) {
+          const int t = i / (D / 4), d = i % (D / 4) * 4, r = r0 + t;
+          if (!sh.ok[r]) continue;
+          const float4 f = *reinterpret_cast<const float4*>(&sh.rows[r][d]);
+          const float s = a.fp8 ? scale[h] : sh.scale[r], y = a.fp8 ? inv[h] : sh.inv[r];
+          *reinterpret_cast<uint32_t*>(dst + (long long)t * D + d) = codes({f.x, f.y, f.z, f.w}, {s, s, s, s}, {y, y, y, y});
+        } else {
+          const int t = i / D * 4, x = i % D, r = r0 + t;
+          const int d = x / (D >> 4) + 16 * (x % (D >> 4));
+          const int have = sh.ok[r] | sh.ok[r + 1] << 1 | sh.ok[r + 2] << 2 | sh.ok[r + 3] << 3;
+          if (!have) continue;
+          float s[4], y[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[e] = a.fp8 ? scale[h] : sh.scale[r + e], y[e] = a.fp8 ? inv[h] : sh.inv[r + e];
+          const uint32_t word = codes({sh.rows[r][d], sh.rows[r + 1][d], sh.rows[r + 2][d], sh.rows[r + 3][d]}, s, y);
+          uint8_t* const p = dst + (long long)t * D + x * 4;
+          if (have == 15) {
+            *reinterpret_cast<uint32_t*>(p) = word;
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (have >> e & 1) p[e] = (uint8_t)(word >> (8 * e));
+          }
         }
       }
     }
@@ -443,26 +569,35 @@ __device__ void do_page(const RopeArgs& a, int block, float (*rows)[256 + 4], fl
 
 template <int T, int LG, bool GENERAL, bool QUANT>
 __global__ void __launch_bounds__(kRopeThreads) rope_kernel(RopeArgs a) {
-  __shared__ __align__(16) float rows[QUANT ? kRopeTokens : 4][256 + 4];
-  if ((int)blockIdx.x < a.row_blocks) {
-    constexpr int kPer = GENERAL ? 4 : kRopeThreads / LG;
-    const long long r = (long long)blockIdx.x * kPer + threadIdx.x / (GENERAL ? 64 : LG);
-    if (r < (long long)a.N * a.heads) do_row<T, LG, GENERAL>(a, r, rows[GENERAL ? threadIdx.x / 64 : 0]);
-    return;
-  }
   if constexpr (QUANT) {
-    __shared__ float row_max[kRopeTokens];
-    __shared__ int row_ok[kRopeTokens];
-    do_page<T, LG, GENERAL>(a, blockIdx.x - a.row_blocks, rows, row_max, row_ok);
+    if ((int)blockIdx.x >= a.row_blocks) {
+      __shared__ __align__(16) PageShared sh;
+      do_page<T, LG, GENERAL>(a, blockIdx.x - a.row_blocks, sh);
+      return;
+    }
   }
+  constexpr int kLanes = GENERAL ? 64 : LG;
+  __shared__ float row[GENERAL ? 4 : 1][GENERAL ? 256 : 1];
+  const uint32_t unit = blockIdx.x * (kRopeThreads / kLanes) + threadIdx.x / kLanes;
+  if (unit < (uint32_t)a.N * a.units) do_unit<T, LG, GENERAL>(a, unit, row[GENERAL ? threadIdx.x / 64 : 0]);
 }
 
 template <int T, bool QUANT>
 void launch_rope(RopeArgs& a, bool fast, hipStream_t st) {
   const int lg = !fast ? 64 : a.D <= 64 ? 4 : a.D <= 128 ? 8 : 16;
   const long long per = kRopeThreads / lg;
-  a.row_blocks = (int)(((long long)a.N * a.heads + per - 1) / per);
-  const long long pages = QUANT ? ((long long)a.N / a.PS + 2LL * a.B) * 2 * a.KH : 0;
+  a.q_units = (a.H + kRopeHeads - 1) / kRopeHeads;
+  a.kv_units = (a.KH + kRopeHeads - 1) / kRopeHeads;
+  a.units = QUANT ? a.q_units : a.q_units + a.kv_units * (a.pool ? 2 : 1);
+  a.units_shift = 0;
+  while ((1LL << a.units_shift) < a.units) ++a.units_shift;
+  if (a.units > 1) {
+    a.units_mul = (uint32_t)(((1ULL << 32) * ((1ULL << a.units_shift) - a.units)) / a.units + 1);
+    --a.units_shift;
+  }
+  a.row_blocks = (int)(((long long)a.N * a.units + per - 1) / per);
+  const long long pages =
+      QUANT ? ((long long)a.N / a.PS + 2LL * a.B) * 2 * ((a.KH + kPageHeads - 1) / kPageHeads) : 0;
   const dim3 grid((unsigned)(a.row_blocks + pages)), block(kRopeThreads);
   if (grid.x == 0) return;
   if (lg == 64)
@@ -511,7 +646,7 @@ int check_rope(int src_dtype, const float* cos_sin, int rot, int top, const void
 bool rope_fast(const RopeArgs& a, int src_dtype) {
   const int per16 = src_dtype == VRM_SRC_F32 ? 4 : 8;
   const auto rows = [&](const void* p, long long n, long long h) { return on16(p) && n % per16 == 0 && h % per16 == 0; };
-  if (a.D % 16 || a.rot % 16 || !on16(a.cos_sin)) return false;
+  if (a.D % 16 || a.rot % 16 || !on16(a.cos_sin) || !on16(a.qw) || !on16(a.kw)) return false;
   if (a.H && (!rows(a.q, a.q_n, a.q_h) || !on16(a.q_out))) return false;
   if (a.KH && (!rows(a.k, a.k_n, a.k_h) || !on16(a.k_out))) return false;
   if (a.pool && (!rows(a.v, a.v_n, a.v_h) || !on16(a.pool))) return false;
@@ -563,7 +698,6 @@ extern "C" int vrm_qk_norm_rope(const void* query, long long q_token_stride, lon
   a.positions = cos_sin ? positions : nullptr, a.pos_bytes = position_bytes;
   a.qw = q_weight, a.kw = k_weight, a.w_type = weight_dtype, a.eps = eps;
   a.N = N, a.H = H, a.KH = KH, a.D = D;
-  a.heads = H + KH;
   return run_rope<false>(a, src_dtype, reinterpret_cast<hipStream_t>(stream), who);
 }
 
@@ -650,7 +784,6 @@ extern "C" int vrm_rope_append(const void* query, long long q_token_stride, long
   a.fp8 = kv_dtype == VRM_KV_FP8E4M3 || kv_dtype == VRM_KV_FP8E4M3_INLINE;
   a.table = page_table, a.lens = context_lens, a.cu = cu_seqlens;
   a.B = B, a.PS = PS, a.P = P, a.max_pp = max_pp;
-  a.heads = quant ? H : H + 2 * KH;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   return quant ? run_rope<true>(a, src_dtype, st, who) : run_rope<false>(a, src_dtype, st, who);
 }
