@@ -25,6 +25,10 @@ Device side, in this library's kernels:
   (``vrm_turboquant_score`` + ``vrm_topk_attend``, :1384-1400);
 * ``compress_page_bulk`` compresses a page's raw K/V for every layer that has
   no codes yet (``vrm_tq_compress_pool``);
+* ``append_chunk`` gives the new tokens of a ragged batch their pages (prompts,
+  chunks of prompts, drafted tokens); ``write_chunk`` norms, rotates and writes
+  them (``paged_chunk.rope_append``) and ``compute_attention_chunk`` attends
+  them (``paged_chunk.paged_attention_chunk``), one launch per layer each;
 * ``from_hf_cache`` stores a prefilled Hugging Face cache in a request's
   pages with one ``vrm_kv_write`` launch per layer, ``to_hf_cache`` gathers
   it back; ``try_prefix_cache`` shares full pages of a token prefix between
@@ -53,7 +57,7 @@ import numpy as np
 
 from . import _lib
 
-__all__ = ["PagedKVConfig", "PhysicalPage", "PageTableEntry", "PagedKVCacheManager", "hf_layers"]
+__all__ = ["PagedKVConfig", "PhysicalPage", "PageTableEntry", "ChunkBatch", "PagedKVCacheManager", "hf_layers"]
 
 # Pool element types: name -> (torch dtype name, bytes per element).
 _POOL_DTYPES = {
@@ -147,6 +151,23 @@ class PageTableEntry:
     pages: List[int] = field(default_factory=list)
     num_tokens: int = 0
     created_at: float = field(default_factory=time.time)
+
+
+@dataclass
+class ChunkBatch:
+    """New tokens of an ordered batch of requests (``append_chunk``), as the
+    chunk operators take them; good until one of the requests changes again."""
+
+    request_ids: List[str]
+    counts: List[int]       # new tokens of each request
+    page_table: Any         # [B, pages] int32
+    context_lens: Any       # [B] int32, the new tokens included
+    cu_seqlens: Any         # [B + 1] int32
+    places: List[Tuple[int, int]]  # (page, slot) of every new token, in row order
+
+    @property
+    def num_tokens(self) -> int:
+        return len(self.places)
 
 
 def _is_gpu(device: str) -> bool:
@@ -346,6 +367,64 @@ class PagedKVCacheManager:
         dev = torch.from_numpy(out).to(self._gpu_pool.device)
         return dev[0], dev[1]
 
+    def append_chunk(self, request_ids: Sequence[str], counts: Sequence[int]) -> ChunkBatch:
+        """Places for ``counts[i]`` new tokens of ``request_ids[i]``, pages
+        allocated where needed: the batch that ``write_chunk`` and
+        ``compute_attention_chunk`` take, rows in the order of the ids.
+
+        All or nothing: an unknown id raises ``KeyError``; an id given twice,
+        a negative count, too few free pages, or two requests (forks) whose
+        new tokens go to one shared page raise ``RuntimeError``, and nothing
+        has changed."""
+        import torch
+
+        self._require_pool("append_chunk")
+        ids, counts = list(request_ids), [int(n) for n in counts]
+        if len(counts) != len(ids):
+            raise RuntimeError(f"{len(ids)} request ids but {len(counts)} counts")
+        if len(set(ids)) < len(ids):
+            raise RuntimeError("a request can be in a chunk once only")
+        if any(n < 0 for n in counts):
+            raise RuntimeError(f"counts must not be negative, got {counts}")
+        PS = self.config.page_size
+        with self._lock:
+            entries = [self._page_tables.get(rid) for rid in ids]
+            missing = [rid for rid, e in zip(ids, entries) if e is None]
+            if missing:
+                raise KeyError(f"unknown request ids {missing}")
+            more = [max(0, -(-(e.num_tokens + n) // PS) - len(e.pages)) if n else 0 for e, n in zip(entries, counts)]
+            if sum(more) > len(self._free_pages):
+                raise RuntimeError(f"no page left: {sum(more)} needed, {len(self._free_pages)} free "
+                                   f"(pool of {self.config.max_pages} pages)")
+            # pages that new tokens go to and that are there already
+            tails = [p for e, n in zip(entries, counts) if n
+                     for p in e.pages[e.num_tokens // PS:-(-(e.num_tokens + n) // PS)]]
+            if len(set(tails)) < len(tails):
+                raise RuntimeError("requests that share the page their next token goes to (forks) cannot be in one "
+                                   "chunk")
+            places: List[Tuple[int, int]] = []
+            now = time.time()
+            for e, n, m in zip(entries, counts, more):
+                e.pages.extend(self._alloc_page() for _ in range(m))
+                for t in range(e.num_tokens, e.num_tokens + n):
+                    places.append((e.pages[t // PS], t % PS))
+                for page in e.pages[e.num_tokens // PS:-(-(e.num_tokens + n) // PS)]:
+                    self._pages[page].last_access = now
+                e.num_tokens += n
+            self._peak_usage = max(self._peak_usage, self.config.max_pages - len(self._free_pages))
+            self._epoch += 1
+            width = max([1] + [len(e.pages) for e in entries])
+            B = len(ids)
+            host = np.full(B * (width + 2) + 1, -1, dtype=np.int32)  # table, lengths, offsets: one upload
+            for b, e in enumerate(entries):
+                host[b * width:b * width + len(e.pages)] = e.pages
+                host[B * width + b] = e.num_tokens
+        host[B * (width + 1)] = 0
+        host[B * (width + 1) + 1:] = np.cumsum(counts)
+        dev = torch.from_numpy(host).to(self._gpu_pool.device)
+        return ChunkBatch(ids, counts, dev[:B * width].view(B, width), dev[B * width:B * (width + 1)],
+                          dev[B * (width + 1):], places)
+
     @property
     def gpu_pool(self) -> Any:
         """The device K/V pool, or ``None`` for a host-only manager."""
@@ -504,6 +583,56 @@ class PagedKVCacheManager:
         if self._kv_compressor is not None:
             self._pending_compress.append((layer_idx, page_ids, slots, key, value,
                                            list(host_slots) if host_slots is not None else None))
+
+    def write_chunk(self, layer_idx: int, chunk: ChunkBatch, key: Any, value: Any, query: Any = None,
+                    cos_sin: Any = None, positions: Any = None, q_weight: Any = None, k_weight: Any = None,
+                    eps: float = 1e-6, interleaved: bool = False) -> Any:
+        """Writes a chunk's K/V ([tokens, num_kv_heads, head_dim], any token
+        and head strides) to its places in ``layer_idx``, normed and rotated
+        on the way where weights and a rotation table are given
+        (``paged_chunk.rope_append``).  Returns the queries, treated alike, or
+        ``None`` without.  With TurboQuant compression the rows also wait in
+        the queue that ``flush_compression`` empties, as the pool holds them."""
+        import torch
+
+        from .paged_chunk import rope_append
+
+        self._require_pool("write_chunk")
+        if key.dim() != 3 or key.shape[0] != chunk.num_tokens:
+            raise RuntimeError(f"key must be [{chunk.num_tokens}, {self.config.num_kv_heads}, {self.config.head_dim}], "
+                               f"got shape {tuple(key.shape)}")
+        out = rope_append(query, key, value, self._gpu_pool, chunk.page_table, chunk.context_lens, chunk.cu_seqlens,
+                          layer_idx, cos_sin, kv_scales=self._kv_scales, positions=positions, q_weight=q_weight,
+                          k_weight=k_weight, eps=eps, interleaved=interleaved)
+        if self._kv_compressor is not None and chunk.num_tokens:
+            at = torch.tensor(chunk.places, dtype=torch.int64).t().to(self._gpu_pool.device)
+            rows = self._gpu_pool[at[0], layer_idx, :, :, at[1]]  # [tokens, 2, KH, D]
+            at = at.to(torch.int32)
+            self._pending_compress.append((layer_idx, at[0], at[1], rows[:, 0].contiguous(), rows[:, 1].contiguous(),
+                                           chunk.places))
+        return out
+
+    def compute_attention_chunk(self, query: Any, chunk: ChunkBatch, layer_idx: int, scale: Optional[float] = None,
+                                causal: bool = True, window: Optional[int] = None) -> Any:
+        """Attention of a chunk's tokens over their requests' pages, which hold
+        them already: query [tokens, H, D] -> the same in its dtype
+        (``paged_chunk.paged_attention_chunk``)."""
+        from .paged_chunk import chunk_workspace, paged_attention_chunk
+
+        self._require_pool("compute_attention_chunk")
+        if query.dim() != 3 or query.shape[0] != chunk.num_tokens:
+            raise RuntimeError(f"query must be [{chunk.num_tokens}, H, {self.config.head_dim}], got shape "
+                               f"{tuple(query.shape)}")
+        B, width = chunk.page_table.shape
+        key = ("chunk", tuple(query.shape), query.dtype, B, width, str(query.device))
+        ws = self._workspaces.get(key)
+        if ws is None:
+            if len(self._workspaces) > 8:
+                self._workspaces.clear()
+            ws = self._workspaces[key] = chunk_workspace(query, self._gpu_pool, B, width)
+        return paged_attention_chunk(query, self._gpu_pool, chunk.page_table, chunk.context_lens, chunk.cu_seqlens,
+                                     layer_idx, scale, kv_scales=self._kv_scales, causal=causal, window=window,
+                                     workspace=ws)
 
     def flush_compression(self) -> None:
         """Compresses every queued row, all layers at once, into the TurboQuant

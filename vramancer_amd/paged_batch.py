@@ -29,10 +29,16 @@ request's prompt through the model with an ordinary cache and stores the
 result in its pages (``from_hf_cache``), as the reference batcher does after
 its prefill (:594-597).
 
-Only decode steps (one new token per request) go through the pages; a
-multi-token update of a ``PagedBatchCache`` raises.  Calls of the attention
-function on any other cache attend with PyTorch's SDPA, causal and unmasked
-(prefill one request at a time, as the reference does).
+Only decode steps (one new token per request) go through a
+``PagedBatchCache``; its multi-token update raises.  ``PagedChunkCache`` is its
+form for several tokens per request: the update writes them into their pages
+and the attention function attends them there
+(``PagedKVCacheManager.append_chunk`` and what takes its batch).  ``chunk_step``
+runs one such step, ``prefill_chunked`` a prompt in chunks, which needs neither
+a second copy of the cache nor scores of the whole prompt.
+
+Calls of the attention function on any other cache attend with PyTorch's SDPA,
+causal and unmasked (prefill one request at a time, as the reference does).
 """
 from __future__ import annotations
 
@@ -43,10 +49,10 @@ import numpy as np
 import torch
 from transformers.cache_utils import Cache, CacheLayerMixin
 
-from .paged_attention import PagedKVCacheManager
+from .paged_attention import ChunkBatch, PagedKVCacheManager
 
-__all__ = ["PagedBatchCache", "PagedBatchLayer", "decode_step", "prefill", "paged_attention_forward",
-           "enable_paged_attention", "ATTENTION_NAME"]
+__all__ = ["PagedBatchCache", "PagedBatchLayer", "PagedChunkCache", "PagedChunkLayer", "decode_step", "chunk_step",
+           "prefill", "prefill_chunked", "paged_attention_forward", "enable_paged_attention", "ATTENTION_NAME"]
 
 ATTENTION_NAME = "vramancer_paged"
 
@@ -144,6 +150,52 @@ class PagedBatchCache(Cache):
         return out.to(query.dtype).unsqueeze(1)
 
 
+class PagedChunkLayer(PagedBatchLayer):
+    """One layer of a ``PagedChunkCache``: writes the step's K/V rows, as many
+    per request as the step has tokens, into the manager's pages."""
+
+    def update(self, key_states: torch.Tensor, value_states: torch.Tensor, *args, **kwargs
+               ) -> Tuple[torch.Tensor, torch.Tensor]:
+        if not self.is_initialized:
+            self.lazy_initialization(key_states, value_states)
+        B, _, q, _ = key_states.shape
+        if B != len(self.cache.request_ids):
+            raise RuntimeError(f"batch of {B} rows for {len(self.cache.request_ids)} request ids")
+        if self.layer_idx == 0:
+            self.cache._begin_chunk(q)
+        chunk = self.cache._step_chunk(q)
+        self.cache.manager.write_chunk(self.layer_idx, chunk, key_states.transpose(1, 2).flatten(0, 1),
+                                       value_states.transpose(1, 2).flatten(0, 1))
+        key_states._vrm_paged_batch = (self.cache, self.layer_idx)
+        return key_states, value_states
+
+
+class PagedChunkCache(PagedBatchCache):
+    """``PagedBatchCache`` for steps of several new tokens per request, the
+    same number for every request of the batch."""
+
+    def __init__(self, manager: PagedKVCacheManager, request_ids: Sequence[str]):
+        super().__init__(manager, request_ids)
+        self._chunk: Optional[ChunkBatch] = None
+        self.layers = [PagedChunkLayer(self, i) for i in range(manager.config.num_layers)]
+
+    def _begin_chunk(self, q: int) -> None:
+        self._chunk = self.manager.append_chunk(self.request_ids, [q] * len(self.request_ids))
+
+    def _step_chunk(self, q: int) -> ChunkBatch:
+        if self._chunk is None or any(n != q for n in self._chunk.counts):
+            raise RuntimeError("a step starts with the update of layer 0, and every layer has its tokens")
+        return self._chunk
+
+    def attend(self, query: torch.Tensor, layer_idx: int, scale: float) -> torch.Tensor:
+        """Attention of one layer over the pages: query [B, H, q, D] ->
+        [B, q, H, D] in the query's dtype."""
+        B, H, q, D = query.shape
+        chunk = self._step_chunk(q)
+        out = self.manager.compute_attention_chunk(query.transpose(1, 2).flatten(0, 1), chunk, layer_idx, scale)
+        return out.view(B, q, H, D)
+
+
 def paged_attention_forward(module, query, key, value, attention_mask, dropout: float = 0.0,
                             scaling: Optional[float] = None, **kwargs):
     """Attention function for ``attn_implementation="vramancer_paged"``.
@@ -195,3 +247,38 @@ def prefill(model, manager: PagedKVCacheManager, request_id: str, input_ids: tor
     out = model(input_ids.reshape(1, -1), use_cache=True)
     manager.from_hf_cache(request_id, out.past_key_values)
     return out.logits[:, -1]
+
+
+def chunk_step(model, manager: PagedKVCacheManager, request_ids: Sequence[str], input_ids: torch.Tensor,
+               cache: Optional[PagedChunkCache] = None) -> torch.Tensor:
+    """One forward over q new tokens ``input_ids`` [B, q] of each request, at
+    the positions after those it has (a prompt's chunk, drafted tokens to
+    verify).  Returns the logits [B, q, vocab].  The model must use
+    ``enable_paged_attention``; pass the ``cache`` of the previous step to
+    reuse it."""
+    if cache is None or cache.request_ids != list(request_ids):
+        cache = PagedChunkCache(manager, request_ids)
+    ids = input_ids.reshape(len(request_ids), -1)
+    pos = torch.from_numpy(cache.token_counts()).to(ids.device).reshape(-1, 1)
+    pos = pos + torch.arange(ids.shape[1], device=ids.device)
+    out = model(ids, position_ids=pos, past_key_values=cache, use_cache=True)
+    return out.logits if hasattr(out, "logits") else out[0]
+
+
+def prefill_chunked(model, manager: PagedKVCacheManager, request_id: str, input_ids: torch.Tensor,
+                    chunk_size: int = 2048) -> torch.Tensor:
+    """Runs a request's prompt [1, S] through the model ``chunk_size`` tokens
+    at a time, straight into its pages, after the tokens that it has already
+    (a prefix, an earlier turn).  Returns the last-position logits [1, vocab].
+
+    Unlike ``prefill`` it keeps no second copy of the cache."""
+    if chunk_size < 1:
+        raise RuntimeError(f"chunk_size must be positive, got {chunk_size}")
+    ids = input_ids.reshape(1, -1)
+    if ids.shape[1] == 0:
+        raise RuntimeError("an empty prompt has no logits")
+    manager.allocate(request_id)
+    cache = PagedChunkCache(manager, [request_id])
+    for start in range(0, ids.shape[1], chunk_size):
+        logits = chunk_step(model, manager, [request_id], ids[:, start:start + chunk_size], cache)
+    return logits[:, -1]

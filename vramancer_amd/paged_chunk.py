@@ -30,7 +30,7 @@ from typing import Any, Optional
 import torch
 
 from . import _lib, kv_quant
-from .rope import check_heads, check_out, check_positions, check_table, check_weights, on_device
+from .rope import check_heads, check_out, check_positions, check_table, check_weights, launch, src_code
 
 __all__ = ["rope_append", "paged_attention_chunk", "chunk_workspace"]
 
@@ -46,7 +46,7 @@ def chunk_workspace(query, kv_pool, batch: int, max_pages_per_seq: int):
     (``workspace=``)."""
     N, H, D = query.shape
     KH, PS = kv_pool.shape[3], kv_pool.shape[4]
-    nbytes = _workspace_bytes(N, batch, H, KH, D, PS, max_pages_per_seq, _lib.src_dtype_code(query.dtype),
+    nbytes = _workspace_bytes(N, batch, H, KH, D, PS, max_pages_per_seq, src_code(query.dtype),
                               _lib.kv_dtype_code(kv_pool.dtype))
     return torch.empty(nbytes, dtype=torch.uint8, device=query.device)
 
@@ -131,7 +131,7 @@ def rope_append(
     key = check_heads("key", key, None, None, None)
     N, KH, D = key.shape
     value = check_heads("value", value, N, D, key.dtype)
-    src = _lib.src_dtype_code(key.dtype)
+    src = src_code(key.dtype)
     code = check_pool(kv_pool, kv_scales, D)
     P, L, _, pool_heads, PS, _ = kv_pool.shape
     if KH != pool_heads or value.shape[1] != KH:
@@ -148,14 +148,15 @@ def rope_append(
     if positions is not None:
         positions = check_positions(positions, N)
     q_weight, k_weight, w_code = check_weights(q_weight, k_weight, D)
-    with on_device(key):
-        rc = _lib.load().vrm_rope_append(
-            _lib.ptr(query), query.stride(0) if H else 0, query.stride(1) if H else 0, _lib.ptr(key), key.stride(0),
-            key.stride(1), _lib.ptr(value), value.stride(0), value.stride(1), src, _lib.ptr(cos_sin), rot, top,
-            _lib.ptr(positions), positions.element_size() if positions is not None else 4, _lib.ptr(q_weight),
-            _lib.ptr(k_weight), w_code, float(eps), int(bool(interleaved)), _lib.ptr(query_out), _lib.ptr(kv_pool),
-            _lib.ptr(kv_scales), code, _lib.ptr(page_table), _lib.ptr(context_lens), _lib.ptr(cu_seqlens), N, B, H, KH,
-            D, PS, L, P, page_table.shape[1], int(layer_idx), _lib.stream_of(key))
+    ptr = _lib.ptr
+    q_n, q_h = query.stride()[:2] if H else (0, 0)
+    (k_n, k_h, _), (v_n, v_h, _) = key.stride(), value.stride()
+    rc = launch(key, _lib.load().vrm_rope_append, ptr(query), q_n, q_h, key.data_ptr(), k_n, k_h, value.data_ptr(), v_n,
+                v_h, src, ptr(cos_sin), rot, top, ptr(positions),
+                positions.element_size() if positions is not None else 4, ptr(q_weight), ptr(k_weight), w_code,
+                float(eps), 1 if interleaved else 0, ptr(query_out), kv_pool.data_ptr(), ptr(kv_scales), code,
+                page_table.data_ptr(), context_lens.data_ptr(), cu_seqlens.data_ptr(), N, B, H, KH, D, PS, L, P,
+                page_table.shape[1], int(layer_idx))
     _lib.check(rc, "rope_append")
     return query_out
 
@@ -195,7 +196,7 @@ def paged_attention_chunk(
     if query.dim() != 3:
         raise RuntimeError(f"query must be [N, H, D], got shape {tuple(query.shape)}")
     N, H, D = query.shape
-    q_code = _lib.src_dtype_code(query.dtype)
+    q_code = src_code(query.dtype)
     code = check_pool(kv_pool, kv_scales, D)
     P, L, _, KH, PS, _ = kv_pool.shape
     page_table, context_lens, cu_seqlens, B = check_batch(page_table, context_lens, cu_seqlens)
@@ -204,8 +205,8 @@ def paged_attention_chunk(
     if query.stride(2) != 1 and D > 1:
         query = query.contiguous()
     if out is None:
-        out = torch.empty((N, H, D), dtype=query.dtype, device=query.device)
-    elif tuple(out.shape) != (N, H, D) or out.dtype != query.dtype or not out.is_contiguous():
+        out = torch.empty_like(query, memory_format=torch.contiguous_format)
+    elif out.shape != query.shape or out.dtype != query.dtype or not out.is_contiguous():
         raise RuntimeError(f"out must be a contiguous {query.dtype} [{N}, {H}, {D}] tensor, got {out.dtype} "
                            f"{tuple(out.shape)}")
     if lse is not None and (tuple(lse.shape) != (N, H) or lse.dtype != torch.float32 or not lse.is_contiguous()):
@@ -218,12 +219,11 @@ def paged_attention_chunk(
     elif not workspace.is_contiguous():
         raise RuntimeError("workspace must be contiguous")
     ws_bytes = workspace.numel() * workspace.element_size() if workspace is not None else 0
-    with on_device(query):
-        rc = _lib.load().vrm_paged_chunk_attention(
-            _lib.ptr(query), q_code, query.stride(0), query.stride(1), _lib.ptr(kv_pool), _lib.ptr(kv_scales),
-            _lib.ptr(page_table), _lib.ptr(context_lens), _lib.ptr(cu_seqlens), _lib.ptr(out), _lib.ptr(lse),
-            _lib.ptr(workspace), ws_bytes, N, B, H, KH, D, PS, L, P, max_pp, int(layer_idx),
-            1.0 / math.sqrt(D) if scale is None else float(scale), int(bool(causal)), window or 0, code,
-            _lib.stream_of(query))
+    ptr = _lib.ptr
+    q_n, q_h, _ = query.stride()
+    rc = launch(query, _lib.load().vrm_paged_chunk_attention, query.data_ptr(), q_code, q_n, q_h, kv_pool.data_ptr(),
+                ptr(kv_scales), page_table.data_ptr(), context_lens.data_ptr(), cu_seqlens.data_ptr(), out.data_ptr(),
+                ptr(lse), ptr(workspace), ws_bytes, N, B, H, KH, D, PS, L, P, max_pp, int(layer_idx),
+                1.0 / math.sqrt(D) if scale is None else float(scale), 1 if causal else 0, window or 0, code)
     _lib.check(rc, "paged_attention_chunk")
     return out

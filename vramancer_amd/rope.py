@@ -11,7 +11,6 @@ frequency scaling.
 """
 from __future__ import annotations
 
-import contextlib
 from typing import Any, Optional, Tuple
 
 import torch
@@ -43,12 +42,21 @@ def rope_table(max_positions: int, rotary_dim: int, base: float = 10000.0, inv_f
     return (torch.cat([angle.cos(), angle.sin()], 1) * attention_scaling).to(torch.float32)
 
 
-def on_device(t):
-    """Makes t's device the current one for a launch on its stream, where it
-    is not."""
-    if torch.cuda.current_device() == t.get_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(t.get_device())
+def launch(t, fn, *args) -> int:
+    """fn(*args, stream) on t's device and its current stream."""
+    index = t.get_device()
+    if torch.cuda.current_device() == index:
+        return fn(*args, _lib.stream_of(t))
+    with torch.cuda.device(index):
+        return fn(*args, _lib.stream_of(t))
+
+
+_SRC_CODES = {torch.float32: _lib.VRM_SRC_F32, torch.float16: _lib.VRM_SRC_F16, torch.bfloat16: _lib.VRM_SRC_BF16}
+
+
+def src_code(dtype) -> int:
+    code = _SRC_CODES.get(dtype)
+    return _lib.src_dtype_code(dtype) if code is None else code  # (raises)
 
 
 def check_heads(name: str, t, N: Optional[int], D: Optional[int], dtype):
@@ -75,7 +83,7 @@ def check_table(cos_sin, D: int) -> Tuple[int, int]:
 
 def check_positions(positions, N: int):
     """Contiguous int32 / int64 [N] positions."""
-    if tuple(positions.shape) != (N,) or positions.dtype not in (torch.int32, torch.int64):
+    if positions.dim() != 1 or positions.shape[0] != N or positions.dtype not in (torch.int32, torch.int64):
         raise RuntimeError(f"positions must be an int32 or int64 [{N}] tensor, got {positions.dtype} "
                            f"{tuple(positions.shape)}")
     return positions.contiguous()
@@ -83,25 +91,20 @@ def check_positions(positions, N: int):
 
 def check_weights(q_weight, k_weight, D: int):
     """(q_weight, k_weight, dtype code), each [D] of one dtype or None."""
-    code, dtype = _lib.VRM_SRC_F32, None
-    out = []
+    first = q_weight if q_weight is not None else k_weight
+    if first is None:
+        return None, None, _lib.VRM_SRC_F32
     for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if w is not None:
-            if tuple(w.shape) != (D,):
-                raise RuntimeError(f"{name} must be [{D}], got {tuple(w.shape)}")
-            if dtype is not None and w.dtype != dtype:
-                raise RuntimeError(f"q_weight and k_weight must share a dtype, got {dtype} and {w.dtype}")
-            dtype = w.dtype
-            code = _lib.src_dtype_code(dtype)
-            w = w.contiguous()
-        out.append(w)
-    return out[0], out[1], code
+        if w is not None and (w.dim() != 1 or w.shape[0] != D or w.dtype != first.dtype):
+            raise RuntimeError(f"{name} must be [{D}], both weights of one dtype; got {w.dtype} {tuple(w.shape)}")
+    return (None if q_weight is None else q_weight.contiguous(), None if k_weight is None else k_weight.contiguous(),
+            src_code(first.dtype))
 
 
 def check_out(name: str, out, like):
     """A contiguous output shaped like `like`, allocated where not given."""
     if out is None:
-        return torch.empty(like.shape, dtype=like.dtype, device=like.device)
+        return torch.empty_like(like, memory_format=torch.contiguous_format)
     if out.shape != like.shape or out.dtype != like.dtype or not out.is_contiguous():
         raise RuntimeError(f"{name} must be a contiguous {like.dtype} {tuple(like.shape)} tensor, got {out.dtype} "
                            f"{tuple(out.shape)}")
@@ -134,7 +137,7 @@ def qk_norm_rope(
     N, H, D = query.shape
     key = check_heads("key", key, N, D, query.dtype)
     KH = key.shape[1]
-    code = _lib.src_dtype_code(query.dtype)
+    code = src_code(query.dtype)
     rot, top = check_table(cos_sin, D)
     if cos_sin is not None:
         if positions is None:
@@ -143,11 +146,11 @@ def qk_norm_rope(
     q_weight, k_weight, w_code = check_weights(q_weight, k_weight, D)
     query_out = check_out("query_out", query_out, query)
     key_out = check_out("key_out", key_out, key)
-    with on_device(query):
-        rc = _lib.load().vrm_qk_norm_rope(
-            _lib.ptr(query), query.stride(0), query.stride(1), _lib.ptr(key), key.stride(0), key.stride(1), code,
-            _lib.ptr(cos_sin), rot, top, _lib.ptr(positions), positions.element_size() if positions is not None else 4,
-            _lib.ptr(q_weight), _lib.ptr(k_weight), w_code, float(eps), int(bool(interleaved)), _lib.ptr(query_out),
-            _lib.ptr(key_out), N, H, KH, D, _lib.stream_of(query))
+    (q_n, q_h, _), (k_n, k_h, _) = query.stride(), key.stride()
+    ptr = _lib.ptr
+    rc = launch(query, _lib.load().vrm_qk_norm_rope, query.data_ptr(), q_n, q_h, key.data_ptr(), k_n, k_h, code,
+                ptr(cos_sin), rot, top, ptr(positions), positions.element_size() if positions is not None else 4,
+                ptr(q_weight), ptr(k_weight), w_code, float(eps), 1 if interleaved else 0, query_out.data_ptr(),
+                key_out.data_ptr(), N, H, KH, D)
     _lib.check(rc, "qk_norm_rope")
     return query_out, key_out
