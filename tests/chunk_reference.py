@@ -102,10 +102,13 @@ def attend(q, vals, table, lens, cu, layer, scale=None, causal=True, window=None
             rows = torch.arange(r0, r1)[any_]
             p = torch.softmax(s, -1)
             vz = v[:, h // G]
-            # a token that a row does not see has no part in it, whatever it holds
-            vz = torch.where(see.any(0)[:, None], vz, torch.zeros((), dtype=torch.float64))
-            out[rows, h] = p @ vz
-            reach[rows, h] = p @ vz.abs()
+            if vz.isfinite().all():
+                out[rows, h] = p @ vz
+                reach[rows, h] = p @ vz.abs()
+            else:  # a token that a row does not see has no part in it, whatever it holds
+                part = torch.where(see[any_][:, :, None], p[:, :, None] * vz[None], 0.0)
+                out[rows, h] = part.sum(1)
+                reach[rows, h] = part.abs().sum(1)
             lse[rows, h] = torch.logsumexp(s, -1)
     return out, lse, reach
 

@@ -154,3 +154,55 @@ def test_scale(scale):
     _say(f"chunk scale {scale}")
     _check("bf16", "bf16", [33, 5], [100, 47], 6, 2, 64, 16, seed=6, scale=scale, q_std=0.5)
     _check("f32", "f32", [33, 5], [100, 47], 6, 2, 64, 16, seed=6, scale=scale, q_std=0.5)
+
+
+@pytest.mark.parametrize("window", [None, 30])
+@pytest.mark.parametrize("qt,kv,D", [("bf16", "bf16", 64), ("f16", "f16", 128), ("f32", "f32", 64), ("bf16", "int8", 64),
+                                     ("bf16", "fp8", 128), ("f16", "fp8", 64), ("f32", "fp8", 64), ("bf16", "f16", 64),
+                                     ("f16", "f16", 256)])
+@pytest.mark.parametrize("q_lens,past", [([40, 3], [70, 130]), ([200], [0]), ([4], [90])])
+def test_values_that_are_not_finite(qt, kv, D, q_lens, past, window):
+    """Infinities and NaN among keys and values that a row does not see (later
+    tokens of its own chunk, tokens before its window) have no part in it; rows
+    that see them get what the definition gives."""
+    _say(f"not finite {qt} over {kv} D={D} q={q_lens} window={window}")
+    gen, P, table, lens, cu = _batch(q_lens, past, 16, 31)
+    pool, scales, vals = make_pool(kv, P, 1, 2, 16, D, gen)
+    for b, (n, p) in enumerate(zip(q_lens, past)):
+        # one token inside the chunk, one before it; the rest of the last page
+        for t, x in ((p + n // 2, math.inf), (max(0, p - 20), math.nan)):
+            pid, slot = int(table[b, t // 16]), t % 16
+            vals[pid, 0, 1, 1, slot, 5] = x
+            if kv in FLOAT:
+                pool[pid, 0, 1, 1, slot, 5] = x
+                pool[pid, 0, 0, 0, slot, 3] = x
+                vals[pid, 0, 0, 0, slot, 3] = x
+            elif kv == "int8":
+                scales[pid, 0, 1, 1, slot] = x
+                vals[pid, 0, 1, 1, slot] = pool_codes(pool, pid, slot).double() * x
+            else:
+                at = ((slot // 4 * 16 + 5) * (D // 16) + 0) * 4 + slot % 4
+                pool.view(torch.uint8)[pid, 0, 1, 1].view(-1)[at] = 0x7f
+                vals[pid, 0, 1, 1, slot, 5] = math.nan
+        end = p + n
+        if end % 16 and kv in FLOAT:
+            pool[int(table[b, end // 16]), 0, :, :, end % 16:] = math.nan
+    q = (torch.randn((int(cu[-1]), 6, D), generator=gen)).to(FLOAT[qt])
+    gp, gs = to_gpu(pool, scales)
+    got = paged_attention_chunk(q.to(DEV), gp, table.to(DEV), lens.to(DEV), cu.to(DEV), 0, kv_scales=gs,
+                                window=window).cpu().double()
+    want, _, reach = attend(q, vals, table, lens, cu, 0, window=window)
+    assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.isinf(), want.isinf())
+    fine = want.isfinite()
+    wide = qt == "f32" or kv == "f32" or (kv in FLOAT and kv != qt)
+    tol = _tolerance(want, reach, q.dtype, wide, D, kv not in FLOAT)
+    assert ((got - want).abs() <= tol)[fine].all()
+    assert fine.any() and not fine.all()
+
+
+def pool_codes(pool, pid, slot):
+    """int8 codes of V, kv-head 1, of a token of a stored pool."""
+    D = pool.shape[-1]
+    d = torch.arange(D)
+    at = ((slot // 4 * 16 + d % 16) * (D // 16) + d // 16) * 4 + slot % 4
+    return pool[pid, 0, 1, 1].reshape(-1)[at]

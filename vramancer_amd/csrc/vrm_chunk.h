@@ -225,6 +225,126 @@ __device__ __forceinline__ uint4 load16(const uint8_t* p, int bytes, bool vec) {
   return make_uint4((uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32));
 }
 
+// Blocks that some row of the tile does not see whole (as far as their tokens
+// are there) are those before whole0 and from whole1 on.
+template <int TN>
+__device__ __forceinline__ void tile_edges(const ChunkArgs& a, const Item& it, int rows, int& whole0, int& whole1) {
+  const int first = it.s.base + it.tile * a.tile_rows / a.G;
+  const int last = it.s.base + (it.tile * a.tile_rows + rows - 1) / a.G;
+  whole0 = a.window ? (max(last - a.window + 1, 0) + TN - 1) / TN : 0;
+  whole1 = a.causal ? max(first + 1, 0) / TN : 0x7fffffff;
+}
+
+__device__ __forceinline__ bool not_finite(float x) { return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u; }
+
+// Whether 16 bytes of values of a pool of this kind hold an infinity or a NaN.
+template <int KIND>
+__device__ __forceinline__ bool not_finite16(const uint4& x) {
+  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (KIND == kSrcF32) bad |= (w[i] & 0x7f800000u) == 0x7f800000u;
+    if constexpr (KIND == kSrcF16 || KIND == kSrcBf16) {
+      constexpr uint32_t e = KIND == kSrcF16 ? 0x7c00u : 0x7f80u;
+      bad |= (w[i] & e) == e || (w[i] >> 16 & e) == e;
+    }
+    if constexpr (KIND == kSrcFp8) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) bad |= (w[i] >> (8 * j) & 0x7fu) == 0x7fu;
+    }
+  }
+  return bad;
+}
+
+__device__ __forceinline__ float load_value(int kind, const uint8_t* p, int i) {
+  switch (kind) {
+    case kSrcF32: return reinterpret_cast<const float*>(p)[i];
+    case kSrcF16: return f16_bits_to_f32(reinterpret_cast<const uint16_t*>(p)[i]);
+    case kSrcBf16: return bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(p)[i]);
+    case kSrcI8: return (float)(int8_t)p[i];
+    default: return e4m3fn_to_f32(p[i]);
+  }
+}
+
+// An item whose edge blocks hold an infinity or a NaN among the values.  There
+// a matrix product's weight 0 makes a NaN of what a row does not see, so such
+// items (a model that has overflowed) are computed again here, a wavefront per
+// row and token by token over those that the row sees.
+template <int TN>
+__device__ __forceinline__ void careful_item(const ChunkArgs& a, const Item& it, int kvh, int kind, int rows, int from,
+                                             int to, int waves) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int32_t* const table = a.table + (long long)it.b * a.max_pp;
+  const uint8_t* const k_base = a.pool + a.layer_off + (long long)kvh * a.g.head;
+  const int row_bytes = kind == kSrcF32 ? 4 * a.D : kind >= kSrcI8 ? a.D : 2 * a.D;
+#pragma unroll 1
+  for (int row = wave; row < rows; row += waves) {
+    const int packed = it.tile * a.tile_rows + row, tok = packed / a.G, head = kvh * a.G + packed % a.G;
+    const int pos = it.s.base + tok;
+    const int t0 = max(from * TN, a.window ? pos - a.window + 1 : 0);
+    const int t1 = min(min(to * TN, it.s.ctx), a.causal ? pos + 1 : it.s.ctx);
+    float q[4], o[4] = {0.f, 0.f, 0.f, 0.f}, m = -INFINITY, l = 0.f;
+    const long long q_at = (long long)(it.s.row0 + tok) * a.q_n + (long long)head * a.q_h;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int d = lane + 64 * e;
+      q[e] = d < a.D && a.q_sign ? load_q(a, q_at + d) * (float)a.q_sign : 0.f;
+    }
+#pragma unroll 1
+    for (int t = t0; t < t1; ++t) {
+      const int pi = page_index(a, t), page = table[pi];
+      if (page < 0 || page >= a.P) continue;
+      const int slot = t - pi * a.PS;
+      const uint8_t* const k = k_base + (long long)page * a.g.page + (long long)slot * row_bytes;
+      const uint8_t* const v = k + a.g.kv - (kind >= kSrcI8 ? (long long)slot * row_bytes : 0);
+      float ks = 1.f, vs = 1.f;
+      if (kind >= kSrcI8) {
+        const float* s = a.scales + a.s_layer_off + (long long)page * a.g.s_page + (long long)kvh * a.g.s_head +
+                         (kind == kSrcI8 ? slot : 0);
+        ks = s[0], vs = s[a.g.s_kv];
+      }
+      float dot = 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (lane + 64 * e < a.D) dot += q[e] * load_value(kind, k, lane + 64 * e);
+      const float s = group_sum<64>(dot) * ks * a.sc;
+      const float next = fmaxf(m, s);
+      const float f = m == -INFINITY ? 0.f : exp2f(m - next), p = s == -INFINITY ? 0.f : exp2f(s - next);
+      m = next;
+      l = l * f + p;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int d = lane + 64 * e;
+        const int i = kind >= kSrcI8 ? (((slot >> 2) * 16 + (d & 15)) * (a.D >> 4) + (d >> 4)) * 4 + (slot & 3) : d;
+        if (d < a.D) o[e] = o[e] * f + p * (load_value(kind, v, i) * vs);
+      }
+    }
+    const long long at = (long long)(it.s.row0 + tok) * a.H + head;
+    const long long share = (long long)blockIdx.x * a.tile_rows + row;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int d = lane + 64 * e;
+      if (d >= a.D) break;
+      const float x = l == 0.f ? 0.f : o[e] / l;
+      if (it.shares > 1)
+        a.part[share * a.dp + d] = o[e];
+      else if (a.q_type == VRM_SRC_F32)
+        static_cast<float*>(a.out)[at * a.D + d] = x;
+      else if (a.q_type == VRM_SRC_F16)
+        static_cast<uint16_t*>(a.out)[at * a.D + d] = __builtin_bit_cast(unsigned short, (_Float16)x);
+      else
+        static_cast<uint16_t*>(a.out)[at * a.D + d] = __builtin_bit_cast(unsigned short, (__bf16)x);
+    }
+    if (lane == 0) {
+      if (it.shares > 1)
+        a.ml[share] = make_float2(m, l);
+      else if (a.lse)
+        a.lse[at] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+    }
+  }
+}
+
 // One launch of the attention kernel: float32 products (pool of kind kSrc*),
 // 16-bit products over float, int8 and fp8 pools.
 void launch_chunk_f32(const ChunkArgs& a, int kind, dim3 grid, hipStream_t st);
