@@ -88,6 +88,13 @@ __device__ __forceinline__ int blocks_of(const ChunkArgs& a, const Sequence& s) 
   return (span + TN - 1) / TN;
 }
 
+// What a block costs a tile of at most 32 rows, whose wavefronts wait for
+// memory, against one of a larger tile.
+constexpr int kFewCost = 2;
+__device__ __forceinline__ int block_cost(const ChunkArgs& a, const Sequence& s) {
+  return s.q_len * a.G <= 32 ? kFewCost : 1;
+}
+
 // Inclusive prefix sum over the wavefront's lanes.
 __device__ __forceinline__ int wave_scan(int v) {
   const int lane = __lane_id();
@@ -134,18 +141,21 @@ __device__ __forceinline__ RowGroup row_group(const ChunkArgs& a, const Item& it
 template <int TN>
 __device__ __forceinline__ bool find_item(const ChunkArgs& a, int idx, Item& it) {
   const int lane = __lane_id();
-  int share_blocks = 0x7fffffff;
+  int share_work = 0x7fffffff;
   if (a.target > 0) {
     float work = 0.f;
+    bool many = false;
     for (int b0 = 0; b0 < a.B; b0 += kWave) {
       const int b = b0 + lane;
       if (b < a.B) {
         const Sequence s = load_sequence(a, b);
-        work += (float)tiles_of(a, s) * (float)blocks_of<TN>(a, s);
+        work += (float)tiles_of(a, s) * (float)block_cost(a, s) * (float)blocks_of<TN>(a, s);
+        many |= block_cost(a, s) == 1 && tiles_of(a, s) > 0;
       }
     }
     work = group_sum<64>(work);
-    share_blocks = max(a.min_blocks, (int)fminf(ceilf(work / (float)a.target), 1e9f));
+    const int unit = __any(many) ? 1 : kFewCost;
+    share_work = unit * (int)fminf(fmaxf(ceilf(work / (float)(a.target * unit)), 1.f), 1e8f);
   }
   int before = 0;
   for (int b0 = 0; b0 < a.B; b0 += kWave) {
@@ -156,7 +166,8 @@ __device__ __forceinline__ bool find_item(const ChunkArgs& a, int idx, Item& it)
       s = load_sequence(a, b);
       tiles = tiles_of(a, s);
       const int blocks = blocks_of<TN>(a, s);
-      shares = max(1, (int)(((long long)blocks + share_blocks - 1) / share_blocks));
+      const long long work = (long long)blocks * block_cost(a, s);
+      shares = max(1, min((int)((work + share_work - 1) / share_work), (blocks + a.min_blocks - 1) / a.min_blocks));
     }
     const int upto = wave_scan(tiles * shares);
     const unsigned long long past = __ballot(before + upto > idx);
@@ -225,38 +236,6 @@ __device__ __forceinline__ uint4 load16(const uint8_t* p, int bytes, bool vec) {
   return make_uint4((uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32));
 }
 
-// Blocks that some row of the tile does not see whole (as far as their tokens
-// are there) are those before whole0 and from whole1 on.
-template <int TN>
-__device__ __forceinline__ void tile_edges(const ChunkArgs& a, const Item& it, int rows, int& whole0, int& whole1) {
-  const int first = it.s.base + it.tile * a.tile_rows / a.G;
-  const int last = it.s.base + (it.tile * a.tile_rows + rows - 1) / a.G;
-  whole0 = a.window ? (max(last - a.window + 1, 0) + TN - 1) / TN : 0;
-  whole1 = a.causal ? max(first + 1, 0) / TN : 0x7fffffff;
-}
-
-__device__ __forceinline__ bool not_finite(float x) { return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u; }
-
-// Whether 16 bytes of values of a pool of this kind hold an infinity or a NaN.
-template <int KIND>
-__device__ __forceinline__ bool not_finite16(const uint4& x) {
-  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-  bool bad = false;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if constexpr (KIND == kSrcF32) bad |= (w[i] & 0x7f800000u) == 0x7f800000u;
-    if constexpr (KIND == kSrcF16 || KIND == kSrcBf16) {
-      constexpr uint32_t e = KIND == kSrcF16 ? 0x7c00u : 0x7f80u;
-      bad |= (w[i] & e) == e || (w[i] >> 16 & e) == e;
-    }
-    if constexpr (KIND == kSrcFp8) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) bad |= (w[i] >> (8 * j) & 0x7fu) == 0x7fu;
-    }
-  }
-  return bad;
-}
-
 __device__ __forceinline__ float load_value(int kind, const uint8_t* p, int i) {
   switch (kind) {
     case kSrcF32: return reinterpret_cast<const float*>(p)[i];
@@ -267,19 +246,63 @@ __device__ __forceinline__ float load_value(int kind, const uint8_t* p, int i) {
   }
 }
 
-// An item whose edge blocks hold an infinity or a NaN among the values.  There
-// a matrix product's weight 0 makes a NaN of what a row does not see, so such
-// items (a model that has overflowed) are computed again here, a wavefront per
-// row and token by token over those that the row sees.
+// Element of a page's V (of a kv-head) that is a slot's dim d.
+__device__ __forceinline__ int value_at(const ChunkArgs& a, int kind, int slot, int d) {
+  if (kind < kSrcI8) return slot * a.D + d;
+  return (((slot >> 2) * 16 + (d & 15)) * (a.D >> 4) + (d >> 4)) * 4 + (slot & 3);
+}
+
+// Whether a row of the wavefront has a NaN in its accumulators (or infinities
+// of both signs).
+template <typename V, int NB>
+__device__ __forceinline__ bool any_nan(const V (&o)[NB], bool real) {
+  V x = o[0];
+#pragma unroll
+  for (int n = 1; n < NB; ++n) x += o[n];
+  float y = x[0];
+#pragma unroll
+  for (int i = 1; i < 16; ++i) y += x[i];
+  return __any(real && y != y);
+}
+
+__device__ __forceinline__ bool not_finite(float x) { return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u; }
+
+// Rows [row0, row1) of an item, of which some have a NaN in their accumulators
+// (called by one wavefront, with the positions of the first and last row).
+// In a matrix product the weight 0 of a token that a row does not see makes a
+// NaN of an infinity or a NaN among its values, so if there is one within the
+// item (a model that has overflowed), the rows are computed again, token by
+// token over those that each sees.  Returns whether it did.
 template <int TN>
-__device__ __forceinline__ void careful_item(const ChunkArgs& a, const Item& it, int kvh, int kind, int rows, int from,
-                                             int to, int waves) {
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+__device__ __forceinline__ bool careful_rows(const ChunkArgs& a, const Item& it, int kvh, int kind, int row0, int row1,
+                                             int first_pos, int last_pos, int from, int to) {
+  const int lane = threadIdx.x & 63;
   const int32_t* const table = a.table + (long long)it.b * a.max_pp;
   const uint8_t* const k_base = a.pool + a.layer_off + (long long)kvh * a.g.head;
-  const int row_bytes = kind == kSrcF32 ? 4 * a.D : kind >= kSrcI8 ? a.D : 2 * a.D;
+  const int end = min(to * TN, it.s.ctx);
+  bool spoilt = false;
 #pragma unroll 1
-  for (int row = wave; row < rows; row += waves) {
+  for (int t = from * TN; t < end; ++t) {
+    const bool unseen = (a.causal && t > first_pos) || (a.window && t <= last_pos - a.window);
+    if (!unseen) {  // on to the tokens after the first row's position
+      if (!a.causal) break;
+      t = max(t, min(first_pos, end));
+      continue;
+    }
+    const int pi = page_index(a, t), page = table[pi];
+    if (page < 0 || page >= a.P) continue;
+    const int slot = t - pi * a.PS;
+    const uint8_t* const v = k_base + a.g.kv + (long long)page * a.g.page;
+    for (int d = lane; d < a.D; d += kWave) spoilt |= not_finite(load_value(kind, v, value_at(a, kind, slot, d)));
+    if (kind >= kSrcI8) {
+      const float vs = a.scales[a.s_layer_off + (long long)page * a.g.s_page + (long long)kvh * a.g.s_head +
+                                (kind == kSrcI8 ? slot : 0) + a.g.s_kv];
+      spoilt |= not_finite(vs);
+    }
+  }
+  if (!__any(spoilt)) return false;
+#pragma unroll 1
+  for (int row = row0; row < row1; ++row) {
     const int packed = it.tile * a.tile_rows + row, tok = packed / a.G, head = kvh * a.G + packed % a.G;
     const int pos = it.s.base + tok;
     const int t0 = max(from * TN, a.window ? pos - a.window + 1 : 0);
@@ -296,8 +319,8 @@ __device__ __forceinline__ void careful_item(const ChunkArgs& a, const Item& it,
       const int pi = page_index(a, t), page = table[pi];
       if (page < 0 || page >= a.P) continue;
       const int slot = t - pi * a.PS;
-      const uint8_t* const k = k_base + (long long)page * a.g.page + (long long)slot * row_bytes;
-      const uint8_t* const v = k + a.g.kv - (kind >= kSrcI8 ? (long long)slot * row_bytes : 0);
+      const uint8_t* const k = k_base + (long long)page * a.g.page;
+      const uint8_t* const v = k + a.g.kv;
       float ks = 1.f, vs = 1.f;
       if (kind >= kSrcI8) {
         const float* s = a.scales + a.s_layer_off + (long long)page * a.g.s_page + (long long)kvh * a.g.s_head +
@@ -307,7 +330,7 @@ __device__ __forceinline__ void careful_item(const ChunkArgs& a, const Item& it,
       float dot = 0.f;
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (lane + 64 * e < a.D) dot += q[e] * load_value(kind, k, lane + 64 * e);
+        if (lane + 64 * e < a.D) dot += q[e] * load_value(kind, k, slot * a.D + lane + 64 * e);
       const float s = group_sum<64>(dot) * ks * a.sc;
       const float next = fmaxf(m, s);
       const float f = m == -INFINITY ? 0.f : exp2f(m - next), p = s == -INFINITY ? 0.f : exp2f(s - next);
@@ -316,8 +339,7 @@ __device__ __forceinline__ void careful_item(const ChunkArgs& a, const Item& it,
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int d = lane + 64 * e;
-        const int i = kind >= kSrcI8 ? (((slot >> 2) * 16 + (d & 15)) * (a.D >> 4) + (d >> 4)) * 4 + (slot & 3) : d;
-        if (d < a.D) o[e] = o[e] * f + p * (load_value(kind, v, i) * vs);
+        if (d < a.D) o[e] = o[e] * f + p * (load_value(kind, v, value_at(a, kind, slot, d)) * vs);
       }
     }
     const long long at = (long long)(it.s.row0 + tok) * a.H + head;
@@ -343,6 +365,7 @@ __device__ __forceinline__ void careful_item(const ChunkArgs& a, const Item& it,
         a.lse[at] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
     }
   }
+  return true;
 }
 
 // One launch of the attention kernel: float32 products (pool of kind kSrc*),

@@ -262,7 +262,6 @@ struct Stage {
   struct Shared {
     unsigned long long there[kRing];  // tokens of a block that are there, a bit each
     alignas(16) float scale[kRing][2][QUANT ? TN : 4];
-    int spoilt;                       // an edge block holds a value that is not finite
   };
 
   const ChunkArgs& a;
@@ -272,18 +271,14 @@ struct Stage {
   const int32_t* table;
   int row_bytes, lane, wave;
   int limit;      // tokens from here on are not there
-  int whole0, whole1;  // edge blocks of the tile: before, and from
   bool one_page;  // a run lies in one page and is contiguous there
   uint4 kr[NP], vr[NP];
   int page;       // lane i: of token i % RUN of the run to be loaded next, -1: none
   uint32_t bits;  // tokens of the run in registers that are there
   float ks, vs;   // lane i < RUN: their scales
 
-  __device__ __forceinline__ Stage(const ChunkArgs& args, const Item& it, int kvh, int rows, int blocks_end,
-                                   Shared& shared)
+  __device__ __forceinline__ Stage(const ChunkArgs& args, const Item& it, int kvh, int blocks_end, Shared& shared)
       : a(args), sh(shared) {
-    tile_edges<TN>(a, it, rows, whole0, whole1);
-    if (threadIdx.x == 0) sh.spoilt = 0;  // (a barrier comes before it is read)
     const int ctx = it.s.ctx, to = blocks_end;
     k_base = a.pool + a.layer_off + (long long)kvh * a.g.head;
     v_base = k_base + a.g.kv;
@@ -357,13 +352,6 @@ struct Stage {
   }
 
   __device__ __forceinline__ void put(int block, uint8_t* k_lds, uint8_t* v_lds) {
-    if (__builtin_expect(block < whole0 || block >= whole1, 0)) {
-      bool bad = QUANT && lane < RUN && not_finite(vs);
-#pragma unroll
-      for (int i = 0; i < NP; ++i)
-        if (!kRagged || lane + 64 * i < kRun) bad |= not_finite16<KIND>(vr[i]);
-      if (bad) sh.spoilt = 1;
-    }
     int first = lane;
     if constexpr (QUANT) asm("" : "+v"(first));  // (as in load: the places in LDS are not worth registers)
     if (QUANT && lane < RUN) {
@@ -435,7 +423,7 @@ __device__ __forceinline__ void scale_weights(const float* vs, int e, int half, 
 // Bound: memory.
 template <typename T, int KIND, int DP, int WAVES>
 __device__ __forceinline__ void few_rows(const ChunkArgs& a, const Item& it, int kvh, int rows, int from, int to,
-                                         uint8_t* lds, float (*own_scale)[2][32], int& spoilt) {
+                                         uint8_t* lds, float (*own_scale)[2][32]) {
   using Tile = ChunkTile<KIND, DP>;
   using PT = std::conditional_t<KIND >= kSrcI8, Bf16, T>;
   constexpr bool QUANT = Tile::kQuant;
@@ -525,9 +513,6 @@ __device__ __forceinline__ void few_rows(const ChunkArgs& a, const Item& it, int
     }
   };
 
-  int whole0, whole1;
-  tile_edges<32>(a, it, rows, whole0, whole1);
-  bool bad = false;  // an edge block holds a value that is not finite
   int sub = 2 * from + wave;
 #pragma unroll
   for (int b = 0; b < DEPTH; ++b) page[b] = page_of(sub + b * WAVES);
@@ -545,19 +530,6 @@ __device__ __forceinline__ void few_rows(const ChunkArgs& a, const Item& it, int
       const int now = sub + b * WAVES, next = now + DEPTH * WAVES, t0 = now * 32;
       if (b > 0 && now >= 2 * to) break;
       const uint32_t there = (uint32_t)__ballot(at[b] >= 0);
-      if (__builtin_expect(now < whole0 || now >= whole1, 0)) {
-        if constexpr (QUANT) {
-          bad |= not_finite(vs[b]);
-          if constexpr (KIND == kSrcFp8) {
-#pragma unroll
-            for (int n = 0; n < NB; ++n)
-              bad |= not_finite16<KIND>(make_uint4(vw[b][0][0][n], vw[b][0][1][n], vw[b][1][0][n], vw[b][1][1][n]));
-          }
-        } else {
-#pragma unroll
-          for (int p = 0; p < KP; ++p) bad |= not_finite16<KIND>(vr[b][p]);
-        }
-      }
       f32x16 s{};
 #pragma unroll
       for (int p = 0; p < KP; ++p) {
@@ -629,18 +601,13 @@ __device__ __forceinline__ void few_rows(const ChunkArgs& a, const Item& it, int
 #pragma unroll
   for (int n = WAVES / 2; n >= 1; n /= 2)
     join<NB>(reinterpret_cast<float*>(lds), wave >= n && wave < 2 * n, wave < n, wave & (n - 1), m, l, o);
-  if (threadIdx.x == 0) spoilt = 0;
-  __syncthreads();
-  if (bad) spoilt = 1;
-  __syncthreads();
-  if (__builtin_expect(spoilt, 0)) {
-    careful_item<64>(a, it, kvh, KIND, rows, from, to, WAVES);
+  if (wave != 0) return;
+  if (__builtin_expect(any_nan(o, g.real), 0) &&
+      careful_rows<64>(a, it, kvh, KIND, 0, rows, g.first_pos, g.last_pos, from, to))
     return;
-  }
-  if (wave == 0)
-    put_rows<T, DP>(a, it, g, m, l, o, [&](int n, int r) {
-      return QUANT && whole ? (r & 15) + 16 * (NB * (r >> 4) + n) : n * 32 + r;
-    });
+  put_rows<T, DP>(a, it, g, m, l, o, [&](int n, int r) {
+    return QUANT && whole ? (r & 15) + 16 * (NB * (r >> 4) + n) : n * 32 + r;
+  });
 }
 
 // Tiles of 128 rows, 32 to a wavefront, two workgroups to a CU: one's
@@ -669,7 +636,7 @@ __global__ void __launch_bounds__(kChunkThreads, DP <= 128 ? 2 : 1) chunk_attn_k
   const int rows = min(a.tile_rows, it.s.q_len * a.G - it.tile * a.tile_rows);
   if constexpr (DP <= 128) {  // (at 256 its operands would not fit the registers)
     if (rows <= 32) {
-      few_rows<T, KIND, DP, 4>(a, it, kvh, rows, from, to, lds, own_scale, shared.spoilt);
+      few_rows<T, KIND, DP, 4>(a, it, kvh, rows, from, to, lds, own_scale);
       return;
     }
   }
@@ -751,7 +718,7 @@ __global__ void __launch_bounds__(kChunkThreads, DP <= 128 ? 2 : 1) chunk_attn_k
       }
   };
 
-  Gather st(a, it, kvh, rows, to, shared);
+  Gather st(a, it, kvh, to, shared);
   st.page = st.page_of(from);
   if (from < to) st.load(from);
   for (int block = from; block < to; ++block) {
@@ -768,11 +735,10 @@ __global__ void __launch_bounds__(kChunkThreads, DP <= 128 ? 2 : 1) chunk_attn_k
   }
   l = xor_add<32>(l);
   if (halves) join<NB>(reinterpret_cast<float*>(lds), active && (wave & 1), active && !(wave & 1), group, m, l, o);
-  if (__builtin_expect(shared.spoilt, 0)) {
-    careful_item<TN>(a, it, kvh, KIND, rows, from, to, 4);
-    return;
-  }
   if (!active || (halves && (wave & 1))) return;
+  if (__builtin_expect(any_nan(o, g.real), 0) &&
+      careful_rows<TN>(a, it, kvh, KIND, group * 32, min(rows, group * 32 + 32), g.first_pos, g.last_pos, from, to))
+    return;
   put_rows<T, DP>(a, it, g, m, l, o, [](int n, int r) { return n * 32 + r; });
 }
 
@@ -804,7 +770,7 @@ __global__ void __launch_bounds__(kLargeThreads, 1) chunk_attn_large_kernel(Chun
   put_record(a, it, kvh);
   const int rows = min(a.tile_rows, it.s.q_len * a.G - it.tile * a.tile_rows);
   if (rows <= 32) {
-    few_rows<T, KIND, DP, 8>(a, it, kvh, rows, from, to, lds, own_scale, shared.spoilt);
+    few_rows<T, KIND, DP, 8>(a, it, kvh, rows, from, to, lds, own_scale);
     return;
   }
 
@@ -823,7 +789,7 @@ __global__ void __launch_bounds__(kLargeThreads, 1) chunk_attn_large_kernel(Chun
   for (int n = 0; n < NB; ++n) o[n] = f32x16{};
   float m = -INFINITY, l = 0.f;
 
-  Gather st(a, it, kvh, rows, to, shared);
+  Gather st(a, it, kvh, to, shared);
   {
     Gather second = st;
     st.page = st.page_of(from);
@@ -992,11 +958,10 @@ __global__ void __launch_bounds__(kLargeThreads, 1) chunk_attn_large_kernel(Chun
     blocks(std::integral_constant<int, 2>{}, std::true_type{}, 0);
   l = xor_add<32>(l);
   if (halves) join<NB>(reinterpret_cast<float*>(lds), active && (wave & 1), active && !(wave & 1), group, m, l, o);
-  if (__builtin_expect(shared.spoilt, 0)) {
-    careful_item<TN>(a, it, kvh, KIND, rows, from, to, 8);
-    return;
-  }
   if (!active || (halves && (wave & 1))) return;
+  if (__builtin_expect(any_nan(o, g.real), 0) &&
+      careful_rows<TN>(a, it, kvh, KIND, group * 32, min(rows, group * 32 + 32), g.first_pos, g.last_pos, from, to))
+    return;
   put_rows<T, DP>(a, it, g, m, l, o, [](int n, int x) { return n * 32 + x; });
 }
 

@@ -56,7 +56,6 @@ __global__ void __launch_bounds__(kChunkThreads, DP <= 128 ? 2 : 1) chunk_attn_f
   __shared__ float scale_lds[2][TN];
   __shared__ long long place_lds[4][TN];
   __shared__ uint32_t there_lds[4];
-  __shared__ int spoilt;  // an edge block holds a value that is not finite
 
   const int kvh = blockIdx.x % a.KH;
   Item it;
@@ -71,9 +70,6 @@ __global__ void __launch_bounds__(kChunkThreads, DP <= 128 ? 2 : 1) chunk_attn_f
   const int rows = min(a.tile_rows, it.s.q_len * a.G - it.tile * a.tile_rows);
   const bool active = wave * 32 < rows;
   const RowGroup g = row_group(a, it, kvh, rows, wave * 32);
-  int whole0, whole1;
-  tile_edges<TN>(a, it, rows, whole0, whole1);
-  if (threadIdx.x == 0) spoilt = 0;
   const bool real = g.real;
 
   float q[DP / 2];
@@ -142,12 +138,6 @@ __global__ void __launch_bounds__(kChunkThreads, DP <= 128 ? 2 : 1) chunk_attn_f
   };
   const auto put_tile = [&](int block) {
     const uint32_t there = there_lds[block & 3];
-    if (block < whole0 || block >= whole1) {
-      bool bad = QUANT && wave == 0 && lane < TN && not_finite(vsc);
-#pragma unroll
-      for (int i = 0; i < NP; ++i) bad |= not_finite16<KIND>(vr[i]);
-      if (bad) spoilt = 1;
-    }
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
       const int c = tid + i * kChunkThreads;
@@ -268,11 +258,11 @@ __global__ void __launch_bounds__(kChunkThreads, DP <= 128 ? 2 : 1) chunk_attn_f
   }
 
   l = xor_add<32>(l);
-  if (spoilt) {
-    careful_item<TN>(a, it, kvh, KIND, rows, from, to, 4);
+  if (!active) return;
+  if (__builtin_expect(any_nan(o, real), 0) &&
+      careful_rows<TN>(a, it, kvh, KIND, wave * 32, min(rows, wave * 32 + 32), g.first_pos, g.last_pos, from, to))
     return;
-  }
-  if (!active || !real) return;
+  if (!real) return;
   if (it.shares > 1) {
     const long long slot = (long long)blockIdx.x * a.tile_rows + g.row;
     float* dst = a.part + slot * DP;
