@@ -22,10 +22,31 @@ import pytest
 import torch
 
 from chunk_reference import FLOAT, HALF, attend, make_pool, make_table, to_gpu
-from vramancer_amd.paged_chunk import chunk_workspace, paged_attention_chunk
+from vramancer_amd import paged_chunk
+from vramancer_amd.paged_chunk import chunk_workspace
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
+
+
+@pytest.fixture(params=["tight", "wide"], autouse=True)
+def table_width(request):
+    """The kernel is chosen by the batch's sizes, the table's width among
+    them: every test runs with a table as wide as its longest sequence, and
+    with one whose further entries are absent pages."""
+    global _wide
+    _wide = request.param == "wide"
+
+
+def paged_attention_chunk(query, pool, table, lens, cu, layer, **kw):
+    rows = query.shape[0] * query.shape[1]
+    need = table.shape[1]
+    if _wide and "workspace" not in kw and rows and table.dim() == 2:
+        width = min(-(-(1 << 24) // (rows * pool.shape[4])), 1 << 15)
+        if width > need:
+            more = torch.full((table.shape[0], width - need), -1, dtype=table.dtype, device=table.device)
+            table = torch.cat([table, more], 1)
+    return paged_chunk.paged_attention_chunk(query, pool, table, lens, cu, layer, **kw)
 
 
 def _say(msg):

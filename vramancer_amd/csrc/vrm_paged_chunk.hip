@@ -105,9 +105,21 @@ struct ChunkPlan {
   size_t rec_bytes, ml_bytes, bytes;
 };
 
-// Tiles that fill the GPU are left whole; fewer are cut into shares, at least
-// kMinBlocks blocks each, for about so many workgroups.
+// Tiles that fill the GPU twice are left whole; fewer are cut into shares for
+// about as many workgroups as are resident at once (for twice as many: a
+// batch of 64 x 4 tokens over 4096 each 130 us for 118, two prompts within a
+// window 123 for 87), at least kMinBlocks blocks each (17 tokens after 1531:
+// 24.4, 21.2 and 21.2 us at 1, 2 and 4).
 constexpr int kMinBlocks = 2;
+
+// Tiles of 256 rows from 128 rows a sequence, 1024 tokens in the table and
+// this much rows x kv-heads x tokens; below, its longer start and its fewer
+// workgroups cost more than its products gain.  Tiles of 128 and of 256 rows,
+// 32 heads over 8 kv-heads of 128, bf16: one sequence after 2000 tokens 19.8
+// and 22.5 us at 128 rows, 37.2 and 36.3 at 1024; 8 such 32.5 and 31.9 at 96,
+// 85.0 and 60.9 at 384; 64 such 114 and 120 at 64, 140 and 135 at 128, 815 and
+// 658 at 1024; 64 after 200 tokens 41 and 60 at 128, 226 and 242 at 1024.
+constexpr double kLargeWork = 1 << 24;
 
 int pool_kind(int kv_dtype) {
   switch (kv_dtype) {
@@ -131,8 +143,10 @@ bool plan_chunk(int N, int B, int H, int KH, int D, int PS, int max_pp, int q_dt
            (q_dtype == VRM_SRC_BF16 && p.kind == kSrcF16);
   p.dp = D <= 64 ? 64 : D <= 96 && !p.wide ? 96 : D <= 128 ? 128 : 256;
   const int block = p.wide ? 32 : 64;
-  const long long blocks = ((long long)max_pp * PS + block - 1) / block;  // of a sequence, at most
-  const bool large = !p.wide && D <= 128 && N * G >= 64LL * B;
+  const long long tokens = (long long)max_pp * PS;           // of a sequence, at most
+  const long long blocks = (tokens + block - 1) / block;
+  const bool large = !p.wide && D <= 128 && N * G >= 128LL * B && tokens >= 1024 &&
+                     (double)(N * G) * KH * (double)tokens >= kLargeWork;
   p.tile_rows = large ? 256 : 128;
   const int wanted = large ? 256 : 512;  // workgroups resident at once
   const long long vtiles = N * G / p.tile_rows + B;
