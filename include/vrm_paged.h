@@ -630,7 +630,9 @@ int vrm_paged_decode_tq_residual(
  * out[n][h] = softmax(scale q[n][h] . K^T) V over the tokens t that row n sees:
  * t < context_lens[b], in a page that is there, with causal != 0 t <= its own
  * position, and with window > 0 t > its position - window.  A row that sees no
- * token gives zeros (lse -inf).  Head h reads kv-head h / (H / KH).
+ * token gives zeros (lse -inf).  What a row does not see has no part in it,
+ * infinities and NaN among the stored values included.  Head h reads kv-head
+ * h / (H / KH).
  *   query       [N][H][D] of q_dtype (VRM_SRC_*), with strides in elements
  *               (last dim contiguous)
  *   kv_pool, kv_scales, page_table as in vrm_paged_decode (any kv_dtype)

@@ -129,6 +129,20 @@ def test_window(kv, window):
     _check("f16", kv, [40, 9], [300, 0], 6, 2, 64, 16, seed=window, window=window, causal=False)
 
 
+@pytest.mark.parametrize("qt,kv", [("bf16", "bf16"), ("f32", "f32")], ids=["bf16", "f32"])
+def test_window_of_every_token(qt, kv):
+    """The widest window is no window, for rows before a context's start too."""
+    _say(f"chunk widest window {qt} over {kv}")
+    gen, P, table, lens, cu = _batch([40, 9], [0, 70], 16, 77)
+    lens = torch.tensor([11, 79], dtype=torch.int32)
+    pool, _, vals = make_pool(kv, P, 1, 2, 16, 64, gen)
+    q = torch.randn((49, 6, 64), generator=gen).to(FLOAT[qt])
+    args = (q.to(DEV), pool.to(DEV), table.to(DEV), lens.to(DEV), cu.to(DEV), 0)
+    out = paged_attention_chunk(*args, window=2 ** 31 - 1)
+    assert torch.equal(out, paged_attention_chunk(*args))
+    assert (out[:29] == 0).all() and (out[29:] != 0).any()
+
+
 @pytest.mark.parametrize("qt,kv", [("bf16", "bf16"), ("f16", "fp8"), ("f32", "int8")], ids=["bf16", "fp8", "f32-int8"])
 def test_not_causal(qt, kv):
     _say(f"chunk not causal {qt} over {kv}")

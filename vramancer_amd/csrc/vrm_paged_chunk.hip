@@ -275,7 +275,7 @@ extern "C" int vrm_paged_chunk_attention(const void* query, int q_dtype, long lo
   a.N = N, a.B = B, a.H = H, a.KH = KH, a.G = H / KH, a.D = D, a.PS = PS, a.P = P, a.max_pp = max_pp;
   a.ps_shift = (PS & (PS - 1)) ? -1 : __builtin_ctz(PS);
   a.causal = causal != 0;
-  a.window = window;
+  a.window = window < 1 << 30 ? window : 1 << 30;  // (positions less it stay in 32 bits)
   a.sc = scale == 0.f ? 1.f : fabsf(scale) * 1.44269504088896341f;
   a.q_sign = scale == 0.f ? 0 : scale < 0.f ? -1 : 1;
   a.target = p.target;

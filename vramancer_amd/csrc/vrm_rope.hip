@@ -133,7 +133,7 @@ __device__ __forceinline__ bool locate(const RopeArgs& a, int n, Token& t) {
       else
         hi = mid - 1;
     }
-    const int c0 = a.cu[lo], c1 = a.cu[lo + 1];
+    const int c0 = a.cu[lo], c1 = min(a.cu[lo + 1], a.N);
     if (n < c0 || n >= c1) return false;
     t.b = lo;
     t.pos = a.lens[lo] - c1 + n;

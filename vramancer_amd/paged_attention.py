@@ -617,22 +617,14 @@ class PagedKVCacheManager:
         """Attention of a chunk's tokens over their requests' pages, which hold
         them already: query [tokens, H, D] -> the same in its dtype
         (``paged_chunk.paged_attention_chunk``)."""
-        from .paged_chunk import chunk_workspace, paged_attention_chunk
+        from .paged_chunk import paged_attention_chunk
 
         self._require_pool("compute_attention_chunk")
         if query.dim() != 3 or query.shape[0] != chunk.num_tokens:
             raise RuntimeError(f"query must be [{chunk.num_tokens}, H, {self.config.head_dim}], got shape "
                                f"{tuple(query.shape)}")
-        B, width = chunk.page_table.shape
-        key = ("chunk", tuple(query.shape), query.dtype, B, width, str(query.device))
-        ws = self._workspaces.get(key)
-        if ws is None:
-            if len(self._workspaces) > 8:
-                self._workspaces.clear()
-            ws = self._workspaces[key] = chunk_workspace(query, self._gpu_pool, B, width)
         return paged_attention_chunk(query, self._gpu_pool, chunk.page_table, chunk.context_lens, chunk.cu_seqlens,
-                                     layer_idx, scale, kv_scales=self._kv_scales, causal=causal, window=window,
-                                     workspace=ws)
+                                     layer_idx, scale, kv_scales=self._kv_scales, causal=causal, window=window)
 
     def flush_compression(self) -> None:
         """Compresses every queued row, all layers at once, into the TurboQuant

@@ -19,7 +19,8 @@ A batch is ragged and described by three int32 device tensors:
   token i of q is at position ``context_lens[b] - q + i``;
 * ``page_table`` [B, max_pages] as the decode takes it.
 
-Everything else is decided on the device; no call reads a tensor back.
+Everything else is decided on the device; no call reads a tensor back.  Like
+the decode these are forward only: outputs carry no gradient.
 """
 from __future__ import annotations
 

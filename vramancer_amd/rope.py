@@ -7,7 +7,7 @@ their cache pages on the way.  The reference leaves both to the model.
 
 Angles come from a table that a program computes once per model
 (``rope_table``): far positions need 64 bits, and a table serves every
-frequency scaling.
+frequency scaling.  Forward only: outputs carry no gradient.
 """
 from __future__ import annotations
 
