@@ -89,7 +89,8 @@ __device__ __forceinline__ int blocks_of(const ChunkArgs& a, const Sequence& s) 
 }
 
 // What a block costs a tile of at most 32 rows, whose wavefronts wait for
-// memory, against one of a larger tile.
+// memory, against one of a larger tile (a prompt's chunk of 509 beside 15
+// single tokens, shares at 1, 2, 3 and 4: 70.6, 65.4, 65.5 and 65.4 us).
 constexpr int kFewCost = 2;
 __device__ __forceinline__ int block_cost(const ChunkArgs& a, const Sequence& s) {
   return s.q_len * a.G <= 32 ? kFewCost : 1;
@@ -135,9 +136,9 @@ __device__ __forceinline__ RowGroup row_group(const ChunkArgs& a, const Item& it
 
 // Item idx of a kv-head: the shares of the first sequence's tiles (later tiles
 // first: under a causal mask they see more keys), then the next sequence's.
-// Shares have about (work of the kv-head) / target blocks, so that sequences
-// of any lengths fill the GPU evenly; every wavefront finds its item itself,
-// lane by lane over the sequences.
+// Shares have about (work of the kv-head) / target, so that sequences of any
+// lengths fill the GPU evenly, and two blocks at least; every wavefront finds
+// its item itself, lane by lane over the sequences.
 template <int TN>
 __device__ __forceinline__ bool find_item(const ChunkArgs& a, int idx, Item& it) {
   const int lane = __lane_id();

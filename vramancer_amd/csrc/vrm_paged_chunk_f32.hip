@@ -8,7 +8,9 @@
 // k-slots of a matrix product may come in any order that both operands
 // share: lane half h takes dims 8 j + 4 h + e of K and Q (16-byte LDS reads),
 // and tokens in the order the scores lie in.
-// Bound: the float32 matrix rate, 1/16 of the 16-bit one.
+// Bound: the float32 matrix rate, 1/16 of the 16-bit one, in long batches;
+// four prompts' chunks of 100 to 160 tokens, 12 heads of 64, are a chain of
+// dependent blocks: 35 us with the merge, 20 TFLOP/s.
 #include <type_traits>
 
 #include "vrm_chunk.h"
