@@ -241,3 +241,63 @@ def pool_codes(pool, pid, slot):
     d = torch.arange(D)
     at = ((slot // 4 * 16 + d % 16) * (D // 16) + d // 16) * 4 + slot % 4
     return pool[pid, 0, 1, 1].reshape(-1)[at]
+
+
+@pytest.mark.parametrize("t,D", [("bf16", 128), ("f16", 80), ("f32", 64)])
+@pytest.mark.parametrize("q_lens", [[3, 1], [150, 20]], ids=["few", "many"])
+def test_strides_and_alignment(t, D, q_lens):
+    """Queries that are slices of a projection, rows and pools that start off
+    16 bytes, outputs that do: the same bits as from dense, aligned ones."""
+    _say(f"chunk strides {t} D={D} q={q_lens}")
+    H, KH = 6, 2
+    gen, P, table, lens, cu = _batch(q_lens, [70, 300], 16, 41)
+    pool, _, _ = make_pool(t, P, 1, KH, 16, D, gen)
+    pool, batch = pool.to(DEV), (table.to(DEV), lens.to(DEV), cu.to(DEV), 0)
+    N = int(cu[-1])
+    proj = torch.randn((N, (H + 2 * KH) * D + 1), generator=gen).to(FLOAT[t]).to(DEV)
+    sliced = proj[:, 1:1 + H * D].view(N, H, D)
+    want = paged_attention_chunk(sliced.contiguous(), pool, *batch)
+    assert torch.equal(paged_attention_chunk(sliced, pool, *batch), want)
+    turned = sliced.transpose(0, 1).contiguous().transpose(0, 1)
+    assert torch.equal(paged_attention_chunk(turned, pool, *batch), want)
+    last = sliced.transpose(1, 2).contiguous().transpose(1, 2)
+    assert torch.equal(paged_attention_chunk(last, pool, *batch), want)
+    odd_pool = torch.empty(pool.numel() + 1, dtype=pool.dtype, device=DEV)[1:].view(pool.shape).copy_(pool)
+    assert torch.equal(paged_attention_chunk(sliced, odd_pool, *batch), want)
+    out = torch.empty(want.numel() + 1, dtype=want.dtype, device=DEV)[1:].view(want.shape)
+    assert torch.equal(paged_attention_chunk(sliced, pool, *batch, out=out), want)
+
+
+@pytest.mark.parametrize("kv,page_bytes", [("bf16", 2 * 8 * 16 * 128 * 2), ("int8", 2 * 8 * 16 * 128)])
+@pytest.mark.parametrize("q_lens", [[4, 1], [90, 40]], ids=["few", "many"])
+def test_pool_past_32_bits(kv, page_bytes, q_lens):
+    """Pages past 4 GiB of a pool give what the same pages give in a small one."""
+    _say(f"chunk pool past 32 bits {kv} q={q_lens}")
+    gen, P, table, lens, cu = _batch(q_lens, [100, 37], 16, 42)
+    pool, scales, _ = make_pool(kv, P, 1, 8, 16, 128, gen, None if kv == "bf16" else "plain")
+    pool = pool.to(DEV)
+    scales = None if scales is None else scales.to(DEV)
+    far = (1 << 32) // page_bytes + 3
+    big = torch.empty((far + P, *pool.shape[1:]), dtype=pool.dtype, device=DEV)
+    big[far:] = pool
+    big_scales = None
+    if scales is not None:
+        big_scales = torch.zeros((far + P, *scales.shape[1:]), device=DEV)
+        big_scales[far:] = scales
+    q = torch.randn((int(cu[-1]), 16, 128), generator=gen).to(torch.bfloat16).to(DEV)
+    far_table = torch.where(table >= 0, table + far, table).to(torch.int32)
+    want = paged_attention_chunk(q, pool, table.to(DEV), lens.to(DEV), cu.to(DEV), 0, kv_scales=scales)
+    got = paged_attention_chunk(q, big, far_table.to(DEV), lens.to(DEV), cu.to(DEV), 0, kv_scales=big_scales)
+    assert torch.equal(got, want) and (want != 0).any()
+
+
+def test_no_pages_and_no_tokens():
+    _say("chunk without pages")
+    pool = torch.zeros((2, 1, 2, 2, 16, 64), dtype=torch.bfloat16, device=DEV)
+    q = torch.ones((5, 4, 64), dtype=torch.bfloat16, device=DEV)
+    cu = torch.tensor([0, 5], dtype=torch.int32, device=DEV)
+    table = torch.empty((1, 0), dtype=torch.int32, device=DEV)
+    for n in (0, 5):
+        out = paged_attention_chunk(q, pool, table, torch.tensor([n], dtype=torch.int32, device=DEV), cu, 0)
+        assert (out == 0).all()
+    assert paged_attention_chunk(q[:0], pool, table, cu[:1], cu, 0).shape == (0, 4, 64)
