@@ -245,3 +245,41 @@ def test_append_matches_quantize_append():
                     torch.arange(B + 1, device=DEV), 0, kv_scales=b[1])
         assert torch.equal(a[0].view(torch.uint8), b[0].view(torch.uint8)), codec
         assert torch.equal(a[1], b[1]), codec
+
+
+@pytest.mark.parametrize("D,rot", [(128, 128), (80, 32), (30, 10)])
+def test_in_place(D, rot):
+    _say(f"rotation in place D={D} rot={rot}")
+    gen = torch.Generator().manual_seed(D)
+    q, k = (torch.randn((37, h, D), generator=gen).to(torch.bfloat16).to(DEV) for h in (9, 3))
+    w = torch.randn(D, generator=gen).to(DEV)
+    pos = torch.randint(0, 50, (37,), generator=gen).to(DEV)
+    table = rope_table(50, rot, device=DEV)
+    want = qk_norm_rope(q, k, table, pos, w, w)
+    got = qk_norm_rope(q, k, table, pos, w, w, query_out=q, key_out=k)
+    assert got[0] is q and got[1] is k and torch.equal(q, want[0]) and torch.equal(k, want[1])
+
+
+@pytest.mark.parametrize("kv", ["bf16", "int8", "fp8"])
+def test_append_past_32_bits(kv):
+    """Pages past 4 GiB of a pool take what the same pages of a small one do."""
+    _say(f"append past 32 bits {kv}")
+    gen = torch.Generator().manual_seed(3)
+    lens = [70, 33]
+    P, table = make_table(lens, 16, gen)
+    pool, scales, _ = make_pool(kv, P, 1, 8, 16, 128, gen, None if kv == "bf16" else "plain")
+    pool, scales = pool.to(DEV), _gpu(scales)
+    far = (1 << 32) // (2 * 8 * 16 * 128 * pool.element_size()) + 3
+    big = torch.empty((far + P, *pool.shape[1:]), dtype=pool.dtype, device=DEV)
+    big[far:] = pool
+    big_scales = None
+    if scales is not None:
+        big_scales = torch.zeros((far + P, *scales.shape[1:]), device=DEV)
+        big_scales[far:] = scales
+    k, v = (torch.randn((43, 8, 128), generator=gen).to(torch.bfloat16).to(DEV) for _ in range(2))
+    batch = (torch.tensor(lens, dtype=torch.int32, device=DEV), torch.tensor([0, 40, 43], dtype=torch.int32, device=DEV), 0)
+    rope_append(None, k, v, pool, table.to(DEV), *batch, kv_scales=scales)
+    rope_append(None, k, v, big, torch.where(table >= 0, table + far, table).to(torch.int32).to(DEV), *batch,
+                kv_scales=big_scales)
+    assert torch.equal(big[far:].view(torch.uint8), pool.view(torch.uint8))
+    assert scales is None or torch.equal(big_scales[far:], scales)
