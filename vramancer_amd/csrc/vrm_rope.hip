@@ -130,7 +130,9 @@ __device__ __forceinline__ bool locate(const RopeArgs& a, int n, Token& t) {
   t.pos = 0;
   if (a.cu) {
     int lo = 0, hi = a.B - 1;
-    if (a.N == a.B && a.cu[n] == n) lo = hi = n;  // one token per sequence
+    // one token per sequence: row n starts sequence n, which is not empty (of
+    // an empty one the row is a later sequence's)
+    if (a.N == a.B && a.cu[n] == n && a.cu[n + 1] > n) lo = hi = n;
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
       if (a.cu[mid] <= n)
