@@ -15,12 +15,17 @@
 //
 // Precision.  Scores, maxima, sums and accumulators are float32.  Int8 and
 // e4m3 codes are exact in bf16 and fp16, so K enters as codes and its scale
-// multiplies the scores.  Weights are rounded to the 16-bit type once (half a
-// step, 2^-9 or 2^-12, independent from token to token: below the rounding of
-// the output for two tokens or more); over quantized values they are bf16
-// (fp16 would overflow under large scales), for fp16 queries as a high and a
-// low part.
+// multiplies the scores.  Weights are rounded to the 16-bit type once, because
+// the second product takes 16-bit operands only: by at most half a step, 2^-8
+// (bf16) or 2^-11 (fp16) of each, independent from token to token, where the
+// output's own rounding is as large.  fp16 has a least step besides, 2^-24:
+// fp16 weights are taken relative to a reference that keeps a row's largest
+// between 2^7 and 2^15 (kMaxBias), so that it is at most 2^-31 of that one.
+// Over quantized values weights are bf16 (fp16 would overflow under large
+// scales), for fp16 queries as a high and a low part.
 #pragma once
+#include <type_traits>
+
 #include "vrm_chunk.h"
 
 namespace vrm {
@@ -141,12 +146,18 @@ __device__ __forceinline__ float top_of(const f32x16& s) {
   return top;
 }
 
-// The running maximum moves only when it would leave weights above 2^8: the
-// accumulators are rescaled a few times per row, not per block.
-template <int NB>
+// Weights are 2^(score - m).  The reference m is moved to kMaxBias below the
+// running maximum, and only when that is kMaxLag above the maximum it was last
+// moved for: the accumulators are rescaled a few times per row, not per block,
+// and a row's largest weight stays between 2^kMaxBias and 2^(kMaxBias +
+// kMaxLag).  P is the weights' type.
+constexpr float kMaxLag = 8.f;
+template <typename P>
+constexpr float kMaxBias = std::is_same_v<P, F16> ? 7.f : 0.f;
+template <typename P, int NB>
 __device__ __forceinline__ void raise_max(float top, float& m, float& l, f32x16 (&o)[NB]) {
-  if (__builtin_expect(__any(top > m + 8.f), 0)) {
-    const float next = fmaxf(m, top);
+  if (__builtin_expect(__any(top > m + (kMaxBias<P> + kMaxLag)), 0)) {
+    const float next = fmaxf(m, top - kMaxBias<P>);
     const float f = next == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - next);
 #pragma unroll
     for (int n = 0; n < NB; ++n)
@@ -556,7 +567,7 @@ __device__ __forceinline__ void few_rows(const ChunkArgs& a, const Item& it, int
       __syncwarp();
       if constexpr (QUANT) scale_scores(own_scale[wave][0], half, s);
       if (needs_mask(a, g, t0, there)) mask_scores(a, it, g, t0, there, half, s);
-      raise_max<NB>(xor_max<32>(top_of(s)) * a.sc, m, l, o);
+      raise_max<PT, NB>(xor_max<32>(top_of(s)) * a.sc, m, l, o);
       const float ref = m == -INFINITY ? 0.f : m;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
@@ -686,7 +697,7 @@ __global__ void __launch_bounds__(kChunkThreads, DP <= 128 ? 2 : 1) chunk_attn_k
       if (needs_mask(a, g, t0 + 32 * u, bits)) mask_scores(a, it, g, t0 + 32 * u, bits, half, s[u]);
       top = fmaxf(top, top_of(s[u]));
     }
-    raise_max<NB>(xor_max<32>(top) * a.sc, m, l, o);
+    raise_max<PT, NB>(xor_max<32>(top) * a.sc, m, l, o);
     const float ref = m == -INFINITY ? 0.f : m;
 #pragma unroll
     for (int u = 0; u < NS; ++u)
@@ -871,7 +882,7 @@ __global__ void __launch_bounds__(kLargeThreads, 1) chunk_attn_large_kernel(Chun
           top = fmaxf(top, top_of(now[u]));
         }
       }
-      raise_max<NB>(xor_max<32>(top) * a.sc, m, l, o);
+      raise_max<PT, NB>(xor_max<32>(top) * a.sc, m, l, o);
       const float ref = m == -INFINITY ? 0.f : m;
       top = -INFINITY;
       typename PT::v8 pb[2 * NS], low[2 * NS];
