@@ -410,6 +410,16 @@ struct Stage {
   }
 };
 
+// Dims D .. DP - 1 of a block's V^T, which no code is staged for: zeros, so that
+// the accumulators of those dims are too (any_nan looks at all).  Once per
+// buffer, by the whole workgroup.
+template <int DP>
+__device__ __forceinline__ void clear_padding(const ChunkArgs& a, uint8_t* v_lds) {
+  const int pad = DP - a.D;
+  for (int i = threadIdx.x; i < 8 * pad; i += blockDim.x)  // [4 steps of 16 tokens][2 halves] of DP x 16 bytes
+    *reinterpret_cast<uint4*>(v_lds + (i / pad * DP + a.D + i % pad) * 16) = make_uint4(0, 0, 0, 0);
+}
+
 // Scores of 32 tokens times their K scales, and weights times their V scales.
 __device__ __forceinline__ void scale_scores(const float* ks, int half, f32x16& s) {
 #pragma unroll
@@ -735,6 +745,7 @@ __global__ void __launch_bounds__(kChunkThreads, DP <= 128 ? 2 : 1) chunk_attn_k
   Gather st(a, it, kvh, to, shared);
   st.page = st.page_of(from);
   if (from < to) st.load(from);
+  if (QUANT && a.D < DP) clear_padding<DP>(a, v_lds);
   for (int block = from; block < to; ++block) {
     __syncthreads();  // the block before is computed
     st.put(block, k_lds, v_lds);
@@ -814,6 +825,8 @@ __global__ void __launch_bounds__(kLargeThreads, 1) chunk_attn_large_kernel(Chun
     second.page = st.page_of(from + 1);
     st.load(from);
     second.load(from + 1);
+    if (QUANT && a.D < DP)
+      for (int i = 0; i < 4; ++i) clear_padding<DP>(a, lds + i * Tile::kBytes + Tile::kKBytes);
     __syncthreads();
     st.put(from, lds, lds + Tile::kKBytes);
     second.put(from + 1, lds + Tile::kBytes, lds + Tile::kBytes + Tile::kKBytes);

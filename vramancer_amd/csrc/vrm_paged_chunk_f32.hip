@@ -107,6 +107,11 @@ __global__ void __launch_bounds__(kChunkThreads, DP <= 128 ? 2 : 1) chunk_attn_f
     const uint32_t mask = (uint32_t)__ballot(there);
     if (lane == 0) there_lds[block & 3] = mask;
   };
+  // dims D .. DP - 1 of V, which no code is staged for, are zeros (any_nan looks at all)
+  if (QUANT && a.D < DP) {
+    const int pad = DP - a.D;
+    for (int i = tid; i < TN * pad; i += kChunkThreads) v_lds[i / pad * VS + a.D + i % pad] = 0.f;
+  }
   uint4 kr[NP], vr[NP];
   float ksc = 0.f, vsc = 0.f;
   constexpr int kPerRow = DP / E;
