@@ -657,6 +657,21 @@ int vrm_paged_chunk_attention(const void* query, int q_dtype, long long q_token_
                               int window, int kv_dtype, vrm_stream_t stream);
 
 /*
+ * The same for a caller that knows about how many tokens a sequence has
+ * (expected_context; the new tokens' mean where sequences differ), which a table
+ * wider than its contexts does not say.  It only bears on the size of the
+ * tiles: any value gives attention over all of context_lens, and 0 is the call
+ * above.  The workspace is the same.
+ */
+int vrm_paged_chunk_attention_expecting(
+    const void* query, int q_dtype, long long q_token_stride, long long q_head_stride,
+    const void* kv_pool, const float* kv_scales, const int32_t* page_table,
+    const int32_t* context_lens, const int32_t* cu_seqlens, void* out, float* lse, void* workspace,
+    size_t workspace_bytes, int N, int B, int H, int KH, int D, int PS, int L, int P, int max_pp,
+    int layer_idx, float scale, int causal, int window, int expected_context, int kv_dtype,
+    vrm_stream_t stream);
+
+/*
  * RMS norm of every query and key head, then the rotation of its first
  * rotary_dim dims by position, in float32 and rounded once:
  *   x' = weight x / sqrt(mean(x^2) + eps)         (where the weight is given)

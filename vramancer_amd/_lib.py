@@ -90,6 +90,8 @@ SIGNATURES = {
                              _p, _p, _i, _p, _p, _p] + [_i] * 10 + [_p]),
     "vrm_paged_chunk_workspace_bytes": (_sz, [_i] * 9),
     "vrm_paged_chunk_attention": (_i, [_p, _i, _ll, _ll] + [_p] * 8 + [_sz] + [_i] * 10 + [_f, _i, _i, _i, _p]),
+    "vrm_paged_chunk_attention_expecting": (_i, [_p, _i, _ll, _ll] + [_p] * 8 + [_sz] + [_i] * 10
+                                            + [_f, _i, _i, _i, _i, _p]),
 }
 
 

@@ -120,7 +120,13 @@ constexpr int kMinBlocks = 2;
 // and 22.5 us at 128 rows, 37.2 and 36.3 at 1024; 8 such 32.5 and 31.9 at 96,
 // 85.0 and 60.9 at 384; 64 such 114 and 120 at 64, 140 and 135 at 128, 815 and
 // 658 at 1024; 64 after 200 tokens 41 and 60 at 128, 226 and 242 at 1024.
+// The tokens are those that a tile sees: the table's width, or what the caller
+// expects, and not more than a window with the tile's own tokens and a block at
+// its edge.  Within windows, after 4000 tokens: 8 sequences of 8192 rows 136
+// and 188 us at a window of 64, 338 and 343 at 768, 417 and 402 at 1000, 730
+// and 622 at 2000; one of 2048 rows 21 and 27, 34 and 36, 36 and 37, 48 and 44.
 constexpr double kLargeWork = 1 << 24;
+constexpr long long kLargeTokens = 1024;
 
 int pool_kind(int kv_dtype) {
   switch (kv_dtype) {
@@ -135,7 +141,11 @@ int pool_kind(int kv_dtype) {
   }
 }
 
-bool plan_chunk(int N, int B, int H, int KH, int D, int PS, int max_pp, int q_dtype, int kv_dtype, ChunkPlan& p) {
+// expected: tokens that a sequence has, as far as the caller knows (0: the table's
+// width).  With window it bears on the tiles' size only; items are counted for
+// the table.
+bool plan_chunk(int N, int B, int H, int KH, int D, int PS, int max_pp, int q_dtype, int kv_dtype, int expected,
+                int window, ChunkPlan& p) {
   const long long G = H / KH;
   if ((long long)N * H > 0x7fff0000LL) return false;
   p.kind = pool_kind(kv_dtype);
@@ -146,8 +156,11 @@ bool plan_chunk(int N, int B, int H, int KH, int D, int PS, int max_pp, int q_dt
   const int block = p.wide ? 32 : 64;
   const long long tokens = (long long)max_pp * PS;           // of a sequence, at most
   const long long blocks = (tokens + block - 1) / block;
-  const bool large = !p.wide && D <= 128 && N * G >= 128LL * B && tokens >= 1024 &&
-                     (double)(N * G) * KH * (double)tokens >= kLargeWork;
+  long long seen = tokens;  // by a large tile
+  if (expected > 0 && expected < seen) seen = expected;
+  if (window > 0 && window + 256 / G + block < seen) seen = window + 256 / G + block;
+  const bool large = !p.wide && D <= 128 && N * G >= 128LL * B && seen >= kLargeTokens &&
+                     (double)(N * G) * KH * (double)seen >= kLargeWork;
   p.tile_rows = large ? 256 : 128;
   const int wanted = large ? 256 : 512;  // workgroups resident at once
   const long long vtiles = N * G / p.tile_rows + B;
@@ -185,11 +198,12 @@ using namespace vrm;
 
 extern "C" size_t vrm_paged_chunk_workspace_bytes(int N, int B, int H, int KH, int D, int PS, int max_pp, int q_dtype,
                                                   int kv_dtype) {
-  ChunkPlan p;
+  ChunkPlan large, small;  // with the larger tiles, if these sizes can have them, and with the others
   if (bad_sizes(N, B, H, KH, D, PS, max_pp) || D > 256 || pool_kind(kv_dtype) < 0 ||
-      !plan_chunk(N, B, H, KH, D, PS, max_pp, q_dtype, kv_dtype, p))
+      !plan_chunk(N, B, H, KH, D, PS, max_pp, q_dtype, kv_dtype, 0, 0, large) ||
+      !plan_chunk(N, B, H, KH, D, PS, max_pp, q_dtype, kv_dtype, 1, 0, small))
     return 0;
-  return p.bytes;
+  return large.bytes > small.bytes ? large.bytes : small.bytes;
 }
 
 extern "C" int vrm_paged_chunk_attention(const void* query, int q_dtype, long long q_token_stride,
@@ -199,10 +213,23 @@ extern "C" int vrm_paged_chunk_attention(const void* query, int q_dtype, long lo
                                          size_t workspace_bytes, int N, int B, int H, int KH, int D, int PS, int L,
                                          int P, int max_pp, int layer_idx, float scale, int causal, int window,
                                          int kv_dtype, vrm_stream_t stream) {
+  return vrm_paged_chunk_attention_expecting(query, q_dtype, q_token_stride, q_head_stride, kv_pool, kv_scales,
+                                             page_table, context_lens, cu_seqlens, out, lse, workspace,
+                                             workspace_bytes, N, B, H, KH, D, PS, L, P, max_pp, layer_idx, scale,
+                                             causal, window, 0, kv_dtype, stream);
+}
+
+extern "C" int vrm_paged_chunk_attention_expecting(
+    const void* query, int q_dtype, long long q_token_stride, long long q_head_stride, const void* kv_pool,
+    const float* kv_scales, const int32_t* page_table, const int32_t* context_lens, const int32_t* cu_seqlens,
+    void* out, float* lse, void* workspace, size_t workspace_bytes, int N, int B, int H, int KH, int D, int PS, int L,
+    int P, int max_pp, int layer_idx, float scale, int causal, int window, int expected_context, int kv_dtype,
+    vrm_stream_t stream) {
   const char* who = "vrm_paged_chunk_attention";
-  if (bad_sizes(N, B, H, KH, D, PS, max_pp) || L <= 0 || P <= 0 || window < 0) {
-    set_error("%s: bad sizes (N=%d B=%d H=%d KH=%d D=%d PS=%d L=%d P=%d max_pp=%d window=%d; H a multiple of KH)", who,
-              N, B, H, KH, D, PS, L, P, max_pp, window);
+  if (bad_sizes(N, B, H, KH, D, PS, max_pp) || L <= 0 || P <= 0 || window < 0 || expected_context < 0) {
+    set_error("%s: bad sizes (N=%d B=%d H=%d KH=%d D=%d PS=%d L=%d P=%d max_pp=%d window=%d "
+              "expected_context=%d; H a multiple of KH)",
+              who, N, B, H, KH, D, PS, L, P, max_pp, window, expected_context);
     return VRM_ERR_ARG;
   }
   if (layer_idx < 0 || layer_idx >= L) {
@@ -232,7 +259,7 @@ extern "C" int vrm_paged_chunk_attention(const void* query, int q_dtype, long lo
     return VRM_ERR_UNSUPPORTED;
   }
   ChunkPlan p;
-  if (!plan_chunk(N, B, H, KH, D, PS, max_pp, q_dtype, kv_dtype, p)) {
+  if (!plan_chunk(N, B, H, KH, D, PS, max_pp, q_dtype, kv_dtype, expected_context, window, p)) {
     set_error("%s: too many rows (N=%d H=%d B=%d)", who, N, H, B);
     return VRM_ERR_UNSUPPORTED;
   }

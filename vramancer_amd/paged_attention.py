@@ -164,6 +164,7 @@ class ChunkBatch:
     context_lens: Any       # [B] int32, the new tokens included
     cu_seqlens: Any         # [B + 1] int32
     places: List[Tuple[int, int]]  # (page, slot) of every new token, in row order
+    expected_context: Optional[int] = None  # mean context of the new tokens
 
     @property
     def num_tokens(self) -> int:
@@ -422,8 +423,10 @@ class PagedKVCacheManager:
         host[B * (width + 1)] = 0
         host[B * (width + 1) + 1:] = np.cumsum(counts)
         dev = torch.from_numpy(host).to(self._gpu_pool.device)
+        lens = host[B * width:B * (width + 1)].tolist()
+        mean = -(-sum(n * c for n, c in zip(lens, counts)) // max(1, sum(counts)))
         return ChunkBatch(ids, counts, dev[:B * width].view(B, width), dev[B * width:B * (width + 1)],
-                          dev[B * (width + 1):], places)
+                          dev[B * (width + 1):], places, mean or None)
 
     @property
     def gpu_pool(self) -> Any:
@@ -624,7 +627,8 @@ class PagedKVCacheManager:
             raise RuntimeError(f"query must be [{chunk.num_tokens}, H, {self.config.head_dim}], got shape "
                                f"{tuple(query.shape)}")
         return paged_attention_chunk(query, self._gpu_pool, chunk.page_table, chunk.context_lens, chunk.cu_seqlens,
-                                     layer_idx, scale, kv_scales=self._kv_scales, causal=causal, window=window)
+                                     layer_idx, scale, kv_scales=self._kv_scales, causal=causal, window=window,
+                                     expected_context=chunk.expected_context)
 
     def flush_compression(self) -> None:
         """Compresses every queued row, all layers at once, into the TurboQuant

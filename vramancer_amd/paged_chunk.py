@@ -176,6 +176,7 @@ def paged_attention_chunk(
     out: Any = None,
     lse: Any = None,
     workspace: Any = None,
+    expected_context: Optional[int] = None,
 ) -> Any:
     """Attention of each sequence's new tokens over its pages; the new tokens'
     keys and values are in the cache already.
@@ -188,6 +189,11 @@ def paged_attention_chunk(
     left as they were, undefined in an output allocated here).  ``lse``
     optionally takes ln sum exp of the scaled scores, [N, H] float32, for
     ``combine_attention``.
+
+    ``expected_context`` is about how many tokens a sequence has (their mean
+    over the new tokens), for callers that know it and whose table is wider
+    than that, as one of a fixed width for a captured graph is.  It chooses the
+    kernel's tiles for such contexts; what is attended does not depend on it.
 
     Calls may run at once on several streams if they share neither output nor
     ``workspace``; results do not depend on what a workspace held before, and
@@ -203,6 +209,8 @@ def paged_attention_chunk(
     page_table, context_lens, cu_seqlens, B = check_batch(page_table, context_lens, cu_seqlens)
     if window is not None and not 0 < window < 1 << 31:
         raise RuntimeError(f"window must be a positive number of tokens, got {window}")
+    if expected_context is not None and expected_context <= 0:
+        raise RuntimeError(f"expected_context must be a positive number of tokens, got {expected_context}")
     if query.stride(2) != 1 and D > 1:
         query = query.contiguous()
     if out is None:
@@ -222,9 +230,10 @@ def paged_attention_chunk(
     ws_bytes = workspace.numel() * workspace.element_size() if workspace is not None else 0
     ptr = _lib.ptr
     q_n, q_h, _ = query.stride()
-    rc = launch(query, _lib.load().vrm_paged_chunk_attention, query.data_ptr(), q_code, q_n, q_h, kv_pool.data_ptr(),
-                ptr(kv_scales), page_table.data_ptr(), context_lens.data_ptr(), cu_seqlens.data_ptr(), out.data_ptr(),
-                ptr(lse), ptr(workspace), ws_bytes, N, B, H, KH, D, PS, L, P, max_pp, int(layer_idx),
-                1.0 / math.sqrt(D) if scale is None else float(scale), 1 if causal else 0, window or 0, code)
+    rc = launch(query, _lib.load().vrm_paged_chunk_attention_expecting, query.data_ptr(), q_code, q_n, q_h,
+                kv_pool.data_ptr(), ptr(kv_scales), page_table.data_ptr(), context_lens.data_ptr(),
+                cu_seqlens.data_ptr(), out.data_ptr(), ptr(lse), ptr(workspace), ws_bytes, N, B, H, KH, D, PS, L, P,
+                max_pp, int(layer_idx), 1.0 / math.sqrt(D) if scale is None else float(scale), 1 if causal else 0,
+                window or 0, min(int(expected_context or 0), 0x7fffffff), code)
     _lib.check(rc, "paged_attention_chunk")
     return out
