@@ -156,7 +156,8 @@ class PageTableEntry:
 @dataclass
 class ChunkBatch:
     """New tokens of an ordered batch of requests (``append_chunk``), as the
-    chunk operators take them; good until one of the requests changes again."""
+    chunk operators take them; good until one of the requests changes again,
+    which ``write_chunk`` and ``compute_attention_chunk`` check."""
 
     request_ids: List[str]
     counts: List[int]       # new tokens of each request
@@ -165,6 +166,11 @@ class ChunkBatch:
     cu_seqlens: Any         # [B + 1] int32
     places: List[Tuple[int, int]]  # (page, slot) of every new token, in row order
     expected_context: Optional[int] = None  # mean context of the new tokens
+    # where it is from: its manager, that manager's epoch when the batch was last
+    # found good, and each request's entry and token count
+    owner: Any = field(default=None, repr=False, compare=False)
+    epoch: int = field(default=0, repr=False, compare=False)
+    states: List[tuple] = field(default_factory=list, repr=False, compare=False)
 
     @property
     def num_tokens(self) -> int:
@@ -414,6 +420,7 @@ class PagedKVCacheManager:
                 e.num_tokens += n
             self._peak_usage = max(self._peak_usage, self.config.max_pages - len(self._free_pages))
             self._epoch += 1
+            epoch, states = self._epoch, [(e, e.num_tokens) for e in entries]
             width = max([1] + [len(e.pages) for e in entries])
             B = len(ids)
             host = np.full(B * (width + 2) + 1, -1, dtype=np.int32)  # table, lengths, offsets: one upload
@@ -426,7 +433,23 @@ class PagedKVCacheManager:
         lens = host[B * width:B * (width + 1)].tolist()
         mean = -(-sum(n * c for n, c in zip(lens, counts)) // max(1, sum(counts)))
         return ChunkBatch(ids, counts, dev[:B * width].view(B, width), dev[B * width:B * (width + 1)],
-                          dev[B * (width + 1):], places, mean or None)
+                          dev[B * (width + 1):], places, mean or None, self, epoch, states)
+
+    def _check_chunk(self, chunk: ChunkBatch, what: str) -> None:
+        """Raises where a request of the batch has changed since append_chunk
+        (freed, appended to, replaced): its pages may be another's by now.  A
+        batch made by hand has no owner and is its maker's concern."""
+        if chunk.owner is None:
+            return
+        if chunk.owner is not self:
+            raise RuntimeError(f"{what} takes a batch that this manager's append_chunk made")
+        if chunk.epoch == self._epoch:
+            return
+        with self._lock:
+            for rid, (entry, n) in zip(chunk.request_ids, chunk.states):
+                if self._page_tables.get(rid) is not entry or entry.num_tokens != n:
+                    raise RuntimeError(f"{what}: request {rid!r} has changed since append_chunk made this batch")
+            chunk.epoch = self._epoch
 
     @property
     def gpu_pool(self) -> Any:
@@ -601,6 +624,7 @@ class PagedKVCacheManager:
         from .paged_chunk import rope_append
 
         self._require_pool("write_chunk")
+        self._check_chunk(chunk, "write_chunk")
         if key.dim() != 3 or key.shape[0] != chunk.num_tokens:
             raise RuntimeError(f"key must be [{chunk.num_tokens}, {self.config.num_kv_heads}, {self.config.head_dim}], "
                                f"got shape {tuple(key.shape)}")
@@ -623,6 +647,7 @@ class PagedKVCacheManager:
         from .paged_chunk import paged_attention_chunk
 
         self._require_pool("compute_attention_chunk")
+        self._check_chunk(chunk, "compute_attention_chunk")
         if query.dim() != 3 or query.shape[0] != chunk.num_tokens:
             raise RuntimeError(f"query must be [{chunk.num_tokens}, H, {self.config.head_dim}], got shape "
                                f"{tuple(query.shape)}")
