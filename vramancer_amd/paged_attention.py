@@ -167,7 +167,7 @@ class ChunkBatch:
     places: List[Tuple[int, int]]  # (page, slot) of every new token, in row order
     expected_context: Optional[int] = None  # mean context of the new tokens
     # where it is from: its manager, that manager's epoch when the batch was last
-    # found good, and each request's entry and token count
+    # found good, and each request's entry, token count and pages added to it
     owner: Any = field(default=None, repr=False, compare=False)
     epoch: int = field(default=0, repr=False, compare=False)
     states: List[tuple] = field(default_factory=list, repr=False, compare=False)
@@ -420,7 +420,7 @@ class PagedKVCacheManager:
                 e.num_tokens += n
             self._peak_usage = max(self._peak_usage, self.config.max_pages - len(self._free_pages))
             self._epoch += 1
-            epoch, states = self._epoch, [(e, e.num_tokens) for e in entries]
+            epoch, states = self._epoch, [(e, e.num_tokens, m) for e, m in zip(entries, more)]
             width = max([1] + [len(e.pages) for e in entries])
             B = len(ids)
             host = np.full(B * (width + 2) + 1, -1, dtype=np.int32)  # table, lengths, offsets: one upload
@@ -446,10 +446,29 @@ class PagedKVCacheManager:
         if chunk.epoch == self._epoch:
             return
         with self._lock:
-            for rid, (entry, n) in zip(chunk.request_ids, chunk.states):
-                if self._page_tables.get(rid) is not entry or entry.num_tokens != n:
-                    raise RuntimeError(f"{what}: request {rid!r} has changed since append_chunk made this batch")
+            self._check_states_locked(chunk, what)
             chunk.epoch = self._epoch
+
+    def _check_states_locked(self, chunk: ChunkBatch, what: str) -> None:
+        for rid, (entry, n, _) in zip(chunk.request_ids, chunk.states):
+            if self._page_tables.get(rid) is not entry or entry.num_tokens != n:
+                raise RuntimeError(f"{what}: request {rid!r} has changed since append_chunk made this batch")
+
+    def _take_back(self, chunk: ChunkBatch) -> None:
+        """Undoes the append_chunk that made a batch, for a step that failed:
+        its tokens, their new pages (in the order they came, so that the free
+        list is as it was) and their rows in the compression queue.  What they
+        wrote lies behind the requests' last tokens; an fp8 page's scale keeps
+        what they raised it to.  Raises, and changes nothing, where a request
+        has changed since."""
+        with self._lock:
+            self._check_states_locked(chunk, "_take_back")
+            for (entry, n, added), count in reversed(list(zip(chunk.states, chunk.counts))):
+                entry.num_tokens = n - count
+                for _ in range(added):
+                    self._release_locked(entry.pages.pop())
+            self._pending_compress = [item for item in self._pending_compress if item[5] is not chunk.places]
+            self._epoch += 1
 
     @property
     def gpu_pool(self) -> Any:
@@ -467,26 +486,29 @@ class PagedKVCacheManager:
             return np.array([e.num_tokens if (e := self._page_tables.get(rid)) is not None else 0
                              for rid in request_ids], dtype=np.int64)
 
+    def _release_locked(self, page_id: int) -> bool:
+        """Drops a request's hold of a page; whether it went back to the free list."""
+        page = self._pages[page_id]
+        page.ref_count -= 1
+        if page.ref_count > 0:
+            return False
+        page.allocated = False
+        page.ref_count = 0
+        if self._tq_slots is not None:
+            # its codes belong to the old request: the next owner's
+            # tokens are compressed afresh
+            self._tq_slots[page_id] = 0
+        self._free_pages.append(page_id)
+        self._total_frees += 1
+        return True
+
     def free(self, request_id: str) -> int:
         """Drops a request; returns how many pages went back to the free list."""
         with self._lock:
             entry = self._page_tables.pop(request_id, None)
             if entry is None:
                 return 0
-            freed = 0
-            for page_id in entry.pages:
-                page = self._pages[page_id]
-                page.ref_count -= 1
-                if page.ref_count <= 0:
-                    page.allocated = False
-                    page.ref_count = 0
-                    if self._tq_slots is not None:
-                        # its codes belong to the old request: the next owner's
-                        # tokens are compressed afresh
-                        self._tq_slots[page_id] = 0
-                    self._free_pages.append(page_id)
-                    freed += 1
-                    self._total_frees += 1
+            freed = sum(self._release_locked(page_id) for page_id in entry.pages)
             self._epoch += 1
             return freed
 

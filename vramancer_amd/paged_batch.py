@@ -182,6 +182,17 @@ class PagedChunkCache(PagedBatchCache):
     def _begin_chunk(self, q: int) -> None:
         self._chunk = self.manager.append_chunk(self.request_ids, [q] * len(self.request_ids))
 
+    def _undo_step(self) -> bool:
+        """Takes the tokens of a step that failed back; False where a request
+        has changed in the meantime, whose tokens stay then."""
+        chunk, self._chunk = self._chunk, None
+        try:
+            if chunk is not None:
+                self.manager._take_back(chunk)
+        except RuntimeError:
+            return False
+        return True
+
     def _step_chunk(self, q: int) -> ChunkBatch:
         if self._chunk is None or any(n != q for n in self._chunk.counts):
             raise RuntimeError("a step starts with the update of layer 0, and every layer has its tokens")
@@ -255,13 +266,18 @@ def chunk_step(model, manager: PagedKVCacheManager, request_ids: Sequence[str], 
     the positions after those it has (a prompt's chunk, drafted tokens to
     verify).  Returns the logits [B, q, vocab].  The model must use
     ``enable_paged_attention``; pass the ``cache`` of the previous step to
-    reuse it."""
-    if cache is None or cache.request_ids != list(request_ids):
+    reuse it.  A forward that raises leaves the requests as they were."""
+    if not isinstance(cache, PagedChunkCache) or cache.manager is not manager or cache.request_ids != list(request_ids):
         cache = PagedChunkCache(manager, request_ids)
     ids = input_ids.reshape(len(request_ids), -1)
     pos = torch.from_numpy(cache.token_counts()).to(ids.device).reshape(-1, 1)
     pos = pos + torch.arange(ids.shape[1], device=ids.device)
-    out = model(ids, position_ids=pos, past_key_values=cache, use_cache=True)
+    cache._chunk = None  # (the step before is no concern of this one)
+    try:
+        out = model(ids, position_ids=pos, past_key_values=cache, use_cache=True)
+    except BaseException:
+        cache._undo_step()
+        raise
     return out.logits if hasattr(out, "logits") else out[0]
 
 
@@ -271,14 +287,29 @@ def prefill_chunked(model, manager: PagedKVCacheManager, request_id: str, input_
     at a time, straight into its pages, after the tokens that it has already
     (a prefix, an earlier turn).  Returns the last-position logits [1, vocab].
 
-    Unlike ``prefill`` it keeps no second copy of the cache."""
+    Unlike ``prefill`` it keeps no second copy of the cache.  Where a chunk
+    fails (no page left, a model that raises) the request is left as it was
+    before the first one."""
     if chunk_size < 1:
         raise RuntimeError(f"chunk_size must be positive, got {chunk_size}")
     ids = input_ids.reshape(1, -1)
     if ids.shape[1] == 0:
         raise RuntimeError("an empty prompt has no logits")
+    new = request_id not in manager.request_ids()
     manager.allocate(request_id)
     cache = PagedChunkCache(manager, [request_id])
-    for start in range(0, ids.shape[1], chunk_size):
-        logits = chunk_step(model, manager, [request_id], ids[:, start:start + chunk_size], cache)
+    done = []
+    try:
+        for start in range(0, ids.shape[1], chunk_size):
+            logits = chunk_step(model, manager, [request_id], ids[:, start:start + chunk_size], cache)
+            done.append(cache._chunk)
+    except BaseException:
+        for chunk in reversed(done):
+            cache._chunk = chunk
+            if not cache._undo_step():
+                break
+        else:
+            if new:
+                manager.free(request_id)
+        raise
     return logits[:, -1]
