@@ -53,7 +53,7 @@ def chunk_workspace(query, kv_pool, batch: int, max_pages_per_seq: int):
 
 
 def check_pool(kv_pool, kv_scales, D: int):
-    """(pool, scales, kv_dtype code) of a pool as the C ABI takes it."""
+    """The kv_dtype code of a pool as the C ABI takes it."""
     if kv_pool.dim() != 6:
         raise RuntimeError(f"kv_pool must be [P, L, 2, KH, PS, D], got shape {tuple(kv_pool.shape)}")
     P, L, two, KH, PS, Dp = kv_pool.shape
