@@ -156,3 +156,24 @@ def test_tokens_taken_back():
     mgr._take_back(chunk)
     assert list(mgr.token_counts(["a", "c"])) == [0, 5] and len(mgr._free_pages) == 11
     assert mgr.append_chunk(["a"], [1]).places[0][0] != mgr._page_tables["c"].pages[0]
+
+
+def test_block_table_after_tokens_taken_back():
+    """A decode between an append and its undoing kept the pages that went
+    back: the next one must not read them."""
+    print("[case] block table after take back", flush=True)
+    mgr = _manager(max_pages=6)
+    gen = torch.Generator().manual_seed(2)
+    for rid in "ab":
+        mgr.allocate(rid)
+    chunk = mgr.append_chunk(["a"], [20])
+    q = torch.randn((1, 4, 64), generator=gen).to(DEV)
+    mgr.compute_attention_decode(q, ["a"], 0)
+    mgr._take_back(chunk)
+    for rid, n in (("b", 16), ("a", 20)):
+        k, v = (torch.randn((n, 2, 64), generator=gen).to(DEV) for _ in range(2))
+        mgr.write_chunk(0, mgr.append_chunk([rid], [n]), k, v)
+    want = torch.nn.functional.scaled_dot_product_attention(  # of a's 20 tokens
+        q[0, :, None].cpu(), k.cpu().transpose(0, 1).repeat_interleave(2, 0), v.cpu().transpose(0, 1).repeat_interleave(2, 0))
+    got = mgr.compute_attention_decode(q, ["a"], 0)[0].cpu()
+    assert ((got - want[:, 0]).abs() <= 2e-3 + 1e-2 * want[:, 0].abs()).all()

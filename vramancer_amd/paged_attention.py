@@ -468,6 +468,7 @@ class PagedKVCacheManager:
                 for _ in range(added):
                     self._release_locked(entry.pages.pop())
             self._pending_compress = [item for item in self._pending_compress if item[5] is not chunk.places]
+            self._table_cache = None  # (its patches take page lists to grow only)
             self._epoch += 1
 
     @property
