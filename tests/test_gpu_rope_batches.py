@@ -10,7 +10,7 @@ from chunk_reference import HALF, attend, norm_rope, rope_angles
 from test_gpu_rope import _append, _close
 from vramancer_amd.paged_attention import PagedKVCacheManager, PagedKVConfig
 from vramancer_amd.paged_chunk import chunk_workspace, paged_attention_chunk, rope_append
-from vramancer_amd.rope import rope_table
+from vramancer_amd.rope import qk_norm_rope, rope_table
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -118,3 +118,16 @@ def test_captured_batch_padded_to_its_sequences():
         want, _, reach = attend(q_out[:n].cpu(), pool.double().cpu(), table.cpu(), lens.cpu(), cu.cpu(), 0)
         tol = HALF[torch.bfloat16] * (want.abs() + reach) + 2.0 ** -16 * reach + 1e-30
         assert ((out[:n].cpu().double() - want).abs() <= tol).all(), step
+
+
+def test_more_rows_than_a_grid_dimension_holds():
+    """More than 2^26 rows, a wavefront to each: more than 2^32 threads."""
+    N, D = 34_000_000, 2
+    _say(f"norms of 2 x {N} rows")
+    q = torch.randn((N, 1, D), device=DEV).bfloat16()
+    w = torch.full((D,), 0.75, device=DEV)
+    got = qk_norm_rope(q, q, None, None, w, w)
+    x = q.double()
+    want = 0.75 * x / (x.pow(2).mean(-1, keepdim=True) + 1e-6).sqrt()
+    for y in got:  # half a step of bf16, and the float32 terms
+        assert ((y.double() - want).abs() <= (HALF[torch.bfloat16] + 2.0 ** -19) * want.abs() + 1e-30).all()

@@ -38,6 +38,7 @@ constexpr int kRopeThreads = 256;
 constexpr int kRopeTokens = 16;  // of a page in LDS at a time
 constexpr int kRopeHeads = 4;    // of a token to a group of lanes
 constexpr int kPageHeads = 2;    // of a page to a workgroup
+constexpr uint32_t kGridX = 1u << 23;  // a launch has less than 2^32 threads along x: further workgroups along y
 
 struct RopeArgs {
   const void *q, *k, *v;
@@ -576,16 +577,17 @@ __device__ __forceinline__ void do_page(const RopeArgs& a, int block, PageShared
 
 template <int T, int LG, bool GENERAL, bool QUANT>
 __global__ void __launch_bounds__(kRopeThreads) rope_kernel(RopeArgs a) {
+  const uint32_t block = blockIdx.y * kGridX + blockIdx.x;
   if constexpr (QUANT) {
-    if ((int)blockIdx.x >= a.row_blocks) {
+    if ((int)block >= a.row_blocks) {
       __shared__ __align__(16) PageShared sh;
-      do_page<T, LG, GENERAL>(a, blockIdx.x - a.row_blocks, sh);
+      do_page<T, LG, GENERAL>(a, block - a.row_blocks, sh);
       return;
     }
   }
   constexpr int kLanes = GENERAL ? 64 : LG;
   __shared__ float row[GENERAL ? 4 : 1][GENERAL ? 256 : 1];
-  const uint32_t unit = blockIdx.x * (kRopeThreads / kLanes) + threadIdx.x / kLanes;
+  const uint32_t unit = block * (kRopeThreads / kLanes) + threadIdx.x / kLanes;
   if (unit < (uint32_t)a.N * a.units) do_unit<T, LG, GENERAL>(a, unit, row[GENERAL ? threadIdx.x / 64 : 0]);
 }
 
@@ -605,8 +607,9 @@ void launch_rope(RopeArgs& a, bool fast, hipStream_t st) {
   a.row_blocks = (int)(((long long)a.N * a.units + per - 1) / per);
   const long long pages =
       QUANT ? ((long long)a.N / a.PS + 2LL * a.B) * 2 * ((a.KH + kPageHeads - 1) / kPageHeads) : 0;
-  const dim3 grid((unsigned)(a.row_blocks + pages)), block(kRopeThreads);
-  if (grid.x == 0) return;
+  const uint32_t blocks = (uint32_t)(a.row_blocks + pages);
+  if (blocks == 0) return;
+  const dim3 grid(blocks < kGridX ? blocks : kGridX, (blocks + kGridX - 1) / kGridX), block(kRopeThreads);
   if (lg == 64)
     hipLaunchKernelGGL((rope_kernel<T, 64, true, QUANT>), grid, block, 0, st, a);
   else if (lg == 4)
