@@ -68,3 +68,12 @@ def test_the_workspace_is_enough_for_any_tiles(lib, N, B, kv):
                 assert 0 < _need(lib, N, B, H, KH, D, 16, max_pp, window, expected, kv=kv) <= have
                 seen += 1
     assert seen
+
+
+def test_calls_past_a_grids_threads(lib):
+    """Batches of so many sequences that a launch would wrap are refused."""
+    args = (16, BF, 128, 128, 16, None, 16, 16, 16, 16, None, 16, 1 << 62)
+    for B, KH in ((1 << 20, 32), (1 << 24, 1), (1 << 30, 64)):
+        rc = lib.vrm_paged_chunk_attention(*args, 4, B, KH, KH, 128, 16, 1, 4, 2, 0, 0.1, 1, 0, KV, None)
+        assert rc == -2 and b"too many" in lib.vrm_last_error()
+        assert lib.vrm_paged_chunk_workspace_bytes(4, B, KH, KH, 128, 16, 2, BF, KV) == 0

@@ -175,7 +175,8 @@ bool plan_chunk(int N, int B, int H, int KH, int D, int PS, int max_pp, int q_dt
     items = vtiles + p.target + p.target / 256 + 2;
     if (items > most) items = most;
   }
-  if (items * KH > 0x7fffffffLL) return false;
+  // (a launch with 2^32 threads along x, the merge's 256 a tile too, would wrap)
+  if (items * KH * (large ? kLargeThreads : kChunkThreads) > 0xffffffffLL) return false;
   p.vtiles = (int)vtiles;
   p.items = (int)items;
   p.rec_bytes = p.ml_bytes = p.bytes = 0;
