@@ -77,3 +77,10 @@ def test_calls_past_a_grids_threads(lib):
         rc = lib.vrm_paged_chunk_attention(*args, 4, B, KH, KH, 128, 16, 1, 4, 2, 0, 0.1, 1, 0, KV, None)
         assert rc == -2 and b"too many" in lib.vrm_last_error()
         assert lib.vrm_paged_chunk_workspace_bytes(4, B, KH, KH, 128, 16, 2, BF, KV) == 0
+
+
+@pytest.mark.parametrize("scale", [3e38, -2.4e38, float("inf"), float("nan")])
+def test_scales_past_float32(lib, scale):
+    args = (16, BF, 1024, 128, 16, None, 16, 16, 16, 16, None, None, 0, 2048, 64, 8, 2, 128, 16, 1, 4, 64, 0)
+    assert lib.vrm_paged_chunk_attention(*args, scale, 1, 0, KV, None) == -1 and b"scale" in lib.vrm_last_error()
+    assert lib.vrm_paged_chunk_attention(*args, 2.3e38, 1, 0, KV, None) == -3  # (as far as the workspace)

@@ -237,8 +237,9 @@ extern "C" int vrm_paged_chunk_attention_expecting(
     set_error("%s: layer_idx %d outside [0, %d)", who, layer_idx, L);
     return VRM_ERR_ARG;
   }
-  if (!isfinite(scale)) {
-    set_error("%s: scale is not finite", who);
+  const float sc = fabsf(scale) * 1.44269504088896341f;  // scores in base-2 logarithms
+  if (!isfinite(sc)) {
+    set_error("%s: scale is not finite, or its product with log2 e is not", who);
     return VRM_ERR_ARG;
   }
   if (q_dtype != VRM_SRC_F32 && q_dtype != VRM_SRC_F16 && q_dtype != VRM_SRC_BF16) {
@@ -305,7 +306,7 @@ extern "C" int vrm_paged_chunk_attention_expecting(
   a.ps_shift = (PS & (PS - 1)) ? -1 : __builtin_ctz(PS);
   a.causal = causal != 0;
   a.window = window < 1 << 30 ? window : 1 << 30;  // (positions less it stay in 32 bits)
-  a.sc = scale == 0.f ? 1.f : fabsf(scale) * 1.44269504088896341f;
+  a.sc = scale == 0.f ? 1.f : sc;
   a.q_sign = scale == 0.f ? 0 : scale < 0.f ? -1 : 1;
   a.target = p.target;
   a.min_blocks = p.min_blocks;
