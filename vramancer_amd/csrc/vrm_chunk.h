@@ -89,8 +89,14 @@ __device__ __forceinline__ int blocks_of(const ChunkArgs& a, const Sequence& s) 
 }
 
 // What a block costs a tile of at most 32 rows, whose wavefronts wait for
-// memory, against one of a larger tile (a prompt's chunk of 509 beside 15
-// single tokens, shares at 1, 2, 3 and 4: 70.6, 65.4, 65.5 and 65.4 us).
+// memory, against one of a larger tile.  A compromise: shares round up to whole
+// items, more of them than are resident at once, and which cost leaves the last
+// ones least to do differs from batch to batch.  At 1, 2 and 4, chunks beside
+// single tokens: 509 beside 15, 28 heads over 4, 54, 48 and 62 us; 2000 beside
+// 31 374, 354 and 311; four of 256 beside 12, 32 over 8, 97, 98 and 115; 512
+// beside 15 at head_dim 256 278, 245 and 246; 512 beside 63 over int8, 40 over
+// 8, 209, 206 and 215, but beside 31 103, 139 and 139; two of 300 beside 30 at
+// head_dim 64 56, 71 and 74.
 constexpr int kFewCost = 2;
 __device__ __forceinline__ int block_cost(const ChunkArgs& a, const Sequence& s) {
   return s.q_len * a.G <= 32 ? kFewCost : 1;

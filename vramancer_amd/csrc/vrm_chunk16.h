@@ -441,8 +441,8 @@ __device__ __forceinline__ void scale_weights(const float* vs, int e, int half, 
 // token's row), refilled as soon as the scores are taken; V of the quantized
 // pools too (its tiling puts a lane's four tokens of a dim in a dword), V of
 // float pools through the wavefront's own LDS.
-// Bound: memory.  64 sequences of 4 tokens after about 3500, 40 heads over 8,
-// int8: 115 us, 4.8 TB/s (a copy reaches 5.0).
+// Bound: memory.  64 sequences of 4 tokens after about 4050, 40 heads over 8,
+// int8: 118 us with the merge, 4.7 TB/s (a copy reaches 5.0).
 template <typename T, int KIND, int DP, int WAVES>
 __device__ __forceinline__ void few_rows(const ChunkArgs& a, const Item& it, int kvh, int rows, int from, int to,
                                          uint8_t* lds, float (*own_scale)[2][32]) {
@@ -774,10 +774,13 @@ __global__ void __launch_bounds__(kChunkThreads, DP <= 128 ? 2 : 1) chunk_attn_k
 // products of K and of V, so that one's masks, maxima and staging fall beside
 // the other's products.  Four blocks are in LDS (the wavefronts ahead write
 // block + 2 while those behind still read block - 1), a fifth in registers.
-// Bound: matrix cores, 2048 of about 4000 cycles of a block at head_dim 128;
-// prompts of thousands of tokens 480 us, 1.0 PFLOP/s in bf16 (a library
-// product of 8192^3 reaches 1.17), 256 tokens after 130,816 over fp8 1207 us,
-// 0.91 PFLOP/s.
+// Bound: matrix cores, 2048 cycles of a block at head_dim 128, and the vector
+// work beside them.  A prompt of 8192 tokens, bf16: 490 us, 1.0 PFLOP/s (a
+// library product of 8192^3 reaches 1.17), matrix cores busy 51 % of the
+// cycles, vector ALUs 50 %; 256 tokens after 130,816 over fp8 1210 us, 0.91
+// PFLOP/s, 40 and 58 % (codes to bf16).  At head_dim 128 all 256 registers are
+// taken: 3 are spilled over float pools, 1 over int8 and fp8, 14 and 15 there
+// with fp16 queries, whose weights are two operands.
 template <typename T, int KIND, int DP>
 __global__ void __launch_bounds__(kLargeThreads, 1) chunk_attn_large_kernel(ChunkArgs a) {
   using Tile = ChunkTile<KIND, DP>;

@@ -109,8 +109,10 @@ struct ChunkPlan {
 // Tiles that fill the GPU twice are left whole; fewer are cut into shares for
 // about as many workgroups as are resident at once (for twice as many: a
 // batch of 64 x 4 tokens over 4096 each 130 us for 118, two prompts within a
-// window 123 for 87), at least kMinBlocks blocks each (17 tokens after 1531:
-// 24.4, 21.2 and 21.2 us at 1, 2 and 4).
+// window 123 for 87), at least kMinBlocks blocks each.  At 1, 2 and 4: 17
+// tokens after 1531 21.5, 19.0 and 21.1 us, four such 27.6, 22.3 and 22.6; 5
+// after 300 13.8, 14.6 and 15.9; 30 after 600 over int8 17.0, 18.1 and 23.0,
+// four such 23.3, 20.4 and 24.2; 40 after 4000 30.1, 29.0 and 25.3.
 constexpr int kMinBlocks = 2;
 
 // Tiles of 256 rows from 128 rows a sequence, 1024 tokens in the table and

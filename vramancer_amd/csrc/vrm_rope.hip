@@ -21,8 +21,11 @@
 // as whole dwords of codes, K token-major, V four tokens of a dim to a dword;
 // an fp8 page's scale needs its tokens' maximum first.
 // Measured, kernels alone: norm and rotation of 2.0e8 bytes of queries and
-// keys 44.7 us (4.5 TB/s; a copy reaches 5.0); prompts of about 8000 tokens,
-// 40 heads over 8, into int8 pages 69 us; one token of a batch 5.5 to 6.7 us.
+// keys 43.6 us (4.6 TB/s; a copy reaches 5.0); prompts of about 8000 tokens,
+// 40 heads over 8, into int8 pages 70 us, vector ALUs busy 65 % of it (codes,
+// and divisions by D in the store loop); one token of a batch 5.9 to 6.9 us.
+// The wavefront-a-row path: the same norm and rotation with 40 dims rotated
+// 122 us for 38 (in a replayed graph).
 // Int8 keys as rows straight from registers were slower (81 us: 130 registers,
 // three wavefronts a SIMD).
 #include <math.h>
