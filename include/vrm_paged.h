@@ -718,6 +718,94 @@ int vrm_rope_append(const void* query, long long q_token_stride, long long q_hea
                     const int32_t* cu_seqlens, int N, int B, int H, int KH, int D, int PS, int L,
                     int P, int max_pp, int layer_idx, vrm_stream_t stream);
 
+/*
+ * The tables of a ragged batch of new tokens from lengths on the device.
+ * Sequence b is request r = requests[b] (b where requests is NULL) with
+ * past_lens[r] tokens stored and counts[b] new ones (negative: 0):
+ *   cu_seqlens   [B + 1] running sums of the counts, cut at N: tokens past N
+ *                have no place and count nowhere
+ *   context_lens [B] past_lens[r] and the new tokens that have a place
+ *   page_table   [B][max_pp] row r of block_table up to the page of the last
+ *                token, -1 behind it
+ *   positions, page_ids, slots, sequences  [N] of every new token: its position,
+ *                the page (-1 past the row's W entries) and the slot there, and
+ *                b; behind the last sequence 0, -1, -1 and -1
+ * block_table is [R] rows of W int32, row_stride elements apart.  A request
+ * outside [0, R) has no tokens and no pages.  A request may stand in several
+ * sequences; their new tokens then have the same places.  Outputs must not
+ * overlap inputs.
+ */
+int vrm_chunk_tables(const int32_t* block_table, long long row_stride, int R, int W,
+                     const int32_t* past_lens, const int32_t* counts, const int32_t* requests,
+                     int B, int N, int PS, int32_t* page_table, int max_pp, int32_t* context_lens,
+                     int32_t* cu_seqlens, int32_t* positions, int32_t* page_ids, int32_t* slots,
+                     int32_t* sequences, vrm_stream_t stream);
+
+/* --------------------------------------------------------------------------
+ * From logits to tokens.  No counterpart in the reference, whose batcher draws
+ * its tokens on the host.
+ *
+ * A row of V logits l (of dtype VRM_SRC_*; row_stride elements from a row to
+ * the next) gives the tokens the weights w_i = exp((l_i - max l) / T).  top_k
+ * keeps the k first in the order (logit descending, index ascending; k <= 0 or
+ * >= V: all), top_p of those the shortest prefix whose weights reach top_p times
+ * the sum of theirs (at least one; >= 1 or NaN: all).  T <= 0 or NaN keeps the
+ * arg max alone, the first of equal ones.  NaN counts as -inf; a row without a
+ * logit above -inf has no token.
+ *
+ * temperature, top_k and top_p are device arrays with a value per sequence, or
+ * NULL: temperature_all, top_k_all, top_p_all hold for every one.  V is at most
+ * VRM_SAMPLE_MAX_V.  Random numbers are taken into [0, 1].
+ *
+ * Weights, their sums and every comparison with them are 64-bit floats (under
+ * top_k and top_p sums of weights rounded to multiples of 2^-S of the largest,
+ * S = min(45, 63 - ceil(log2 V)), which is where the shortest prefix is found).
+ * Results are the same from call to call.  The workspace is 16-byte aligned and
+ * written before it is read.
+ * -------------------------------------------------------------------------- */
+#define VRM_SAMPLE_MAX_V (1 << 24)
+
+/*
+ * tokens[n] = the lowest i with sum_{j <= i} w_j > uniforms[n] sum_j w_j over
+ * the tokens of row n that are kept; -1 for a row that has no token.
+ *   probs   [N][V] float32 or NULL: w_i over the sum, 0 for what is not kept
+ *   workspace of vrm_sample_workspace_bytes; filtered: whether a top_k or top_p
+ *   is given that could drop a token, with_probs: whether probs is
+ */
+size_t vrm_sample_workspace_bytes(int N, int V, int filtered, int with_probs);
+int vrm_sample_tokens(const void* logits, int dtype, long long row_stride, const float* uniforms,
+                      const float* temperature, float temperature_all, const int32_t* top_k,
+                      int top_k_all, const float* top_p, float top_p_all, float* probs,
+                      int64_t* tokens, void* workspace, size_t workspace_bytes, int N, int V,
+                      vrm_stream_t stream);
+
+/*
+ * Drafted tokens against the target's distributions.  Sequence b has n_b =
+ * min(q_b - 1, K) drafts x_0 .. and the rows cu_seqlens[b] .. of the logits (q_b
+ * rows; K + 1 each where cu_seqlens is NULL): row i is the distribution p of
+ * what follows draft i - 1.  Draft i is accepted where
+ *      accept_uniforms[b][i] q_i(x_i) < p_i(x_i)
+ * and all before it are; q is draft_probs[b][i] (float32, strides in elements,
+ * negative values 0, a NaN more than any p), or 1 at x_i where draft_probs is NULL.  A draft outside
+ * [0, V) is not accepted.  With a drafts accepted the token after them comes
+ * from p_a where all were, or draft a was outside [0, V); otherwise from
+ * max(p_a - q_a, 0) over its sum (p_a where nothing is left of it): the lowest
+ * index whose running sum passes draw_uniforms[b] of the whole.
+ *   tokens    [B][K + 1]: the accepted drafts, that token (-1 where p_a has
+ *             none), then -1; all -1 for a sequence without rows
+ *   accepted  [B]: a
+ *   drafts    [B][K] integers of draft_bytes (4 or 8)
+ */
+size_t vrm_verify_workspace_bytes(int B, int K, int V, int filtered);
+int vrm_verify_drafts(const void* logits, int dtype, long long row_stride,
+                      const int32_t* cu_seqlens, const void* drafts, int draft_bytes,
+                      const float* draft_probs, long long probs_seq_stride,
+                      long long probs_draft_stride, const float* accept_uniforms,
+                      const float* draw_uniforms, const float* temperature, float temperature_all,
+                      const int32_t* top_k, int top_k_all, const float* top_p, float top_p_all,
+                      int64_t* tokens, int32_t* accepted, void* workspace, size_t workspace_bytes,
+                      int N, int B, int K, int V, vrm_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -92,6 +92,12 @@ SIGNATURES = {
     "vrm_paged_chunk_attention": (_i, [_p, _i, _ll, _ll] + [_p] * 8 + [_sz] + [_i] * 10 + [_f, _i, _i, _i, _p]),
     "vrm_paged_chunk_attention_expecting": (_i, [_p, _i, _ll, _ll] + [_p] * 8 + [_sz] + [_i] * 10
                                             + [_f, _i, _i, _i, _i, _p]),
+    "vrm_chunk_tables": (_i, [_p, _ll, _i, _i, _p, _p, _p, _i, _i, _i, _p, _i] + [_p] * 6 + [_p]),
+    "vrm_sample_workspace_bytes": (_sz, [_i] * 4),
+    "vrm_sample_tokens": (_i, [_p, _i, _ll, _p, _p, _f, _p, _i, _p, _f, _p, _p, _p, _sz, _i, _i, _p]),
+    "vrm_verify_workspace_bytes": (_sz, [_i] * 4),
+    "vrm_verify_drafts": (_i, [_p, _i, _ll, _p, _p, _i, _p, _ll, _ll, _p, _p, _p, _f, _p, _i, _p, _f, _p, _p, _p, _sz]
+                          + [_i] * 4 + [_p]),
 }
 
 

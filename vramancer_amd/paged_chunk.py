@@ -19,6 +19,10 @@ A batch is ragged and described by three int32 device tensors:
   token i of q is at position ``context_lens[b] - q + i``;
 * ``page_table`` [B, max_pages] as the decode takes it.
 
+``chunk_tables`` makes them, and the place of every new token, from lengths
+that are on the device: a step whose lengths follow from the one before it
+(``sampling.verify_drafts``) needs no copy to the host.
+
 Everything else is decided on the device; no call reads a tensor back.  Like
 the decode these are forward only: outputs carry no gradient.
 """
@@ -26,6 +30,7 @@ from __future__ import annotations
 
 import functools
 import math
+from dataclasses import dataclass
 from typing import Any, Optional
 
 import torch
@@ -33,7 +38,7 @@ import torch
 from . import _lib, kv_quant
 from .rope import check_heads, check_out, check_positions, check_table, check_weights, launch, src_code
 
-__all__ = ["rope_append", "paged_attention_chunk", "chunk_workspace"]
+__all__ = ["rope_append", "paged_attention_chunk", "chunk_workspace", "chunk_tables", "ChunkTables"]
 
 
 @functools.lru_cache(maxsize=256)
@@ -236,4 +241,86 @@ def paged_attention_chunk(
                 max_pp, int(layer_idx), 1.0 / math.sqrt(D) if scale is None else float(scale), 1 if causal else 0,
                 window or 0, min(int(expected_context or 0), 0x7fffffff), code)
     _lib.check(rc, "paged_attention_chunk")
+    return out
+
+
+@dataclass
+class ChunkTables:
+    """A ragged batch of new tokens (``chunk_tables``), int32 on the device."""
+
+    page_table: Any    # [B, max_pages]
+    context_lens: Any  # [B], the new tokens included
+    cu_seqlens: Any    # [B + 1]
+    positions: Any     # [N] position of every new token, 0 behind the last sequence
+    page_ids: Any      # [N] its page, -1 where there is none
+    slots: Any         # [N] its slot there, -1 behind the last sequence
+    sequences: Any     # [N] its sequence, -1 behind the last one
+
+
+def _ints(name: str, t, n: Optional[int]):
+    if t.dim() != 1 or (n is not None and t.shape[0] != n):
+        raise RuntimeError(f"{name} must be [{'R' if n is None else n}], got shape {tuple(t.shape)}")
+    if t.dtype != torch.int32:
+        if t.dtype not in (torch.int64, torch.int16, torch.int8, torch.uint8):
+            raise RuntimeError(f"{name} must be integers, got {t.dtype}")
+        t = t.to(torch.int32)
+    return t.contiguous()
+
+
+def chunk_tables(
+    block_table: Any,  # [R, W] int32, rows may be strided
+    past_lens: Any,    # [R] tokens stored
+    counts: Any,       # [B] new tokens
+    num_rows: int,     # N
+    page_size: int,
+    requests: Any = None,  # [B] rows of block_table; default: the first B
+    max_pages: Optional[int] = None,
+    out: Optional[ChunkTables] = None,
+) -> ChunkTables:
+    """What ``rope_append``, ``paged_attention_chunk`` and
+    ``PagedKVCacheManager.write_kv_batch`` take, for ``counts[b]`` new tokens of
+    each request ``requests[b]``, from a block table that stays on the device
+    and holds the pages of the new tokens already
+    (``PagedKVCacheManager.reserve``).
+
+    ``num_rows`` is the N of the batch's tensors: tokens past it get no place
+    (``cu_seqlens`` ends at it), rows behind the last token belong to no
+    sequence.  ``max_pages`` (default W) is the page table's width; a row holds
+    the pages up to its last token's, -1 behind them.  A request outside
+    [0, R) and a negative count have no tokens.  ``out`` takes the tensors of
+    an earlier call of the same sizes, for a captured graph that reads them."""
+    if block_table.dim() != 2 or block_table.dtype != torch.int32:
+        raise RuntimeError(f"block_table must be int32 [R, W], got {block_table.dtype} {tuple(block_table.shape)}")
+    R, W = block_table.shape
+    N, PS = int(num_rows), int(page_size)
+    max_pp = W if max_pages is None else int(max_pages)
+    if N < 0 or PS < 1 or max_pp < 0:
+        raise RuntimeError(f"num_rows and max_pages must not be negative and page_size positive, got {N}, {max_pp}, "
+                           f"{PS}")
+    if block_table.stride(1) != 1 and W > 1:
+        block_table = block_table.contiguous()
+    past_lens = _ints("past_lens", past_lens, R)
+    counts = _ints("counts", counts, None if requests is None else requests.shape[0])
+    B = counts.shape[0]
+    if requests is not None:
+        requests = _ints("requests", requests, B)
+    if out is None:
+        sizes = [B * max_pp, B, B + 1, N, N, N, N]
+        parts = torch.empty(sum(sizes), dtype=torch.int32, device=block_table.device).split(sizes)
+        out = ChunkTables(parts[0].view(B, max_pp), *parts[1:])
+    else:
+        for name, shape in (("page_table", (B, max_pp)), ("context_lens", (B,)), ("cu_seqlens", (B + 1,)),
+                            ("positions", (N,)), ("page_ids", (N,)), ("slots", (N,)), ("sequences", (N,))):
+            t = getattr(out, name)
+            if tuple(t.shape) != shape or t.dtype != torch.int32 or not t.is_contiguous():
+                raise RuntimeError(f"out.{name} must be a contiguous int32 {list(shape)} tensor, got {t.dtype} "
+                                   f"{tuple(t.shape)}")
+    _lib.require_cuda(block_table, past_lens, counts, requests, out.page_table, out.context_lens, out.cu_seqlens,
+                      out.positions, out.page_ids, out.slots, out.sequences)
+    ptr = _lib.ptr
+    rc = launch(block_table, _lib.load().vrm_chunk_tables, block_table.data_ptr(), block_table.stride(0), R, W,
+                past_lens.data_ptr(), counts.data_ptr(), ptr(requests), B, N, PS, out.page_table.data_ptr(), max_pp,
+                out.context_lens.data_ptr(), out.cu_seqlens.data_ptr(), out.positions.data_ptr(),
+                out.page_ids.data_ptr(), out.slots.data_ptr(), out.sequences.data_ptr())
+    _lib.check(rc, "chunk_tables")
     return out
