@@ -1,21 +1,24 @@
 // Weights of the tokens of a row of logits, in 64 bits, as the kernels that
 // draw and verify tokens share them (vrm_sample.hip, vrm_sample_cut.hip).
 //
-// A row's token i has weight w_i = 2^((l_i - m) c), c = log2(e) / T, m the
-// row's maximum; the probability is w_i over their sum.  A token is an answer
-// in whole numbers that follows running sums over up to 10^5 weights next to
-// borders, so that an error of 1e-7 in each weight would change one in some
-// thousand draws from flat rows.  Weights are therefore float64: a conversion,
-// a subtraction, a product and a polynomial of 10 steps, on a vector unit whose
-// float64 rate is its float32 rate.  Logits that are -inf or NaN weigh nothing.
+// Token i of a row weighs w_i = 2^((l_i - max l) c), c = log2(e) / T; its
+// probability is w_i over their sum.  A token is an answer in whole numbers
+// that follows running sums over up to 10^5 weights next to borders, so that an
+// error of 1e-7 in each weight would change one in some thousand draws from
+// flat rows.  Weights are therefore float64, at 15 instructions each on a vector
+// unit whose float64 rate is its float32 rate (4.7 to 5.6 cycles a wavefront's
+// instruction, float32 4.0 to 4.4).  The largest weight is exactly 1, so that
+// draws from tokens that are all equal to it are exact where their number times
+// the random number is whole.  Logits that are -inf or NaN weigh nothing.
 #pragma once
 #include "vrm_common.h"
 
 namespace vrm {
 
 constexpr int kSampleThreads = 256;
-constexpr int kSamplePer = 32;                               // logits of a thread in a chunk
-constexpr int kSampleChunk = kSampleThreads * kSamplePer;    // logits of a chunk
+constexpr int kSamplePer = 32;                     // logits of a lane in a segment
+constexpr int kSegment = kWave * kSamplePer;       // logits of a wavefront
+constexpr int kSampleBlock = 4 * kSegment;         // of a workgroup
 
 // Rows of logits and the parameters of the sequence they belong to.  Sequence
 // b has rows cu[b] .. cu[b + 1] (K + 1 each without cu), of which the first
@@ -39,11 +42,13 @@ struct SampleRows {
   __device__ __forceinline__ float temp(int b) const { return temperature ? temperature[b] : temperature_all; }
   __device__ __forceinline__ int limit(int b) const { return top_k ? top_k[b] : top_k_all; }
   __device__ __forceinline__ float nucleus(int b) const { return top_p ? top_p[b] : top_p_all; }
+  __host__ __device__ __forceinline__ int segments() const { return (V + kSegment - 1) / kSegment; }
 };
 
-// What a chunk of a row says about it: its maximum, that one's first place,
-// and the sum of its weights relative to it.
-struct ChunkRec {
+// What a segment of a row says about it: a maximum (of the segment or of some
+// more of the row around it), that one's first place, and the sum of the
+// segment's weights by the scale of that maximum.
+struct SegRec {
   double sum;
   float top;
   int arg;
@@ -56,46 +61,88 @@ struct RowCut {
   double sum;
 };
 
-// A sequence's draw: the row it draws from, with the row's scale, and the
-// drafted token that is refused (-1: none), whose place in the drafts is `at`.
+// A sequence's draw: the row it draws from, and the drafted token that is
+// refused (-1: none), whose place in the drafts is `at`.
 struct DrawRec {
-  double c;                // 0 with greedy
   double sum;              // of the row's weights that stay
   unsigned long long cut;
   float top;
   int row;                 // -1: the sequence has none
-  int arg;                 // greedy: the answer; otherwise -2
+  int arg;                 // the answer where it is known (greedy, no token); otherwise -2
   int refused;
   int at;
   int pad;
 };
 
-__device__ __forceinline__ double sample_scale(float t) { return 1.4426950408889634074 / (double)t; }
+// The scale of a row, or of a part of one.
+struct Scale {
+  double top, c, low;  // low: a difference from top at which the weight is 0
+  bool infinite;       // the maximum is +inf: those tokens alone
+};
 
-// 2^y for y <= 0, to 6e-16 of the value: y = n + r, 2^r = 1 + r q(r) with q
-// interpolated at Chebyshev nodes of [-1/2, 1/2]; exactly 1 at 0.
-__device__ __forceinline__ double exp2_neg(double y) {
-  const double big = y + 6755399441055744.0;  // 1.5 2^52: the sum's last digits are the nearest integer
-  const double r = y - (big - 6755399441055744.0);
-  double q = 0x1.e5e9f548e5725p-28;
-  q = fma(q, r, 0x1.b6571de2f2351p-24);
-  q = fma(q, r, 0x1.62bfe46117445p-20);
-  q = fma(q, r, 0x1.ffcb76789860fp-17);
-  q = fma(q, r, 0x1.4309130378460p-13);
-  q = fma(q, r, 0x1.5d87fe908f88ap-10);
-  q = fma(q, r, 0x1.3b2ab6fba385fp-7);
-  q = fma(q, r, 0x1.c6b08d7044119p-5);
-  q = fma(q, r, 0x1.ebfbdff82c590p-3);
-  q = fma(q, r, 0x1.62e42fefa39f7p-1);
-  return __builtin_ldexp(fma(q, r, 1.0), (int)__double_as_longlong(big));
+__device__ __forceinline__ Scale make_scale(float top, float t) {
+  Scale s;
+  s.infinite = top == INFINITY;
+  s.top = top;
+  s.c = fmax(1.4426950408889634074 / (double)t, 1e-290);  // (an infinite temperature: every weight is 1)
+  s.low = -1100.0 / s.c;
+  return s;
 }
 
-// Weight of a logit against the row's maximum.  A NaN (of the logit, of
-// inf - inf) is taken as the lower bound by the maximum and weighs nothing;
-// rows whose maximum is +inf weigh their +inf alone.
-__device__ __forceinline__ double sample_weight(float l, float top, double c) {
-  if (top == INFINITY) return l == INFINITY ? 1.0 : 0.0;
-  return exp2_neg(fmax(((double)l - (double)top) * c, -1100.0));
+// Weights of N logits.  (l - top) c = n + r; 2^r = 1 + r q(r) with q
+// interpolated at 8 Chebyshev nodes of [-1/2, 1/2], to 2.2e-12 of the value
+// (the same for equal logits).  n comes out of an addition at 2^52, r of the
+// same product again.  A NaN (of the logit, of -inf against -inf) is taken as
+// the lower bound by fmax.
+// The polynomial's steps, four values side by side, are written out with their
+// coefficients in scalar registers: the compiler takes the form of the
+// instruction that adds onto its result, and copies each coefficient into
+// vector registers first, two instructions more for each step (the sums of 960
+// rows of 131072 took 123 us with them).
+template <int N>
+__device__ __forceinline__ void sample_weights(const float* l, const Scale& s, double* w) {
+  static_assert(N % 4 == 0, "four values side by side");
+  if (s.infinite) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) w[e] = l[e] == INFINITY ? 1.0 : 0.0;
+    return;
+  }
+  constexpr double kBig = 6755399441055744.0;  // 1.5 2^52: a sum's last digits are the nearest integer
+#pragma unroll
+  for (int e = 0; e < N; e += 4) {
+    double r[4], q[4];
+    int n[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const double x = fmax((double)l[e + i] - s.top, s.low);
+      const double big = fma(x, s.c, kBig);
+      n[i] = (int)__double_as_longlong(big);
+      r[i] = fma(x, s.c, -(big - kBig));
+    }
+#define VRM_STEP(c)                          \
+  "v_fma_f64 %0, %0, %4, " c "\n\t"          \
+  "v_fma_f64 %1, %1, %5, " c "\n\t"          \
+  "v_fma_f64 %2, %2, %6, " c "\n\t"          \
+  "v_fma_f64 %3, %3, %7, " c "\n\t"
+    asm("v_fma_f64 %0, %15, %4, %8\n\t"
+        "v_fma_f64 %1, %15, %5, %8\n\t"
+        "v_fma_f64 %2, %15, %6, %8\n\t"
+        "v_fma_f64 %3, %15, %7, %8\n\t" VRM_STEP("%9") VRM_STEP("%10") VRM_STEP("%11") VRM_STEP("%12")
+            VRM_STEP("%13") VRM_STEP("%14") VRM_STEP("1.0")
+        : "=&v"(q[0]), "=&v"(q[1]), "=&v"(q[2]), "=&v"(q[3])
+        : "v"(r[0]), "v"(r[1]), "v"(r[2]), "v"(r[3]), "s"(0x1.00c0e4e15189cp-16), "s"(0x1.4308c7183d6a2p-13),
+          "s"(0x1.5d877598350dep-10), "s"(0x1.3b2ab70ad2565p-7), "s"(0x1.c6b08da70cce3p-5),
+          "s"(0x1.ebfbdff82a734p-3), "s"(0x1.62e42fef9cc69p-1), "v"(0x1.63b2d7971923fp-20));
+#undef VRM_STEP
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[e + i] = __builtin_ldexp(q[i], n[i]);
+  }
+}
+__device__ __forceinline__ double sample_weight(float l, const Scale& s) {
+  const float x[4] = {l, l, l, l};
+  double w[4];
+  sample_weights<4>(x, s, w);
+  return w[0];
 }
 
 // Order value of token i: larger for what comes first (larger logit, then
@@ -155,17 +202,37 @@ __device__ __forceinline__ const typename Logit<SRC>::Raw* row_at(const SampleRo
   return static_cast<const typename Logit<SRC>::Raw*>(r.logits) + (long long)row * r.stride;
 }
 
-// A chunk's elements of this thread: vector i is elements (i 256 + tid) kVec ..
+// The first element of a lane's vector i of a segment; a wavefront's load is
+// 1 KB without a gap.
 template <int SRC>
-__device__ __forceinline__ void load_chunk(const typename Logit<SRC>::Raw* row, int chunk, int V, float* x) {
-  constexpr int kVec = Logit<SRC>::kVec;
-#pragma unroll
-  for (int i = 0; i < kSamplePer / kVec; ++i)
-    load_vec<SRC>(row, chunk * kSampleChunk + (i * kSampleThreads + (int)threadIdx.x) * kVec, V, x + i * kVec);
+__device__ __forceinline__ int segment_element(int seg, int i) {
+  return seg * kSegment + (i * kWave + (int)(threadIdx.x & 63)) * Logit<SRC>::kVec;
 }
 
-// Sums, largest and smallest values over a wavefront, every lane has them; the
-// sums' order is fixed.
+// A lane's elements of a segment.  All loads of a whole segment are under way
+// before the first is waited for.
+template <int SRC>
+__device__ __forceinline__ void load_segment(const typename Logit<SRC>::Raw* row, int seg, int V, float* x) {
+  using L = Logit<SRC>;
+  constexpr int kVec = L::kVec, kGroups = kSamplePer / kVec;
+  const int e0 = segment_element<SRC>(seg, 0);
+  if ((seg + 1) * kSegment <= V) {
+    Unaligned16<typename L::Raw> raw[kGroups];
+#pragma unroll
+    for (int i = 0; i < kGroups; ++i)
+      raw[i] = *reinterpret_cast<const Unaligned16<typename L::Raw>*>(row + e0 + i * kWave * kVec);
+#pragma unroll
+    for (int i = 0; i < kSamplePer; ++i) x[i] = L::value(raw[i / kVec].v[i % kVec]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kSamplePer; ++i) {
+      const int e = e0 + (i / kVec) * kWave * kVec + i % kVec;
+      x[i] = e < V ? L::value(row[e]) : -INFINITY;
+    }
+  }
+}
+
+// Sums, prefixes and smallest values over a wavefront, in a fixed order.
 __device__ __forceinline__ double wave_sum(double v) {
 #pragma unroll
   for (int m = 1; m < kWave; m <<= 1) v += __shfl_xor(v, m);
@@ -185,26 +252,75 @@ __device__ __forceinline__ int wave_min(int v) {
   return v;
 }
 
-// A row's maximum, the sum of its weights relative to it (scale c, 0 for
-// greedy rows, whose sum is not asked for) and the maximum's first place, from
-// its chunks; by one wavefront.
-__device__ __forceinline__ void combine_chunks(const ChunkRec* rec, int nc, double c, float& top, double& sum, int& arg) {
-  const int lane = threadIdx.x & 63;
-  float m = -INFINITY;
-  for (int j = lane; j < nc; j += kWave) m = fmaxf(m, rec[j].top);
-  m = group_max<64>(m);
-  double s = 0.0;
-  int first = 0x7fffffff;
-  for (int j = lane; j < nc; j += kWave) {
-    const ChunkRec r = rec[j];
-    if (r.top == m) first = min(first, r.arg);
-    if (r.top > -INFINITY) s += r.sum * sample_weight(r.top, m, c);
-  }
-  top = m;
-  sum = wave_sum(s);
-  arg = wave_min(first);
+// A segment's sum by its row's scale.
+__device__ __forceinline__ double segment_sum(const SegRec& r, const Scale& s) {
+  return r.top > -INFINITY ? r.sum * sample_weight(r.top, s) : 0.0;
 }
 
-int launch_sample_cut(const SampleRows& r, int dtype, int nc, const ChunkRec* rec, RowCut* cuts, hipStream_t st);
+// A row from its segments, by one wavefront: its maximum, that one's first
+// place (greedy rows), its scale and the sum of its weights (the others).
+__device__ __forceinline__ void combine_segments(const SegRec* rec, int ns, float t, float& top, int& arg, Scale& scale,
+                                                 double& sum) {
+  const int lane = threadIdx.x & 63;
+  float m = -INFINITY;
+  for (int j = lane; j < ns; j += kWave) m = fmaxf(m, rec[j].top);
+  top = group_max<64>(m);
+  arg = -1;
+  sum = 0.0;
+  if (top == -INFINITY) return;
+  if (!(t > 0.0f)) {
+    int first = 0x7fffffff;
+    for (int j = lane; j < ns; j += kWave)
+      if (rec[j].top == top) first = min(first, rec[j].arg);
+    arg = wave_min(first);
+    sum = 1.0;
+    return;
+  }
+  arg = -2;
+  scale = make_scale(top, t);
+  double s = 0.0;
+  for (int j = lane; j < ns; j += kWave) s += segment_sum(rec[j], scale);
+  sum = wave_sum(s);
+}
+
+// Histograms of the workgroups' parts of a row, for top_k and top_p: bins are
+// steps of a tenth of a factor of 2 in the weight, counted from the bin of the
+// part's maximum on.  The steps are absolute (floor of l times 10 c, within 24
+// bits), so that the parts of a row differ by a shift only; the bin of a logit
+// is monotone in it, and what is past the last bin weighs less than 2^-51 of
+// the part's maximum.  Where the maximum is +inf, that is the top bin and the
+// finite logits are past the last one.  Sums are integers, weights times 2^49
+// rounded: they do not depend on the order of the atomics.
+constexpr int kBins = 512;
+constexpr int kBinBits = 49;
+constexpr float kBinMost = 8000000.0f;
+
+struct Histogram {
+  unsigned long long sum[kBins];
+  uint32_t count[kBins];  // (where a top_k is given)
+};
+
+__device__ __forceinline__ float bin_scale(const Scale& s) { return s.infinite ? 1e-30f : (float)fmin(10.0 * s.c, 3e38); }
+__device__ __forceinline__ int bin_of(float l, float c) {
+  return (int)floorf(fminf(fmaxf(l * c, -kBinMost), kBinMost));
+}
+
+// Weight as an integer, in units of 2^-bits.
+__device__ __forceinline__ unsigned long long fixed_weight(double w, double unit) {
+  return (unsigned long long)__double_as_longlong(fma(w, unit, 4503599627370496.0)) & 0xfffffffffffffULL;  // 2^52
+}
+
+// Whether a row's parameters may drop tokens.
+__device__ __forceinline__ bool row_filters(const SampleRows& r, int b, float t, bool& by_k, bool& by_p) {
+  const int k = r.limit(b);
+  by_k = k > 0 && k < r.V;
+  by_p = r.nucleus(b) < 1.0f;
+  return t > 0.0f && (by_k || by_p);
+}
+
+// Finds every row's cut from the histograms of its parts; with draws (sequences
+// of one row) its draw too.
+int launch_sample_cut(const SampleRows& r, int dtype, const SegRec* rec, const Histogram* hist, RowCut* cuts,
+                      DrawRec* draws, hipStream_t st);
 
 }  // namespace vrm

@@ -2,69 +2,132 @@
 // tokens verified against the target's probabilities (vrm_verify_drafts).  No
 // counterpart in the reference, whose batcher samples on the host.
 //
-// Both are passes over rows of V logits, cut into chunks of 8192 so that few
-// rows fill the chip too:
-//   1. sample_chunk_kernel  every row's chunks: maximum, sum of weights
-//   2. sample_cut_kernel    (top_k, top_p) which tokens stay (vrm_sample_cut.hip)
-//   3. sample_choose_kernel a sequence's drafts: accepted ones, the row its next
-//                           token is drawn from
-//   4. sample_mass_kernel   that row's chunks: the mass to draw from
-//   5. sample_pick_kernel   the chunk and the token where the running sum
-//                           passes the random number
-// A plain draw without top_k, top_p and probabilities is 1 and 5.
+// Both are passes over rows of V logits, cut into segments of 2048, one for a
+// wavefront, so that few rows fill the chip too:
+//   1. sample_segment_kernel    every row's segments: maximum, sum of weights;
+//      sample_histogram_kernel  the same and histograms, where top_k or top_p
+//                               may drop tokens
+//   2. sample_cut_kernel        which tokens stay (vrm_sample_cut.hip)
+//   3. sample_choose_kernel     a sequence's drafts: accepted ones, the row its
+//                               next token is drawn from
+//   4. sample_mass_kernel       that row's segments: the mass to draw from
+//   5. sample_pick_kernel       the segment and the token where the running sum
+//                               passes the random number
+// A draw without top_k and top_p is 1 and 5, one with them 1, 2, 4 and 5.
 #include "vrm_sample.h"
 
 namespace vrm {
 namespace {
 
+// The first place of a segment's maximum.
+template <int SRC>
+__device__ __forceinline__ int first_place(const float* x, float m, int seg) {
+  constexpr int kVec = Logit<SRC>::kVec;
+  int arg = 0x7fffffff;
+#pragma unroll
+  for (int e = kSamplePer - 1; e >= 0; --e)
+    if (x[e] == m) arg = segment_element<SRC>(seg, e / kVec) + e % kVec;
+  return wave_min(arg);
+}
+
 // ---------------------------------------------------------------------------
-// 1. Chunks of rows
+// 1. Segments of rows
 // ---------------------------------------------------------------------------
 
 template <int SRC>
-__global__ void __launch_bounds__(kSampleThreads) sample_chunk_kernel(SampleRows r, int nc, ChunkRec* rec) {
-  __shared__ float tops[4];
-  __shared__ double sums[4];
-  __shared__ int args[4];
-  const int slot = blockIdx.x / nc, chunk = blockIdx.x % nc;
+__global__ void __launch_bounds__(kSampleThreads) sample_segment_kernel(SampleRows r, int ns, int blocks, SegRec* rec) {
+  const int slot = blockIdx.x / blocks, seg = (blockIdx.x % blocks) * 4 + (threadIdx.x >> 6);
   const int b = slot / (r.K + 1), i = slot % (r.K + 1);
-  if (i >= r.count(b)) return;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  if (seg >= ns || i >= r.count(b)) return;
   float x[kSamplePer];
-  load_chunk<SRC>(row_at<SRC>(r, r.first(b) + i), chunk, r.V, x);
+  load_segment<SRC>(row_at<SRC>(r, r.first(b) + i), seg, r.V, x);
+  const float t = r.temp(b);
   float m = -INFINITY;
 #pragma unroll
   for (int e = 0; e < kSamplePer; ++e) m = fmaxf(m, x[e]);
   m = group_max<64>(m);
-  if (lane == 0) tops[wave] = m;
+  SegRec g{0.0, m, -1};
+  if (m > -INFINITY) {
+    if (t > 0.0f) {
+      const Scale s = make_scale(m, t);
+#pragma unroll
+      for (int e = 0; e < kSamplePer; e += 8) {
+        double w[8];
+        sample_weights<8>(x + e, s, w);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) g.sum += w[j];
+      }
+      g.sum = wave_sum(g.sum);
+    } else {
+      g.arg = first_place<SRC>(x, m, seg);
+    }
+  }
+  if ((threadIdx.x & 63) == 0) rec[(long long)slot * ns + seg] = g;
+}
+
+// The same with the histogram of the workgroup's four segments, whose common
+// maximum gives the scale.
+template <int SRC>
+__global__ void __launch_bounds__(kSampleThreads)
+    sample_histogram_kernel(SampleRows r, int ns, int blocks, SegRec* rec, Histogram* hist) {
+  __shared__ Histogram h;
+  __shared__ float tops[4];
+  const int slot = blockIdx.x / blocks, wave = threadIdx.x >> 6, seg = (blockIdx.x % blocks) * 4 + wave;
+  const int b = slot / (r.K + 1), i = slot % (r.K + 1);
+  if (i >= r.count(b)) return;
+  for (int j = threadIdx.x; j < kBins; j += kSampleThreads) {
+    h.sum[j] = 0;
+    h.count[j] = 0;
+  }
+  float x[kSamplePer];
+  load_segment<SRC>(row_at<SRC>(r, r.first(b) + i), seg, r.V, x);
+  const float t = r.temp(b);
+  bool by_k, by_p;
+  const bool filters = row_filters(r, b, t, by_k, by_p);
+  float m = -INFINITY;
+#pragma unroll
+  for (int e = 0; e < kSamplePer; ++e) m = fmaxf(m, x[e]);
+  m = group_max<64>(m);
+  if ((threadIdx.x & 63) == 0) tops[wave] = m;
   __syncthreads();
   m = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-  const float t = r.temp(b);
-  double s = 0.0;
-  int arg = 0x7fffffff;
-  if (t > 0.0f) {
-    const double c = sample_scale(t);
-    if (m > -INFINITY) {
+  SegRec g{0.0, m, -1};
+  if (m > -INFINITY) {
+    if (t > 0.0f) {
+      const Scale s = make_scale(m, t);
+      const float bins = bin_scale(s);
+      const int top_bin = bin_of(m, bins);
+      constexpr double kUnit = (double)(1ULL << kBinBits);
 #pragma unroll
-      for (int e = 0; e < kSamplePer; ++e) s += sample_weight(x[e], m, c);
+      for (int e = 0; e < kSamplePer; e += 8) {
+        double w[8];
+        sample_weights<8>(x + e, s, w);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) g.sum += w[j];
+        if (filters) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int bin = top_bin - bin_of(x[e + j], bins);
+            if (bin < kBins && x[e + j] > -INFINITY) {
+              if (by_k) atomicAdd(&h.count[bin], 1u);
+              atomicAdd(&h.sum[bin], fixed_weight(w[j], kUnit));
+            }
+          }
+        }
+      }
+      g.sum = wave_sum(g.sum);
+    } else {
+      g.arg = first_place<SRC>(x, m, seg);
     }
-  } else if (m > -INFINITY) {
-    constexpr int kVec = Logit<SRC>::kVec;
-#pragma unroll
-    for (int e = kSamplePer - 1; e >= 0; --e)
-      if (x[e] == m)
-        arg = chunk * kSampleChunk + ((e / kVec) * kSampleThreads + (int)threadIdx.x) * kVec + e % kVec;
   }
-  s = wave_sum(s);
-  arg = wave_min(arg);
-  if (lane == 0) {
-    sums[wave] = s;
-    args[wave] = arg;
-  }
+  if ((threadIdx.x & 63) == 0 && seg < ns) rec[(long long)slot * ns + seg] = g;
+  if (!filters) return;
   __syncthreads();
-  if (threadIdx.x == 0)
-    rec[(long long)slot * nc + chunk] = ChunkRec{(sums[0] + sums[1]) + (sums[2] + sums[3]), m,
-                                                 min(min(args[0], args[1]), min(args[2], args[3]))};
+  Histogram& to = hist[blockIdx.x];
+  for (int j = threadIdx.x; j < kBins; j += kSampleThreads) {
+    to.sum[j] = h.sum[j];
+    if (by_k) to.count[j] = h.count[j];
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -87,7 +150,7 @@ struct Drafts {
 
 template <int SRC>
 __global__ void __launch_bounds__(kSampleThreads)
-    sample_choose_kernel(SampleRows r, Drafts d, int nc, const ChunkRec* rec, const RowCut* cuts, DrawRec* draws,
+    sample_choose_kernel(SampleRows r, Drafts d, int ns, const SegRec* rec, const RowCut* cuts, DrawRec* draws,
                          long long* tokens, int32_t* accepted) {
   __shared__ int stop;  // the first row whose draft is refused, or the last row
   const int b = blockIdx.x, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -95,60 +158,53 @@ __global__ void __launch_bounds__(kSampleThreads)
   if (threadIdx.x == 0) stop = n - 1;
   __syncthreads();
   const float t = r.temp(b);
-  const bool greedy = !(t > 0.0f);
-  const double c = greedy ? 0.0 : sample_scale(t);
   for (int i = wave; i < n - 1; i += kSampleThreads / kWave) {
     const long long slot = (long long)b * (r.K + 1) + i, at = (long long)b * r.K + i;
-    float top;
-    double sum;
-    int arg;
-    combine_chunks(rec + slot * nc, nc, c, top, sum, arg);
     const long long x = d.id(at);
+    const bool known = x >= 0 && x < r.V;
+    const float u = fmaxf(d.accept[at], 0.0f);
+    const float l = known ? Logit<SRC>::value(row_at<SRC>(r, first + i)[x]) : 0.0f;
+    const float qx = known && d.probs ? d.probs[b * d.seq_stride + i * d.draft_stride + x] : 1.0f;
+    float top;
+    int arg;
+    Scale scale;
+    double sum;
+    combine_segments(rec + slot * ns, ns, t, top, arg, scale, sum);
     bool ok = false;
-    if (x >= 0 && x < r.V && top > -INFINITY) {
-      double w;
-      if (greedy) {
-        w = x == arg ? 1.0 : 0.0;
-        sum = 1.0;
-      } else {
-        const float l = Logit<SRC>::value(row_at<SRC>(r, first + i)[x]);
-        w = sample_weight(l, top, c);
+    if (known && arg != -1) {
+      double w = x == arg ? 1.0 : 0.0;
+      if (arg == -2) {
+        w = sample_weight(l, scale);
         if (cuts) {
           const RowCut cut = cuts[slot];
           sum = cut.sum;
           if (order_value(l, (int)x) < cut.cut) w = 0.0;
         }
       }
-      const double q = d.probs ? (double)d.probs[b * d.seq_stride + i * d.draft_stride + x] : 1.0;
-      const double u = (double)fmaxf(d.accept[at], 0.0f);
-      ok = u * (q < 0.0 ? 0.0 : q) * sum < w;
+      ok = (double)u * (double)(qx < 0.0f ? 0.0f : qx) * sum < w;
     }
     if (!ok && lane == 0) atomicMin(&stop, i);
   }
   __syncthreads();
   const int a = max(stop, 0);
-  if (tokens) {
-    for (int i = threadIdx.x; i <= r.K; i += kSampleThreads)
-      tokens[(long long)b * (r.K + 1) + i] = i < a && n > 0 ? d.id((long long)b * r.K + i) : -1;
-    if (threadIdx.x == 0) accepted[b] = n > 0 ? a : 0;
-  }
+  for (int i = threadIdx.x; i <= r.K; i += kSampleThreads)
+    tokens[(long long)b * (r.K + 1) + i] = i < a && n > 0 ? d.id((long long)b * r.K + i) : -1;
+  if (threadIdx.x == 0) accepted[b] = n > 0 ? a : 0;
   if (wave != 0) return;
   DrawRec w{};
   w.row = -1;
   if (n > 0) {
     const long long slot = (long long)b * (r.K + 1) + a;
-    int arg;
-    combine_chunks(rec + slot * nc, nc, c, w.top, w.sum, arg);
-    w.c = c;
+    Scale scale;
+    combine_segments(rec + slot * ns, ns, t, w.top, w.arg, scale, w.sum);
     w.row = first + a;
-    w.arg = w.top == -INFINITY ? -1 : greedy ? arg : -2;
     w.at = a;
     w.refused = -1;
     if (a < n - 1) {
       const long long x = d.id((long long)b * r.K + a);
       if (x >= 0 && x < r.V) w.refused = (int)x;
     }
-    if (cuts && !greedy) {
+    if (cuts && w.arg == -2) {
       w.cut = cuts[slot].cut;
       w.sum = cuts[slot].sum;
     }
@@ -160,39 +216,60 @@ __global__ void __launch_bounds__(kSampleThreads)
 // 4. and 5. The mass of a row's tokens and the token
 // ---------------------------------------------------------------------------
 
-// What the tokens of the vector at e0 weigh in the draw: p, or where a draft
-// was refused max(p - q, 0), in units of 1 / sum.
-template <int SRC>
-__device__ __forceinline__ void draw_weights(const DrawRec& w, const float* q, bool rest, int e0, int V, const float* x,
-                                             double* out) {
-  constexpr int kVec = Logit<SRC>::kVec;
-  float qx[kVec];
+// A sequence's draw; without one made before, the whole of row b (by one
+// wavefront).
+__device__ __forceinline__ DrawRec draw_of(const SampleRows& r, const DrawRec* draws, const SegRec* rec, int ns, int b,
+                                           Scale& scale) {
+  DrawRec w{};
+  const float t = r.temp(b);
+  if (draws) {
+    w = draws[b];
+    if (w.row >= 0 && w.arg == -2) scale = make_scale(w.top, t);
+  } else {
+    combine_segments(rec + (long long)b * ns, ns, t, w.top, w.arg, scale, w.sum);
+    w.row = b;
+    w.refused = -1;
+  }
+  return w;
+}
+
+// What the tokens e0 .. e0 + N weigh in the draw: p, or where a draft was
+// refused max(p - q, 0), in units of 1 / sum.
+template <int N>
+__device__ __forceinline__ void draw_weights(const DrawRec& w, const Scale& scale, const float* q, bool rest, int e0,
+                                             int V, const float* x, double* out) {
+  float qx[N];
   if (rest && q) {
-    if (e0 + kVec <= V) {
+    if (e0 + N <= V) {
 #pragma unroll
-      for (int h = 0; h < kVec; h += 4) {
+      for (int h = 0; h < N; h += 4) {
         const auto raw = *reinterpret_cast<const Unaligned16<uint32_t>*>(q + e0 + h);
 #pragma unroll
         for (int e = 0; e < 4; ++e) qx[h + e] = __uint_as_float(raw.v[e]);
       }
     } else {
 #pragma unroll
-      for (int e = 0; e < kVec; ++e) qx[e] = e0 + e < V ? q[e0 + e] : 0.0f;
+      for (int e = 0; e < N; ++e) qx[e] = e0 + e < V ? q[e0 + e] : 0.0f;
     }
   }
+  sample_weights<N>(x, scale, out);
+  if (w.cut) {
 #pragma unroll
-  for (int e = 0; e < kVec; ++e) {
-    double p = sample_weight(x[e], w.top, w.c);
-    if (w.cut && order_value(x[e], e0 + e) < w.cut) p = 0.0;
-    if (rest) {
-      if (q) {
-        const double d = fma(-(double)(qx[e] < 0.0f ? 0.0f : qx[e]), w.sum, p);
-        p = d > 0.0 ? d : 0.0;  // (nothing where q is NaN)
-      } else if (e0 + e == w.refused) {
-        p = 0.0;
+    for (int e = 0; e < N; ++e)
+      if (order_value(x[e], e0 + e) < w.cut) out[e] = 0.0;
+  }
+  if (rest) {
+    if (q) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const double d = fma(-(double)(qx[e] < 0.0f ? 0.0f : qx[e]), w.sum, out[e]);
+        out[e] = d > 0.0 ? d : 0.0;  // (nothing where q is NaN)
       }
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        if (e0 + e == w.refused) out[e] = 0.0;
     }
-    out[e] = p;
   }
 }
 
@@ -202,213 +279,165 @@ __device__ __forceinline__ const float* draft_row(const Drafts& d, const DrawRec
 
 template <int SRC>
 __global__ void __launch_bounds__(kSampleThreads)
-    sample_mass_kernel(SampleRows r, Drafts d, int nc, const DrawRec* draws, double* mass, float* probs) {
-  __shared__ double sums[4];
-  const int b = blockIdx.x / nc, chunk = blockIdx.x % nc;
-  const DrawRec w = draws[b];
-  if (w.row < 0) return;
-  constexpr int kVec = Logit<SRC>::kVec;
-  if (w.arg >= -1) {  // greedy, or nothing to draw from
-    if (probs) {
-      for (int i = threadIdx.x; i < kSampleChunk; i += kSampleThreads) {
-        const long long e = (long long)chunk * kSampleChunk + i;
-        if (e < r.V) probs[(long long)b * r.V + e] = e == w.arg ? 1.0f : 0.0f;
-      }
-    }
-    return;
-  }
+    sample_mass_kernel(SampleRows r, Drafts d, int ns, int blocks, const SegRec* rec, const DrawRec* draws, double* mass,
+                       float* probs) {
+  const int b = blockIdx.x / blocks, seg = (blockIdx.x % blocks) * 4 + (threadIdx.x >> 6);
+  if (seg >= ns) return;
+  constexpr int kVec = Logit<SRC>::kVec, kGroups = kSamplePer / kVec;
+  Scale scale;
+  const DrawRec w = draw_of(r, draws, rec, ns, b, scale);
+  if (w.row < 0 || (w.arg != -2 && !probs)) return;
+  const bool known = w.arg != -2;  // greedy, or no token
+  const bool rest = w.refused >= 0;
   const auto* row = row_at<SRC>(r, w.row);
   const float* q = draft_row(d, w, b);
   const double inv = 1.0 / w.sum;
+  float x[kSamplePer];
+  if (!known) load_segment<SRC>(row, seg, r.V, x);
   double s = 0.0;
-#pragma unroll 2
-  for (int i = 0; i < kSamplePer / kVec; ++i) {
-    const int e0 = chunk * kSampleChunk + (i * kSampleThreads + (int)threadIdx.x) * kVec;
-    float x[kVec];
-    double p[kVec];
-    load_vec<SRC>(row, e0, r.V, x);
-    draw_weights<SRC>(w, q, w.refused >= 0, e0, r.V, x, p);
 #pragma unroll
-    for (int e = 0; e < kVec; ++e) s += p[e];
+  for (int i = 0; i < kGroups; ++i) {
+    const int e0 = segment_element<SRC>(seg, i);
+    double p[kVec];
+    if (known) {
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) p[e] = e0 + e == w.arg ? w.sum : 0.0;
+    } else {
+      draw_weights<kVec>(w, scale, q, rest, e0, r.V, x + i * kVec, p);
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) s += p[e];
+    }
     if (probs) {
       float* to = probs + (long long)b * r.V + e0;
+      const double by = known ? 1.0 : inv;
+      if (e0 + kVec <= r.V) {
 #pragma unroll
-      for (int e = 0; e < kVec; ++e)
-        if (e0 + e < r.V) to[e] = (float)(p[e] * inv);
+        for (int h = 0; h < kVec; h += 4) {
+          Unaligned16<uint32_t> raw;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) raw.v[e] = __float_as_uint((float)(p[h + e] * by));
+          *reinterpret_cast<Unaligned16<uint32_t>*>(to + h) = raw;
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < kVec; ++e)
+          if (e0 + e < r.V) to[e] = (float)(p[e] * by);
+      }
     }
   }
+  if (known) return;
   s = wave_sum(s);
-  if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = s;
-  __syncthreads();
-  if (threadIdx.x == 0) mass[(long long)b * nc + chunk] = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+  if ((threadIdx.x & 63) == 0) mass[(long long)b * ns + seg] = s;
 }
 
-// One workgroup per sequence.  mass == NULL: a draw from a row by its chunk
-// records alone (slot b); draws == NULL then.
+// One wavefront per sequence.  mass == NULL: a draw from row b by its segments'
+// sums.
 template <int SRC>
-__global__ void __launch_bounds__(kSampleThreads)
-    sample_pick_kernel(SampleRows r, Drafts d, int nc, const ChunkRec* rec, const DrawRec* draws, const double* mass,
+__global__ void __launch_bounds__(kWave)
+    sample_pick_kernel(SampleRows r, Drafts d, int ns, const SegRec* rec, const DrawRec* draws, const double* mass,
                        const float* uniforms, long long* tokens) {
-  __shared__ double totals[kSamplePer / 4][4];
-  __shared__ double base;
-  __shared__ int where, found, last;
   constexpr int kVec = Logit<SRC>::kVec, kGroups = kSamplePer / kVec;
-  const int b = blockIdx.x, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  DrawRec w{};
-  if (draws) {
-    w = draws[b];
-  } else {
-    const float t = r.temp(b);
-    const bool greedy = !(t > 0.0f);
-    w.c = greedy ? 0.0 : sample_scale(t);
-    int arg;
-    combine_chunks(rec + (long long)b * nc, nc, w.c, w.top, w.sum, arg);
-    w.row = b;
-    w.arg = w.top == -INFINITY ? -1 : greedy ? arg : -2;
-    w.refused = -1;
-  }
+  const int b = blockIdx.x, lane = threadIdx.x;
+  Scale scale;
+  const DrawRec w = draw_of(r, draws, rec, ns, b, scale);
   if (w.row < 0) return;
-  long long* out = tokens + (draws ? (long long)b * (r.K + 1) + w.at : b);
-  if (w.arg >= -1) {
-    if (threadIdx.x == 0) *out = w.arg;
+  long long* out = tokens + (long long)b * (r.K + 1) + w.at;
+  if (w.arg != -2) {
+    if (lane == 0) *out = w.arg;
     return;
   }
   const auto* row = row_at<SRC>(r, w.row);
   const float* q = draft_row(d, w, b);
   const double u = fmin(fmax((double)uniforms[b], 0.0), 1.0);
   bool rest = w.refused >= 0;
-  // The chunk: by one wavefront, 64 at a time.
-  const auto chunk_mass = [&](int j) -> double {
-    if (mass) return mass[(long long)b * nc + j];
-    const ChunkRec g = rec[(long long)b * nc + j];
-    return g.top > -INFINITY ? g.sum * sample_weight(g.top, w.top, w.c) : 0.0;
+  const auto segment_mass = [&](int j) -> double {
+    if (j >= ns) return 0.0;
+    return mass ? mass[(long long)b * ns + j] : segment_sum(rec[(long long)b * ns + j], scale);
   };
-  if (wave == 0) {
-    double total = 0.0;
-    for (int j0 = 0; j0 < nc; j0 += kWave) total += wave_sum(j0 + lane < nc ? chunk_mass(j0 + lane) : 0.0);
-    const double target = u * total;
-    double before = 0.0;
-    int at = -1, some = -1;
-    double left = 0.0, some_left = 0.0;
-    for (int j0 = 0; j0 < nc && at < 0; j0 += kWave) {
-      const double v = j0 + lane < nc ? chunk_mass(j0 + lane) : 0.0;
-      const double run = before + wave_prefix(v);
-      const unsigned long long hit = __ballot(v > 0.0 && run > target), any = __ballot(v > 0.0);
-      if (hit) {
-        const int l = __ffsll(hit) - 1;
-        at = j0 + l;
-        left = target - (__shfl(run, l) - __shfl(v, l));
-      } else if (any) {
-        const int l = 63 - __clzll(any);
-        some = j0 + l;
-        some_left = target - (__shfl(run, l) - __shfl(v, l));
-      }
-      before = __shfl(run, 63);
+  // The segment: the first whose running sum passes u of the whole, or the last
+  // that weighs anything (rounding of the sums, a random number of 1).
+  double total = 0.0;
+  for (int j0 = 0; j0 < ns; j0 += kWave) total += wave_sum(segment_mass(j0 + lane));
+  double target = u * total, before = 0.0, left = 0.0;
+  int seg = -1;
+  bool passed = false;
+  for (int j0 = 0; j0 < ns && !passed; j0 += kWave) {
+    const double v = segment_mass(j0 + lane);
+    const double run = before + wave_prefix(v);
+    const unsigned long long some = __ballot(v > 0.0), hit = __ballot(v > 0.0 && run > target);
+    if (some) {
+      passed = hit != 0;
+      const int at = passed ? __ffsll(hit) - 1 : 63 - __clzll(some);
+      seg = j0 + at;
+      left = target - (__shfl(run, at) - __shfl(v, at));
     }
-    if (at < 0) {  // rounding of the sums, or a random number of 1: the last token that weighs anything
-      at = some;
-      left = some_left;
-    }
-    if (lane == 0) {
-      where = at;
-      base = left;
-      found = 0x7fffffff;
-      last = -1;
-    }
+    before = __shfl(run, 63);
   }
-  __syncthreads();
-  int chunk = where;
-  double target = base;
-  if (chunk < 0) {
-    // Nothing is left of p - q: the row's p itself.  Its chunks have not been
-    // summed, so this (a q that is p but for rounding, or no distribution) walks
-    // the row twice.
-    if (!rest) {
-      if (threadIdx.x == 0) *out = -1;
-      return;
-    }
-    rest = false;
-    double total = 0.0, goal = 0.0, before = 0.0;
-    int lastc = -1;
-    double lastg = 0.0;
-    for (int turn = 0; turn < 2; ++turn) {
+  if (seg < 0) {
+    // Nothing is left of p - q: the row's p itself, whose segments have not
+    // been summed (its cut tokens out), so that this walks the row twice.
+    for (int turn = 0; turn < 2 && rest; ++turn) {
+      if (turn == 1) rest = false;
+      target = u * before;  // (turn 1: of the whole, summed in the same order)
       before = 0.0;
-      for (int j = 0; j < nc; ++j) {
+      for (int j = 0; j < ns; ++j) {
         double s = 0.0;
+#pragma unroll 1
         for (int i = 0; i < kGroups; ++i) {
-          const int e0 = j * kSampleChunk + (i * kSampleThreads + (int)threadIdx.x) * kVec;
+          const int e0 = segment_element<SRC>(j, i);
           float x[kVec];
           double p[kVec];
           load_vec<SRC>(row, e0, r.V, x);
-          draw_weights<SRC>(w, nullptr, false, e0, r.V, x, p);
+          draw_weights<kVec>(w, scale, nullptr, false, e0, r.V, x, p);
 #pragma unroll
           for (int e = 0; e < kVec; ++e) s += p[e];
         }
         s = wave_sum(s);
-        __syncthreads();
-        if (lane == 0) totals[0][wave] = s;
-        __syncthreads();
-        s = (totals[0][0] + totals[0][1]) + (totals[0][2] + totals[0][3]);
         if (turn == 1 && s > 0.0) {
-          lastc = j;
-          lastg = goal - before;
-          if (before + s > goal) break;
+          seg = j;
+          left = target - before;
+          if (before + s > target) break;
         }
         before += s;
       }
-      if (turn == 0) {
-        total = before;
-        goal = u * total;
-      }
-    }
-    __syncthreads();
-    chunk = lastc;
-    target = lastg;
-    if (chunk < 0) {
-      if (threadIdx.x == 0) *out = -1;
-      return;
     }
   }
-  // The token: running sums over the chunk in the order of its indices.
-  double p[kSamplePer], run[kGroups];
-#pragma unroll
-  for (int i = 0; i < kGroups; ++i) {
-    const int e0 = chunk * kSampleChunk + (i * kSampleThreads + (int)threadIdx.x) * kVec;
-    float x[kVec];
-    load_vec<SRC>(row, e0, r.V, x);
-    draw_weights<SRC>(w, rest ? q : nullptr, rest, e0, r.V, x, p + i * kVec);
-    double s = 0.0;
-#pragma unroll
-    for (int e = 0; e < kVec; ++e) s += p[i * kVec + e];
-    run[i] = wave_prefix(s) - s;
-    if (lane == 63) totals[i][wave] = run[i] + s;
+  if (seg < 0) {
+    if (lane == 0) *out = -1;
+    return;
   }
-  __syncthreads();
-  double before = 0.0;
+  // The token: running sums over the segment in the order of its indices.
+  float x[kSamplePer];
+  load_segment<SRC>(row, seg, r.V, x);
+  int token = -1;
+  before = 0.0;
 #pragma unroll
   for (int i = 0; i < kGroups; ++i) {
+    const int e0 = segment_element<SRC>(seg, i);
+    double p[kVec], s = 0.0;
+    draw_weights<kVec>(w, scale, q, rest, e0, r.V, x + i * kVec, p);
 #pragma unroll
-    for (int v = 0; v < 4; ++v) {
-      if (v == wave) {
-        double sum = before + run[i];
-        int hit = -1, some = -1;
+    for (int e = 0; e < kVec; ++e) s += p[e];
+    const double run = before + wave_prefix(s);
+    const unsigned long long some = __ballot(s > 0.0), hit = __ballot(s > 0.0 && run > left);
+    if (some) {
+      const int at = hit ? __ffsll(hit) - 1 : 63 - __clzll(some);
+      double sum = run - s;
+      int last = 0, first = -1;
 #pragma unroll
-        for (int e = 0; e < kVec; ++e) {
-          sum += p[i * kVec + e];
-          if (p[i * kVec + e] > 0.0) {
-            some = e;
-            if (hit < 0 && sum > target) hit = e;
-          }
+      for (int e = 0; e < kVec; ++e) {
+        sum += p[e];
+        if (p[e] > 0.0) {
+          last = e;
+          if (first < 0 && sum > left) first = e;
         }
-        const int e0 = chunk * kSampleChunk + (i * kSampleThreads + (int)threadIdx.x) * kVec;
-        if (hit >= 0) atomicMin(&found, e0 + hit);
-        if (some >= 0) atomicMax(&last, e0 + some);
       }
-      before += totals[i][v];
+      token = __shfl(e0 + (hit && first >= 0 ? first : last), at);
+      if (hit) break;
     }
+    before = __shfl(run, 63);
   }
-  __syncthreads();
-  if (threadIdx.x == 0) *out = found != 0x7fffffff ? found : last;
+  if (lane == 0) *out = token;
 }
 
 // ---------------------------------------------------------------------------
@@ -417,29 +446,36 @@ __global__ void __launch_bounds__(kSampleThreads)
 
 size_t up(size_t n) { return (n + 255) & ~(size_t)255; }
 
+// What a call runs and where its workspace holds what.
 struct Plan {
   long long slots;
-  int nc;
-  bool filtered, direct;  // direct: chunks and pick alone
-  size_t rec, cuts, draws, mass, bytes;
+  int ns, blocks;  // segments and workgroups of a row
+  bool filtered, drafts, masses;
+  size_t hist, cuts, draws, mass, bytes;
 };
 
-Plan plan_of(long long B, int K, int V, bool filtered, bool direct) {
+Plan plan_of(long long B, int K, int V, bool filtered, bool drafts, bool probs) {
   Plan p{};
   p.slots = B * (K + 1);
-  p.nc = (V + kSampleChunk - 1) / kSampleChunk;
+  p.ns = (V + kSegment - 1) / kSegment;
+  p.blocks = (V + kSampleBlock - 1) / kSampleBlock;
   p.filtered = filtered;
-  p.direct = direct && !filtered;
-  size_t at = up((size_t)p.slots * p.nc * sizeof(ChunkRec));
+  p.drafts = drafts;
+  p.masses = filtered || drafts || probs;
+  size_t at = up((size_t)p.slots * p.ns * sizeof(SegRec));
   if (filtered) {
+    p.hist = at;
+    at += up((size_t)p.slots * p.blocks * sizeof(Histogram));
     p.cuts = at;
     at += up((size_t)p.slots * sizeof(RowCut));
   }
-  if (!p.direct) {
+  if (filtered || drafts) {
     p.draws = at;
     at += up((size_t)B * sizeof(DrawRec));
+  }
+  if (p.masses) {
     p.mass = at;
-    at += up((size_t)B * p.nc * sizeof(double));
+    at += up((size_t)B * p.ns * sizeof(double));
   }
   p.bytes = at;
   return p;
@@ -451,26 +487,27 @@ constexpr long long kMostBlocks = (1LL << 32) / 1024 - 1;
 template <int SRC>
 int run(const SampleRows& r, const Drafts& d, const Plan& p, char* ws, const float* uniforms, float* probs,
         long long* tokens, int32_t* accepted, hipStream_t st, const char* who) {
-  auto* rec = reinterpret_cast<ChunkRec*>(ws);
-  auto* cuts = p.filtered ? reinterpret_cast<RowCut*>(ws + p.cuts) : nullptr;
-  hipLaunchKernelGGL((sample_chunk_kernel<SRC>), dim3((unsigned)(p.slots * p.nc)), dim3(kSampleThreads), 0, st, r, p.nc,
-                     rec);
-  DrawRec* draws = nullptr;
-  double* mass = nullptr;
-  if (!p.direct) {
-    draws = reinterpret_cast<DrawRec*>(ws + p.draws);
-    mass = reinterpret_cast<double*>(ws + p.mass);
-    if (cuts) {
-      const int rc = launch_sample_cut(r, SRC, p.nc, rec, cuts, st);
-      if (rc) return rc;
-    }
-    hipLaunchKernelGGL((sample_choose_kernel<SRC>), dim3(r.B), dim3(kSampleThreads), 0, st, r, d, p.nc, rec, cuts,
-                       draws, accepted ? tokens : nullptr, accepted);
-    hipLaunchKernelGGL((sample_mass_kernel<SRC>), dim3((unsigned)((long long)r.B * p.nc)), dim3(kSampleThreads), 0, st,
-                       r, d, p.nc, draws, mass, probs);
+  auto* rec = reinterpret_cast<SegRec*>(ws);
+  auto* draws = p.draws ? reinterpret_cast<DrawRec*>(ws + p.draws) : nullptr;
+  auto* mass = p.masses ? reinterpret_cast<double*>(ws + p.mass) : nullptr;
+  const dim3 row_blocks((unsigned)(p.slots * p.blocks)), threads(kSampleThreads);
+  RowCut* cuts = nullptr;
+  if (p.filtered) {
+    auto* hist = reinterpret_cast<Histogram*>(ws + p.hist);
+    cuts = reinterpret_cast<RowCut*>(ws + p.cuts);
+    hipLaunchKernelGGL((sample_histogram_kernel<SRC>), row_blocks, threads, 0, st, r, p.ns, p.blocks, rec, hist);
+    if (int rc = launch_sample_cut(r, SRC, rec, hist, cuts, p.drafts ? nullptr : draws, st)) return rc;
+  } else {
+    hipLaunchKernelGGL((sample_segment_kernel<SRC>), row_blocks, threads, 0, st, r, p.ns, p.blocks, rec);
   }
-  hipLaunchKernelGGL((sample_pick_kernel<SRC>), dim3(r.B), dim3(kSampleThreads), 0, st, r, d, p.nc, rec, draws, mass,
-                     uniforms, tokens);
+  if (p.drafts)
+    hipLaunchKernelGGL((sample_choose_kernel<SRC>), dim3(r.B), threads, 0, st, r, d, p.ns, rec, cuts, draws, tokens,
+                       accepted);
+  if (p.masses)
+    hipLaunchKernelGGL((sample_mass_kernel<SRC>), dim3((unsigned)((long long)r.B * p.blocks)), threads, 0, st, r, d,
+                       p.ns, p.blocks, rec, draws, mass, probs);
+  hipLaunchKernelGGL((sample_pick_kernel<SRC>), dim3(r.B), dim3(kWave), 0, st, r, d, p.ns, rec, draws, mass, uniforms,
+                     tokens);
   return launch_status(who);
 }
 
@@ -496,8 +533,8 @@ int check_sizes(long long B, int K, int V, int dtype, long long stride, const ch
     set_error("%s: V=%d above %d", who, V, VRM_SAMPLE_MAX_V);
     return VRM_ERR_UNSUPPORTED;
   }
-  const long long nc = (V + kSampleChunk - 1) / kSampleChunk;
-  if (B > 0 && ((long long)K + 1 > kMostBlocks / nc / B)) {
+  const long long blocks = (V + kSampleBlock - 1) / kSampleBlock;
+  if (B > 0 && ((long long)K + 1 > kMostBlocks / blocks / B)) {
     set_error("%s: %lld sequences of %d rows of %d logits are too many for one call", who, B, K + 1, V);
     return VRM_ERR_UNSUPPORTED;
   }
@@ -528,7 +565,7 @@ using namespace vrm;
 
 extern "C" size_t vrm_sample_workspace_bytes(int N, int V, int filtered, int with_probs) {
   if (check_sizes(N, 0, V, VRM_SRC_F32, 0, "vrm_sample_workspace_bytes")) return 0;
-  return plan_of(N, 0, V, filtered != 0, !with_probs).bytes;
+  return plan_of(N, 0, V, filtered != 0, false, with_probs != 0).bytes;
 }
 
 extern "C" int vrm_sample_tokens(const void* logits, int dtype, long long row_stride, const float* uniforms,
@@ -545,7 +582,7 @@ extern "C" int vrm_sample_tokens(const void* logits, int dtype, long long row_st
     set_error("%s: null pointer argument", who);
     return VRM_ERR_ARG;
   }
-  const Plan p = plan_of(N, 0, V, filters(top_k, top_k_all, top_p, top_p_all, V), !probs);
+  const Plan p = plan_of(N, 0, V, filters(top_k, top_k_all, top_p, top_p_all, V), false, probs != nullptr);
   if (int rc = check_workspace(workspace, workspace_bytes, p.bytes, who)) return rc;
   const SampleRows r{logits, row_stride, nullptr, N, N, 0, V, temperature, temperature_all, top_k, top_k_all, top_p,
                      top_p_all};
@@ -555,7 +592,7 @@ extern "C" int vrm_sample_tokens(const void* logits, int dtype, long long row_st
 
 extern "C" size_t vrm_verify_workspace_bytes(int B, int K, int V, int filtered) {
   if (check_sizes(B, K, V, VRM_SRC_F32, 0, "vrm_verify_workspace_bytes")) return 0;
-  return plan_of(B, K, V, filtered != 0, false).bytes;
+  return plan_of(B, K, V, filtered != 0, true, false).bytes;
 }
 
 extern "C" int vrm_verify_drafts(const void* logits, int dtype, long long row_stride, const int32_t* cu_seqlens,
@@ -587,7 +624,7 @@ extern "C" int vrm_verify_drafts(const void* logits, int dtype, long long row_st
     set_error("%s: null pointer argument", who);
     return VRM_ERR_ARG;
   }
-  const Plan p = plan_of(B, K, V, filters(top_k, top_k_all, top_p, top_p_all, V), false);
+  const Plan p = plan_of(B, K, V, filters(top_k, top_k_all, top_p, top_p_all, V), true, false);
   if (int rc = check_workspace(workspace, workspace_bytes, p.bytes, who)) return rc;
   const SampleRows r{logits, row_stride, cu_seqlens, N, B, K, V, temperature, temperature_all, top_k, top_k_all, top_p,
                      top_p_all};
