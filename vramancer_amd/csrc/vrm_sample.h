@@ -138,11 +138,21 @@ __device__ __forceinline__ void sample_weights(const float* l, const Scale& s, d
     for (int i = 0; i < 4; ++i) w[e + i] = __builtin_ldexp(q[i], n[i]);
   }
 }
+// The same for one logit, to the same bits (the steps are the same).
 __device__ __forceinline__ double sample_weight(float l, const Scale& s) {
-  const float x[4] = {l, l, l, l};
-  double w[4];
-  sample_weights<4>(x, s, w);
-  return w[0];
+  if (s.infinite) return l == INFINITY ? 1.0 : 0.0;
+  constexpr double kBig = 6755399441055744.0;
+  const double x = fmax((double)l - s.top, s.low);
+  const double big = fma(x, s.c, kBig);
+  const double r = fma(x, s.c, -(big - kBig));
+  double q = fma(0x1.63b2d7971923fp-20, r, 0x1.00c0e4e15189cp-16);
+  q = fma(q, r, 0x1.4308c7183d6a2p-13);
+  q = fma(q, r, 0x1.5d877598350dep-10);
+  q = fma(q, r, 0x1.3b2ab70ad2565p-7);
+  q = fma(q, r, 0x1.c6b08da70cce3p-5);
+  q = fma(q, r, 0x1.ebfbdff82a734p-3);
+  q = fma(q, r, 0x1.62e42fef9cc69p-1);
+  return __builtin_ldexp(fma(q, r, 1.0), (int)__double_as_longlong(big));
 }
 
 // Order value of token i: larger for what comes first (larger logit, then
@@ -232,24 +242,62 @@ __device__ __forceinline__ void load_segment(const typename Logit<SRC>::Raw* row
   }
 }
 
-// Sums, prefixes and smallest values over a wavefront, in a fixed order.
-__device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-  for (int m = 1; m < kWave; m <<= 1) v += __shfl_xor(v, m);
-  return v;
-}
-__device__ __forceinline__ double wave_prefix(double v) {  // inclusive
-#pragma unroll
-  for (int m = 1; m < kWave; m <<= 1) {
-    const double o = __shfl_up(v, m);
-    if ((int)(threadIdx.x & 63) >= m) v += o;
+// Prefixes over a wavefront on the vector ALU, and from them sums, largest and
+// smallest values as scalars: within a row of 16 lanes, then from row to row.
+// (Exchanges through the LDS unit answer after some 100 cycles, and 16
+// wavefronts that all reduce wait for each other there: a bin of the cut took
+// 12,000 cycles to find with them.)  The order of a sum is fixed.
+template <typename T>
+__device__ __forceinline__ T lane_value(T v, int lane) {  // lane: the same in all
+  if constexpr (sizeof(T) == 4) {
+    return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
+  } else {
+    const auto u = __builtin_bit_cast(unsigned long long, v);
+    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)u, lane);
+    const uint32_t hi = __builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), lane);
+    return __builtin_bit_cast(T, ((unsigned long long)hi << 32) | lo);
   }
+}
+
+template <int CTRL, int ROWS, typename T>
+__device__ __forceinline__ T lane_move(T v, T identity) {
+  if constexpr (sizeof(T) == 4) {
+    return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, identity),
+                                                             __builtin_bit_cast(int, v), CTRL, ROWS, 0xf, false));
+  } else {
+    const auto u = __builtin_bit_cast(unsigned long long, v), i = __builtin_bit_cast(unsigned long long, identity);
+    const uint32_t lo = __builtin_amdgcn_update_dpp((int)(uint32_t)i, (int)(uint32_t)u, CTRL, ROWS, 0xf, false);
+    const uint32_t hi =
+        __builtin_amdgcn_update_dpp((int)(uint32_t)(i >> 32), (int)(uint32_t)(u >> 32), CTRL, ROWS, 0xf, false);
+    return __builtin_bit_cast(T, ((unsigned long long)hi << 32) | lo);
+  }
+}
+
+template <typename T, typename Op>
+__device__ __forceinline__ T wave_scan(T v, T identity, Op op) {  // inclusive
+  v = op(v, lane_move<0x111, 0xf>(v, identity));  // row_shr 1, 2, 4, 8
+  v = op(v, lane_move<0x112, 0xf>(v, identity));
+  v = op(v, lane_move<0x114, 0xf>(v, identity));
+  v = op(v, lane_move<0x118, 0xf>(v, identity));
+  v = op(v, lane_move<0x142, 0xa>(v, identity));  // row_bcast 15 into rows 1 and 3
+  v = op(v, lane_move<0x143, 0xc>(v, identity));  // row_bcast 31 into rows 2 and 3
   return v;
 }
-__device__ __forceinline__ int wave_min(int v) {
-#pragma unroll
-  for (int m = 1; m < kWave; m <<= 1) v = min(v, __shfl_xor(v, m));
-  return v;
+template <typename T>
+__device__ __forceinline__ T wave_prefix(T v) {
+  return wave_scan(v, T(0), [](T a, T b) { return a + b; });
+}
+template <typename T>
+__device__ __forceinline__ T wave_sum(T v) {
+  return lane_value(wave_prefix(v), 63);
+}
+template <typename T>
+__device__ __forceinline__ T wave_min(T v, T most) {
+  return lane_value(wave_scan(v, most, [](T a, T b) { return a < b ? a : b; }), 63);
+}
+template <typename T>
+__device__ __forceinline__ T wave_max(T v, T least) {
+  return lane_value(wave_scan(v, least, [](T a, T b) { return a < b ? b : a; }), 63);
 }
 
 // A segment's sum by its row's scale.
@@ -264,7 +312,7 @@ __device__ __forceinline__ void combine_segments(const SegRec* rec, int ns, floa
   const int lane = threadIdx.x & 63;
   float m = -INFINITY;
   for (int j = lane; j < ns; j += kWave) m = fmaxf(m, rec[j].top);
-  top = group_max<64>(m);
+  top = wave_max(m, -INFINITY);
   arg = -1;
   sum = 0.0;
   if (top == -INFINITY) return;
@@ -272,7 +320,7 @@ __device__ __forceinline__ void combine_segments(const SegRec* rec, int ns, floa
     int first = 0x7fffffff;
     for (int j = lane; j < ns; j += kWave)
       if (rec[j].top == top) first = min(first, rec[j].arg);
-    arg = wave_min(first);
+    arg = wave_min(first, 0x7fffffff);
     sum = 1.0;
     return;
   }

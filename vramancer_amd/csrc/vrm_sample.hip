@@ -27,7 +27,7 @@ __device__ __forceinline__ int first_place(const float* x, float m, int seg) {
 #pragma unroll
   for (int e = kSamplePer - 1; e >= 0; --e)
     if (x[e] == m) arg = segment_element<SRC>(seg, e / kVec) + e % kVec;
-  return wave_min(arg);
+  return wave_min(arg, 0x7fffffff);
 }
 
 // ---------------------------------------------------------------------------
@@ -45,7 +45,7 @@ __global__ void __launch_bounds__(kSampleThreads) sample_segment_kernel(SampleRo
   float m = -INFINITY;
 #pragma unroll
   for (int e = 0; e < kSamplePer; ++e) m = fmaxf(m, x[e]);
-  m = group_max<64>(m);
+  m = wave_max(m, -INFINITY);
   SegRec g{0.0, m, -1};
   if (m > -INFINITY) {
     if (t > 0.0f) {
@@ -87,7 +87,7 @@ __global__ void __launch_bounds__(kSampleThreads)
   float m = -INFINITY;
 #pragma unroll
   for (int e = 0; e < kSamplePer; ++e) m = fmaxf(m, x[e]);
-  m = group_max<64>(m);
+  m = wave_max(m, -INFINITY);
   if ((threadIdx.x & 63) == 0) tops[wave] = m;
   __syncthreads();
   m = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
@@ -369,9 +369,9 @@ __global__ void __launch_bounds__(kWave)
       passed = hit != 0;
       const int at = passed ? __ffsll(hit) - 1 : 63 - __clzll(some);
       seg = j0 + at;
-      left = target - (__shfl(run, at) - __shfl(v, at));
+      left = target - (lane_value(run, at) - lane_value(v, at));
     }
-    before = __shfl(run, 63);
+    before = lane_value(run, 63);
   }
   if (seg < 0) {
     // Nothing is left of p - q: the row's p itself, whose segments have not
@@ -432,10 +432,10 @@ __global__ void __launch_bounds__(kWave)
           if (first < 0 && sum > left) first = e;
         }
       }
-      token = __shfl(e0 + (hit && first >= 0 ? first : last), at);
+      token = lane_value(e0 + (hit && first >= 0 ? first : last), at);
       if (hit) break;
     }
-    before = __shfl(run, 63);
+    before = lane_value(run, 63);
   }
   if (lane == 0) *out = token;
 }
