@@ -366,9 +366,28 @@ __device__ __forceinline__ bool row_filters(const SampleRows& r, int b, float t,
   return t > 0.0f && (by_k || by_p);
 }
 
+// What a row's cut looks for (vrm_sample_cut.hip).  Bins are absolute; first is
+// the one of the larger logits.
+constexpr int kListed = 4096;  // tokens that a row's list holds
+
+struct CutPlan {
+  double kept;                // the sum of the row's weights, all of them
+  double total;               // the same by the histograms
+  double k_before, p_before;  // sums before the bins of the borders
+  float top;
+  int arg;                    // as DrawRec's
+  int filters;                // whether anything is cut
+  int k;                      // top_k's, 0 where it cuts nothing
+  uint32_t k_count;           // tokens before its bin
+  int by_p;
+  int k_first, k_last, p_first, p_last;
+  int list_first, list_last, also, also_first, also_last;  // bins to list
+  int listed;                 // how many tokens they have
+};
+
 // Finds every row's cut from the histograms of its parts; with draws (sequences
-// of one row) its draw too.
-int launch_sample_cut(const SampleRows& r, int dtype, const SegRec* rec, const Histogram* hist, RowCut* cuts,
-                      DrawRec* draws, hipStream_t st);
+// of one row) its draw too.  lists: kListed order values a row.
+int launch_sample_cut(const SampleRows& r, int dtype, const SegRec* rec, const Histogram* hist, CutPlan* plans,
+                      unsigned long long* lists, RowCut* cuts, DrawRec* draws, hipStream_t st);
 
 }  // namespace vrm

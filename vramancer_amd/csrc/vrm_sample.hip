@@ -7,7 +7,7 @@
 //   1. sample_segment_kernel    every row's segments: maximum, sum of weights;
 //      sample_histogram_kernel  the same and histograms, where top_k or top_p
 //                               may drop tokens
-//   2. sample_cut_kernel        which tokens stay (vrm_sample_cut.hip)
+//   2. launch_sample_cut        which tokens stay (vrm_sample_cut.hip)
 //   3. sample_choose_kernel     a sequence's drafts: accepted ones, the row its
 //                               next token is drawn from
 //   4. sample_mass_kernel       that row's segments: the mass to draw from
@@ -451,7 +451,7 @@ struct Plan {
   long long slots;
   int ns, blocks;  // segments and workgroups of a row
   bool filtered, drafts, masses;
-  size_t hist, cuts, draws, mass, bytes;
+  size_t hist, plans, lists, cuts, draws, mass, bytes;
 };
 
 Plan plan_of(long long B, int K, int V, bool filtered, bool drafts, bool probs) {
@@ -466,6 +466,10 @@ Plan plan_of(long long B, int K, int V, bool filtered, bool drafts, bool probs) 
   if (filtered) {
     p.hist = at;
     at += up((size_t)p.slots * p.blocks * sizeof(Histogram));
+    p.plans = at;
+    at += up((size_t)p.slots * sizeof(CutPlan));
+    p.lists = at;
+    at += up((size_t)p.slots * kListed * sizeof(unsigned long long));
     p.cuts = at;
     at += up((size_t)p.slots * sizeof(RowCut));
   }
@@ -496,7 +500,10 @@ int run(const SampleRows& r, const Drafts& d, const Plan& p, char* ws, const flo
     auto* hist = reinterpret_cast<Histogram*>(ws + p.hist);
     cuts = reinterpret_cast<RowCut*>(ws + p.cuts);
     hipLaunchKernelGGL((sample_histogram_kernel<SRC>), row_blocks, threads, 0, st, r, p.ns, p.blocks, rec, hist);
-    if (int rc = launch_sample_cut(r, SRC, rec, hist, cuts, p.drafts ? nullptr : draws, st)) return rc;
+    if (int rc = launch_sample_cut(r, SRC, rec, hist, reinterpret_cast<CutPlan*>(ws + p.plans),
+                                   reinterpret_cast<unsigned long long*>(ws + p.lists), cuts,
+                                   p.drafts ? nullptr : draws, st))
+      return rc;
   } else {
     hipLaunchKernelGGL((sample_segment_kernel<SRC>), row_blocks, threads, 0, st, r, p.ns, p.blocks, rec);
   }
