@@ -17,6 +17,8 @@
 // on the device already (tokens stored and new tokens of each request, a block
 // table that stays there), so that a step whose lengths follow from the one
 // before it, as accepted drafts do, starts without a copy to the host.
+#include <algorithm>
+
 #include "vrm_common.h"
 
 namespace vrm {
@@ -68,32 +70,138 @@ struct ChunkTableArgs {
   }
 };
 
-constexpr int kScanThreads = 1024;
+constexpr int kScanThreads = 512;
+constexpr int kScanPer = 4;
+constexpr int kScanMost = kScanThreads * kScanPer;  // sequences whose offsets every workgroup can have
+constexpr int kEntries = 4 * kScanThreads;          // page table entries of a workgroup
 
-// Offsets of the new tokens, cut at N, and the lengths that follow from them.
+// Running sum over the workgroup's values, inclusive; `all` the whole.
+__device__ __forceinline__ long long block_prefix(long long v, long long* waves, long long& all) {
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) {
+    const long long o = __shfl_up(v, m);
+    if (lane >= m) v += o;
+  }
+  __syncthreads();
+  if (lane == 63) waves[wave] = v;
+  __syncthreads();
+  all = 0;
+  for (int w = 0; w < kScanThreads / 64; ++w) {
+    if (w < wave) v += waves[w];
+    all += waves[w];
+  }
+  return v;
+}
+
+// Every `parts`-th kEntries of one sequence's row of the page table.  (wide:
+// rows of both tables start on 16 bytes and have whole vectors.)
+__device__ __forceinline__ void fill_row(const ChunkTableArgs& a, int b, int part, int parts, int context, bool wide) {
+  const int r = a.request(b);
+  const int held = r >= 0 ? (int)min(((long long)context + a.PS - 1) / a.PS, (long long)a.W) : 0;
+  const int32_t* from = a.block_table + (r >= 0 ? r : 0) * a.row_stride;
+  int32_t* to = a.page_table + (size_t)b * a.max_pp;
+  for (long long p0 = (long long)part * kEntries; p0 < a.max_pp; p0 += (long long)parts * kEntries) {
+    if (wide) {
+      const int p = (int)p0 + 4 * threadIdx.x;
+      if (p >= a.max_pp) return;
+      int4 v = make_int4(-1, -1, -1, -1);
+      if (p < held) {
+        v = *reinterpret_cast<const int4*>(from + p);
+        if (p + 1 >= held) v.y = -1;
+        if (p + 2 >= held) v.z = -1;
+        if (p + 3 >= held) v.w = -1;
+      }
+      *reinterpret_cast<int4*>(to + p) = v;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const long long p = p0 + i * kScanThreads + threadIdx.x;
+        if (p < a.max_pp) to[p] = p < held ? from[p] : -1;
+      }
+    }
+  }
+}
+
+// The place of new token n.
+__device__ __forceinline__ void place_token(const ChunkTableArgs& a, const int* cu, int n) {
+  int pos = 0, page = -1, slot = -1, seq = -1;
+  if (n < cu[a.B]) {
+    int lo = 0, hi = a.B - 1;  // the sequence that ends first after n
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (cu[mid + 1] > n) hi = mid;
+      else lo = mid + 1;
+    }
+    seq = lo;
+    const int r = a.request(seq);
+    pos = a.stored(r) + n - cu[seq];
+    slot = pos % a.PS;
+    const int p = pos / a.PS;
+    if (r >= 0 && p < a.W) page = a.block_table[r * a.row_stride + p];
+  }
+  a.positions[n] = pos;
+  a.page_ids[n] = page;
+  a.slots[n] = slot;
+  a.sequences[n] = seq;
+}
+
+// Everything in one launch: up to kScanMost sequences each workgroup sums the
+// counts by itself (12 bytes a sequence, from L2 but for the first), which costs
+// less than a launch of its own for it.  Blocks 0 .. table_blocks fill the page
+// table, the others place 512 new tokens each; the last one writes the offsets.
+__global__ void __launch_bounds__(kScanThreads)
+    chunk_tables_kernel(ChunkTableArgs a, int per_row, int table_blocks, bool wide) {
+  __shared__ int cu[kScanMost + 1];
+  __shared__ long long waves[kScanThreads / 64];
+  int n[kScanPer], past[kScanPer];
+  long long sum = 0, all;
+#pragma unroll
+  for (int i = 0; i < kScanPer; ++i) {
+    const int b = kScanPer * threadIdx.x + i;
+    const int r = b < a.B ? a.request(b) : -1;
+    past[i] = a.stored(r);
+    n[i] = r >= 0 ? a.asked(b, r) : 0;
+    sum += n[i];
+  }
+  long long run = block_prefix(sum, waves, all) - sum;
+  if (threadIdx.x == 0) cu[0] = 0;
+  const bool writes = blockIdx.x == gridDim.x - 1;
+  if (writes && threadIdx.x == 0) a.cu[0] = 0;
+#pragma unroll
+  for (int i = 0; i < kScanPer; ++i) {
+    const int b = kScanPer * threadIdx.x + i;
+    const int beg = (int)min(run, (long long)a.N);
+    run += n[i];
+    const int end = (int)min(run, (long long)a.N);
+    if (b < a.B) {
+      cu[b + 1] = end;
+      if (writes) {
+        a.cu[b + 1] = end;
+        a.context_lens[b] = past[i] + (end - beg);
+      }
+    }
+  }
+  __syncthreads();
+  if ((int)blockIdx.x < table_blocks) {
+    const int b = blockIdx.x / per_row;
+    fill_row(a, b, blockIdx.x % per_row, per_row, a.stored(a.request(b)) + cu[b + 1] - cu[b], wide);
+    return;
+  }
+  const int token = ((int)blockIdx.x - table_blocks) * kScanThreads + threadIdx.x;
+  if (token < a.N) place_token(a, cu, token);
+}
+
+// More sequences: the offsets first, by one workgroup.
 __global__ void __launch_bounds__(kScanThreads) chunk_offsets_kernel(ChunkTableArgs a) {
   __shared__ long long waves[kScanThreads / 64];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  long long before = 0;
+  long long before = 0, all;
   if (threadIdx.x == 0) a.cu[0] = 0;
   for (int b0 = 0; b0 < a.B; b0 += kScanThreads) {
     const int b = b0 + threadIdx.x;
     const int r = b < a.B ? a.request(b) : -1;
-    const long long n = b < a.B ? a.asked(b, r) : 0;
-    long long run = n;
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) {
-      const long long o = __shfl_up(run, m);
-      if (lane >= m) run += o;
-    }
-    __syncthreads();
-    if (lane == 63) waves[wave] = run;
-    __syncthreads();
-    long long all = 0;
-    for (int v = 0; v < kScanThreads / 64; ++v) {
-      if (v == wave) run += before + all;
-      all += waves[v];
-    }
+    const long long n = r >= 0 ? a.asked(b, r) : 0;
+    const long long run = before + block_prefix(n, waves, all);
     before += all;
     if (b < a.B) {
       const long long end = min(run, (long long)a.N), beg = min(run - n, (long long)a.N);
@@ -103,42 +211,15 @@ __global__ void __launch_bounds__(kScanThreads) chunk_offsets_kernel(ChunkTableA
   }
 }
 
-// Blocks 0 .. table_blocks: 1024 entries of a sequence's row of the page table
-// each; the others 256 new tokens each.
-__global__ void __launch_bounds__(kTableThreads) chunk_places_kernel(ChunkTableArgs a, int per_row, int table_blocks) {
+__global__ void __launch_bounds__(kScanThreads)
+    chunk_places_kernel(ChunkTableArgs a, int per_row, int table_blocks, bool wide) {
   if ((int)blockIdx.x < table_blocks) {
-    const int b = blockIdx.x / per_row, p0 = (blockIdx.x % per_row) * 4 * kTableThreads;
-    const int r = a.request(b);
-    const int held = (int)min(((long long)a.context_lens[b] + a.PS - 1) / a.PS, (long long)a.W);
-    const int32_t* from = a.block_table + (r >= 0 ? r : 0) * a.row_stride;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int p = p0 + i * kTableThreads + threadIdx.x;
-      if (p < a.max_pp) a.page_table[(size_t)b * a.max_pp + p] = r >= 0 && p < held ? from[p] : -1;
-    }
+    const int b = blockIdx.x / per_row;
+    fill_row(a, b, blockIdx.x % per_row, per_row, a.context_lens[b], wide);
     return;
   }
-  const int n = ((int)blockIdx.x - table_blocks) * kTableThreads + threadIdx.x;
-  if (n >= a.N) return;
-  int pos = 0, page = -1, slot = -1, seq = -1;
-  if (n < a.cu[a.B]) {
-    int lo = 0, hi = a.B - 1;  // the last sequence that starts at or before n and is not empty
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (a.cu[mid + 1] > n) hi = mid;
-      else lo = mid + 1;
-    }
-    seq = lo;
-    const int r = a.request(seq);
-    pos = a.stored(r) + n - a.cu[seq];
-    slot = pos % a.PS;
-    const int p = pos / a.PS;
-    if (r >= 0 && p < a.W) page = a.block_table[r * a.row_stride + p];
-  }
-  a.positions[n] = pos;
-  a.page_ids[n] = page;
-  a.slots[n] = slot;
-  a.sequences[n] = seq;
+  const int token = ((int)blockIdx.x - table_blocks) * kScanThreads + threadIdx.x;
+  if (token < a.N) place_token(a, a.cu, token);
 }
 
 template <int SRC>
@@ -256,19 +337,30 @@ extern "C" int vrm_chunk_tables(const int32_t* block_table, long long row_stride
     set_error("%s: null pointer argument", who);
     return VRM_ERR_ARG;
   }
-  const long long per_row = (max_pp + 4LL * kTableThreads - 1) / (4 * kTableThreads);
-  const long long table_blocks = per_row * B, blocks = table_blocks + (N + kTableThreads - 1LL) / kTableThreads;
-  if (blocks > (1LL << 32) / kTableThreads - 1) {  // a launch counts its threads in 32 bits
+  // Workgroups of a row: one, or more where rows are few (a thousand in all fill
+  // the chip, and each sums the counts first).
+  const long long per_row =
+      max_pp == 0 ? 0 : B >= 1024 ? 1 : std::min((max_pp + kEntries - 1LL) / kEntries, 1024LL / std::max(B, 1));
+  const long long table_blocks = per_row * B;
+  const long long blocks = table_blocks + (N + kScanThreads - 1LL) / kScanThreads;
+  if (blocks > (1LL << 32) / kScanThreads - 2) {  // a launch counts its threads in 32 bits
     set_error("%s: %d rows of %d pages and %d tokens are too many for one call", who, B, max_pp, N);
     return VRM_ERR_UNSUPPORTED;
   }
   const ChunkTableArgs a{block_table, row_stride, R, W, past_lens, counts, requests, B, N, PS, page_table, max_pp,
                          context_lens, cu_seqlens, positions, page_ids, slots, sequences};
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  hipLaunchKernelGGL(chunk_offsets_kernel, dim3(1), dim3(kScanThreads), 0, st, a);
-  if (blocks > 0)
-    hipLaunchKernelGGL(chunk_places_kernel, dim3((unsigned)blocks), dim3(kTableThreads), 0, st, a, (int)per_row,
-                       (int)table_blocks);
+  const bool wide = !(((uintptr_t)block_table | (uintptr_t)page_table) & 15) && !(row_stride & 3) && !(max_pp & 3) &&
+                    !(W & 3);
+  if (B <= kScanMost) {
+    hipLaunchKernelGGL(chunk_tables_kernel, dim3((unsigned)(blocks > 0 ? blocks : 1)), dim3(kScanThreads), 0, st, a,
+                       (int)per_row, (int)table_blocks, wide);
+  } else {
+    hipLaunchKernelGGL(chunk_offsets_kernel, dim3(1), dim3(kScanThreads), 0, st, a);
+    if (blocks > 0)
+      hipLaunchKernelGGL(chunk_places_kernel, dim3((unsigned)blocks), dim3(kScanThreads), 0, st, a, (int)per_row,
+                         (int)table_blocks, wide);
+  }
   return launch_status(who);
 }
 

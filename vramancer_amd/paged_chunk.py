@@ -305,9 +305,16 @@ def chunk_tables(
     if requests is not None:
         requests = _ints("requests", requests, B)
     if out is None:
-        sizes = [B * max_pp, B, B + 1, N, N, N, N]
-        parts = torch.empty(sum(sizes), dtype=torch.int32, device=block_table.device).split(sizes)
-        out = ChunkTables(parts[0].view(B, max_pp), *parts[1:])
+        _lib.require_cuda(block_table, past_lens, counts, requests)
+        sizes = (B * max_pp, B, B + 1, N, N, N, N)
+        parts = torch.empty(sum(sizes), dtype=torch.int32, device=block_table.device)
+        at = parts.data_ptr()
+        ptrs = []
+        for n in sizes:
+            ptrs.append(at)
+            at += 4 * n
+        table, ctx, cu, pos, page, slot, seq = parts.split(sizes)
+        out = ChunkTables(table.view(B, max_pp), ctx, cu, pos, page, slot, seq)
     else:
         for name, shape in (("page_table", (B, max_pp)), ("context_lens", (B,)), ("cu_seqlens", (B + 1,)),
                             ("positions", (N,)), ("page_ids", (N,)), ("slots", (N,)), ("sequences", (N,))):
@@ -315,12 +322,12 @@ def chunk_tables(
             if tuple(t.shape) != shape or t.dtype != torch.int32 or not t.is_contiguous():
                 raise RuntimeError(f"out.{name} must be a contiguous int32 {list(shape)} tensor, got {t.dtype} "
                                    f"{tuple(t.shape)}")
-    _lib.require_cuda(block_table, past_lens, counts, requests, out.page_table, out.context_lens, out.cu_seqlens,
-                      out.positions, out.page_ids, out.slots, out.sequences)
-    ptr = _lib.ptr
+        tensors = (out.page_table, out.context_lens, out.cu_seqlens, out.positions, out.page_ids, out.slots,
+                   out.sequences)
+        _lib.require_cuda(block_table, past_lens, counts, requests, *tensors)
+        ptrs = [t.data_ptr() for t in tensors]
     rc = launch(block_table, _lib.load().vrm_chunk_tables, block_table.data_ptr(), block_table.stride(0), R, W,
-                past_lens.data_ptr(), counts.data_ptr(), ptr(requests), B, N, PS, out.page_table.data_ptr(), max_pp,
-                out.context_lens.data_ptr(), out.cu_seqlens.data_ptr(), out.positions.data_ptr(),
-                out.page_ids.data_ptr(), out.slots.data_ptr(), out.sequences.data_ptr())
+                past_lens.data_ptr(), counts.data_ptr(), None if requests is None else requests.data_ptr(), B, N, PS,
+                ptrs[0], max_pp, *ptrs[1:])
     _lib.check(rc, "chunk_tables")
     return out
