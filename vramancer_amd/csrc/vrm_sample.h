@@ -331,6 +331,150 @@ __device__ __forceinline__ void combine_segments(const SegRec* rec, int ns, floa
   sum = wave_sum(s);
 }
 
+// What the tokens e0 .. e0 + N weigh in the draw: p, or where a draft was
+// refused max(p - q, 0), in units of 1 / sum.
+template <int N>
+__device__ __forceinline__ void draw_weights(const DrawRec& w, const Scale& scale, const float* q, bool rest, int e0,
+                                             int V, const float* x, double* out) {
+  float qx[N];
+  if (rest && q) {
+    if (e0 + N <= V) {
+#pragma unroll
+      for (int h = 0; h < N; h += 4) {
+        const auto raw = *reinterpret_cast<const Unaligned16<uint32_t>*>(q + e0 + h);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) qx[h + e] = __uint_as_float(raw.v[e]);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; ++e) qx[e] = e0 + e < V ? q[e0 + e] : 0.0f;
+    }
+  }
+  bool in[N], any = true;
+  if (w.cut) {
+    any = false;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      in[e] = order_value(x[e], e0 + e) >= w.cut;
+      any |= in[e];
+    }
+  }
+  if (!__any(any)) {  // (what is cut weighs nothing, and most wavefronts of a short list have nothing else)
+#pragma unroll
+    for (int e = 0; e < N; ++e) out[e] = 0.0;
+    return;
+  }
+  sample_weights<N>(x, scale, out);
+  if (w.cut) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) out[e] = in[e] ? out[e] : 0.0;
+  }
+  if (rest) {
+    if (q) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const double d = fma(-(double)(qx[e] < 0.0f ? 0.0f : qx[e]), w.sum, out[e]);
+        out[e] = d > 0.0 ? d : 0.0;  // (nothing where q is NaN)
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        if (e0 + e == w.refused) out[e] = 0.0;
+    }
+  }
+}
+
+// The token at which the running sum passes u of the whole, -1 without mass: by
+// one wavefront.  mass(j): the sum of segment j's weights.
+template <int SRC, typename Mass>
+__device__ __forceinline__ long long pick_token(const typename Logit<SRC>::Raw* row, int V, int ns, const DrawRec& w,
+                                                const Scale& scale, const float* q, bool rest, double u, Mass mass) {
+  constexpr int kVec = Logit<SRC>::kVec, kGroups = kSamplePer / kVec;
+  const int lane = threadIdx.x & 63;
+  const auto segment_mass = [&](int j) -> double { return j < ns ? mass(j) : 0.0; };
+  // The segment: the first whose running sum passes u of the whole, or the last
+  // that weighs anything (rounding of the sums, a random number of 1).
+  double total = 0.0;
+  for (int j0 = 0; j0 < ns; j0 += kWave) total += wave_sum(segment_mass(j0 + lane));
+  double target = u * total, before = 0.0, left = 0.0;
+  int seg = -1;
+  bool passed = false;
+  for (int j0 = 0; j0 < ns && !passed; j0 += kWave) {
+    const double v = segment_mass(j0 + lane);
+    const double run = before + wave_prefix(v);
+    const unsigned long long some = __ballot(v > 0.0), hit = __ballot(v > 0.0 && run > target);
+    if (some) {
+      passed = hit != 0;
+      const int at = passed ? __ffsll(hit) - 1 : 63 - __clzll(some);
+      seg = j0 + at;
+      left = target - (lane_value(run, at) - lane_value(v, at));
+    }
+    before = lane_value(run, 63);
+  }
+  if (seg < 0) {
+    // Nothing is left of p - q: the row's p itself, whose segments have not
+    // been summed (its cut tokens out), so that this walks the row twice.
+    for (int turn = 0; turn < 2 && rest; ++turn) {
+      if (turn == 1) rest = false;
+      target = u * before;  // (turn 1: of the whole, summed in the same order)
+      before = 0.0;
+      for (int j = 0; j < ns; ++j) {
+        double s = 0.0;
+#pragma unroll 1
+        for (int i = 0; i < kGroups; ++i) {
+          const int e0 = segment_element<SRC>(j, i);
+          float x[kVec];
+          double p[kVec];
+          load_vec<SRC>(row, e0, V, x);
+          draw_weights<kVec>(w, scale, nullptr, false, e0, V, x, p);
+#pragma unroll
+          for (int e = 0; e < kVec; ++e) s += p[e];
+        }
+        s = wave_sum(s);
+        if (turn == 1 && s > 0.0) {
+          seg = j;
+          left = target - before;
+          if (before + s > target) break;
+        }
+        before += s;
+      }
+    }
+  }
+  if (seg < 0) return -1;
+  // The token: running sums over the segment in the order of its indices.
+  float x[kSamplePer];
+  load_segment<SRC>(row, seg, V, x);
+  int token = -1;
+  before = 0.0;
+#pragma unroll
+  for (int i = 0; i < kGroups; ++i) {
+    const int e0 = segment_element<SRC>(seg, i);
+    double p[kVec], s = 0.0;
+    draw_weights<kVec>(w, scale, q, rest, e0, V, x + i * kVec, p);
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) s += p[e];
+    const double run = before + wave_prefix(s);
+    const unsigned long long some = __ballot(s > 0.0), hit = __ballot(s > 0.0 && run > left);
+    if (some) {
+      const int at = hit ? __ffsll(hit) - 1 : 63 - __clzll(some);
+      double sum = run - s;
+      int last = 0, first = -1;
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) {
+        sum += p[e];
+        if (p[e] > 0.0) {
+          last = e;
+          if (first < 0 && sum > left) first = e;
+        }
+      }
+      token = lane_value(e0 + (hit && first >= 0 ? first : last), at);
+      if (hit) break;
+    }
+    before = lane_value(run, 63);
+  }
+  return token;
+}
+
 // Histograms of the workgroups' parts of a row, for top_k and top_p: bins are
 // steps of a tenth of a factor of 2 in the weight, counted from the bin of the
 // part's maximum on.  The steps are absolute (floor of l times 10 c, within 24
@@ -382,12 +526,17 @@ struct CutPlan {
   int by_p;
   int k_first, k_last, p_first, p_last;
   int list_first, list_last, also, also_first, also_last;  // bins to list
+  int all_listed;             // every token that can stay is in them
   int listed;                 // how many tokens they have
 };
 
-// Finds every row's cut from the histograms of its parts; with draws (sequences
-// of one row) its draw too.  lists: kListed order values a row.
+// Finds every row's cut from the histograms of its parts (cuts; with draws,
+// sequences of one row, its draw too), or with tokens draws from it: mass then
+// takes the sums of a row's segments, at most kDrawSegments.  lists: kListed
+// order values a row.
+constexpr int kDrawSegments = 1024;
 int launch_sample_cut(const SampleRows& r, int dtype, const SegRec* rec, const Histogram* hist, CutPlan* plans,
-                      unsigned long long* lists, RowCut* cuts, DrawRec* draws, hipStream_t st);
+                      unsigned long long* lists, RowCut* cuts, DrawRec* draws, double* mass, const float* uniforms,
+                      long long* tokens, hipStream_t st);
 
 }  // namespace vrm

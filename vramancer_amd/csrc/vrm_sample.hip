@@ -13,7 +13,8 @@
 //   4. sample_mass_kernel       that row's segments: the mass to draw from
 //   5. sample_pick_kernel       the segment and the token where the running sum
 //                               passes the random number
-// A draw without top_k and top_p is 1 and 5, one with them 1, 2, 4 and 5.
+// A draw without top_k and top_p is 1 and 5, one with them 1 and 2 (which picks
+// too), and 1, 2, 4 and 5 where its distribution is asked for.
 #include "vrm_sample.h"
 
 namespace vrm {
@@ -233,46 +234,6 @@ __device__ __forceinline__ DrawRec draw_of(const SampleRows& r, const DrawRec* d
   return w;
 }
 
-// What the tokens e0 .. e0 + N weigh in the draw: p, or where a draft was
-// refused max(p - q, 0), in units of 1 / sum.
-template <int N>
-__device__ __forceinline__ void draw_weights(const DrawRec& w, const Scale& scale, const float* q, bool rest, int e0,
-                                             int V, const float* x, double* out) {
-  float qx[N];
-  if (rest && q) {
-    if (e0 + N <= V) {
-#pragma unroll
-      for (int h = 0; h < N; h += 4) {
-        const auto raw = *reinterpret_cast<const Unaligned16<uint32_t>*>(q + e0 + h);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) qx[h + e] = __uint_as_float(raw.v[e]);
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < N; ++e) qx[e] = e0 + e < V ? q[e0 + e] : 0.0f;
-    }
-  }
-  sample_weights<N>(x, scale, out);
-  if (w.cut) {
-#pragma unroll
-    for (int e = 0; e < N; ++e)
-      if (order_value(x[e], e0 + e) < w.cut) out[e] = 0.0;
-  }
-  if (rest) {
-    if (q) {
-#pragma unroll
-      for (int e = 0; e < N; ++e) {
-        const double d = fma(-(double)(qx[e] < 0.0f ? 0.0f : qx[e]), w.sum, out[e]);
-        out[e] = d > 0.0 ? d : 0.0;  // (nothing where q is NaN)
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < N; ++e)
-        if (e0 + e == w.refused) out[e] = 0.0;
-    }
-  }
-}
-
 __device__ __forceinline__ const float* draft_row(const Drafts& d, const DrawRec& w, int b) {
   return d.probs ? d.probs + b * d.seq_stride + w.at * d.draft_stride : nullptr;
 }
@@ -336,7 +297,6 @@ template <int SRC>
 __global__ void __launch_bounds__(kWave)
     sample_pick_kernel(SampleRows r, Drafts d, int ns, const SegRec* rec, const DrawRec* draws, const double* mass,
                        const float* uniforms, long long* tokens) {
-  constexpr int kVec = Logit<SRC>::kVec, kGroups = kSamplePer / kVec;
   const int b = blockIdx.x, lane = threadIdx.x;
   Scale scale;
   const DrawRec w = draw_of(r, draws, rec, ns, b, scale);
@@ -346,97 +306,11 @@ __global__ void __launch_bounds__(kWave)
     if (lane == 0) *out = w.arg;
     return;
   }
-  const auto* row = row_at<SRC>(r, w.row);
-  const float* q = draft_row(d, w, b);
-  const double u = fmin(fmax((double)uniforms[b], 0.0), 1.0);
-  bool rest = w.refused >= 0;
-  const auto segment_mass = [&](int j) -> double {
-    if (j >= ns) return 0.0;
-    return mass ? mass[(long long)b * ns + j] : segment_sum(rec[(long long)b * ns + j], scale);
-  };
-  // The segment: the first whose running sum passes u of the whole, or the last
-  // that weighs anything (rounding of the sums, a random number of 1).
-  double total = 0.0;
-  for (int j0 = 0; j0 < ns; j0 += kWave) total += wave_sum(segment_mass(j0 + lane));
-  double target = u * total, before = 0.0, left = 0.0;
-  int seg = -1;
-  bool passed = false;
-  for (int j0 = 0; j0 < ns && !passed; j0 += kWave) {
-    const double v = segment_mass(j0 + lane);
-    const double run = before + wave_prefix(v);
-    const unsigned long long some = __ballot(v > 0.0), hit = __ballot(v > 0.0 && run > target);
-    if (some) {
-      passed = hit != 0;
-      const int at = passed ? __ffsll(hit) - 1 : 63 - __clzll(some);
-      seg = j0 + at;
-      left = target - (lane_value(run, at) - lane_value(v, at));
-    }
-    before = lane_value(run, 63);
-  }
-  if (seg < 0) {
-    // Nothing is left of p - q: the row's p itself, whose segments have not
-    // been summed (its cut tokens out), so that this walks the row twice.
-    for (int turn = 0; turn < 2 && rest; ++turn) {
-      if (turn == 1) rest = false;
-      target = u * before;  // (turn 1: of the whole, summed in the same order)
-      before = 0.0;
-      for (int j = 0; j < ns; ++j) {
-        double s = 0.0;
-#pragma unroll 1
-        for (int i = 0; i < kGroups; ++i) {
-          const int e0 = segment_element<SRC>(j, i);
-          float x[kVec];
-          double p[kVec];
-          load_vec<SRC>(row, e0, r.V, x);
-          draw_weights<kVec>(w, scale, nullptr, false, e0, r.V, x, p);
-#pragma unroll
-          for (int e = 0; e < kVec; ++e) s += p[e];
-        }
-        s = wave_sum(s);
-        if (turn == 1 && s > 0.0) {
-          seg = j;
-          left = target - before;
-          if (before + s > target) break;
-        }
-        before += s;
-      }
-    }
-  }
-  if (seg < 0) {
-    if (lane == 0) *out = -1;
-    return;
-  }
-  // The token: running sums over the segment in the order of its indices.
-  float x[kSamplePer];
-  load_segment<SRC>(row, seg, r.V, x);
-  int token = -1;
-  before = 0.0;
-#pragma unroll
-  for (int i = 0; i < kGroups; ++i) {
-    const int e0 = segment_element<SRC>(seg, i);
-    double p[kVec], s = 0.0;
-    draw_weights<kVec>(w, scale, q, rest, e0, r.V, x + i * kVec, p);
-#pragma unroll
-    for (int e = 0; e < kVec; ++e) s += p[e];
-    const double run = before + wave_prefix(s);
-    const unsigned long long some = __ballot(s > 0.0), hit = __ballot(s > 0.0 && run > left);
-    if (some) {
-      const int at = hit ? __ffsll(hit) - 1 : 63 - __clzll(some);
-      double sum = run - s;
-      int last = 0, first = -1;
-#pragma unroll
-      for (int e = 0; e < kVec; ++e) {
-        sum += p[e];
-        if (p[e] > 0.0) {
-          last = e;
-          if (first < 0 && sum > left) first = e;
-        }
-      }
-      token = lane_value(e0 + (hit && first >= 0 ? first : last), at);
-      if (hit) break;
-    }
-    before = lane_value(run, 63);
-  }
+  const long long token = pick_token<SRC>(row_at<SRC>(r, w.row), r.V, ns, w, scale, draft_row(d, w, b), w.refused >= 0,
+                                          fmin(fmax((double)uniforms[b], 0.0), 1.0), [&](int j) {
+                                            return mass ? mass[(long long)b * ns + j]
+                                                        : segment_sum(rec[(long long)b * ns + j], scale);
+                                          });
   if (lane == 0) *out = token;
 }
 
@@ -451,6 +325,7 @@ struct Plan {
   long long slots;
   int ns, blocks;  // segments and workgroups of a row
   bool filtered, drafts, masses;
+  bool fused;  // the cut draws by itself
   size_t hist, plans, lists, cuts, draws, mass, bytes;
 };
 
@@ -462,6 +337,7 @@ Plan plan_of(long long B, int K, int V, bool filtered, bool drafts, bool probs) 
   p.filtered = filtered;
   p.drafts = drafts;
   p.masses = filtered || drafts || probs;
+  p.fused = filtered && !drafts && !probs && p.ns <= kDrawSegments;
   size_t at = up((size_t)p.slots * p.ns * sizeof(SegRec));
   if (filtered) {
     p.hist = at;
@@ -502,8 +378,9 @@ int run(const SampleRows& r, const Drafts& d, const Plan& p, char* ws, const flo
     hipLaunchKernelGGL((sample_histogram_kernel<SRC>), row_blocks, threads, 0, st, r, p.ns, p.blocks, rec, hist);
     if (int rc = launch_sample_cut(r, SRC, rec, hist, reinterpret_cast<CutPlan*>(ws + p.plans),
                                    reinterpret_cast<unsigned long long*>(ws + p.lists), cuts,
-                                   p.drafts ? nullptr : draws, st))
+                                   p.drafts ? nullptr : draws, mass, uniforms, p.fused ? tokens : nullptr, st))
       return rc;
+    if (p.fused) return launch_status(who);
   } else {
     hipLaunchKernelGGL((sample_segment_kernel<SRC>), row_blocks, threads, 0, st, r, p.ns, p.blocks, rec);
   }

@@ -9,6 +9,9 @@
 //   sample_collect_kernel  lists those bins' tokens (a wavefront per segment)
 //   sample_border_kernel   narrows the list down by bins of order values until
 //                          64 tokens are left, which it compares with each other
+// A draw that needs nothing else comes out of the same launches: the second one
+// adds up what the segments hold above the border's bins, the third adds the
+// listed tokens that stay and picks.
 // Three launches where one workgroup per row could do all of it: what it takes
 // that workgroup to look through its row alone is 8 to 30 us, at 16 bytes a
 // cycle and with 2 wavefronts a SIMD; all wavefronts of the chip do it in 3.
@@ -33,6 +36,7 @@ constexpr int kSubBits = 10;
 constexpr int kSub = 1 << kSubBits;  // steps of order values: two a thread
 constexpr int kFew = 64;             // tokens that are compared with each other
 constexpr int kPartsAhead = 24;
+static_assert(kSub >= kDrawSegments, "a sum for each segment");
 
 using u64 = unsigned long long;
 
@@ -205,6 +209,7 @@ __global__ void __launch_bounds__(kCutThreads)
         plan.p_last = top_bin - at;
         plan.p_before = 0.0;
         plan.by_p = by_p;
+        plan.all_listed = 1;
         by_p = false;
       } else {
         plan.list_first = plan.list_last = top_bin - at;
@@ -244,18 +249,22 @@ __global__ void __launch_bounds__(kCutThreads)
 
 // A wavefront per segment: the tokens of the bins of the plan go to the row's
 // list, by their order values; plan.listed counts them, and only kListed fit.
-template <int SRC>
+// With MASS, mass takes the weights of the segment's tokens above the first of
+// those bins, which stay whatever the border.  (The segment is under way before
+// the plan that says whether it is needed.)
+template <int SRC, bool MASS>
 __global__ void __launch_bounds__(kSampleThreads)
-    sample_collect_kernel(SampleRows r, int ns, int blocks, CutPlan* plans, u64* lists) {
+    sample_collect_kernel(SampleRows r, int ns, int blocks, CutPlan* plans, u64* lists, double* mass) {
   const int slot = blockIdx.x / blocks, seg = (blockIdx.x % blocks) * 4 + (threadIdx.x >> 6);
   const int b = slot / (r.K + 1), i = slot % (r.K + 1);
   if (seg >= ns || i >= r.count(b)) return;
   CutPlan& plan = plans[slot];
-  if (!plan.filters) return;
   constexpr int kVec = Logit<SRC>::kVec;
   float x[kSamplePer];
   load_segment<SRC>(row_at<SRC>(r, r.first(b) + i), seg, r.V, x);
-  const float bins = bin_scale(make_scale(plan.top, r.temp(b)));
+  if (!plan.filters) return;
+  const Scale scale = make_scale(plan.top, r.temp(b));
+  const float bins = bin_scale(scale);
   const BinRange main(plan.list_last, plan.list_first), second(plan.also_last, plan.also_first);
   const bool two = plan.also != 0;
   uint32_t hits = 0;
@@ -266,24 +275,46 @@ __global__ void __launch_bounds__(kSampleThreads)
   }
   const int mine = __popc(hits);
   const int up_to = wave_prefix(mine), all = lane_value(up_to, 63);
-  if (all == 0) return;
-  int at = 0;
-  if ((threadIdx.x & 63) == 0) at = atomicAdd(&plan.listed, all);
-  at = lane_value(at, 0) + up_to - mine;
-  u64* list = lists + (long long)slot * kListed;
+  if (all != 0) {
+    int at = 0;
+    if ((threadIdx.x & 63) == 0) at = atomicAdd(&plan.listed, all);
+    at = lane_value(at, 0) + up_to - mine;
+    u64* list = lists + (long long)slot * kListed;
 #pragma unroll
-  for (int e = 0; e < kSamplePer; ++e) {
-    if (hits & (1u << e)) {
-      if (at < kListed) list[at] = order_value(x[e], segment_element<SRC>(seg, e / kVec) + e % kVec);
-      ++at;
+    for (int e = 0; e < kSamplePer; ++e) {
+      if (hits & (1u << e)) {
+        if (at < kListed) list[at] = order_value(x[e], segment_element<SRC>(seg, e / kVec) + e % kVec);
+        ++at;
+      }
     }
   }
+  if constexpr (!MASS) return;
+  if (plan.all_listed) return;
+  const float above = plan.by_p ? BinRange(0, plan.p_first).high : BinRange(0, plan.k_first).high;
+  double s = 0.0;
+#pragma unroll
+  for (int e = 0; e < kSamplePer; e += 8) {
+    bool in[8], any = false;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      in[j] = x[e + j] * bins >= above;
+      any |= in[j];
+    }
+    if (!__any(any)) continue;
+    double w[8];
+    sample_weights<8>(x + e, scale, w);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s += in[j] ? w[j] : 0.0;
+  }
+  s = wave_sum(s);
+  if ((threadIdx.x & 63) == 0) mass[(long long)slot * ns + seg] = s;
 }
 
-// One workgroup per row: the borders.
+// One workgroup per row: the borders, and where tokens are asked for the draw.
 template <int SRC>
 __global__ void __launch_bounds__(kCutThreads)
-    sample_border_kernel(SampleRows r, int bits, const CutPlan* plans, const u64* lists, RowCut* cuts, DrawRec* draws) {
+    sample_border_kernel(SampleRows r, int ns, int bits, const SegRec* rec, const CutPlan* plans, const u64* lists,
+                         RowCut* cuts, DrawRec* draws, double* mass, const float* uniforms, long long* tokens) {
   __shared__ u64 list[kListed];  // order values
   __shared__ u64 sub_sum[kSub];
   __shared__ uint32_t sub_count[kSub];
@@ -298,8 +329,11 @@ __global__ void __launch_bounds__(kCutThreads)
   const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
   if (i >= r.count(b)) return;
   const CutPlan plan = plans[slot];
+  const u64 ahead = lists[(long long)slot * kListed + t];  // (under way with the plan; what is not listed is not used)
   u64 cut = 0;
   double kept = plan.kept;
+  bool fits = true, of_p = false;  // whether the cut is top_p's
+  int listed = 0;
   if (plan.filters) {
     using L = Logit<SRC>;
     const auto* row = row_at<SRC>(r, r.first(b) + i);
@@ -308,9 +342,10 @@ __global__ void __launch_bounds__(kCutThreads)
     const float bins = bin_scale(scale);
     const double unit = (double)(1ULL << bits);
     const auto weight_of = [&](u64 o) { return fixed_weight(sample_weight(order_logit(o), scale), unit); };
-    const bool fits = plan.listed <= kListed;
-    int listed = fits ? plan.listed : 0;
-    for (int j = t; j < listed; j += kCutThreads) list[j] = lists[(long long)slot * kListed + j];
+    fits = plan.listed <= kListed;
+    listed = fits ? plan.listed : 0;
+    if (t < listed) list[t] = ahead;
+    for (int j = t + kCutThreads; j < listed; j += kCutThreads) list[j] = lists[(long long)slot * kListed + j];
     kept = plan.total;
 #pragma unroll 1
     for (int turn = 0; turn < 2; ++turn) {
@@ -490,48 +525,106 @@ __global__ void __launch_bounds__(kCutThreads)
       }
       __syncthreads();
       cut = s_border;
+      of_p = !by_count;
       kept = before + (double)s_before_fixed / unit;
       __syncthreads();
     }
     if (cut == 0) kept = plan.kept;
   }
-  if (t != 0) return;
-  cuts[slot] = RowCut{cut, kept};
-  if (draws) {
-    DrawRec w{};
-    w.sum = kept;
-    w.cut = cut;
-    w.top = plan.top;
-    w.row = r.first(b);
-    w.arg = plan.arg;
-    w.refused = -1;
-    draws[b] = w;
+  DrawRec w{};
+  w.sum = kept;
+  w.cut = cut;
+  w.top = plan.top;
+  w.row = r.first(b) + i;
+  w.arg = plan.arg;
+  w.refused = -1;
+  if (!tokens) {
+    if (t == 0) {
+      cuts[slot] = RowCut{cut, kept};
+      if (draws) draws[b] = w;
+    }
+    return;
   }
+  // The draw (rows and sequences are the same here, ns is at most kSub).
+  if (w.arg != -2) {
+    if (t == 0) tokens[b] = w.arg;
+    return;
+  }
+  const auto* row = row_at<SRC>(r, w.row);
+  const Scale scale = make_scale(w.top, r.temp(b));
+  double* masses = mass + (long long)slot * ns;
+  const double unit = (double)(1ULL << bits);
+  // What the second launch summed is right where the cut is in the bins that it
+  // listed; the segments are summed here otherwise.
+  const bool summed = plan.filters && cut != 0 && fits && (plan.all_listed || of_p == (plan.by_p != 0));
+  if (summed) {
+    for (int j = t; j < ns; j += kCutThreads) sub_sum[j] = 0;
+    __syncthreads();
+    const BinRange range(plan.by_p ? plan.p_last : plan.k_last, plan.by_p ? plan.p_first : plan.k_first);
+    const float bins = bin_scale(scale);
+    for (int j = t; j < listed; j += kCutThreads) {
+      const u64 o = list[j];
+      const float l = order_logit(o);
+      if (o >= cut && (plan.all_listed || range.holds(l * bins)))
+        atomicAdd(&sub_sum[(uint32_t)~o / kSegment], fixed_weight(sample_weight(l, scale), unit));
+    }
+  } else if (cut != 0) {
+    for (int seg = wave; seg < ns; seg += kCutWaves) {
+      float x[kSamplePer];
+      load_segment<SRC>(row, seg, r.V, x);
+      constexpr int kVec = Logit<SRC>::kVec;
+      double s = 0.0;
+#pragma unroll
+      for (int g = 0; g < kSamplePer / kVec; ++g) {
+        double p[kVec];
+        draw_weights<kVec>(w, scale, nullptr, false, segment_element<SRC>(seg, g), r.V, x + g * kVec, p);
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) s += p[e];
+      }
+      s = wave_sum(s);
+      if (lane == 0) masses[seg] = s;
+    }
+  }
+  __syncthreads();
+  if (wave != 0) return;
+  const SegRec* recs = rec + (long long)slot * ns;
+  const long long token =
+      pick_token<SRC>(row, r.V, ns, w, scale, nullptr, false, fmin(fmax((double)uniforms[b], 0.0), 1.0), [&](int j) {
+        if (cut == 0) return segment_sum(recs[j], scale);
+        if (!summed) return masses[j];
+        return (plan.all_listed ? 0.0 : masses[j]) + (double)sub_sum[j] / unit;
+      });
+  if (lane == 0) tokens[b] = token;
 }
 
 template <int SRC>
 void launch(const SampleRows& r, int bits, const SegRec* rec, const Histogram* hist, CutPlan* plans, u64* lists,
-            RowCut* cuts, DrawRec* draws, hipStream_t st) {
+            RowCut* cuts, DrawRec* draws, double* mass, const float* uniforms, long long* tokens, hipStream_t st) {
   const int blocks = (r.V + kSampleBlock - 1) / kSampleBlock;
   const long long slots = (long long)r.B * (r.K + 1);
   hipLaunchKernelGGL(sample_bins_kernel, dim3((unsigned)slots), dim3(kCutThreads), 0, st, r, r.segments(), blocks, rec,
                      hist, plans);
-  hipLaunchKernelGGL((sample_collect_kernel<SRC>), dim3((unsigned)(slots * blocks)), dim3(kSampleThreads), 0, st, r,
-                     r.segments(), blocks, plans, lists);
-  hipLaunchKernelGGL((sample_border_kernel<SRC>), dim3((unsigned)slots), dim3(kCutThreads), 0, st, r, bits, plans, lists,
-                     cuts, draws);
+  if (tokens)
+    hipLaunchKernelGGL((sample_collect_kernel<SRC, true>), dim3((unsigned)(slots * blocks)), dim3(kSampleThreads), 0, st,
+                       r, r.segments(), blocks, plans, lists, mass);
+  else
+    hipLaunchKernelGGL((sample_collect_kernel<SRC, false>), dim3((unsigned)(slots * blocks)), dim3(kSampleThreads), 0,
+                       st, r, r.segments(), blocks, plans, lists, nullptr);
+  hipLaunchKernelGGL((sample_border_kernel<SRC>), dim3((unsigned)slots), dim3(kCutThreads), 0, st, r, r.segments(), bits,
+                     rec, plans, lists, cuts, draws, mass, uniforms, tokens);
 }
 
 }  // namespace
 
 int launch_sample_cut(const SampleRows& r, int dtype, const SegRec* rec, const Histogram* hist, CutPlan* plans,
-                      u64* lists, RowCut* cuts, DrawRec* draws, hipStream_t st) {
+                      u64* lists, RowCut* cuts, DrawRec* draws, double* mass, const float* uniforms, long long* tokens,
+                      hipStream_t st) {
   int bits = 45;
   while ((1LL << (62 - bits)) < (long long)r.V) --bits;
   switch (dtype) {
-    case VRM_SRC_F32: launch<VRM_SRC_F32>(r, bits, rec, hist, plans, lists, cuts, draws, st); break;
-    case VRM_SRC_F16: launch<VRM_SRC_F16>(r, bits, rec, hist, plans, lists, cuts, draws, st); break;
-    default: launch<VRM_SRC_BF16>(r, bits, rec, hist, plans, lists, cuts, draws, st); break;
+    case VRM_SRC_F32: launch<VRM_SRC_F32>(r, bits, rec, hist, plans, lists, cuts, draws, mass, uniforms, tokens, st); break;
+    case VRM_SRC_F16: launch<VRM_SRC_F16>(r, bits, rec, hist, plans, lists, cuts, draws, mass, uniforms, tokens, st); break;
+    default: launch<VRM_SRC_BF16>(r, bits, rec, hist, plans, lists, cuts, draws, mass, uniforms, tokens, st); break;
   }
   return launch_status("sample_cut");
 }
