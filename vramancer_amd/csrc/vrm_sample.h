@@ -165,6 +165,11 @@ __device__ __forceinline__ unsigned long long order_value(float l, int i) {
   return ((unsigned long long)logit_key(l) << 32) | (uint32_t)~i;
 }
 
+__device__ __forceinline__ float order_logit(unsigned long long order) {
+  const uint32_t key = (uint32_t)(order >> 32);
+  return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
+}
+
 template <int SRC>
 struct Logit;  // element type of a row
 template <>
@@ -353,9 +358,11 @@ __device__ __forceinline__ void draw_weights(const DrawRec& w, const Scale& scal
   bool in[N], any = true;
   if (w.cut) {
     any = false;
+    const float border = order_logit(w.cut);
+    const int last = (int)(uint32_t)~w.cut - e0;
 #pragma unroll
     for (int e = 0; e < N; ++e) {
-      in[e] = order_value(x[e], e0 + e) >= w.cut;
+      in[e] = x[e] > border || (x[e] == border && e <= last);
       any |= in[e];
     }
   }
@@ -480,7 +487,7 @@ __device__ __forceinline__ long long pick_token(const typename Logit<SRC>::Raw* 
 // part's maximum on.  The steps are absolute (floor of l times 10 c, within 24
 // bits), so that the parts of a row differ by a shift only; the bin of a logit
 // is monotone in it, and what is past the last bin weighs less than 2^-51 of
-// the part's maximum.  Where the maximum is +inf, that is the top bin and the
+// the part's maximum, which is 0 as an integer.  Where the maximum is +inf, that is the top bin and the
 // finite logits are past the last one.  Sums are integers, weights times 2^49
 // rounded: they do not depend on the order of the atomics.
 constexpr int kBins = 512;
@@ -493,13 +500,17 @@ struct Histogram {
 };
 
 __device__ __forceinline__ float bin_scale(const Scale& s) { return s.infinite ? 1e-30f : (float)fmin(10.0 * s.c, 3e38); }
-__device__ __forceinline__ int bin_of(float l, float c) {
-  return (int)floorf(fminf(fmaxf(l * c, -kBinMost), kBinMost));
+__device__ __forceinline__ int bin_of(float l, float c, float most = kBinMost) {
+  int bin;  // floor and conversion in one instruction
+  asm("v_cvt_flr_i32_f32 %0, %1" : "=v"(bin) : "v"(__builtin_amdgcn_fmed3f(l * c, -most, most)));
+  return bin;
 }
 
-// Weight as an integer, in units of 2^-bits.
+// Weight as an integer, in units of 2^-bits (the rounding of a sum at 2^52).
 __device__ __forceinline__ unsigned long long fixed_weight(double w, double unit) {
-  return (unsigned long long)__double_as_longlong(fma(w, unit, 4503599627370496.0)) & 0xfffffffffffffULL;  // 2^52
+  double sum;
+  asm("v_fma_f64 %0, %1, %2, %3" : "=v"(sum) : "v"(w), "v"(unit), "s"(4503599627370496.0));
+  return (unsigned long long)__double_as_longlong(sum) & 0xfffffffffffffULL;
 }
 
 // Whether a row's parameters may drop tokens.

@@ -40,11 +40,6 @@ static_assert(kSub >= kDrawSegments, "a sum for each segment");
 
 using u64 = unsigned long long;
 
-__device__ __forceinline__ float order_logit(u64 order) {
-  const uint32_t key = (uint32_t)(order >> 32);
-  return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
-}
-
 // Whether a logit's bin, floor of the clamped product with `bins`, is within
 // last .. first, as two comparisons.
 struct BinRange {
