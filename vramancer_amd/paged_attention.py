@@ -29,6 +29,10 @@ Device side, in this library's kernels:
   chunks of prompts, drafted tokens); ``write_chunk`` norms, rotates and writes
   them (``paged_chunk.rope_append``) and ``compute_attention_chunk`` attends
   them (``paged_chunk.paged_attention_chunk``), one launch per layer each;
+  ``keep_chunk`` takes refused drafts back;
+* ``reserve`` gives requests pages for tokens to come and puts their block table
+  and lengths on the device, where ``paged_chunk.chunk_tables`` makes a step's
+  tables from them; ``commit`` counts the tokens that such steps have stored;
 * ``from_hf_cache`` stores a prefilled Hugging Face cache in a request's
   pages with one ``vrm_kv_write`` launch per layer, ``to_hf_cache`` gathers
   it back; ``try_prefix_cache`` shares full pages of a token prefix between
@@ -151,6 +155,7 @@ class PageTableEntry:
     pages: List[int] = field(default_factory=list)
     num_tokens: int = 0
     created_at: float = field(default_factory=time.time)
+    reserved: bool = False  # may hold pages that no token is in yet (``reserve``)
 
 
 @dataclass
@@ -471,6 +476,131 @@ class PagedKVCacheManager:
             self._table_cache = None  # (its patches take page lists to grow only)
             self._epoch += 1
 
+    def keep_chunk(self, chunk: ChunkBatch, counts: Sequence[int]) -> None:
+        """Keeps the first ``counts[i]`` new tokens of each request of a batch
+        (``append_chunk``) and takes the others back, with the pages that were
+        added for them alone and their rows in the compression queue: drafted
+        tokens that were refused.  What those wrote lies behind the requests'
+        last tokens; an fp8 page's scale keeps what they raised it to.  The
+        batch is spent unless all of it is kept.  Raises, and changes nothing,
+        where a request has changed since append_chunk."""
+        counts = [int(n) for n in counts]
+        if len(counts) != len(chunk.counts) or any(not 0 <= n <= had for n, had in zip(counts, chunk.counts)):
+            raise RuntimeError(f"keep_chunk takes a number of tokens for each request, at most {chunk.counts}, "
+                               f"got {counts}")
+        if chunk.owner is not self:
+            raise RuntimeError("keep_chunk takes a batch that this manager's append_chunk made")
+        if counts == chunk.counts:
+            self._check_chunk(chunk, "keep_chunk")
+            return
+        PS = self.config.page_size
+        with self._lock:
+            self._check_states_locked(chunk, "keep_chunk")
+            for (entry, n, added), had, kept in reversed(list(zip(chunk.states, chunk.counts, counts))):
+                entry.num_tokens = n - had + kept
+                for _ in range(added):
+                    if (len(entry.pages) - 1) * PS < entry.num_tokens:
+                        break
+                    self._release_locked(entry.pages.pop())
+            rows = [at + i for at, kept in zip(itertools.accumulate([0] + chunk.counts), counts) for i in range(kept)]
+            places = [chunk.places[i] for i in rows]
+            pending = []
+            for item in self._pending_compress:
+                if item[5] is chunk.places:
+                    if not rows:
+                        continue
+                    layer, pages, slots, key, value, _ = item
+                    item = (layer, pages[rows], slots[rows], key[rows], value[rows], places)
+                pending.append(item)
+            self._pending_compress = pending
+            self._table_cache = None  # (its patches take page lists to grow only)
+            self._epoch += 1
+
+    def reserve(self, request_ids: Sequence[str], counts: Sequence[int]) -> Tuple[Any, Any]:
+        """Pages for ``counts[i]`` tokens of ``request_ids[i]`` to come, and
+        (block_table [B, pages], past_lens [B]) int32 on the device, in the
+        order of the ids: what ``paged_chunk.chunk_tables`` makes the tables of
+        steps from whose lengths are known on the device alone.  ``past_lens``
+        is the caller's to advance.  The requests' token counts stay as they
+        are until ``commit``; pages that end up without a token are the
+        request's next ones.
+
+        All or nothing: an unknown id raises ``KeyError``; an id given twice, a
+        negative count, too few free pages, or requests (forks) that share a
+        page their next tokens go to raise ``RuntimeError``, and nothing has
+        changed."""
+        import torch
+
+        self._require_pool("reserve")
+        ids, counts = list(request_ids), [int(n) for n in counts]
+        if len(counts) != len(ids):
+            raise RuntimeError(f"{len(ids)} request ids but {len(counts)} counts")
+        if len(set(ids)) < len(ids):
+            raise RuntimeError("a request can be reserved for once only")
+        if any(n < 0 for n in counts):
+            raise RuntimeError(f"counts must not be negative, got {counts}")
+        PS = self.config.page_size
+        with self._lock:
+            entries = [self._page_tables.get(rid) for rid in ids]
+            missing = [rid for rid, e in zip(ids, entries) if e is None]
+            if missing:
+                raise KeyError(f"unknown request ids {missing}")
+            more = [max(0, -(-(e.num_tokens + n) // PS) - len(e.pages)) if n else 0 for e, n in zip(entries, counts)]
+            if sum(more) > len(self._free_pages):
+                raise RuntimeError(f"no page left: {sum(more)} needed, {len(self._free_pages)} free "
+                                   f"(pool of {self.config.max_pages} pages)")
+            tails = [p for e, n in zip(entries, counts) if n
+                     for p in e.pages[e.num_tokens // PS:-(-(e.num_tokens + n) // PS)]]
+            if len(set(tails)) < len(tails):
+                raise RuntimeError("requests that share the page their next token goes to (forks) cannot be reserved "
+                                   "for together")
+            for e, m in zip(entries, more):
+                if m:
+                    e.pages.extend(self._alloc_page() for _ in range(m))
+                    e.reserved = True
+            if any(more):
+                self._peak_usage = max(self._peak_usage, self.config.max_pages - len(self._free_pages))
+                self._epoch += 1
+            width = max([1] + [len(e.pages) for e in entries])
+            B = len(ids)
+            host = np.full(B * (width + 1), -1, dtype=np.int32)  # table and lengths: one upload
+            for b, e in enumerate(entries):
+                host[b * width:b * width + len(e.pages)] = e.pages
+                host[B * width + b] = e.num_tokens
+        dev = torch.from_numpy(host).to(self._gpu_pool.device)
+        return dev[:B * width].view(B, width), dev[B * width:]
+
+    def commit(self, request_ids: Sequence[str], counts: Sequence[int]) -> None:
+        """Counts ``counts[i]`` tokens that steps over reserved pages have
+        stored for ``request_ids[i]``.  All or nothing: an unknown id raises
+        ``KeyError``, a negative count or more tokens than the request has
+        pages for ``RuntimeError``."""
+        ids, counts = list(request_ids), [int(n) for n in counts]
+        if len(counts) != len(ids):
+            raise RuntimeError(f"{len(ids)} request ids but {len(counts)} counts")
+        if len(set(ids)) < len(ids):
+            raise RuntimeError("a request can be committed once only")
+        if self._kv_compressor is not None and any(counts):
+            raise RuntimeError("tokens stored on the device alone do not enter the compression queue: commit is for "
+                               "managers without kv_compression")
+        PS = self.config.page_size
+        with self._lock:
+            entries = [self._page_tables.get(rid) for rid in ids]
+            missing = [rid for rid, e in zip(ids, entries) if e is None]
+            if missing:
+                raise KeyError(f"unknown request ids {missing}")
+            for rid, e, n in zip(ids, entries, counts):
+                if n < 0 or e.num_tokens + n > len(e.pages) * PS:
+                    raise RuntimeError(f"request {rid!r} has pages for {len(e.pages) * PS - e.num_tokens} more tokens, "
+                                       f"not {n}")
+            now = time.time()
+            for e, n in zip(entries, counts):
+                for page in e.pages[e.num_tokens // PS:-(-(e.num_tokens + n) // PS)] if n else []:
+                    self._pages[page].last_access = now
+                e.num_tokens += n
+                e.reserved = len(e.pages) * PS - e.num_tokens >= PS
+            self._epoch += 1
+
     @property
     def gpu_pool(self) -> Any:
         """The device K/V pool, or ``None`` for a host-only manager."""
@@ -520,6 +650,8 @@ class PagedKVCacheManager:
             if src is None:
                 return None
             entry = PageTableEntry(request_id=dst_request_id, pages=list(src.pages), num_tokens=src.num_tokens)
+            if src.reserved:  # (the pages of tokens to come are the source's own)
+                del entry.pages[-(-src.num_tokens // self.config.page_size):]
             for page_id in entry.pages:
                 self._pages[page_id].ref_count += 1
             self._page_tables[dst_request_id] = entry
@@ -540,6 +672,8 @@ class PagedKVCacheManager:
         PS = self.config.page_size
         with self._lock:
             entry = self._page_tables.get(request_id)
+            if entry is not None and entry.reserved:
+                raise RuntimeError(f"request {request_id!r} has reserved pages: a prefix comes before them")
             if entry is None:
                 entry = self._page_tables[request_id] = PageTableEntry(request_id=request_id)
             hits = 0

@@ -37,6 +37,11 @@ and the attention function attends them there
 runs one such step, ``prefill_chunked`` a prompt in chunks, which needs neither
 a second copy of the cache nor scores of the whole prompt.
 
+``sample_step`` is a decode step up to its tokens, drawn on the GPU
+(``sampling.sample_tokens``); ``speculative_step`` runs drafted tokens through
+the model, verifies them (``sampling.verify_drafts``) and takes those that are
+refused out of the pages again.
+
 Calls of the attention function on any other cache attend with PyTorch's SDPA,
 causal and unmasked (prefill one request at a time, as the reference does).
 """
@@ -52,7 +57,7 @@ from transformers.cache_utils import Cache, CacheLayerMixin
 from .paged_attention import ChunkBatch, PagedKVCacheManager
 
 __all__ = ["PagedBatchCache", "PagedBatchLayer", "PagedChunkCache", "PagedChunkLayer", "decode_step", "chunk_step",
-           "prefill", "prefill_chunked", "paged_attention_forward", "enable_paged_attention", "ATTENTION_NAME"]
+           "sample_step", "speculative_step", "prefill", "prefill_chunked", "paged_attention_forward", "enable_paged_attention", "ATTENTION_NAME"]
 
 ATTENTION_NAME = "vramancer_paged"
 
@@ -279,6 +284,52 @@ def chunk_step(model, manager: PagedKVCacheManager, request_ids: Sequence[str], 
         cache._undo_step()
         raise
     return out.logits if hasattr(out, "logits") else out[0]
+
+
+def sample_step(model, manager: PagedKVCacheManager, request_ids: Sequence[str], input_ids: torch.Tensor,
+                uniforms: torch.Tensor, temperature: Any = None, top_k: Any = None, top_p: Any = None,
+                probs: Any = None, cache: Optional[PagedBatchCache] = None) -> torch.Tensor:
+    """``decode_step`` and a token for each request, int64 [B], drawn from its
+    logits with ``uniforms`` [B] (``sampling.sample_tokens``)."""
+    from .sampling import sample_tokens
+
+    logits = decode_step(model, manager, request_ids, input_ids, cache)
+    return sample_tokens(logits, uniforms, temperature=temperature, top_k=top_k, top_p=top_p, probs=probs)
+
+
+def speculative_step(model, manager: PagedKVCacheManager, request_ids: Sequence[str], input_ids: torch.Tensor,
+                     drafts: torch.Tensor, accept_uniforms: torch.Tensor, draw_uniforms: torch.Tensor,
+                     draft_probs: Any = None, temperature: Any = None, top_k: Any = None, top_p: Any = None,
+                     cache: Optional[PagedChunkCache] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """One forward over each request's pending token ``input_ids`` [B] and its
+    ``drafts`` [B, K], the drafts verified against the model's distributions:
+    (tokens [B, K + 1], accepted [B]) of ``sampling.verify_drafts``.
+
+    Afterwards a request has its pending token and the accepted drafts in its
+    pages; the token after them, ``tokens[b, accepted[b]]``, is its next
+    pending one.  Reads ``accepted`` back, since the pages are the host's.  A
+    step that raises leaves the requests as they were."""
+    from .sampling import verify_drafts
+
+    B = len(request_ids)
+    if drafts.dim() != 2 or drafts.shape[0] != B:
+        raise RuntimeError(f"drafts must be [{B}, K], got shape {tuple(drafts.shape)}")
+    if not isinstance(cache, PagedChunkCache) or cache.manager is not manager or cache.request_ids != list(request_ids):
+        cache = PagedChunkCache(manager, request_ids)
+    # (a draft outside the vocabulary ends the list: the model gets some token there)
+    vocab = model.get_input_embeddings().weight.shape[0]
+    known = drafts.clamp(0, vocab - 1).to(input_ids.dtype)
+    logits = chunk_step(model, manager, request_ids, torch.cat([input_ids.reshape(B, 1), known], 1), cache)
+    try:
+        tokens, accepted = verify_drafts(logits, drafts, accept_uniforms, draw_uniforms, draft_probs=draft_probs,
+                                         temperature=temperature, top_k=top_k, top_p=top_p)
+        kept = [1 + n for n in accepted.tolist()]
+    except BaseException:
+        cache._undo_step()
+        raise
+    chunk, cache._chunk = cache._chunk, None
+    manager.keep_chunk(chunk, kept)
+    return tokens, accepted
 
 
 def prefill_chunked(model, manager: PagedKVCacheManager, request_id: str, input_ids: torch.Tensor,
