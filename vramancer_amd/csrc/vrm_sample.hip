@@ -9,7 +9,8 @@
 //                               may drop tokens
 //   2. launch_sample_cut        which tokens stay (vrm_sample_cut.hip)
 //   3. sample_choose_kernel     a sequence's drafts: accepted ones, the row its
-//                               next token is drawn from
+//                               next token is drawn from (for small batches in
+//                               the launch that follows)
 //   4. sample_mass_kernel       that row's segments: the mass to draw from
 //   5. sample_pick_kernel       the segment and the token where the running sum
 //                               passes the random number
@@ -152,12 +153,16 @@ struct Drafts {
   }
 };
 
+// The drafts that sequence b accepts and its draw, for every thread of the
+// workgroup.  Answers (tokens, accepted, draws) are written by the workgroup
+// that has `writes`.
 template <int SRC>
-__global__ void __launch_bounds__(kSampleThreads)
-    sample_choose_kernel(SampleRows r, Drafts d, int ns, const SegRec* rec, const RowCut* cuts, DrawRec* draws,
-                         long long* tokens, int32_t* accepted) {
+__device__ __forceinline__ DrawRec choose(const SampleRows& r, const Drafts& d, int ns, const SegRec* rec,
+                                          const RowCut* cuts, int b, bool writes, DrawRec* draws, long long* tokens,
+                                          int32_t* accepted, Scale& scale) {
   __shared__ int stop;  // the first row whose draft is refused, or the last row
-  const int b = blockIdx.x, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  __shared__ DrawRec draw;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int n = r.count(b), first = r.first(b);
   if (threadIdx.x == 0) stop = n - 1;
   __syncthreads();
@@ -171,14 +176,14 @@ __global__ void __launch_bounds__(kSampleThreads)
     const float qx = known && d.probs ? d.probs[b * d.seq_stride + i * d.draft_stride + x] : 1.0f;
     float top;
     int arg;
-    Scale scale;
+    Scale at_row;
     double sum;
-    combine_segments(rec + slot * ns, ns, t, top, arg, scale, sum);
+    combine_segments(rec + slot * ns, ns, t, top, arg, at_row, sum);
     bool ok = false;
     if (known && arg != -1) {
       double w = x == arg ? 1.0 : 0.0;
       if (arg == -2) {
-        w = sample_weight(l, scale);
+        w = sample_weight(l, at_row);
         if (cuts) {
           const RowCut cut = cuts[slot];
           sum = cut.sum;
@@ -191,29 +196,47 @@ __global__ void __launch_bounds__(kSampleThreads)
   }
   __syncthreads();
   const int a = max(stop, 0);
-  for (int i = threadIdx.x; i <= r.K; i += kSampleThreads)
-    tokens[(long long)b * (r.K + 1) + i] = i < a && n > 0 ? d.id((long long)b * r.K + i) : -1;
-  if (threadIdx.x == 0) accepted[b] = n > 0 ? a : 0;
-  if (wave != 0) return;
-  DrawRec w{};
-  w.row = -1;
-  if (n > 0) {
-    const long long slot = (long long)b * (r.K + 1) + a;
-    Scale scale;
-    combine_segments(rec + slot * ns, ns, t, w.top, w.arg, scale, w.sum);
-    w.row = first + a;
-    w.at = a;
-    w.refused = -1;
-    if (a < n - 1) {
-      const long long x = d.id((long long)b * r.K + a);
-      if (x >= 0 && x < r.V) w.refused = (int)x;
+  if (writes) {
+    for (int i = threadIdx.x; i <= r.K; i += kSampleThreads)
+      tokens[(long long)b * (r.K + 1) + i] = i < a && n > 0 ? d.id((long long)b * r.K + i) : -1;
+    if (threadIdx.x == 0) accepted[b] = n > 0 ? a : 0;
+  }
+  if (wave == 0) {
+    DrawRec w{};
+    w.row = -1;
+    if (n > 0) {
+      const long long slot = (long long)b * (r.K + 1) + a;
+      Scale at_row;
+      combine_segments(rec + slot * ns, ns, t, w.top, w.arg, at_row, w.sum);
+      w.row = first + a;
+      w.at = a;
+      w.refused = -1;
+      if (a < n - 1) {
+        const long long x = d.id((long long)b * r.K + a);
+        if (x >= 0 && x < r.V) w.refused = (int)x;
+      }
+      if (cuts && w.arg == -2) {
+        w.cut = cuts[slot].cut;
+        w.sum = cuts[slot].sum;
+      }
     }
-    if (cuts && w.arg == -2) {
-      w.cut = cuts[slot].cut;
-      w.sum = cuts[slot].sum;
+    if (lane == 0) {
+      draw = w;
+      if (writes) draws[b] = w;
     }
   }
-  if (lane == 0) draws[b] = w;
+  __syncthreads();
+  const DrawRec w = draw;
+  if (w.row >= 0 && w.arg == -2) scale = make_scale(w.top, t);
+  return w;
+}
+
+template <int SRC>
+__global__ void __launch_bounds__(kSampleThreads)
+    sample_choose_kernel(SampleRows r, Drafts d, int ns, const SegRec* rec, const RowCut* cuts, DrawRec* draws,
+                         long long* tokens, int32_t* accepted) {
+  Scale scale;
+  choose<SRC>(r, d, ns, rec, cuts, blockIdx.x, true, draws, tokens, accepted, scale);
 }
 
 // ---------------------------------------------------------------------------
@@ -241,15 +264,19 @@ __device__ __forceinline__ const float* draft_row(const Drafts& d, const DrawRec
   return d.probs ? d.probs + b * d.seq_stride + w.at * d.draft_stride : nullptr;
 }
 
-template <int SRC>
+// With CHOOSE each workgroup finds its sequence's draw by itself first (the first
+// one of a sequence writes tokens and accepted): a few KB of segment records
+// each, and no launch between.
+template <int SRC, bool CHOOSE>
 __global__ void __launch_bounds__(kSampleThreads)
-    sample_mass_kernel(SampleRows r, Drafts d, int ns, int blocks, const SegRec* rec, const DrawRec* draws, double* mass,
-                       float* probs) {
-  const int b = blockIdx.x / blocks, seg = (blockIdx.x % blocks) * 4 + (threadIdx.x >> 6);
-  if (seg >= ns) return;
+    sample_mass_kernel(SampleRows r, Drafts d, int ns, int blocks, const SegRec* rec, const RowCut* cuts, DrawRec* draws,
+                       double* mass, float* probs, long long* tokens, int32_t* accepted) {
+  const int b = blockIdx.x / blocks, part = blockIdx.x % blocks, seg = part * 4 + (threadIdx.x >> 6);
   constexpr int kVec = Logit<SRC>::kVec, kGroups = kSamplePer / kVec;
   Scale scale;
-  const DrawRec w = draw_of(r, draws, rec, ns, b, scale);
+  const DrawRec w = CHOOSE ? choose<SRC>(r, d, ns, rec, cuts, b, part == 0, draws, tokens, accepted, scale)
+                           : draw_of(r, draws, rec, ns, b, scale);
+  if (seg >= ns) return;
   if (w.row < 0 || (w.arg != -2 && !probs)) return;
   const bool known = w.arg != -2;  // greedy, or no token
   const bool rest = w.refused >= 0;
@@ -364,6 +391,13 @@ Plan plan_of(long long B, int K, int V, bool filtered, bool drafts, bool probs) 
   return p;
 }
 
+// Up to this many workgroups, which the chip has at once, every one of a
+// sequence's masses tests its drafts (for a few drafts): 9.7 us against 5.2 + 7.0
+// in two launches for 8 sequences of 3 drafts and 32000 logits (32 workgroups),
+// 15.6 against 7.0 + 10.7 for 37 of 7 and 100003 (481); 23.5 against 6.0 + 15.8
+// for 64 of 4 and 152000 (1216).
+constexpr int kChooseBlocks = 768, kChooseDrafts = 12;
+
 // A launch counts its threads in 32 bits.
 constexpr long long kMostBlocks = (1LL << 32) / 1024 - 1;
 
@@ -387,12 +421,18 @@ int run(const SampleRows& r, const Drafts& d, const Plan& p, char* ws, const flo
   } else {
     hipLaunchKernelGGL((sample_segment_kernel<SRC>), row_blocks, threads, 0, st, r, p.ns, p.blocks, rec);
   }
-  if (p.drafts)
-    hipLaunchKernelGGL((sample_choose_kernel<SRC>), dim3(r.B), threads, 0, st, r, d, p.ns, rec, cuts, draws, tokens,
-                       accepted);
-  if (p.masses)
-    hipLaunchKernelGGL((sample_mass_kernel<SRC>), dim3((unsigned)((long long)r.B * p.blocks)), threads, 0, st, r, d,
-                       p.ns, p.blocks, rec, draws, mass, probs);
+  const dim3 mass_blocks((unsigned)((long long)r.B * p.blocks));
+  if (p.drafts && r.K <= kChooseDrafts && mass_blocks.x <= (unsigned)kChooseBlocks) {
+    hipLaunchKernelGGL((sample_mass_kernel<SRC, true>), mass_blocks, threads, 0, st, r, d, p.ns, p.blocks, rec, cuts,
+                       draws, mass, nullptr, tokens, accepted);
+  } else {
+    if (p.drafts)
+      hipLaunchKernelGGL((sample_choose_kernel<SRC>), dim3(r.B), threads, 0, st, r, d, p.ns, rec, cuts, draws, tokens,
+                         accepted);
+    if (p.masses)
+      hipLaunchKernelGGL((sample_mass_kernel<SRC, false>), mass_blocks, threads, 0, st, r, d, p.ns, p.blocks, rec, cuts,
+                         draws, mass, probs, nullptr, nullptr);
+  }
   hipLaunchKernelGGL((sample_pick_kernel<SRC>), dim3(r.B), dim3(kWave), 0, st, r, d, p.ns, rec, draws, mass, uniforms,
                      tokens);
   return launch_status(who);
