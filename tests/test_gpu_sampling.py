@@ -305,6 +305,50 @@ def test_verified_tokens_are_the_targets():
     assert abs(accepted.double().mean().item() - agree) <= 6 * math.sqrt(agree * (1 - agree) / n)
 
 
+@pytest.mark.parametrize("B,K,V", [(3, 14, 700), (900, 2, 40), (300, 1, 20000)])
+@pytest.mark.parametrize("kw", [dict(), dict(top_k=20, top_p=0.9)])
+def test_verify_many(B, K, V, kw):
+    # many drafts, many sequences: the drafts are tested in a launch of their own
+    x, d, ua, u, q = drafts_of(B, K, V, torch.bfloat16, B)
+    ws = sampling.verify_workspace(B, K, V, device=DEV)
+    ws.fill_(255)
+    some = slice(0, B, max(1, B // 40))  # (the reference is slow)
+    tokens, accepted = sampling.verify_drafts(x, d, ua, u, q, workspace=ws, **kw)
+    want = verify(x[some], d[some], ua[some], u[some], q[some], **kw)
+    assert tokens[some].cpu().tolist() == want[0].tolist() and accepted[some].cpu().tolist() == want[1].tolist()
+    again = sampling.verify_drafts(x, d, ua, u, q, **kw)
+    assert torch.equal(again[0], tokens) and torch.equal(again[1], accepted)
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(top_k=70), dict(top_p=0.9)])
+def test_a_very_long_row(kw):
+    # more segments than the draw of a cut takes
+    V = 2_200_003
+    x, u = make(2, V, torch.float16, 3)
+    check(x, u, **kw)
+
+
+def test_rows_of_a_mixed_batch():
+    # greedy, cut and whole rows, masked and empty ones, of one call
+    N, V = 24, 9000
+    x, u = make(N, V, torch.bfloat16, 31)
+    x[5] = -math.inf
+    x[6, 100:] = -math.inf
+    x[7] = 2.0
+    k = torch.zeros(N, dtype=torch.int32)
+    k[::3] = torch.tensor([1, 5, 50, 4000, 5000, 8999, 9000, 20000], dtype=torch.int32)
+    p = torch.ones(N)
+    p[::2] = torch.linspace(0.0, 0.999, 12)
+    t = torch.ones(N)
+    t[::7] = 0.0
+    check(x, u, temperature=t.to(DEV), top_k=k.to(DEV), top_p=p.to(DEV))
+    ws = sampling.sample_workspace(N, V, device=DEV)
+    ws.fill_(255)
+    want = sampling.sample_tokens(x, u, temperature=t.to(DEV), top_k=k.to(DEV), top_p=p.to(DEV))
+    got = sampling.sample_tokens(x, u, temperature=t.to(DEV), top_k=k.to(DEV), top_p=p.to(DEV), workspace=ws)
+    assert torch.equal(got, want)
+
+
 def test_repeats_and_streams():
     x, u = make(40, 30011, torch.bfloat16, 12)
     first = sampling.sample_tokens(x, u, top_p=0.9)

@@ -43,8 +43,6 @@ FILE_FLAGS = {
     # 168 VGPRs with no scratch, and the other stream kernels of the file run
     # as fast or faster (c5 -5 us, head_dim 64 -2 us, bf16 unchanged).
     "vrm_decode_mfma.hip": ["-mllvm", "-disable-machine-licm"],
-    # The same: 30 spilled registers instead of 86 in the one kernel of the file.
-    "vrm_sample_cut.hip": ["-mllvm", "-disable-machine-licm"],
 }
 
 

@@ -321,27 +321,42 @@ __global__ void __launch_bounds__(kSampleThreads)
   if ((threadIdx.x & 63) == 0) mass[(long long)b * ns + seg] = s;
 }
 
-// One wavefront per sequence.  mass == NULL: a draw from row b by its segments'
+// One workgroup per sequence.  mass == NULL: a draw from row b by its segments'
 // sums.
 template <int SRC>
-__global__ void __launch_bounds__(kWave)
+__global__ void __launch_bounds__(kSampleThreads)
     sample_pick_kernel(SampleRows r, Drafts d, int ns, const SegRec* rec, const DrawRec* draws, const double* mass,
                        const float* uniforms, long long* tokens) {
-  const int b = blockIdx.x, lane = threadIdx.x;
+  __shared__ PickShared<SRC> shared;
+  __shared__ DrawRec draw;
+  const int b = blockIdx.x;
+  const float u = uniforms[b];
   Scale scale;
-  const DrawRec w = draw_of(r, draws, rec, ns, b, scale);
+  DrawRec w;
+  if (draws) {
+    w = draw_of(r, draws, rec, ns, b, scale);
+  } else {
+    if (threadIdx.x < kWave) {
+      w = draw_of(r, draws, rec, ns, b, scale);
+      if (threadIdx.x == 0) draw = w;
+    }
+    __syncthreads();
+    w = draw;
+    if (w.arg == -2) scale = make_scale(w.top, r.temp(b));
+  }
   if (w.row < 0) return;
   long long* out = tokens + (long long)b * (r.K + 1) + w.at;
   if (w.arg != -2) {
-    if (lane == 0) *out = w.arg;
+    if (threadIdx.x == 0) *out = w.arg;
     return;
   }
-  const long long token = pick_token<SRC>(row_at<SRC>(r, w.row), r.V, ns, w, scale, draft_row(d, w, b), w.refused >= 0,
-                                          fmin(fmax((double)uniforms[b], 0.0), 1.0), [&](int j) {
+  pick_token<SRC, kSampleThreads / kWave>(shared, row_at<SRC>(r, w.row), r.V, ns, w, scale, draft_row(d, w, b),
+                                          w.refused >= 0, fmin(fmax((double)u, 0.0), 1.0),
+                                          [&](int j) {
                                             return mass ? mass[(long long)b * ns + j]
                                                         : segment_sum(rec[(long long)b * ns + j], scale);
-                                          });
-  if (lane == 0) *out = token;
+                                          },
+                                          out);
 }
 
 // ---------------------------------------------------------------------------
@@ -433,7 +448,7 @@ int run(const SampleRows& r, const Drafts& d, const Plan& p, char* ws, const flo
       hipLaunchKernelGGL((sample_mass_kernel<SRC, false>), mass_blocks, threads, 0, st, r, d, p.ns, p.blocks, rec, cuts,
                          draws, mass, probs, nullptr, nullptr);
   }
-  hipLaunchKernelGGL((sample_pick_kernel<SRC>), dim3(r.B), dim3(kWave), 0, st, r, d, p.ns, rec, draws, mass, uniforms,
+  hipLaunchKernelGGL((sample_pick_kernel<SRC>), dim3(r.B), threads, 0, st, r, d, p.ns, rec, draws, mass, uniforms,
                      tokens);
   return launch_status(who);
 }

@@ -12,9 +12,10 @@
 // A draw that needs nothing else comes out of the same launches: the second one
 // adds up what the segments hold above the border's bins, the third adds the
 // listed tokens that stay and picks.
-// Three launches where one workgroup per row could do all of it: what it takes
-// that workgroup to look through its row alone is 8 to 30 us, at 16 bytes a
-// cycle and with 2 wavefronts a SIMD; all wavefronts of the chip do it in 3.
+// Three launches where one workgroup per row could do all of it: to look through
+// its row alone took that workgroup 7 us (131072 float32) to 12 (152000 bf16) at
+// 16 to 24 bytes a cycle, and 512 rows 28; a launch of the whole chip takes as
+// long for 64 rows as for one.
 //
 // Counts and sums do not depend on the order in which tokens are listed: the
 // parts' sums are integers, added in 64-bit floats part by part; among listed
@@ -319,11 +320,13 @@ __global__ void __launch_bounds__(kCutThreads)
   __shared__ u64 s_before_fixed, s_border;
   __shared__ uint32_t s_before_count, s_count;
   __shared__ int s_bin, s_fill;
+  __shared__ PickShared<SRC> pick;
 
   const int slot = blockIdx.x, b = slot / (r.K + 1), i = slot % (r.K + 1);
   const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
   if (i >= r.count(b)) return;
   const CutPlan plan = plans[slot];
+  const float u = tokens ? uniforms[b] : 0.0f;
   const u64 ahead = lists[(long long)slot * kListed + t];  // (under way with the plan; what is not listed is not used)
   u64 cut = 0;
   double kept = plan.kept;
@@ -581,15 +584,14 @@ __global__ void __launch_bounds__(kCutThreads)
     }
   }
   __syncthreads();
-  if (wave != 0) return;
   const SegRec* recs = rec + (long long)slot * ns;
-  const long long token =
-      pick_token<SRC>(row, r.V, ns, w, scale, nullptr, false, fmin(fmax((double)uniforms[b], 0.0), 1.0), [&](int j) {
-        if (cut == 0) return segment_sum(recs[j], scale);
-        if (!summed) return masses[j];
-        return (plan.all_listed ? 0.0 : masses[j]) + (double)sub_sum[j] / unit;
-      });
-  if (lane == 0) tokens[b] = token;
+  pick_token<SRC, kCutWaves>(pick, row, r.V, ns, w, scale, nullptr, false, fmin(fmax((double)u, 0.0), 1.0),
+                             [&](int j) {
+                               if (cut == 0) return segment_sum(recs[j], scale);
+                               if (!summed) return masses[j];
+                               return (plan.all_listed ? 0.0 : masses[j]) + (double)sub_sum[j] / unit;
+                             },
+                             tokens + b);
 }
 
 template <int SRC>
