@@ -102,8 +102,12 @@ def test_python_refusals():
         chunk_tables(table, lens[:2], lens, 3, 16)
     with pytest.raises(RuntimeError, match="counts must be integers"):
         chunk_tables(table, lens, lens.float(), 3, 16)
-    with pytest.raises(RuntimeError, match="counts must be"):
+    with pytest.raises(RuntimeError, match="requests must be"):
         chunk_tables(table, lens, lens, 3, 16, requests=lens[:2])
+    with pytest.raises(RuntimeError, match="requests must be"):
+        chunk_tables(table, lens, lens, 3, 16, requests=lens[0])
+    with pytest.raises(RuntimeError, match="counts must be"):
+        chunk_tables(table, lens, lens[None], 3, 16)
     short = ChunkTables(table, lens, lens, lens, lens, lens, lens)
     with pytest.raises(RuntimeError, match="out.cu_seqlens"):
         chunk_tables(table, lens, lens, 3, 16, out=short)

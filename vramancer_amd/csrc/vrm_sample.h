@@ -591,7 +591,7 @@ struct CutPlan {
 // Finds every row's cut from the histograms of its parts (cuts; with draws,
 // sequences of one row, its draw too), or with tokens draws from it: mass then
 // takes the sums of a row's segments, at most kDrawSegments.  lists: kListed
-// order values a row.
+// order values a row, V where that is less.
 constexpr int kDrawSegments = 1024;
 int launch_sample_cut(const SampleRows& r, int dtype, const SegRec* rec, const Histogram* hist, CutPlan* plans,
                       unsigned long long* lists, RowCut* cuts, DrawRec* draws, double* mass, const float* uniforms,

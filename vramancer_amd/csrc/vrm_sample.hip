@@ -390,7 +390,7 @@ Plan plan_of(long long B, int K, int V, bool filtered, bool drafts, bool probs) 
     p.plans = at;
     at += up((size_t)p.slots * sizeof(CutPlan));
     p.lists = at;
-    at += up((size_t)p.slots * kListed * sizeof(unsigned long long));
+    at += up((size_t)p.slots * (V < kListed ? V : kListed) * sizeof(unsigned long long));
     p.cuts = at;
     at += up((size_t)p.slots * sizeof(RowCut));
   }

@@ -20,12 +20,14 @@
 // Counts and sums do not depend on the order in which tokens are listed: the
 // parts' sums are integers, added in 64-bit floats part by part; among listed
 // tokens weights are integers in units of 2^-S, S such that V of them stay below
-// 2^62 (S = 45 for V up to 2^17).  Tokens below 2^-51 of the row's largest may
-// weigh nothing here; where such a token would be the border nothing is cut.
+// 2^62 (S = 45 for V up to 2^17).  Tokens below 2^-50 of the row's largest may
+// count and weigh nothing here: a border among them may lie further down.
 //
 // A workgroup of the first and the last kernel runs each part of its code a few
 // times at most, so that fetching it is what short code saves (170 KB, with a
 // copy of the narrowing for each use, took 42 us for a row of 131072).
+#include <algorithm>
+
 #include "vrm_sample.h"
 
 namespace vrm {
@@ -244,13 +246,15 @@ __global__ void __launch_bounds__(kCutThreads)
 }
 
 // A wavefront per segment: the tokens of the bins of the plan go to the row's
-// list, by their order values; plan.listed counts them, and only kListed fit.
+// list, by their order values; plan.listed counts them, and only `most` (kListed,
+// or V where that is less) fit.
 // With MASS, mass takes the weights of the segment's tokens above the first of
 // those bins, which stay whatever the border.  (The segment is under way before
 // the plan that says whether it is needed.)
 template <int SRC, bool MASS>
 __global__ void __launch_bounds__(kSampleThreads)
-    sample_collect_kernel(SampleRows r, int ns, int blocks, CutPlan* plans, u64* lists, double* mass) {
+    sample_collect_kernel(SampleRows r, int ns, int blocks, CutPlan* plans, u64* lists, int most,
+                          double* mass) {
   const int slot = blockIdx.x / blocks, seg = (blockIdx.x % blocks) * 4 + (threadIdx.x >> 6);
   const int b = slot / (r.K + 1), i = slot % (r.K + 1);
   if (seg >= ns || i >= r.count(b)) return;
@@ -275,11 +279,11 @@ __global__ void __launch_bounds__(kSampleThreads)
     int at = 0;
     if ((threadIdx.x & 63) == 0) at = atomicAdd(&plan.listed, all);
     at = lane_value(at, 0) + up_to - mine;
-    u64* list = lists + (long long)slot * kListed;
+    u64* list = lists + (long long)slot * most;
 #pragma unroll
     for (int e = 0; e < kSamplePer; ++e) {
       if (hits & (1u << e)) {
-        if (at < kListed) list[at] = order_value(x[e], segment_element<SRC>(seg, e / kVec) + e % kVec);
+        if (at < most) list[at] = order_value(x[e], segment_element<SRC>(seg, e / kVec) + e % kVec);
         ++at;
       }
     }
@@ -310,7 +314,7 @@ __global__ void __launch_bounds__(kSampleThreads)
 template <int SRC>
 __global__ void __launch_bounds__(kCutThreads)
     sample_border_kernel(SampleRows r, int ns, int bits, const SegRec* rec, const CutPlan* plans, const u64* lists,
-                         RowCut* cuts, DrawRec* draws, double* mass, const float* uniforms, long long* tokens) {
+                         int most, RowCut* cuts, DrawRec* draws, double* mass, const float* uniforms, long long* tokens) {
   __shared__ u64 list[kListed];  // order values
   __shared__ u64 sub_sum[kSub];
   __shared__ uint32_t sub_count[kSub];
@@ -327,7 +331,8 @@ __global__ void __launch_bounds__(kCutThreads)
   if (i >= r.count(b)) return;
   const CutPlan plan = plans[slot];
   const float u = tokens ? uniforms[b] : 0.0f;
-  const u64 ahead = lists[(long long)slot * kListed + t];  // (under way with the plan; what is not listed is not used)
+  // (under way with the plan; what is not listed is not used)
+  const u64 ahead = t < most ? lists[(long long)slot * most + t] : 0;
   u64 cut = 0;
   double kept = plan.kept;
   bool fits = true, of_p = false;  // whether the cut is top_p's
@@ -340,10 +345,10 @@ __global__ void __launch_bounds__(kCutThreads)
     const float bins = bin_scale(scale);
     const double unit = (double)(1ULL << bits);
     const auto weight_of = [&](u64 o) { return fixed_weight(sample_weight(order_logit(o), scale), unit); };
-    fits = plan.listed <= kListed;
+    fits = plan.listed <= most;
     listed = fits ? plan.listed : 0;
     if (t < listed) list[t] = ahead;
-    for (int j = t + kCutThreads; j < listed; j += kCutThreads) list[j] = lists[(long long)slot * kListed + j];
+    for (int j = t + kCutThreads; j < listed; j += kCutThreads) list[j] = lists[(long long)slot * most + j];
     kept = plan.total;
 #pragma unroll 1
     for (int turn = 0; turn < 2; ++turn) {
@@ -599,16 +604,17 @@ void launch(const SampleRows& r, int bits, const SegRec* rec, const Histogram* h
             RowCut* cuts, DrawRec* draws, double* mass, const float* uniforms, long long* tokens, hipStream_t st) {
   const int blocks = (r.V + kSampleBlock - 1) / kSampleBlock;
   const long long slots = (long long)r.B * (r.K + 1);
+  const int most = std::min(kListed, r.V);
   hipLaunchKernelGGL(sample_bins_kernel, dim3((unsigned)slots), dim3(kCutThreads), 0, st, r, r.segments(), blocks, rec,
                      hist, plans);
   if (tokens)
     hipLaunchKernelGGL((sample_collect_kernel<SRC, true>), dim3((unsigned)(slots * blocks)), dim3(kSampleThreads), 0, st,
-                       r, r.segments(), blocks, plans, lists, mass);
+                       r, r.segments(), blocks, plans, lists, most, mass);
   else
     hipLaunchKernelGGL((sample_collect_kernel<SRC, false>), dim3((unsigned)(slots * blocks)), dim3(kSampleThreads), 0,
-                       st, r, r.segments(), blocks, plans, lists, nullptr);
+                       st, r, r.segments(), blocks, plans, lists, most, nullptr);
   hipLaunchKernelGGL((sample_border_kernel<SRC>), dim3((unsigned)slots), dim3(kCutThreads), 0, st, r, r.segments(), bits,
-                     rec, plans, lists, cuts, draws, mass, uniforms, tokens);
+                     rec, plans, lists, most, cuts, draws, mass, uniforms, tokens);
 }
 
 }  // namespace

@@ -259,7 +259,7 @@ class ChunkTables:
 
 def _ints(name: str, t, n: Optional[int]):
     if t.dim() != 1 or (n is not None and t.shape[0] != n):
-        raise RuntimeError(f"{name} must be [{'R' if n is None else n}], got shape {tuple(t.shape)}")
+        raise RuntimeError(f"{name} must be [{'B' if n is None else n}], got shape {tuple(t.shape)}")
     if t.dtype != torch.int32:
         if t.dtype not in (torch.int64, torch.int16, torch.int8, torch.uint8):
             raise RuntimeError(f"{name} must be integers, got {t.dtype}")
@@ -300,7 +300,7 @@ def chunk_tables(
     if block_table.stride(1) != 1 and W > 1:
         block_table = block_table.contiguous()
     past_lens = _ints("past_lens", past_lens, R)
-    counts = _ints("counts", counts, None if requests is None else requests.shape[0])
+    counts = _ints("counts", counts, None)
     B = counts.shape[0]
     if requests is not None:
         requests = _ints("requests", requests, B)
