@@ -305,7 +305,7 @@ def test_verified_tokens_are_the_targets():
     assert abs(accepted.double().mean().item() - agree) <= 6 * math.sqrt(agree * (1 - agree) / n)
 
 
-@pytest.mark.parametrize("B,K,V", [(3, 14, 700), (900, 2, 40), (300, 1, 20000)])
+@pytest.mark.parametrize("B,K,V", [(3, 14, 700), (900, 2, 40), (300, 1, 20000), (500, 3, 9000), (40, 9, 60001)])
 @pytest.mark.parametrize("kw", [dict(), dict(top_k=20, top_p=0.9)])
 def test_verify_many(B, K, V, kw):
     # many drafts, many sequences: the drafts are tested in a launch of their own
@@ -318,6 +318,73 @@ def test_verify_many(B, K, V, kw):
     assert tokens[some].cpu().tolist() == want[0].tolist() and accepted[some].cpu().tolist() == want[1].tolist()
     again = sampling.verify_drafts(x, d, ua, u, q, **kw)
     assert torch.equal(again[0], tokens) and torch.equal(again[1], accepted)
+
+
+def borders(B, K, V, dtype, seed, near):
+    """Drafts whose random number lies next to p / q, and draft distributions
+    that are p but for 1e-6 of it (near) and a few tokens."""
+    g = torch.Generator().manual_seed(seed)
+    x = (torch.randn((B, K + 1, V), generator=g) * 2.5).to(dtype)
+    p = torch.softmax(x.double(), -1)[:, :K]
+    q = p * (1 + near * torch.randn((B, K, V), generator=g).double())
+    up = torch.randint(0, V, (B, K, 1), generator=g)
+    down = torch.randint(0, V, (B, K, 9), generator=g)
+    q = q.scatter(2, down, q.gather(2, down) * 0.3)
+    d = p.argmax(-1) if near else up[..., 0]
+    q = q.scatter(2, d[..., None], (p.gather(2, d[..., None]) * 1.7 + 1e-3).clamp(max=1.0)).float()
+    ratio = (p.gather(2, d[..., None]) / q.double().gather(2, d[..., None]))[..., 0].float()
+    step = torch.randint(-3, 4, (B, K), generator=g)
+    step[:, -1] = 4  # (the last is refused if the others pass)
+    ua = ratio
+    for i in range(1, 5):
+        ua = torch.where(step >= i, torch.nextafter(ua, torch.tensor(2.0)), ua)
+        ua = torch.where(step <= -i, torch.nextafter(ua, torch.tensor(0.0)), ua)
+    return x.to(DEV), d.to(DEV), ua.to(DEV), torch.rand(B, generator=g).to(DEV), q.to(DEV)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("near", [0.0, 1e-6, 1e-7])
+@pytest.mark.parametrize("B,K,V,only", [(6, 3, 3000, None), (700, 3, 300, 60), (120, 2, 50001, 12)])
+def test_verify_at_the_borders(B, K, V, only, near, dtype):
+    # small and large batches take different sums; both decide as 64 bits do
+    x, d, ua, u, q = borders(B, K, V, dtype, V + B, near)
+    tokens, accepted = sampling.verify_drafts(x, d, ua, u, q)
+    n = only or B
+    want = verify(x[:n], d[:n], ua[:n], u[:n], q[:n])
+    assert accepted[:n].cpu().tolist() == want[1].tolist()
+    assert tokens[:n].cpu().tolist() == want[0].tolist()
+    if only:
+        tokens, accepted = sampling.verify_drafts(x, d, ua, u)
+        want = verify(x[:n], d[:n], ua[:n], u[:n])
+        assert tokens[:n].cpu().tolist() == want[0].tolist() and accepted[:n].cpu().tolist() == want[1].tolist()
+
+
+def test_verify_large_masked():
+    # what test_verify_masked, _greedy_rows and _nothing_left hold, in a large batch
+    B, K, V = 600, 3, 900
+    x, d, ua, u, q = drafts_of(B, K, V, torch.float32, 16)
+    x[0, 0] = -math.inf
+    x[1, :, ::2] = -math.inf
+    x[2, 1, d[2, 1]] = -math.inf
+    x[3, 0, :] = math.nan
+    x[4, 0, 10] = math.inf
+    x[5, 0, 700:] = math.nan
+    q = q.clone()
+    q[6, 0, 5] = math.nan
+    q[7, 1, :] = -1.0
+    q[8] = 2.0
+    d[9, 0], d[10, 1] = -1, V
+    t = torch.full((B,), 0.7, device=DEV)
+    t[11:14] = 0.0
+    t[14], t[15], t[16] = math.inf, 1e-38, 1e4
+    d[12] = x[12, :K].argmax(-1)
+    ua[8] = 0.9
+    for kw in (dict(), dict(temperature=t)):
+        for probs in (q, None):
+            tokens, accepted = sampling.verify_drafts(x, d, ua, u, probs, **kw)
+            part = {k: v[:40] for k, v in kw.items()}
+            want = verify(x[:40], d[:40], ua[:40], u[:40], None if probs is None else q[:40], **part)
+            assert tokens[:40].cpu().tolist() == want[0].tolist() and accepted[:40].cpu().tolist() == want[1].tolist()
 
 
 @pytest.mark.parametrize("kw", [dict(), dict(top_k=70), dict(top_p=0.9)])

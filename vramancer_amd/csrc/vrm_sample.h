@@ -336,25 +336,29 @@ __device__ __forceinline__ void combine_segments(const SegRec* rec, int ns, floa
   sum = wave_sum(s);
 }
 
+// Probabilities e0 .. e0 + N of a row of V, 0 past its end.
+template <int N>
+__device__ __forceinline__ void load_probs(const float* q, int e0, int V, float* x) {
+  if (e0 + N <= V) {
+#pragma unroll
+    for (int h = 0; h < N; h += 4) {
+      const auto raw = *reinterpret_cast<const Unaligned16<uint32_t>*>(q + e0 + h);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[h + e] = __uint_as_float(raw.v[e]);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e) x[e] = e0 + e < V ? q[e0 + e] : 0.0f;
+  }
+}
+
 // What the tokens e0 .. e0 + N weigh in the draw: p, or where a draft was
 // refused max(p - q, 0), in units of 1 / sum.
 template <int N>
 __device__ __forceinline__ void draw_weights(const DrawRec& w, const Scale& scale, const float* q, bool rest, int e0,
                                              int V, const float* x, double* out) {
   float qx[N];
-  if (rest && q) {
-    if (e0 + N <= V) {
-#pragma unroll
-      for (int h = 0; h < N; h += 4) {
-        const auto raw = *reinterpret_cast<const Unaligned16<uint32_t>*>(q + e0 + h);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) qx[h + e] = __uint_as_float(raw.v[e]);
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < N; ++e) qx[e] = e0 + e < V ? q[e0 + e] : 0.0f;
-    }
-  }
+  if (rest && q) load_probs<N>(q, e0, V, qx);
   bool in[N], any = true;
   if (w.cut) {
     any = false;

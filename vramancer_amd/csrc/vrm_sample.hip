@@ -14,6 +14,8 @@
 //   4. sample_mass_kernel       that row's segments: the mass to draw from
 //   5. sample_pick_kernel       the segment and the token where the running sum
 //                               passes the random number
+// Large batches of drafts run 1, 4 and 5 in forms of their own, in float32 where
+// that decides (sample_rough_*).
 // A draw without top_k and top_p is 1 and 5, one with them 1 and 2 (which picks
 // too), and 1, 2, 4 and 5 where its distribution is asked for.
 #include "vrm_sample.h"
@@ -135,6 +137,64 @@ __global__ void __launch_bounds__(kSampleThreads)
   }
 }
 
+// The same as sample_segment_kernel in float32, for large batches of drafts: all
+// that most rows are for is the test of one draft.  Sums are within kRough of the
+// exact ones: a term errs by 3 2^-24 |y| ln 2 + 2^-23 of itself (the difference,
+// the scale and their product, and the exponential's last place), which is
+// 4.1e-6 for |y| <= 32; what lies below weighs V 2^-32 of the largest at most;
+// 32 terms of a lane, added in pairs, add 5 2^-24: 4.4e-6 in all.
+constexpr double kRough = 5e-6;
+
+template <int SRC>
+__global__ void __launch_bounds__(kSampleThreads) sample_rough_kernel(SampleRows r, int ns, int blocks, SegRec* rec) {
+  const int slot = blockIdx.x / blocks, seg = (blockIdx.x % blocks) * 4 + (threadIdx.x >> 6);
+  const int b = slot / (r.K + 1), i = slot % (r.K + 1);
+  if (seg >= ns || i >= r.count(b)) return;
+  float x[kSamplePer];
+  load_segment<SRC>(row_at<SRC>(r, r.first(b) + i), seg, r.V, x);
+  const float t = r.temp(b);
+  float m = -INFINITY;
+#pragma unroll
+  for (int e = 0; e < kSamplePer; ++e) m = fmaxf(m, x[e]);
+  m = wave_max(m, -INFINITY);
+  SegRec g{0.0, m, -1};
+  if (m > -INFINITY) {
+    if (t > 0.0f) {
+      const float c = fminf((float)(1.4426950408889634074 / (double)t), 3e38f);
+#pragma unroll
+      for (int e = 0; e < kSamplePer; ++e) {
+        const float y = fmaxf((x[e] - m) * c, -200.0f);  // (a NaN is the lower bound, which underflows)
+        x[e] = m == INFINITY ? (x[e] == m ? 1.0f : 0.0f) : __builtin_amdgcn_exp2f(y);
+      }
+#pragma unroll
+      for (int n = kSamplePer / 2; n > 0; n /= 2)
+#pragma unroll
+        for (int e = 0; e < n; ++e) x[e] += x[e + n];
+      g.sum = wave_sum((double)x[0]);
+    } else {
+      g.arg = first_place<SRC>(x, m, seg);
+    }
+  }
+  if ((threadIdx.x & 63) == 0) rec[(long long)slot * ns + seg] = g;
+}
+
+// The exact sum of a row's weights, by one wavefront.
+template <int SRC>
+__device__ __forceinline__ double exact_sum(const typename Logit<SRC>::Raw* row, int V, int ns, const Scale& scale) {
+  constexpr int kVec = Logit<SRC>::kVec;
+  double sum = 0.0;
+#pragma unroll 1
+  for (int g = 0; g < ns * (kSamplePer / kVec); ++g) {
+    float x[kVec];
+    double w[kVec];
+    load_vec<SRC>(row, segment_element<SRC>(g / (kSamplePer / kVec), g % (kSamplePer / kVec)), V, x);
+    sample_weights<kVec>(x, scale, w);
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) sum += w[e];
+  }
+  return wave_sum(sum);
+}
+
 // ---------------------------------------------------------------------------
 // 3. Accepted drafts and the row to draw from: one workgroup per sequence, a
 // wavefront per row in turn.  The drafts are tested at once and not one after
@@ -155,8 +215,10 @@ struct Drafts {
 
 // The drafts that sequence b accepts and its draw, for every thread of the
 // workgroup.  Answers (tokens, accepted, draws) are written by the workgroup
-// that has `writes`.
-template <int SRC>
+// that has `writes`.  With ROUGH sums are within kRough: a test that lies
+// within that of its border is made again with the exact sum (one in 10^5), and
+// the draw's sum is the rough one.
+template <int SRC, bool ROUGH>
 __device__ __forceinline__ DrawRec choose(const SampleRows& r, const Drafts& d, int ns, const SegRec* rec,
                                           const RowCut* cuts, int b, bool writes, DrawRec* draws, long long* tokens,
                                           int32_t* accepted, Scale& scale) {
@@ -190,7 +252,10 @@ __device__ __forceinline__ DrawRec choose(const SampleRows& r, const Drafts& d, 
           if (order_value(l, (int)x) < cut.cut) w = 0.0;
         }
       }
-      ok = (double)u * (double)(qx < 0.0f ? 0.0f : qx) * sum < w;
+      const double uq = (double)u * (double)(qx < 0.0f ? 0.0f : qx);
+      if (ROUGH && arg == -2 && uq * sum * (1.0 - kRough) < w && !(uq * sum * (1.0 + kRough) < w))
+        sum = exact_sum<SRC>(row_at<SRC>(r, first + i), r.V, ns, at_row);
+      ok = uq * sum < w;
     }
     if (!ok && lane == 0) atomicMin(&stop, i);
   }
@@ -231,12 +296,12 @@ __device__ __forceinline__ DrawRec choose(const SampleRows& r, const Drafts& d, 
   return w;
 }
 
-template <int SRC>
+template <int SRC, bool ROUGH>
 __global__ void __launch_bounds__(kSampleThreads)
     sample_choose_kernel(SampleRows r, Drafts d, int ns, const SegRec* rec, const RowCut* cuts, DrawRec* draws,
                          long long* tokens, int32_t* accepted) {
   Scale scale;
-  choose<SRC>(r, d, ns, rec, cuts, blockIdx.x, true, draws, tokens, accepted, scale);
+  choose<SRC, ROUGH>(r, d, ns, rec, cuts, blockIdx.x, true, draws, tokens, accepted, scale);
 }
 
 // ---------------------------------------------------------------------------
@@ -274,7 +339,7 @@ __global__ void __launch_bounds__(kSampleThreads)
   const int b = blockIdx.x / blocks, part = blockIdx.x % blocks, seg = part * 4 + (threadIdx.x >> 6);
   constexpr int kVec = Logit<SRC>::kVec, kGroups = kSamplePer / kVec;
   Scale scale;
-  const DrawRec w = CHOOSE ? choose<SRC>(r, d, ns, rec, cuts, b, part == 0, draws, tokens, accepted, scale)
+  const DrawRec w = CHOOSE ? choose<SRC, false>(r, d, ns, rec, cuts, b, part == 0, draws, tokens, accepted, scale)
                            : draw_of(r, draws, rec, ns, b, scale);
   if (seg >= ns) return;
   if (w.row < 0 || (w.arg != -2 && !probs)) return;
@@ -319,6 +384,110 @@ __global__ void __launch_bounds__(kSampleThreads)
   if (known) return;
   s = wave_sum(s);
   if ((threadIdx.x & 63) == 0) mass[(long long)b * ns + seg] = s;
+}
+
+// The masses of a draw whose row's sum is known roughly: what max(p - q, 0) adds
+// up to is the weight of the tokens that are above q by more than the sum can
+// be off, less their q times the exact sum, which is the sum of `all`.  Segments
+// with tokens nearer to their border than that (a few in a row) are marked.
+struct RoughMass {
+  double all, above, q;
+  int near, pad;
+};
+
+template <int SRC>
+__global__ void __launch_bounds__(kSampleThreads)
+    sample_rough_mass_kernel(SampleRows r, Drafts d, int ns, int blocks, const DrawRec* draws, RoughMass* mass) {
+  const int b = blockIdx.x / blocks, seg = (blockIdx.x % blocks) * 4 + (threadIdx.x >> 6);
+  if (seg >= ns) return;
+  constexpr int kVec = Logit<SRC>::kVec, kGroups = kSamplePer / kVec;
+  const DrawRec w = draws[b];
+  if (w.row < 0 || w.arg != -2) return;
+  const Scale scale = make_scale(w.top, r.temp(b));
+  const float* q = w.refused >= 0 ? draft_row(d, w, b) : nullptr;
+  const double low = w.sum * (1.0 - 1.01 * kRough), high = w.sum * (1.0 + 1.01 * kRough);
+  float x[kSamplePer];
+  load_segment<SRC>(row_at<SRC>(r, w.row), seg, r.V, x);
+  RoughMass g{};
+#pragma unroll
+  for (int i = 0; i < kGroups; ++i) {
+    const int e0 = segment_element<SRC>(seg, i);
+    float qx[kVec];
+    double p[kVec];
+    if (q) load_probs<kVec>(q, e0, r.V, qx);
+    sample_weights<kVec>(x + i * kVec, scale, p);
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) {
+      g.all += p[e];
+      if (q) {
+        const double qe = qx[e] < 0.0f ? 0.0f : qx[e];
+        const bool above = p[e] > qe * high;
+        g.above += above ? p[e] : 0.0;
+        g.q += above ? qe : 0.0;
+        if (!above && p[e] > qe * low) g.near = 1;
+      } else {
+        g.above += e0 + e == w.refused ? 0.0 : p[e];
+      }
+    }
+  }
+  g.all = wave_sum(g.all);
+  g.above = wave_sum(g.above);
+  g.q = wave_sum(g.q);
+  g.near = __any(g.near) ? 1 : 0;
+  if ((threadIdx.x & 63) == 0) mass[(long long)b * ns + seg] = g;
+}
+
+// The exact masses from these, and the token; one workgroup per sequence.
+template <int SRC>
+__global__ void __launch_bounds__(kSampleThreads)
+    sample_rough_pick_kernel(SampleRows r, Drafts d, int ns, const DrawRec* draws, const RoughMass* rough, double* mass,
+                             const float* uniforms, long long* tokens) {
+  __shared__ PickShared<SRC> shared;
+  const int b = blockIdx.x, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const float u = uniforms[b];
+  DrawRec w = draws[b];
+  if (w.row < 0) return;
+  long long* out = tokens + (long long)b * (r.K + 1) + w.at;
+  if (w.arg != -2) {
+    if (threadIdx.x == 0) *out = w.arg;
+    return;
+  }
+  constexpr int kVec = Logit<SRC>::kVec, kGroups = kSamplePer / kVec;
+  const auto* row = row_at<SRC>(r, w.row);
+  const float* q = draft_row(d, w, b);
+  const bool rest = w.refused >= 0;
+  const Scale scale = make_scale(w.top, r.temp(b));
+  const RoughMass* from = rough + (long long)b * ns;
+  double* to = mass + (long long)b * ns;
+  double sum = 0.0;
+  for (int j = lane; j < ns; j += kWave) sum += from[j].all;
+  w.sum = wave_sum(sum);
+  int turn = 0;  // the marked segments, to the wavefronts in turn
+  for (int j0 = 0; j0 < ns; j0 += kWave) {
+    const int j = j0 + lane;
+    const RoughMass g = j < ns ? from[j] : RoughMass{};
+    if (wave == 0 && j < ns && !g.near) to[j] = rest ? fmax(fma(-g.q, w.sum, g.above), 0.0) : g.all;
+    unsigned long long near = __ballot(g.near != 0);
+    for (; near; near &= near - 1, ++turn) {
+      if (turn % (kSampleThreads / kWave) != wave) continue;
+      const int at = __ffsll(near) - 1;
+      float x[kSamplePer];
+      load_segment<SRC>(row, j0 + at, r.V, x);
+      double s = 0.0;
+#pragma unroll
+      for (int i = 0; i < kGroups; ++i) {
+        double p[kVec];
+        draw_weights<kVec>(w, scale, q, rest, segment_element<SRC>(j0 + at, i), r.V, x + i * kVec, p);
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) s += p[e];
+      }
+      s = wave_sum(s);
+      if (lane == at) to[j] = s;
+    }
+  }
+  __syncthreads();
+  pick_token<SRC, kSampleThreads / kWave>(shared, row, r.V, ns, w, scale, q, rest, fmin(fmax((double)u, 0.0), 1.0),
+                                          [&](int j) { return to[j]; }, out);
 }
 
 // One workgroup per sequence.  mass == NULL: a draw from row b by its segments'
@@ -371,8 +540,12 @@ struct Plan {
   int ns, blocks;  // segments and workgroups of a row
   bool filtered, drafts, masses;
   bool fused;  // the cut draws by itself
-  size_t hist, plans, lists, cuts, draws, mass, bytes;
+  bool rough;  // rows summed in float32 first
+  size_t rough_mass, hist, plans, lists, cuts, draws, mass, bytes;
 };
+
+// From how many workgroups of all rows on they are summed in float32 first.
+constexpr long long kRoughBlocks = 2048;
 
 Plan plan_of(long long B, int K, int V, bool filtered, bool drafts, bool probs) {
   Plan p{};
@@ -383,7 +556,12 @@ Plan plan_of(long long B, int K, int V, bool filtered, bool drafts, bool probs) 
   p.drafts = drafts;
   p.masses = filtered || drafts || probs;
   p.fused = filtered && !drafts && !probs && p.ns <= kDrawSegments;
+  p.rough = drafts && !filtered && p.slots * p.blocks > kRoughBlocks;
   size_t at = up((size_t)p.slots * p.ns * sizeof(SegRec));
+  if (p.rough) {
+    p.rough_mass = at;
+    at += up((size_t)B * p.ns * sizeof(RoughMass));
+  }
   if (filtered) {
     p.hist = at;
     at += up((size_t)p.slots * p.blocks * sizeof(Histogram));
@@ -433,16 +611,27 @@ int run(const SampleRows& r, const Drafts& d, const Plan& p, char* ws, const flo
                                    p.drafts ? nullptr : draws, mass, uniforms, p.fused ? tokens : nullptr, st))
       return rc;
     if (p.fused) return launch_status(who);
+  } else if (p.rough) {
+    hipLaunchKernelGGL((sample_rough_kernel<SRC>), row_blocks, threads, 0, st, r, p.ns, p.blocks, rec);
   } else {
     hipLaunchKernelGGL((sample_segment_kernel<SRC>), row_blocks, threads, 0, st, r, p.ns, p.blocks, rec);
   }
   const dim3 mass_blocks((unsigned)((long long)r.B * p.blocks));
+  if (p.rough) {
+    auto* rough = reinterpret_cast<RoughMass*>(ws + p.rough_mass);
+    hipLaunchKernelGGL((sample_choose_kernel<SRC, true>), dim3(r.B), threads, 0, st, r, d, p.ns, rec, nullptr, draws,
+                       tokens, accepted);
+    hipLaunchKernelGGL((sample_rough_mass_kernel<SRC>), mass_blocks, threads, 0, st, r, d, p.ns, p.blocks, draws, rough);
+    hipLaunchKernelGGL((sample_rough_pick_kernel<SRC>), dim3(r.B), threads, 0, st, r, d, p.ns, draws, rough, mass,
+                       uniforms, tokens);
+    return launch_status(who);
+  }
   if (p.drafts && r.K <= kChooseDrafts && mass_blocks.x <= (unsigned)kChooseBlocks) {
     hipLaunchKernelGGL((sample_mass_kernel<SRC, true>), mass_blocks, threads, 0, st, r, d, p.ns, p.blocks, rec, cuts,
                        draws, mass, nullptr, tokens, accepted);
   } else {
     if (p.drafts)
-      hipLaunchKernelGGL((sample_choose_kernel<SRC>), dim3(r.B), threads, 0, st, r, d, p.ns, rec, cuts, draws, tokens,
+      hipLaunchKernelGGL((sample_choose_kernel<SRC, false>), dim3(r.B), threads, 0, st, r, d, p.ns, rec, cuts, draws, tokens,
                          accepted);
     if (p.masses)
       hipLaunchKernelGGL((sample_mass_kernel<SRC, false>), mass_blocks, threads, 0, st, r, d, p.ns, p.blocks, rec, cuts,
