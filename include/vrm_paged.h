@@ -757,10 +757,11 @@ int vrm_chunk_tables(const int32_t* block_table, long long row_stride, int R, in
  * NULL: temperature_all, top_k_all, top_p_all hold for every one.  V is at most
  * VRM_SAMPLE_MAX_V.  Random numbers are taken into [0, 1].
  *
- * Weights, their sums and every comparison with them are 64-bit floats (under
- * top_k and top_p sums of weights rounded to multiples of 2^-S of the largest,
- * S = min(45, 63 - ceil(log2 V)), which is where the shortest prefix is found).
- * Results are the same from call to call.  The workspace is 16-byte aligned and
+ * Weights, their sums and every comparison with them are 64-bit floats, weights
+ * to 2.2e-12 of themselves, or decided as with those (under top_k and top_p a
+ * border is found in sums of weights rounded to multiples of 2^-S of the
+ * largest, S = min(45, 62 - ceil(log2 V)); tokens below 2^-50 of the largest may
+ * count for nothing there).  Results are the same from call to call.  The workspace is 16-byte aligned and
  * written before it is read.
  * -------------------------------------------------------------------------- */
 #define VRM_SAMPLE_MAX_V (1 << 24)

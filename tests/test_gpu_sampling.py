@@ -178,6 +178,15 @@ def drafts_of(B, K, V, dtype, seed, near=0.7):
             q.to(DEV))
 
 
+def many_drafts(B, K, V, dtype, seed):
+    """The same, made on the GPU."""
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    x = torch.randn((B, K + 1, V), generator=g, device=DEV) * 2.5
+    q = torch.softmax(x[:, :K] + torch.randn((B, K, V), generator=g, device=DEV) * 0.7, -1)
+    d = (q / -torch.rand((B, K, V), generator=g, device=DEV).clamp(min=1e-30).log()).argmax(-1)
+    return (x.to(dtype), d, torch.rand((B, K), generator=g, device=DEV), torch.rand(B, generator=g, device=DEV), q)
+
+
 def check_verify(x, d, ua, u, q=None, cu=None, **kw):
     tokens, accepted = sampling.verify_drafts(x, d, ua, u, draft_probs=q, cu_seqlens=cu, **kw)
     want_t, want_a = verify(x, d, ua, u, q, cu, **kw)
@@ -305,14 +314,15 @@ def test_verified_tokens_are_the_targets():
     assert abs(accepted.double().mean().item() - agree) <= 6 * math.sqrt(agree * (1 - agree) / n)
 
 
-@pytest.mark.parametrize("B,K,V", [(3, 14, 700), (900, 2, 40), (300, 1, 20000), (500, 3, 9000), (40, 9, 60001)])
+@pytest.mark.parametrize("B,K,V", [(3, 14, 700), (900, 2, 40), (300, 1, 20000), (90, 9, 40001), (9000, 3, 1000)])
 @pytest.mark.parametrize("kw", [dict(), dict(top_k=20, top_p=0.9)])
 def test_verify_many(B, K, V, kw):
-    # many drafts, many sequences: the drafts are tested in a launch of their own
-    x, d, ua, u, q = drafts_of(B, K, V, torch.bfloat16, B)
+    # many drafts, many sequences: drafts tested in a launch of their own, and
+    # from 2^25 logits on sums in float32 first
+    x, d, ua, u, q = many_drafts(B, K, V, torch.bfloat16, B)
     ws = sampling.verify_workspace(B, K, V, device=DEV)
     ws.fill_(255)
-    some = slice(0, B, max(1, B // 40))  # (the reference is slow)
+    some = slice(0, B, max(1, B // 30))  # (the reference is slow)
     tokens, accepted = sampling.verify_drafts(x, d, ua, u, q, workspace=ws, **kw)
     want = verify(x[some], d[some], ua[some], u[some], q[some], **kw)
     assert tokens[some].cpu().tolist() == want[0].tolist() and accepted[some].cpu().tolist() == want[1].tolist()
@@ -323,28 +333,28 @@ def test_verify_many(B, K, V, kw):
 def borders(B, K, V, dtype, seed, near):
     """Drafts whose random number lies next to p / q, and draft distributions
     that are p but for 1e-6 of it (near) and a few tokens."""
-    g = torch.Generator().manual_seed(seed)
-    x = (torch.randn((B, K + 1, V), generator=g) * 2.5).to(dtype)
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    at = dict(generator=g, device=DEV)
+    x = (torch.randn((B, K + 1, V), **at) * 2.5).to(dtype)
     p = torch.softmax(x.double(), -1)[:, :K]
-    q = p * (1 + near * torch.randn((B, K, V), generator=g).double())
-    up = torch.randint(0, V, (B, K, 1), generator=g)
-    down = torch.randint(0, V, (B, K, 9), generator=g)
-    q = q.scatter(2, down, q.gather(2, down) * 0.3)
+    q = p * (1 + near * torch.randn((B, K, V), **at))
+    up = torch.randint(0, V, (B, K, 1), **at)
+    down = torch.randint(0, V, (B, K, 9), **at)
+    q = q.scatter(2, down, p.gather(2, down) * 0.3)
     d = p.argmax(-1) if near else up[..., 0]
     q = q.scatter(2, d[..., None], (p.gather(2, d[..., None]) * 1.7 + 1e-3).clamp(max=1.0)).float()
-    ratio = (p.gather(2, d[..., None]) / q.double().gather(2, d[..., None]))[..., 0].float()
-    step = torch.randint(-3, 4, (B, K), generator=g)
+    ua = (p.gather(2, d[..., None]) / q.double().gather(2, d[..., None]))[..., 0].float()
+    step = torch.randint(-3, 4, (B, K), **at)
     step[:, -1] = 4  # (the last is refused if the others pass)
-    ua = ratio
     for i in range(1, 5):
-        ua = torch.where(step >= i, torch.nextafter(ua, torch.tensor(2.0)), ua)
-        ua = torch.where(step <= -i, torch.nextafter(ua, torch.tensor(0.0)), ua)
-    return x.to(DEV), d.to(DEV), ua.to(DEV), torch.rand(B, generator=g).to(DEV), q.to(DEV)
+        ua = torch.where(step >= i, torch.nextafter(ua, torch.full_like(ua, 2.0)), ua)
+        ua = torch.where(step <= -i, torch.nextafter(ua, torch.zeros_like(ua)), ua)
+    return x, d, ua, torch.rand(B, **at), q
 
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("near", [0.0, 1e-6, 1e-7])
-@pytest.mark.parametrize("B,K,V,only", [(6, 3, 3000, None), (700, 3, 300, 60), (120, 2, 50001, 12)])
+@pytest.mark.parametrize("B,K,V,only", [(6, 3, 3000, None), (700, 3, 300, 60), (230, 2, 50001, 12), (12000, 3, 800, 100)])
 def test_verify_at_the_borders(B, K, V, only, near, dtype):
     # small and large batches take different sums; both decide as 64 bits do
     x, d, ua, u, q = borders(B, K, V, dtype, V + B, near)
@@ -361,8 +371,8 @@ def test_verify_at_the_borders(B, K, V, only, near, dtype):
 
 def test_verify_large_masked():
     # what test_verify_masked, _greedy_rows and _nothing_left hold, in a large batch
-    B, K, V = 600, 3, 900
-    x, d, ua, u, q = drafts_of(B, K, V, torch.float32, 16)
+    B, K, V = 600, 3, 14001
+    x, d, ua, u, q = many_drafts(B, K, V, torch.float32, 16)
     x[0, 0] = -math.inf
     x[1, :, ::2] = -math.inf
     x[2, 1, d[2, 1]] = -math.inf
