@@ -255,13 +255,15 @@ template <int SRC, bool MASS>
 __global__ void __launch_bounds__(kSampleThreads)
     sample_collect_kernel(SampleRows r, int ns, int blocks, CutPlan* plans, u64* lists, int most,
                           double* mass) {
-  const int slot = blockIdx.x / blocks, seg = (blockIdx.x % blocks) * 4 + (threadIdx.x >> 6);
+  __shared__ int wave_hits[kSampleThreads / kWave], base;
+  const int wave = threadIdx.x >> 6, slot = blockIdx.x / blocks, seg = (blockIdx.x % blocks) * 4 + wave;
   const int b = slot / (r.K + 1), i = slot % (r.K + 1);
-  if (seg >= ns || i >= r.count(b)) return;
+  if (i >= r.count(b)) return;
   CutPlan& plan = plans[slot];
   constexpr int kVec = Logit<SRC>::kVec;
+  const auto* row = row_at<SRC>(r, r.first(b) + i);
   float x[kSamplePer];
-  load_segment<SRC>(row_at<SRC>(r, r.first(b) + i), seg, r.V, x);
+  load_segment<SRC>(row, seg, r.V, x);
   if (!plan.filters) return;
   const Scale scale = make_scale(plan.top, r.temp(b));
   const float bins = bin_scale(scale);
@@ -275,17 +277,28 @@ __global__ void __launch_bounds__(kSampleThreads)
   }
   const int mine = __popc(hits);
   const int up_to = wave_prefix(mine), all = lane_value(up_to, 63);
+  // (One addition to the row's counter for a workgroup: with one for each
+  // wavefront 76 of a row waited for each other.)
+  if ((threadIdx.x & 63) == 0) wave_hits[wave] = all;
+  __syncthreads();
+  int at = up_to - mine, block = 0;
+  for (int v = 0; v < kSampleThreads / kWave; ++v) {
+    if (v < wave) at += wave_hits[v];
+    block += wave_hits[v];
+  }
+  if (block != 0) {  // (the same for every thread)
+    if (threadIdx.x == 0) base = atomicAdd(&plan.listed, block);
+    __syncthreads();
+  }
   if (all != 0) {
-    int at = 0;
-    if ((threadIdx.x & 63) == 0) at = atomicAdd(&plan.listed, all);
-    at = lane_value(at, 0) + up_to - mine;
+    at += base;
     u64* list = lists + (long long)slot * most;
-#pragma unroll
-    for (int e = 0; e < kSamplePer; ++e) {
-      if (hits & (1u << e)) {
-        if (at < most) list[at] = order_value(x[e], segment_element<SRC>(seg, e / kVec) + e % kVec);
-        ++at;
-      }
+    // (A lane has three at most, mostly: their logits are read again, since
+    // registers have no index.)
+#pragma unroll 1
+    for (; hits; hits &= hits - 1, ++at) {
+      const int bit = __ffs(hits) - 1, e = segment_element<SRC>(seg, bit / kVec) + bit % kVec;
+      if (at < most) list[at] = order_value(Logit<SRC>::value(row[e]), e);
     }
   }
   if constexpr (!MASS) return;
@@ -307,7 +320,7 @@ __global__ void __launch_bounds__(kSampleThreads)
     for (int j = 0; j < 8; ++j) s += in[j] ? w[j] : 0.0;
   }
   s = wave_sum(s);
-  if ((threadIdx.x & 63) == 0) mass[(long long)slot * ns + seg] = s;
+  if ((threadIdx.x & 63) == 0 && seg < ns) mass[(long long)slot * ns + seg] = s;
 }
 
 // One workgroup per row: the borders, and where tokens are asked for the draw.
