@@ -313,7 +313,7 @@ def chunk_tables(
         for n in sizes:
             ptrs.append(at)
             at += 4 * n
-        table, ctx, cu, pos, page, slot, seq = parts.split(sizes)
+        table, ctx, cu, pos, page, slot, seq = parts.split_with_sizes(sizes)
         out = ChunkTables(table.view(B, max_pp), ctx, cu, pos, page, slot, seq)
     else:
         for name, shape in (("page_table", (B, max_pp)), ("context_lens", (B,)), ("cu_seqlens", (B + 1,)),
