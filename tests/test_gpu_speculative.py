@@ -210,6 +210,26 @@ def test_keep_chunk_refusals():
         mgr.keep_chunk(chunk, [4])
 
 
+def test_keep_chunk_after_a_reservation():
+    """Pages that reserve gave out behind a chunk's stay the request's."""
+    mgr = _manager()
+    mgr.allocate("a"), mgr.allocate("b")
+    chunk = mgr.append_chunk(["a", "b"], [9, 3])
+    table, past = mgr.reserve(["a"], [20])
+    assert past.tolist() == [9] and table.tolist() == [mgr._page_tables["a"].pages]
+    before = _state(mgr)
+    for call in (lambda: mgr.keep_chunk(chunk, [1, 3]), lambda: mgr._take_back(chunk)):
+        with pytest.raises(RuntimeError, match="has changed"):
+            call()
+        assert _state(mgr) == before
+    mgr.keep_chunk(chunk, [9, 3])  # (takes nothing back)
+    assert _state(mgr) == before
+    held = list(mgr._page_tables["a"].pages)
+    chunk = mgr.append_chunk(["a"], [9])  # into reserved pages: none of its own to give back
+    mgr.keep_chunk(chunk, [2])
+    assert mgr._page_tables["a"].pages == held and list(mgr.token_counts(["a"])) == [11]
+
+
 def test_reserve_and_commit():
     mgr = _manager(max_pages=10)
     for rid, n in (("a", 5), ("b", 16)):

@@ -454,9 +454,13 @@ class PagedKVCacheManager:
             self._check_states_locked(chunk, what)
             chunk.epoch = self._epoch
 
-    def _check_states_locked(self, chunk: ChunkBatch, what: str) -> None:
-        for rid, (entry, n, _) in zip(chunk.request_ids, chunk.states):
-            if self._page_tables.get(rid) is not entry or entry.num_tokens != n:
+    def _check_states_locked(self, chunk: ChunkBatch, what: str, pages: bool = False) -> None:
+        # With ``pages``, for callers that take the batch's last pages back: they
+        # are not the last ones any more where ``reserve`` has added some.
+        PS = self.config.page_size
+        for rid, (entry, n, added) in zip(chunk.request_ids, chunk.states):
+            if (self._page_tables.get(rid) is not entry or entry.num_tokens != n
+                    or (pages and added and len(entry.pages) != -(-n // PS))):
                 raise RuntimeError(f"{what}: request {rid!r} has changed since append_chunk made this batch")
 
     def _take_back(self, chunk: ChunkBatch) -> None:
@@ -467,7 +471,7 @@ class PagedKVCacheManager:
         what they raised it to.  Raises, and changes nothing, where a request
         has changed since."""
         with self._lock:
-            self._check_states_locked(chunk, "_take_back")
+            self._check_states_locked(chunk, "_take_back", pages=True)
             for (entry, n, added), count in reversed(list(zip(chunk.states, chunk.counts))):
                 entry.num_tokens = n - count
                 for _ in range(added):
@@ -495,7 +499,7 @@ class PagedKVCacheManager:
             return
         PS = self.config.page_size
         with self._lock:
-            self._check_states_locked(chunk, "keep_chunk")
+            self._check_states_locked(chunk, "keep_chunk", pages=True)
             for (entry, n, added), had, kept in reversed(list(zip(chunk.states, chunk.counts, counts))):
                 entry.num_tokens = n - had + kept
                 for _ in range(added):
