@@ -733,7 +733,7 @@ int vrm_rope_append(const void* query, long long q_token_stride, long long q_hea
  * block_table is [R] rows of W int32, row_stride elements apart.  A request
  * outside [0, R) has no tokens and no pages.  A request may stand in several
  * sequences; their new tokens then have the same places.  Outputs must not
- * overlap inputs.
+ * overlap inputs (VRM_ERR_ARG).
  */
 int vrm_chunk_tables(const int32_t* block_table, long long row_stride, int R, int W,
                      const int32_t* past_lens, const int32_t* counts, const int32_t* requests,
@@ -761,8 +761,9 @@ int vrm_chunk_tables(const int32_t* block_table, long long row_stride, int R, in
  * to 2.2e-12 of themselves, or decided as with those (under top_k and top_p a
  * border is found in sums of weights rounded to multiples of 2^-S of the
  * largest, S = min(45, 62 - ceil(log2 V)); tokens below 2^-50 of the largest may
- * count for nothing there).  Results are the same from call to call.  The workspace is 16-byte aligned and
- * written before it is read.
+ * count for nothing there).  Results are the same from call to call.  The
+ * workspace is 16-byte aligned and written before it is read.  Outputs and the
+ * workspace must not overlap inputs (VRM_ERR_ARG).
  * -------------------------------------------------------------------------- */
 #define VRM_SAMPLE_MAX_V (1 << 24)
 

@@ -70,6 +70,37 @@ def test_tables_refusals(lib, bad, rc, text):
     assert _tables(lib, **bad) == rc and text in lib.vrm_last_error()
 
 
+_MB = 1 << 20  # (distinct places for every argument of a call that never runs)
+
+
+@pytest.mark.parametrize("over", [
+    dict(probs=_MB), dict(probs=_MB + 15996), dict(probs=_MB - 12), dict(tokens=_MB + 8), dict(tokens=2 * _MB),
+    dict(tokens=3 * _MB - 16, t=3 * _MB), dict(tokens=3 * _MB, k=3 * _MB), dict(probs=3 * _MB, p=3 * _MB + 8),
+    dict(ws=_MB + 1024), dict(ws=2 * _MB)])
+def test_sample_outputs_on_inputs(lib, over):
+    a = dict(logits=_MB, u=2 * _MB, tokens=5 * _MB, ws=6 * _MB, wsb=_MB)
+    assert _sample(lib, **{**a, **over}) == -1 and b"overlap" in lib.vrm_last_error()
+
+
+@pytest.mark.parametrize("over", [
+    dict(tokens=2 * _MB), dict(tokens=2 * _MB - 8), dict(tokens=_MB), dict(tokens=3 * _MB + 23996), dict(tokens=4 * _MB),
+    dict(accepted=5 * _MB + 4), dict(accepted=9 * _MB + 8, cu=9 * _MB), dict(accepted=9 * _MB, t=9 * _MB + 4),
+    dict(accepted=9 * _MB, k=9 * _MB), dict(accepted=9 * _MB, p=9 * _MB), dict(ws=2 * _MB)])
+def test_verify_outputs_on_inputs(lib, over):
+    a = dict(logits=_MB, drafts=2 * _MB, q=3 * _MB, ua=4 * _MB, u=5 * _MB, tokens=6 * _MB, accepted=7 * _MB, ws=8 * _MB,
+             wsb=_MB)
+    assert _verify(lib, **{**a, **over}) == -1 and b"overlap" in lib.vrm_last_error()
+
+
+@pytest.mark.parametrize("over", [
+    dict(cl=2 * _MB), dict(cl=2 * _MB - 4), dict(pt=_MB), dict(pt=_MB + 124), dict(cu=3 * _MB), dict(pos=2 * _MB + 12),
+    dict(page=4 * _MB + 4), dict(slot=3 * _MB + 4), dict(seq=4 * _MB - 16)])
+def test_tables_outputs_on_inputs(lib, over):
+    a = dict(table=_MB, past=2 * _MB, counts=3 * _MB, requests=4 * _MB, pt=5 * _MB, cl=6 * _MB, cu=7 * _MB, pos=8 * _MB,
+             page=9 * _MB, slot=10 * _MB, seq=11 * _MB)
+    assert _tables(lib, **{**a, **over}) == -1 and b"overlap" in lib.vrm_last_error()
+
+
 def test_nothing_to_do(lib):
     assert _sample(lib, N=0, logits=None, tokens=None, u=None, ws=None) == 0
     assert _verify(lib, B=0, N=0, logits=None, tokens=None, u=None, ws=None) == 0

@@ -347,6 +347,20 @@ extern "C" int vrm_chunk_tables(const int32_t* block_table, long long row_stride
     set_error("%s: %d rows of %d pages and %d tokens are too many for one call", who, B, max_pp, N);
     return VRM_ERR_UNSUPPORTED;
   }
+  const size_t seqs = B, rows = N;
+  if (int rc = check_apart({{page_table, seqs * max_pp * 4},
+                            {context_lens, seqs * 4},
+                            {cu_seqlens, (seqs + 1) * 4},
+                            {positions, rows * 4},
+                            {page_ids, rows * 4},
+                            {slots, rows * 4},
+                            {sequences, rows * 4}},
+                           {{block_table, R > 0 && W > 0 ? (size_t)((R - 1) * row_stride + W) * 4 : 0},
+                            {past_lens, (size_t)R * 4},
+                            {counts, seqs * 4},
+                            {requests, seqs * 4}},
+                           who))
+    return rc;
   const ChunkTableArgs a{block_table, row_stride, R, W, past_lens, counts, requests, B, N, PS, page_table, max_pp,
                          context_lens, cu_seqlens, positions, page_ids, slots, sequences};
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);

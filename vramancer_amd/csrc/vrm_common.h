@@ -16,6 +16,28 @@ void clear_error();
 // Converts the launch status of the last kernel into the ABI status.
 int launch_status(const char* what);
 
+// Bytes of an argument.
+struct Span {
+  const void* at;
+  size_t bytes;
+};
+
+// VRM_ERR_ARG with a message where an output lies on an input: kernels that
+// read an input after another workgroup has written there would answer by luck.
+template <size_t OUTS, size_t INS>
+inline int check_apart(const Span (&outs)[OUTS], const Span (&ins)[INS], const char* who) {
+  for (const Span& o : outs) {
+    for (const Span& i : ins) {
+      const auto a = reinterpret_cast<uintptr_t>(o.at), b = reinterpret_cast<uintptr_t>(i.at);
+      if (a && b && o.bytes && i.bytes && a < b + i.bytes && b < a + o.bytes) {
+        set_error("%s: outputs must not overlap inputs", who);
+        return VRM_ERR_ARG;
+      }
+    }
+  }
+  return VRM_OK;
+}
+
 constexpr int kWave = 64;
 
 // Butterfly exchange across lanes lane ^ mask of a 64-wide wavefront, on the

@@ -687,6 +687,11 @@ int check_workspace(const void* ws, size_t bytes, size_t need, const char* who) 
   return VRM_OK;
 }
 
+// Bytes of n rows of V elements, stride elements apart.
+size_t row_bytes(long long n, int V, long long stride, int dtype) {
+  return n > 0 ? (size_t)((n - 1) * stride + V) * (dtype == VRM_SRC_F32 ? 4 : 2) : 0;
+}
+
 // Whether any row may lose tokens to top_k or top_p.
 bool filters(const int32_t* top_k, int top_k_all, const float* top_p, float top_p_all, int V) {
   return top_k || (top_k_all > 0 && top_k_all < V) || top_p || top_p_all < 1.0f;
@@ -718,6 +723,15 @@ extern "C" int vrm_sample_tokens(const void* logits, int dtype, long long row_st
   }
   const Plan p = plan_of(N, 0, V, filters(top_k, top_k_all, top_p, top_p_all, V), false, probs != nullptr);
   if (int rc = check_workspace(workspace, workspace_bytes, p.bytes, who)) return rc;
+  const size_t n = N;
+  if (int rc = check_apart({{tokens, n * 8}, {probs, n * V * 4}, {workspace, p.bytes}},
+                           {{logits, row_bytes(N, V, row_stride, dtype)},
+                            {uniforms, n * 4},
+                            {temperature, n * 4},
+                            {top_k, n * 4},
+                            {top_p, n * 4}},
+                           who))
+    return rc;
   const SampleRows r{logits, row_stride, nullptr, N, N, 0, V, temperature, temperature_all, top_k, top_k_all, top_p,
                      top_p_all};
   return run_typed(r, dtype, Drafts{}, p, static_cast<char*>(workspace), uniforms, probs,
@@ -760,6 +774,20 @@ extern "C" int vrm_verify_drafts(const void* logits, int dtype, long long row_st
   }
   const Plan p = plan_of(B, K, V, filters(top_k, top_k_all, top_p, top_p_all, V), true, false);
   if (int rc = check_workspace(workspace, workspace_bytes, p.bytes, who)) return rc;
+  const size_t n = B, k = K;
+  const size_t last_draft = K > 0 ? (n - 1) * probs_seq_stride + (k - 1) * probs_draft_stride + V : 0;
+  if (int rc = check_apart({{tokens, n * (k + 1) * 8}, {accepted, n * 4}, {workspace, p.bytes}},
+                           {{logits, row_bytes(N, V, row_stride, dtype)},
+                            {cu_seqlens, (n + 1) * 4},
+                            {drafts, n * k * draft_bytes},
+                            {draft_probs, last_draft * 4},
+                            {accept_uniforms, n * k * 4},
+                            {draw_uniforms, n * 4},
+                            {temperature, n * 4},
+                            {top_k, n * 4},
+                            {top_p, n * 4}},
+                           who))
+    return rc;
   const SampleRows r{logits, row_stride, cu_seqlens, N, B, K, V, temperature, temperature_all, top_k, top_k_all, top_p,
                      top_p_all};
   const Drafts d{drafts, draft_bytes, draft_probs, probs_seq_stride, probs_draft_stride, accept_uniforms};

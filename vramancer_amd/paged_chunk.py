@@ -288,7 +288,9 @@ def chunk_tables(
     sequence.  ``max_pages`` (default W) is the page table's width; a row holds
     the pages up to its last token's, -1 behind them.  A request outside
     [0, R) and a negative count have no tokens.  ``out`` takes the tensors of
-    an earlier call of the same sizes, for a captured graph that reads them."""
+    an earlier call of the same sizes, for a captured graph that reads them;
+    none of them may be an input too (lengths move on in a tensor of their own,
+    not from ``context_lens`` of one call into the next one's ``out``)."""
     if block_table.dim() != 2 or block_table.dtype != torch.int32:
         raise RuntimeError(f"block_table must be int32 [R, W], got {block_table.dtype} {tuple(block_table.shape)}")
     R, W = block_table.shape

@@ -19,7 +19,8 @@ tokens that cannot be drawn; a row of nothing else gives token -1.
 
 ``temperature``, ``top_k`` and ``top_p`` are a number for all sequences or a
 tensor [B] with one for each (k <= 0, p >= 1: all tokens); temperatures and
-top_p are taken as float32.  No call reads a tensor back.
+top_p are taken as float32.  No call reads a tensor back.  An output that lies
+on an input's memory is refused.
 """
 from __future__ import annotations
 
