@@ -159,6 +159,17 @@ def test_crowded_bins(V):
         check(x, u, **kw)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("kw", [dict(top_k=9000), dict(top_p=0.45), dict(top_k=25000, top_p=0.8)])
+def test_ties_of_both_signs(kw, dtype):
+    # few values on both sides of 0, close together and far apart, in lists that
+    # fit and that do not
+    g = torch.Generator().manual_seed(3)
+    x = torch.randint(-3, 4, (4, 30001), generator=g).float()
+    x = (x * torch.tensor([2.0 ** -12, 2.0 ** -5, 0.125, 1.0])[:, None]).to(dtype).to(DEV)
+    check(x, torch.tensor([0.2, 0.45, 0.7, 0.95], device=DEV), **kw)
+
+
 def test_no_rows_and_out():
     x, u = make(4, 100, torch.float32, 9)
     assert sampling.sample_tokens(x[:0], u[:0]).shape == (0,)

@@ -175,19 +175,19 @@ struct Logit;  // element type of a row
 template <>
 struct Logit<VRM_SRC_F32> {
   using Raw = uint32_t;
-  static constexpr int kVec = 4;
+  static constexpr int kVec = 4, kZeros = 0;  // (last bits that are 0 in every value as float32)
   static __device__ __forceinline__ float value(uint32_t u) { return __uint_as_float(u); }
 };
 template <>
 struct Logit<VRM_SRC_F16> {
   using Raw = uint16_t;
-  static constexpr int kVec = 8;
+  static constexpr int kVec = 8, kZeros = 13;
   static __device__ __forceinline__ float value(uint16_t u) { return f16_bits_to_f32(u); }
 };
 template <>
 struct Logit<VRM_SRC_BF16> {
   using Raw = uint16_t;
-  static constexpr int kVec = 8;
+  static constexpr int kVec = 8, kZeros = 16;
   static __device__ __forceinline__ float value(uint16_t u) { return bf16_bits_to_f32(u); }
 };
 

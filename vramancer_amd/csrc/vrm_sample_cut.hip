@@ -37,7 +37,7 @@ constexpr int kCutThreads = 512;  // = kBins
 constexpr int kCutWaves = kCutThreads / kWave;
 constexpr int kSubBits = 10;
 constexpr int kSub = 1 << kSubBits;  // steps of order values: two a thread
-constexpr int kFew = 64;             // tokens that are compared with each other
+constexpr int kFew = 64;            // tokens that are compared with each other
 constexpr int kPartsAhead = 24;
 static_assert(kSub >= kDrawSegments, "a sum for each segment");
 
@@ -323,15 +323,42 @@ __global__ void __launch_bounds__(kSampleThreads)
   if ((threadIdx.x & 63) == 0 && seg < ns) mass[(long long)slot * ns + seg] = s;
 }
 
-// One workgroup per row: the borders, and where tokens are asked for the draw.
+// Order values without the bits that are the same for all of a row: the zeros
+// that end 16-bit logits as float32 and the ones above an index of V.  Ten bits
+// of the distance between two of them then tell equal logits apart by index:
+// 775 bf16 logits of a bin are down to 64 in one step of the narrowing, where
+// plain order values took two (the kernel 18.2 us for 64 rows of 152000, 15.4 with
+// this and the weights worked out once).
 template <int SRC>
-__global__ void __launch_bounds__(kCutThreads)
+struct Packed {
+  static constexpr int kZeros = Logit<SRC>::kZeros;
+  int index_bits;
+  uint32_t mask;
+
+  __device__ __forceinline__ explicit Packed(int V) : index_bits(32 - __clz(V)), mask((1u << index_bits) - 1) {}
+  __device__ __forceinline__ int bits() const { return 32 - kZeros + index_bits; }
+  __device__ __forceinline__ u64 pack(u64 order) const {
+    return (order >> (32 + kZeros)) << index_bits | ((uint32_t)order & mask);
+  }
+  __device__ __forceinline__ u64 order(u64 p) const {
+    uint32_t key = (uint32_t)(p >> index_bits) << kZeros;
+    if (!(key & 0x80000000u)) key |= (1u << kZeros) - 1;  // (of negative logits the bits are inverted)
+    return (u64)key << 32 | ((uint32_t)p & mask) | (uint32_t)~mask;
+  }
+  __device__ __forceinline__ float logit(u64 p) const { return order_logit(order(p)); }
+  __device__ __forceinline__ int index(u64 p) const { return (int)(~(uint32_t)p & mask); }
+};
+
+// One workgroup per row: the borders, and where tokens are asked for the draw.
+// (128 registers, so that a compute unit has two rows.)
+template <int SRC>
+__global__ void __launch_bounds__(kCutThreads, 4)
     sample_border_kernel(SampleRows r, int ns, int bits, const SegRec* rec, const CutPlan* plans, const u64* lists,
                          int most, RowCut* cuts, DrawRec* draws, double* mass, const float* uniforms, long long* tokens) {
-  __shared__ u64 list[kListed];  // order values
+  __shared__ u64 list[kListed], weight[kListed];  // packed order values, weights as integers
   __shared__ u64 sub_sum[kSub];
   __shared__ uint32_t sub_count[kSub];
-  __shared__ u64 few[kFew], few_weight[kFew];
+  __shared__ ulonglong2 few[kFew];  // (order, weight)
   __shared__ u64 wave_fixed[kCutWaves], wave_low[kCutWaves], wave_high[kCutWaves];
   __shared__ uint32_t wave_count[kCutWaves];
   __shared__ u64 s_before_fixed, s_border;
@@ -346,7 +373,8 @@ __global__ void __launch_bounds__(kCutThreads)
   const float u = tokens ? uniforms[b] : 0.0f;
   // (under way with the plan; what is not listed is not used)
   const u64 ahead = t < most ? lists[(long long)slot * most + t] : 0;
-  u64 cut = 0;
+  const Packed<SRC> packed(r.V);
+  u64 border = 0;  // packed; 0: no cut
   double kept = plan.kept;
   bool fits = true, of_p = false;  // whether the cut is top_p's
   int listed = 0;
@@ -357,11 +385,14 @@ __global__ void __launch_bounds__(kCutThreads)
     const Scale scale = make_scale(plan.top, r.temp(b));
     const float bins = bin_scale(scale);
     const double unit = (double)(1ULL << bits);
-    const auto weight_of = [&](u64 o) { return fixed_weight(sample_weight(order_logit(o), scale), unit); };
+    const auto put = [&](int at, u64 order) {
+      list[at] = packed.pack(order);
+      weight[at] = fixed_weight(sample_weight(order_logit(order), scale), unit);
+    };
     fits = plan.listed <= most;
     listed = fits ? plan.listed : 0;
-    if (t < listed) list[t] = ahead;
-    for (int j = t + kCutThreads; j < listed; j += kCutThreads) list[j] = lists[(long long)slot * most + j];
+    if (t < listed) put(t, ahead);
+    for (int j = t + kCutThreads; j < listed; j += kCutThreads) put(j, lists[(long long)slot * most + j]);
     kept = plan.total;
 #pragma unroll 1
     for (int turn = 0; turn < 2; ++turn) {
@@ -373,7 +404,7 @@ __global__ void __launch_bounds__(kCutThreads)
       const double before = by_count ? plan.k_before : plan.p_before;
       const double goal = fmin(fmax((double)r.nucleus(b) * kept, 0x1p-200), kept);
       uint32_t before_count = by_count ? plan.k_count : 0;
-      u64 low = 0, high = ~0ULL, fixed_goal = 0, before_fixed = 0;
+      u64 low = 0, high = (1ULL << packed.bits()) - 1, fixed_goal = 0, before_fixed = 0;
       bool have_goal = by_count, lost = false;
 
       // The part of the goal that is among these tokens, at most what their
@@ -425,7 +456,7 @@ __global__ void __launch_bounds__(kCutThreads)
         // The list does not hold these bins' tokens (logits that lie closer
         // together than a bin is wide): passes over the row narrow their order
         // values by 10 bits each until what is left fits it.
-        int shift = 64 - kSubBits;
+        int shift = max(0, packed.bits() - kSubBits);
 #pragma unroll 1
         while (true) {
           __syncthreads();
@@ -439,13 +470,13 @@ __global__ void __launch_bounds__(kCutThreads)
           for (int e = t; e < V; e += kCutThreads) {
             const float l = L::value(row[e]);
             if (!range.holds(l * bins) || !(l > -INFINITY)) continue;
-            const u64 o = order_value(l, e);
+            const u64 order = order_value(l, e), o = packed.pack(order);
             if (o < low || o > high) continue;
             if (shift < 0) {
-              list[atomicAdd(&s_fill, 1)] = o;  // (there are as many as the last pass counted)
+              put(atomicAdd(&s_fill, 1), order);  // (there are as many as the last pass counted)
             } else {
               atomicAdd(&sub_count[(high - o) >> shift], 1u);
-              atomicAdd(&sub_sum[(high - o) >> shift], weight_of(o));
+              atomicAdd(&sub_sum[(high - o) >> shift], fixed_weight(sample_weight(l, scale), unit));
             }
           }
           __syncthreads();
@@ -457,19 +488,20 @@ __global__ void __launch_bounds__(kCutThreads)
         listed = lost ? 0 : s_fill;
       }
 
-      // Narrow the listed tokens of the bins that are within low .. high.
+      // Narrow the listed tokens of the bins that are within low .. high.  (A
+      // bin's tokens are an interval of order values: the first look finds it.)
       uint32_t n;
 #pragma unroll 1
-      while (true) {
+      for (bool first_look = true;; first_look = false) {
         __syncthreads();
         // How many there are, what they weigh, and the interval that they take.
         u64 a = ~0ULL, z = 0, sum = 0;
         uint32_t count = 0;
         for (int j = t; j < listed; j += kCutThreads) {
           const u64 o = list[j];
-          if (o >= low && o <= high && range.holds(order_logit(o) * bins)) {
+          if (o >= low && o <= high && (!first_look || range.holds(packed.logit(o) * bins))) {
             ++count;
-            if (!have_goal) sum += weight_of(o);
+            if (!have_goal) sum += weight[j];
             a = min(a, o);
             z = max(z, o);
           }
@@ -488,6 +520,7 @@ __global__ void __launch_bounds__(kCutThreads)
           sub_count[j] = 0;
           sub_sum[j] = 0;
         }
+        if (t < kFew) few[t] = make_ulonglong2(0, 0);
         if (t == 0) s_fill = 0;
         __syncthreads();
         n = 0;
@@ -499,54 +532,73 @@ __global__ void __launch_bounds__(kCutThreads)
           z = max(z, wave_high[v]);
         }
         if (!have_goal) set_goal(sum);
-        if (n <= (uint32_t)kFew || lost) break;
         low = a;
         high = z;
+        if (n <= (uint32_t)kFew || lost) break;
         const int shift = max(0, 64 - __clzll(high - low) - kSubBits);  // (high - low) >> shift is below kSub
         for (int j = t; j < listed; j += kCutThreads) {
           const u64 o = list[j];
-          if (o >= low && o <= high && range.holds(order_logit(o) * bins)) {
+          if (o >= low && o <= high) {
             atomicAdd(&sub_count[(high - o) >> shift], 1u);
-            atomicAdd(&sub_sum[(high - o) >> shift], weight_of(o));
+            atomicAdd(&sub_sum[(high - o) >> shift], weight[j]);
           }
         }
         __syncthreads();
         narrow(shift);
       }
       if (lost || n == 0) continue;  // (the same for every thread)
-      // The few that are left, each against the others.
+      // The few that are left, each against the others: a thread has one and a
+      // part of the others.  (One wavefront with all of them took 3.8 us for 50;
+      // 128 instead of 64 take 1 us longer where they are not needed and save as
+      // much where they are.)
       for (int j = t; j < listed; j += kCutThreads) {
         const u64 o = list[j];
-        if (o >= low && o <= high && range.holds(order_logit(o) * bins)) {
+        if (o >= low && o <= high) {
           const int f = atomicAdd(&s_fill, 1);
-          few[f] = o;
-          few_weight[f] = weight_of(o);
+          few[f] = make_ulonglong2(o, weight[j]);
+        }
+      }
+      __syncthreads();
+      constexpr int kEach = kFew * kFew / kCutThreads;
+      const int mine = t % kFew, others = t / kFew * kEach;
+      if (others < (int)n) {
+        const u64 o = few[mine].x;
+        uint32_t c = 0;
+        u64 w = 0;
+#pragma unroll 1
+        for (int j = 0; j < kEach; j += 8) {
+          ulonglong2 other[8];  // (0 behind the last one)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) other[e] = few[others + j + e];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            c += other[e].x > o ? 1 : 0;
+            w += other[e].x > o ? other[e].y : 0;
+          }
+        }
+        if (c != 0) {
+          atomicAdd(&sub_count[mine], c);
+          atomicAdd(&sub_sum[mine], w);
         }
       }
       __syncthreads();
       if (t < (int)n) {
-        const u64 o = few[t], w = few_weight[t];
-        uint32_t c = before_count;
-        u64 up_to = before_fixed;
-        for (uint32_t j = 0; j < n; ++j) {
-          if (few[j] > o) {
-            ++c;
-            up_to += few_weight[j];
-          }
-        }
+        const uint32_t c = before_count + sub_count[t];
+        const u64 up_to = before_fixed + sub_sum[t], w = few[t].y;
         if (by_count ? c + 1 == k : up_to < fixed_goal && up_to + w >= fixed_goal) {  // (one of them)
-          s_border = o;
+          s_border = few[t].x;
           s_before_fixed = up_to + w;
         }
       }
       __syncthreads();
-      cut = s_border;
+      border = s_border;
       of_p = !by_count;
       kept = before + (double)s_before_fixed / unit;
       __syncthreads();
     }
-    if (cut == 0) kept = plan.kept;
+    if (border == 0) kept = plan.kept;
   }
+  const u64 cut = border ? packed.order(border) : 0;
   DrawRec w{};
   w.sum = kept;
   w.cut = cut;
@@ -580,9 +632,8 @@ __global__ void __launch_bounds__(kCutThreads)
     const float bins = bin_scale(scale);
     for (int j = t; j < listed; j += kCutThreads) {
       const u64 o = list[j];
-      const float l = order_logit(o);
-      if (o >= cut && (plan.all_listed || range.holds(l * bins)))
-        atomicAdd(&sub_sum[(uint32_t)~o / kSegment], fixed_weight(sample_weight(l, scale), unit));
+      if (o >= border && (plan.all_listed || range.holds(packed.logit(o) * bins)))
+        atomicAdd(&sub_sum[packed.index(o) / kSegment], weight[j]);
     }
   } else if (cut != 0) {
     for (int seg = wave; seg < ns; seg += kCutWaves) {
