@@ -213,95 +213,119 @@ struct Drafts {
   }
 };
 
+// What a row's segments and cut say about it.
+struct RowSum {
+  double sum;
+  unsigned long long cut;
+  float top;
+  int arg;
+  int id;  // its draft, -1: none, or outside the vocabulary
+};
+constexpr int kHeldRows = 16;  // rows of a sequence whose sums are held for the draw
+
+// A row's, by one wavefront.
+__device__ __forceinline__ RowSum row_sum(const SegRec* rec, const RowCut* cuts, long long slot, int ns, float t,
+                                          Scale& scale) {
+  RowSum g;
+  combine_segments(rec + slot * ns, ns, t, g.top, g.arg, scale, g.sum);
+  g.cut = 0;
+  g.id = -1;
+  if (cuts && g.arg == -2) {
+    g.cut = cuts[slot].cut;
+    g.sum = cuts[slot].sum;
+  }
+  return g;
+}
+
 // The drafts that sequence b accepts and its draw, for every thread of the
 // workgroup.  Answers (tokens, accepted, draws) are written by the workgroup
-// that has `writes`.  With ROUGH sums are within kRough: a test that lies
-// within that of its border is made again with the exact sum (one in 10^5), and
-// the draw's sum is the rough one.
-template <int SRC, bool ROUGH>
+// that has `writes`.  Every row is summed with the drafts' tests, also the one
+// behind the last draft, so that the draw waits for nothing more.  With ROUGH
+// sums are within kRough: a test that lies within that of its border is made
+// again with the exact sum (one in 10^5), and the draw's sum is a rough one.
+template <int SRC, bool ROUGH, int THREADS>
 __device__ __forceinline__ DrawRec choose(const SampleRows& r, const Drafts& d, int ns, const SegRec* rec,
                                           const RowCut* cuts, int b, bool writes, DrawRec* draws, long long* tokens,
                                           int32_t* accepted, Scale& scale) {
   __shared__ int stop;  // the first row whose draft is refused, or the last row
-  __shared__ DrawRec draw;
+  __shared__ RowSum held[kHeldRows];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int n = r.count(b), first = r.first(b);
   if (threadIdx.x == 0) stop = n - 1;
   __syncthreads();
   const float t = r.temp(b);
-  for (int i = wave; i < n - 1; i += kSampleThreads / kWave) {
+  for (int i = wave; i < n; i += THREADS / kWave) {
+    if (i == n - 1 && i >= kHeldRows) break;
     const long long slot = (long long)b * (r.K + 1) + i, at = (long long)b * r.K + i;
-    const long long x = d.id(at);
+    const bool draft = i < n - 1;
+    const long long x = draft ? d.id(at) : -1;
     const bool known = x >= 0 && x < r.V;
-    const float u = fmaxf(d.accept[at], 0.0f);
+    const float u = draft ? fmaxf(d.accept[at], 0.0f) : 0.0f;
     const float l = known ? Logit<SRC>::value(row_at<SRC>(r, first + i)[x]) : 0.0f;
     const float qx = known && d.probs ? d.probs[b * d.seq_stride + i * d.draft_stride + x] : 1.0f;
-    float top;
-    int arg;
     Scale at_row;
-    double sum;
-    combine_segments(rec + slot * ns, ns, t, top, arg, at_row, sum);
+    RowSum g = row_sum(rec, cuts, slot, ns, t, at_row);
+    if (known) g.id = (int)x;
+    if (i < kHeldRows && lane == 0) held[i] = g;
+    if (!draft) break;
     bool ok = false;
-    if (known && arg != -1) {
-      double w = x == arg ? 1.0 : 0.0;
-      if (arg == -2) {
+    if (known && g.arg != -1) {
+      double w = x == g.arg ? 1.0 : 0.0;
+      if (g.arg == -2) {
         w = sample_weight(l, at_row);
-        if (cuts) {
-          const RowCut cut = cuts[slot];
-          sum = cut.sum;
-          if (order_value(l, (int)x) < cut.cut) w = 0.0;
-        }
+        if (cuts && order_value(l, (int)x) < g.cut) w = 0.0;
       }
       const double uq = (double)u * (double)(qx < 0.0f ? 0.0f : qx);
-      if (ROUGH && arg == -2 && uq * sum * (1.0 - kRough) < w && !(uq * sum * (1.0 + kRough) < w))
-        sum = exact_sum<SRC>(row_at<SRC>(r, first + i), r.V, ns, at_row);
-      ok = uq * sum < w;
+      if (ROUGH && g.arg == -2 && uq * g.sum * (1.0 - kRough) < w && !(uq * g.sum * (1.0 + kRough) < w))
+        g.sum = exact_sum<SRC>(row_at<SRC>(r, first + i), r.V, ns, at_row);
+      ok = uq * g.sum < w;
     }
     if (!ok && lane == 0) atomicMin(&stop, i);
   }
   __syncthreads();
   const int a = max(stop, 0);
   if (writes) {
-    for (int i = threadIdx.x; i <= r.K; i += kSampleThreads)
+    for (int i = threadIdx.x; i <= r.K; i += THREADS)
       tokens[(long long)b * (r.K + 1) + i] = i < a && n > 0 ? d.id((long long)b * r.K + i) : -1;
     if (threadIdx.x == 0) accepted[b] = n > 0 ? a : 0;
   }
-  if (wave == 0) {
-    DrawRec w{};
-    w.row = -1;
-    if (n > 0) {
-      const long long slot = (long long)b * (r.K + 1) + a;
+  if (a >= kHeldRows && n > 0) {  // (the same for every thread)
+    if (wave == 0) {
       Scale at_row;
-      combine_segments(rec + slot * ns, ns, t, w.top, w.arg, at_row, w.sum);
-      w.row = first + a;
-      w.at = a;
-      w.refused = -1;
+      RowSum g = row_sum(rec, cuts, (long long)b * (r.K + 1) + a, ns, t, at_row);
       if (a < n - 1) {
         const long long x = d.id((long long)b * r.K + a);
-        if (x >= 0 && x < r.V) w.refused = (int)x;
+        if (x >= 0 && x < r.V) g.id = (int)x;
       }
-      if (cuts && w.arg == -2) {
-        w.cut = cuts[slot].cut;
-        w.sum = cuts[slot].sum;
-      }
+      if (lane == 0) held[0] = g;
     }
-    if (lane == 0) {
-      draw = w;
-      if (writes) draws[b] = w;
-    }
+    __syncthreads();
   }
-  __syncthreads();
-  const DrawRec w = draw;
-  if (w.row >= 0 && w.arg == -2) scale = make_scale(w.top, t);
+  DrawRec w{};
+  w.row = -1;
+  if (n > 0) {
+    const RowSum g = held[a < kHeldRows ? a : 0];
+    w.sum = g.sum;
+    w.cut = g.cut;
+    w.top = g.top;
+    w.row = first + a;
+    w.arg = g.arg;
+    w.refused = g.id;
+    w.at = a;
+    if (g.arg == -2) scale = make_scale(g.top, t);
+  }
+  if (writes && threadIdx.x == 0) draws[b] = w;
   return w;
 }
 
+constexpr int kChooseThreads = 512;  // (256 waited for a second row of a wavefront: 6.5 us, 5.1 now)
+
 template <int SRC, bool ROUGH>
-__global__ void __launch_bounds__(kSampleThreads)
+__global__ void __launch_bounds__(kChooseThreads)
     sample_choose_kernel(SampleRows r, Drafts d, int ns, const SegRec* rec, const RowCut* cuts, DrawRec* draws,
                          long long* tokens, int32_t* accepted) {
   Scale scale;
-  choose<SRC, ROUGH>(r, d, ns, rec, cuts, blockIdx.x, true, draws, tokens, accepted, scale);
+  choose<SRC, ROUGH, kChooseThreads>(r, d, ns, rec, cuts, blockIdx.x, true, draws, tokens, accepted, scale);
 }
 
 // ---------------------------------------------------------------------------
@@ -339,7 +363,8 @@ __global__ void __launch_bounds__(kSampleThreads)
   const int b = blockIdx.x / blocks, part = blockIdx.x % blocks, seg = part * 4 + (threadIdx.x >> 6);
   constexpr int kVec = Logit<SRC>::kVec, kGroups = kSamplePer / kVec;
   Scale scale;
-  const DrawRec w = CHOOSE ? choose<SRC, false>(r, d, ns, rec, cuts, b, part == 0, draws, tokens, accepted, scale)
+  const DrawRec w = CHOOSE ? choose<SRC, false, kSampleThreads>(r, d, ns, rec, cuts, b, part == 0, draws, tokens,
+                                                                accepted, scale)
                            : draw_of(r, draws, rec, ns, b, scale);
   if (seg >= ns) return;
   if (w.row < 0 || (w.arg != -2 && !probs)) return;
@@ -388,11 +413,13 @@ __global__ void __launch_bounds__(kSampleThreads)
 
 // The masses of a draw whose row's sum is known roughly: what max(p - q, 0) adds
 // up to is the weight of the tokens that are above q by more than the sum can
-// be off, less their q times the exact sum, which is the sum of `all`.  Segments
-// with tokens nearer to their border than that (a few in a row) are marked.
+// be off, less their q times the exact sum, which is the sum of `all`.  A token
+// nearer to its border than that (a few in a row) is kept beside them; segments
+// with more than one (near > 1) are summed again (with all of them summed again
+// the pick took 10.2 us for 160 rows of 131072, 5.6 now).
 struct RoughMass {
-  double all, above, q;
-  int near, pad;
+  double all, above, q, near_weight, near_q;
+  long long near;
 };
 
 template <int SRC>
@@ -409,6 +436,7 @@ __global__ void __launch_bounds__(kSampleThreads)
   float x[kSamplePer];
   load_segment<SRC>(row_at<SRC>(r, w.row), seg, r.V, x);
   RoughMass g{};
+  uint32_t near = 0;
 #pragma unroll
   for (int i = 0; i < kGroups; ++i) {
     const int e0 = segment_element<SRC>(seg, i);
@@ -424,7 +452,7 @@ __global__ void __launch_bounds__(kSampleThreads)
         const bool above = p[e] > qe * high;
         g.above += above ? p[e] : 0.0;
         g.q += above ? qe : 0.0;
-        if (!above && p[e] > qe * low) g.near = 1;
+        if (!above && p[e] > qe * low) near |= 1u << (i * kVec + e);
       } else {
         g.above += e0 + e == w.refused ? 0.0 : p[e];
       }
@@ -433,7 +461,19 @@ __global__ void __launch_bounds__(kSampleThreads)
   g.all = wave_sum(g.all);
   g.above = wave_sum(g.above);
   g.q = wave_sum(g.q);
-  g.near = __any(g.near) ? 1 : 0;
+  const unsigned long long some = __ballot(near != 0);
+  if (some) {
+    const int lane = __ffsll(some) - 1;
+    const uint32_t bits = lane_value(near, lane);
+    g.near = (some & (some - 1)) || (bits & (bits - 1)) ? 2 : 1;
+    if (near) {  // (read again: registers have no index)
+      const int bit = __ffs(near) - 1, at = segment_element<SRC>(seg, bit / kVec) + bit % kVec;
+      g.near_weight = sample_weight(Logit<SRC>::value(row_at<SRC>(r, w.row)[at]), scale);
+      g.near_q = q[at];
+    }
+    g.near_weight = lane_value(g.near_weight, lane);
+    g.near_q = lane_value(g.near_q, lane);
+  }
   if ((threadIdx.x & 63) == 0) mass[(long long)b * ns + seg] = g;
 }
 
@@ -466,8 +506,11 @@ __global__ void __launch_bounds__(kSampleThreads)
   for (int j0 = 0; j0 < ns; j0 += kWave) {
     const int j = j0 + lane;
     const RoughMass g = j < ns ? from[j] : RoughMass{};
-    if (wave == 0 && j < ns && !g.near) to[j] = rest ? fmax(fma(-g.q, w.sum, g.above), 0.0) : g.all;
-    unsigned long long near = __ballot(g.near != 0);
+    if (wave == 0 && j < ns && g.near <= 1) {
+      const double near = g.near ? fmax(fma(-g.near_q, w.sum, g.near_weight), 0.0) : 0.0;
+      to[j] = rest ? fmax(fma(-g.q, w.sum, g.above), 0.0) + near : g.all;
+    }
+    unsigned long long near = __ballot(g.near > 1);
     for (; near; near &= near - 1, ++turn) {
       if (turn % (kSampleThreads / kWave) != wave) continue;
       const int at = __ffsll(near) - 1;
@@ -622,8 +665,8 @@ int run(const SampleRows& r, const Drafts& d, const Plan& p, char* ws, const flo
   const dim3 mass_blocks((unsigned)((long long)r.B * p.blocks));
   if (p.rough) {
     auto* rough = reinterpret_cast<RoughMass*>(ws + p.rough_mass);
-    hipLaunchKernelGGL((sample_choose_kernel<SRC, true>), dim3(r.B), threads, 0, st, r, d, p.ns, rec, nullptr, draws,
-                       tokens, accepted);
+    hipLaunchKernelGGL((sample_choose_kernel<SRC, true>), dim3(r.B), dim3(kChooseThreads), 0, st, r, d, p.ns, rec,
+                       nullptr, draws, tokens, accepted);
     hipLaunchKernelGGL((sample_rough_mass_kernel<SRC>), mass_blocks, threads, 0, st, r, d, p.ns, p.blocks, draws, rough);
     hipLaunchKernelGGL((sample_rough_pick_kernel<SRC>), dim3(r.B), threads, 0, st, r, d, p.ns, draws, rough, mass,
                        uniforms, tokens);
@@ -634,8 +677,8 @@ int run(const SampleRows& r, const Drafts& d, const Plan& p, char* ws, const flo
                        draws, mass, nullptr, tokens, accepted);
   } else {
     if (p.drafts)
-      hipLaunchKernelGGL((sample_choose_kernel<SRC, false>), dim3(r.B), threads, 0, st, r, d, p.ns, rec, cuts, draws, tokens,
-                         accepted);
+      hipLaunchKernelGGL((sample_choose_kernel<SRC, false>), dim3(r.B), dim3(kChooseThreads), 0, st, r, d, p.ns, rec,
+                         cuts, draws, tokens, accepted);
     if (p.masses)
       hipLaunchKernelGGL((sample_mass_kernel<SRC, false>), mass_blocks, threads, 0, st, r, d, p.ns, p.blocks, rec, cuts,
                          draws, mass, probs, nullptr, nullptr);
