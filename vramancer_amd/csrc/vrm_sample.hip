@@ -70,9 +70,10 @@ __global__ void __launch_bounds__(kSampleThreads) sample_segment_kernel(SampleRo
 }
 
 // The same with the histogram of the workgroup's four segments, whose common
-// maximum gives the scale.
+// maximum gives the scale.  (Five wavefronts a SIMD, at the price of three
+// registers that spill: 64 rows of 152000 are 4.75 of them, one round.)
 template <int SRC>
-__global__ void __launch_bounds__(kSampleThreads)
+__global__ void __launch_bounds__(kSampleThreads, 5)
     sample_histogram_kernel(SampleRows r, int ns, int blocks, SegRec* rec, Histogram* hist) {
   __shared__ Histogram h;
   __shared__ float tops[4];

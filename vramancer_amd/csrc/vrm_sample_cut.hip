@@ -250,9 +250,10 @@ __global__ void __launch_bounds__(kCutThreads)
 // or V where that is less) fit.
 // With MASS, mass takes the weights of the segment's tokens above the first of
 // those bins, which stay whatever the border.  (The segment is under way before
-// the plan that says whether it is needed.)
+// the plan that says whether it is needed.  Five wavefronts a SIMD, as the
+// histograms: with four each the draw of 64 rows of 152000 took 55.2 us, 51.8 now.)
 template <int SRC, bool MASS>
-__global__ void __launch_bounds__(kSampleThreads)
+__global__ void __launch_bounds__(kSampleThreads, 5)
     sample_collect_kernel(SampleRows r, int ns, int blocks, CutPlan* plans, u64* lists, int most,
                           double* mass) {
   __shared__ int wave_hits[kSampleThreads / kWave], base;
