@@ -170,6 +170,30 @@ def test_ties_of_both_signs(kw, dtype):
     check(x, torch.tensor([0.2, 0.45, 0.7, 0.95], device=DEV), **kw)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V", [2047, 2048, 2049, 6145, 8191, 8192, 8193])
+def test_rows_around_one_part(V, dtype):
+    # lists that fit and that do not, each row with parameters of its own
+    g = torch.Generator().manual_seed(V)
+    x = torch.randn((12, V), generator=g) * 2.0
+    x[0] = 0.75
+    x[1] = -torch.finfo(dtype).max
+    x[2] = torch.randint(0, 3, (V,), generator=g) * 0.01
+    x[3] = -math.inf
+    x[4] = math.nan
+    x[4, V - 1] = -3.0
+    x[5, : V // 2] = math.inf
+    x[6, ::3] = -math.inf
+    x = x.to(dtype).to(DEV)
+    u = torch.rand(12, generator=g).to(DEV)
+    k = torch.tensor([V // 2, V - 1, 1500, 5, 5, 700, 0, 1, 1000, V, 50, 40], dtype=torch.int32)
+    p = torch.tensor([0.8, 1.0, 0.999, 0.5, 0.5, 0.3, 0.97, 0.5, 1.0, 0.9, 0.9, 1.0])
+    t = torch.tensor([1.0, 0.7, 3.0, 1.0, 1.0, 1.0, 0.5, 1.0, 2.0, 0.6, 1.5, 0.0])
+    check(x, u, temperature=t.to(DEV), top_k=k.to(DEV), top_p=p.to(DEV))
+    check(x, u, top_k=V - 1)
+    check(x, u, top_p=0.62, temperature=1.3)
+
+
 def test_no_rows_and_out():
     x, u = make(4, 100, torch.float32, 9)
     assert sampling.sample_tokens(x[:0], u[:0]).shape == (0,)

@@ -572,6 +572,64 @@ __device__ __forceinline__ bool row_filters(const SampleRows& r, int b, float t,
   return t > 0.0f && (by_k || by_p);
 }
 
+// The first place of a segment's maximum.
+template <int SRC>
+__device__ __forceinline__ int first_place(const float* x, float m, int seg) {
+  constexpr int kVec = Logit<SRC>::kVec;
+  int arg = 0x7fffffff;
+#pragma unroll
+  for (int e = kSamplePer - 1; e >= 0; --e)
+    if (x[e] == m) arg = segment_element<SRC>(seg, e / kVec) + e % kVec;
+  return wave_min(arg, 0x7fffffff);
+}
+
+// A segment's record by the maximum of its workgroup's part of a row, and in h,
+// which is clear, the histogram of the part where tokens may be dropped.
+template <int SRC>
+__device__ __forceinline__ SegRec part_sums(const float* x, int seg, float t, bool filters, bool by_k, float* tops,
+                                            Histogram& h) {
+  float m = -INFINITY;
+#pragma unroll
+  for (int e = 0; e < kSamplePer; ++e) m = fmaxf(m, x[e]);
+  m = wave_max(m, -INFINITY);
+  if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+  SegRec g{0.0, m, -1};
+  if (m > -INFINITY) {
+    if (t > 0.0f) {
+      const Scale s = make_scale(m, t);
+      const float bins = bin_scale(s);
+      const int top_bin = bin_of(m, bins);
+      constexpr double kUnit = (double)(1ULL << kBinBits);
+      float most = kBinMost;
+      asm("" : "+v"(most));  // (kept in a register: one move less for each logit)
+#pragma unroll
+      for (int e = 0; e < kSamplePer; e += 8) {
+        double w[8];
+        sample_weights<8>(x + e, s, w);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) g.sum += w[j];
+        if (filters) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int bin = top_bin - bin_of(x[e + j], bins, most);
+            const unsigned long long fixed = fixed_weight(w[j], kUnit);
+            if (fixed != 0) {  // (bin is below kBins then)
+              if (by_k) atomicAdd(&h.count[bin], 1u);
+              atomicAdd(&h.sum[bin], fixed);
+            }
+          }
+        }
+      }
+      g.sum = wave_sum(g.sum);
+    } else {
+      g.arg = first_place<SRC>(x, m, seg);
+    }
+  }
+  return g;
+}
+
 // What a row's cut looks for (vrm_sample_cut.hip).  Bins are absolute; first is
 // the one of the larger logits.
 constexpr int kListed = 4096;  // tokens that a row's list holds
@@ -595,9 +653,10 @@ struct CutPlan {
 // Finds every row's cut from the histograms of its parts (cuts; with draws,
 // sequences of one row, its draw too), or with tokens draws from it: mass then
 // takes the sums of a row's segments, at most kDrawSegments.  lists: kListed
-// order values a row, V where that is less.
+// order values a row.  Rows of one part are summed here (rec, which is input
+// otherwise) and need no histograms, plans and lists.
 constexpr int kDrawSegments = 1024;
-int launch_sample_cut(const SampleRows& r, int dtype, const SegRec* rec, const Histogram* hist, CutPlan* plans,
+int launch_sample_cut(const SampleRows& r, int dtype, SegRec* rec, const Histogram* hist, CutPlan* plans,
                       unsigned long long* lists, RowCut* cuts, DrawRec* draws, double* mass, const float* uniforms,
                       long long* tokens, hipStream_t st);
 

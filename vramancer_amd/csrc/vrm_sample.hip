@@ -7,7 +7,8 @@
 //   1. sample_segment_kernel    every row's segments: maximum, sum of weights;
 //      sample_histogram_kernel  the same and histograms, where top_k or top_p
 //                               may drop tokens
-//   2. launch_sample_cut        which tokens stay (vrm_sample_cut.hip)
+//   2. launch_sample_cut        which tokens stay (vrm_sample_cut.hip); for rows
+//                               of up to 8192 logits also 1, in one launch
 //   3. sample_choose_kernel     a sequence's drafts: accepted ones, the row its
 //                               next token is drawn from (for small batches in
 //                               the launch that follows)
@@ -22,17 +23,6 @@
 
 namespace vrm {
 namespace {
-
-// The first place of a segment's maximum.
-template <int SRC>
-__device__ __forceinline__ int first_place(const float* x, float m, int seg) {
-  constexpr int kVec = Logit<SRC>::kVec;
-  int arg = 0x7fffffff;
-#pragma unroll
-  for (int e = kSamplePer - 1; e >= 0; --e)
-    if (x[e] == m) arg = segment_element<SRC>(seg, e / kVec) + e % kVec;
-  return wave_min(arg, 0x7fffffff);
-}
 
 // ---------------------------------------------------------------------------
 // 1. Segments of rows
@@ -89,45 +79,7 @@ __global__ void __launch_bounds__(kSampleThreads, 5)
   const float t = r.temp(b);
   bool by_k, by_p;
   const bool filters = row_filters(r, b, t, by_k, by_p);
-  float m = -INFINITY;
-#pragma unroll
-  for (int e = 0; e < kSamplePer; ++e) m = fmaxf(m, x[e]);
-  m = wave_max(m, -INFINITY);
-  if ((threadIdx.x & 63) == 0) tops[wave] = m;
-  __syncthreads();
-  m = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-  SegRec g{0.0, m, -1};
-  if (m > -INFINITY) {
-    if (t > 0.0f) {
-      const Scale s = make_scale(m, t);
-      const float bins = bin_scale(s);
-      const int top_bin = bin_of(m, bins);
-      constexpr double kUnit = (double)(1ULL << kBinBits);
-      float most = kBinMost;
-      asm("" : "+v"(most));  // (kept in a register: one move less for each logit)
-#pragma unroll
-      for (int e = 0; e < kSamplePer; e += 8) {
-        double w[8];
-        sample_weights<8>(x + e, s, w);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) g.sum += w[j];
-        if (filters) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const int bin = top_bin - bin_of(x[e + j], bins, most);
-            const unsigned long long fixed = fixed_weight(w[j], kUnit);
-            if (fixed != 0) {  // (bin is below kBins then)
-              if (by_k) atomicAdd(&h.count[bin], 1u);
-              atomicAdd(&h.sum[bin], fixed);
-            }
-          }
-        }
-      }
-      g.sum = wave_sum(g.sum);
-    } else {
-      g.arg = first_place<SRC>(x, m, seg);
-    }
-  }
+  const SegRec g = part_sums<SRC>(x, seg, t, filters, by_k, tops, h);
   if ((threadIdx.x & 63) == 0 && seg < ns) rec[(long long)slot * ns + seg] = g;
   if (!filters) return;
   __syncthreads();
@@ -610,12 +562,14 @@ Plan plan_of(long long B, int K, int V, bool filtered, bool drafts, bool probs) 
     at += up((size_t)B * p.ns * sizeof(RoughMass));
   }
   if (filtered) {
-    p.hist = at;
-    at += up((size_t)p.slots * p.blocks * sizeof(Histogram));
-    p.plans = at;
-    at += up((size_t)p.slots * sizeof(CutPlan));
-    p.lists = at;
-    at += up((size_t)p.slots * (V < kListed ? V : kListed) * sizeof(unsigned long long));
+    if (p.blocks > 1) {
+      p.hist = at;
+      at += up((size_t)p.slots * p.blocks * sizeof(Histogram));
+      p.plans = at;
+      at += up((size_t)p.slots * sizeof(CutPlan));
+      p.lists = at;
+      at += up((size_t)p.slots * kListed * sizeof(unsigned long long));
+    }
     p.cuts = at;
     at += up((size_t)p.slots * sizeof(RowCut));
   }
@@ -652,7 +606,8 @@ int run(const SampleRows& r, const Drafts& d, const Plan& p, char* ws, const flo
   if (p.filtered) {
     auto* hist = reinterpret_cast<Histogram*>(ws + p.hist);
     cuts = reinterpret_cast<RowCut*>(ws + p.cuts);
-    hipLaunchKernelGGL((sample_histogram_kernel<SRC>), row_blocks, threads, 0, st, r, p.ns, p.blocks, rec, hist);
+    if (p.blocks > 1)
+      hipLaunchKernelGGL((sample_histogram_kernel<SRC>), row_blocks, threads, 0, st, r, p.ns, p.blocks, rec, hist);
     if (int rc = launch_sample_cut(r, SRC, rec, hist, reinterpret_cast<CutPlan*>(ws + p.plans),
                                    reinterpret_cast<unsigned long long*>(ws + p.lists), cuts,
                                    p.drafts ? nullptr : draws, mass, uniforms, p.fused ? tokens : nullptr, st))

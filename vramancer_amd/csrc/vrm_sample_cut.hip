@@ -26,20 +26,16 @@
 // A workgroup of the first and the last kernel runs each part of its code a few
 // times at most, so that fetching it is what short code saves (170 KB, with a
 // copy of the narrowing for each use, took 42 us for a row of 131072).
-#include <algorithm>
-
 #include "vrm_sample.h"
 
 namespace vrm {
 namespace {
 
 constexpr int kCutThreads = 512;  // = kBins
-constexpr int kCutWaves = kCutThreads / kWave;
-constexpr int kSubBits = 10;
-constexpr int kSub = 1 << kSubBits;  // steps of order values: two a thread
 constexpr int kFew = 64;            // tokens that are compared with each other
 constexpr int kPartsAhead = 24;
-static_assert(kSub >= kDrawSegments, "a sum for each segment");
+constexpr int kShortListed = 2048;   // tokens of a short row's list
+static_assert(2 * kCutThreads >= kDrawSegments, "a sum for each segment");
 
 using u64 = unsigned long long;
 
@@ -103,6 +99,69 @@ struct BinScan {
     return which * kPer + lane_value(at, which);
   }
 };
+
+// The bins of a row's borders, by one wavefront.
+__device__ __forceinline__ void plan_cut(CutPlan& plan, const BinScan& scan, const SampleRows& r, int b, int top_bin,
+                                         bool by_k, bool by_p) {
+  const double p = fmax((double)r.nucleus(b), 0.0);
+  plan.k = by_k ? r.limit(b) : 0;
+  double least = scan.total, most = scan.total;  // what top_p takes its part of
+  int last = kBins - 1;                          // the last bin that it can end in
+  if (by_k) {
+    uint32_t n_before, n_bin;
+    double s_before, s_bin;
+    const int at = scan.find(true, (uint32_t)plan.k, 0.0, n_before, s_before, n_bin, s_bin);
+    if (at == kBins) {
+      plan.k = 0;  // (all that weighs anything stays)
+    } else {
+      plan.k_first = plan.k_last = top_bin - at;
+      plan.k_count = n_before;
+      plan.k_before = s_before;
+      if (n_before + n_bin <= (uint32_t)kListed) {
+        // All tokens down to this bin are listed: the border of a top_p is
+        // among them.
+        plan.list_first = top_bin;
+        plan.list_last = top_bin - at;
+        plan.p_first = top_bin;
+        plan.p_last = top_bin - at;
+        plan.p_before = 0.0;
+        plan.by_p = by_p;
+        plan.all_listed = 1;
+        by_p = false;
+      } else {
+        plan.list_first = plan.list_last = top_bin - at;
+      }
+      least = s_before;
+      most = s_before + s_bin;
+      last = at;
+    }
+  }
+  plan.filters = plan.k > 0;
+  plan.total = scan.total;
+  if (by_p) {
+    // One bin; after a top_k, whose sum lies between two values still, what the
+    // border of the smaller and of the larger one enclose.
+    uint32_t n;
+    double s, before, unused;
+    const int from = scan.find(false, 0, fmin(fmax(p * least, 0x1p-200), least), n, before, n, s);
+    const int to = scan.find(false, 0, fmin(fmax(p * most, 0x1p-200), most), n, unused, n, s);
+    if (from < kBins) {
+      plan.by_p = 1;
+      plan.filters = 1;
+      plan.p_first = top_bin - from;
+      plan.p_last = top_bin - min(to, last);
+      plan.p_before = before;
+      if (plan.k > 0) {
+        plan.also_first = plan.p_first;
+        plan.also_last = plan.p_last;
+        plan.also = 1;
+      } else {
+        plan.list_first = plan.p_first;
+        plan.list_last = plan.p_last;
+      }
+    }
+  }
+}
 
 // One workgroup per row.
 __global__ void __launch_bounds__(kCutThreads)
@@ -183,79 +242,32 @@ __global__ void __launch_bounds__(kCutThreads)
   bin_count[t] = count;
   __syncthreads();
   if (t >= kWave) return;
-  const BinScan scan(bin_count, bin_sum);
-  const double p = fmax((double)r.nucleus(b), 0.0);
-  plan.k = by_k ? r.limit(b) : 0;
-  double least = scan.total, most = scan.total;  // what top_p takes its part of
-  int last = kBins - 1;                          // the last bin that it can end in
-  if (by_k) {
-    uint32_t n_before, n_bin;
-    double s_before, s_bin;
-    const int at = scan.find(true, (uint32_t)plan.k, 0.0, n_before, s_before, n_bin, s_bin);
-    if (at == kBins) {
-      plan.k = 0;  // (all that weighs anything stays)
-    } else {
-      plan.k_first = plan.k_last = top_bin - at;
-      plan.k_count = n_before;
-      plan.k_before = s_before;
-      if (n_before + n_bin <= (uint32_t)kListed) {
-        // All tokens down to this bin are listed: the border of a top_p is
-        // among them.
-        plan.list_first = top_bin;
-        plan.list_last = top_bin - at;
-        plan.p_first = top_bin;
-        plan.p_last = top_bin - at;
-        plan.p_before = 0.0;
-        plan.by_p = by_p;
-        plan.all_listed = 1;
-        by_p = false;
-      } else {
-        plan.list_first = plan.list_last = top_bin - at;
-      }
-      least = s_before;
-      most = s_before + s_bin;
-      last = at;
-    }
-  }
-  plan.filters = plan.k > 0;
-  plan.total = scan.total;
-  if (by_p) {
-    // One bin; after a top_k, whose sum lies between two values still, what the
-    // border of the smaller and of the larger one enclose.
-    uint32_t n;
-    double s, before, unused;
-    const int from = scan.find(false, 0, fmin(fmax(p * least, 0x1p-200), least), n, before, n, s);
-    const int to = scan.find(false, 0, fmin(fmax(p * most, 0x1p-200), most), n, unused, n, s);
-    if (from < kBins) {
-      plan.by_p = 1;
-      plan.filters = 1;
-      plan.p_first = top_bin - from;
-      plan.p_last = top_bin - min(to, last);
-      plan.p_before = before;
-      if (plan.k > 0) {
-        plan.also_first = plan.p_first;
-        plan.also_last = plan.p_last;
-        plan.also = 1;
-      } else {
-        plan.list_first = plan.p_first;
-        plan.list_last = plan.p_last;
-      }
-    }
-  }
+  plan_cut(plan, BinScan(bin_count, bin_sum), r, b, top_bin, by_k, by_p);
   if (lane == 0) plans[slot] = plan;
 }
 
+// Which of a lane's logits are in the bins to list.
+__device__ __forceinline__ uint32_t plan_hits(const CutPlan& plan, const float* x, float bins) {
+  const BinRange main(plan.list_last, plan.list_first), second(plan.also_last, plan.also_first);
+  const bool two = plan.also != 0;
+  uint32_t hits = 0;
+#pragma unroll
+  for (int e = 0; e < kSamplePer; ++e) {
+    const float y = x[e] * bins;
+    if ((main.holds(y) || (two && second.holds(y))) && x[e] > -INFINITY) hits |= 1u << e;
+  }
+  return hits;
+}
+
 // A wavefront per segment: the tokens of the bins of the plan go to the row's
-// list, by their order values; plan.listed counts them, and only `most` (kListed,
-// or V where that is less) fit.
+// list, by their order values; plan.listed counts them, and only kListed fit.
 // With MASS, mass takes the weights of the segment's tokens above the first of
 // those bins, which stay whatever the border.  (The segment is under way before
 // the plan that says whether it is needed.  Five wavefronts a SIMD, as the
 // histograms: with four each the draw of 64 rows of 152000 took 55.2 us, 51.8 now.)
 template <int SRC, bool MASS>
 __global__ void __launch_bounds__(kSampleThreads, 5)
-    sample_collect_kernel(SampleRows r, int ns, int blocks, CutPlan* plans, u64* lists, int most,
-                          double* mass) {
+    sample_collect_kernel(SampleRows r, int ns, int blocks, CutPlan* plans, u64* lists, double* mass) {
   __shared__ int wave_hits[kSampleThreads / kWave], base;
   const int wave = threadIdx.x >> 6, slot = blockIdx.x / blocks, seg = (blockIdx.x % blocks) * 4 + wave;
   const int b = slot / (r.K + 1), i = slot % (r.K + 1);
@@ -268,14 +280,7 @@ __global__ void __launch_bounds__(kSampleThreads, 5)
   if (!plan.filters) return;
   const Scale scale = make_scale(plan.top, r.temp(b));
   const float bins = bin_scale(scale);
-  const BinRange main(plan.list_last, plan.list_first), second(plan.also_last, plan.also_first);
-  const bool two = plan.also != 0;
-  uint32_t hits = 0;
-#pragma unroll
-  for (int e = 0; e < kSamplePer; ++e) {
-    const float y = x[e] * bins;
-    if ((main.holds(y) || (two && second.holds(y))) && x[e] > -INFINITY) hits |= 1u << e;
-  }
+  uint32_t hits = plan_hits(plan, x, bins);
   const int mine = __popc(hits);
   const int up_to = wave_prefix(mine), all = lane_value(up_to, 63);
   // (One addition to the row's counter for a workgroup: with one for each
@@ -293,13 +298,13 @@ __global__ void __launch_bounds__(kSampleThreads, 5)
   }
   if (all != 0) {
     at += base;
-    u64* list = lists + (long long)slot * most;
+    u64* list = lists + (long long)slot * kListed;
     // (A lane has three at most, mostly: their logits are read again, since
     // registers have no index.)
 #pragma unroll 1
     for (; hits; hits &= hits - 1, ++at) {
       const int bit = __ffs(hits) - 1, e = segment_element<SRC>(seg, bit / kVec) + bit % kVec;
-      if (at < most) list[at] = order_value(Logit<SRC>::value(row[e]), e);
+      if (at < kListed) list[at] = order_value(Logit<SRC>::value(row[e]), e);
     }
   }
   if constexpr (!MASS) return;
@@ -350,30 +355,41 @@ struct Packed {
   __device__ __forceinline__ int index(u64 p) const { return (int)(~(uint32_t)p & mask); }
 };
 
-// One workgroup per row: the borders, and where tokens are asked for the draw.
-// (128 registers, so that a compute unit has two rows.)
-template <int SRC>
-__global__ void __launch_bounds__(kCutThreads, 4)
-    sample_border_kernel(SampleRows r, int ns, int bits, const SegRec* rec, const CutPlan* plans, const u64* lists,
-                         int most, RowCut* cuts, DrawRec* draws, double* mass, const float* uniforms, long long* tokens) {
-  __shared__ u64 list[kListed], weight[kListed];  // packed order values, weights as integers
-  __shared__ u64 sub_sum[kSub];
-  __shared__ uint32_t sub_count[kSub];
-  __shared__ ulonglong2 few[kFew];  // (order, weight)
-  __shared__ u64 wave_fixed[kCutWaves], wave_low[kCutWaves], wave_high[kCutWaves];
-  __shared__ uint32_t wave_count[kCutWaves];
-  __shared__ u64 s_before_fixed, s_border;
-  __shared__ uint32_t s_before_count, s_count;
-  __shared__ int s_bin, s_fill;
-  __shared__ PickShared<SRC> pick;
+// What a workgroup of THREADS needs to find the borders of a row whose list has
+// up to LISTED tokens.
+template <int SRC, int THREADS, int LISTED>
+struct CutShared {
+  static constexpr int kThreads = THREADS, kWaves = THREADS / kWave;
+  static constexpr int kSub = 2 * THREADS, kSubBits = 31 - __builtin_clz(kSub);  // steps of order values
+  u64 list[LISTED], weight[LISTED];  // packed order values, weights as integers
+  u64 sub_sum[kSub];
+  uint32_t sub_count[kSub];
+  ulonglong2 few[kFew];  // (order, weight)
+  u64 wave_fixed[kWaves], wave_low[kWaves], wave_high[kWaves];
+  u64 before_fixed_, border_;
+  uint32_t wave_count[kWaves];
+  uint32_t before_count_, count_;
+  int bin_, fill_;
+  PickShared<SRC> pick;
 
+  __device__ __forceinline__ void put(int at, u64 order, const Packed<SRC>& packed, const Scale& scale, double unit) {
+    list[at] = packed.pack(order);
+    weight[at] = fixed_weight(sample_weight(order_logit(order), scale), unit);
+  }
+};
+
+// The borders of a row, and where tokens are asked for the draw, by a workgroup.
+// `listing` tokens are those of the plan's bins: in `lists` (thread t has one of
+// them, ahead), or where that is NULL in sh.list already; more than LISTED are
+// in neither.  With lists, mass has the sums of sample_collect_kernel.
+template <int SRC, int THREADS, int LISTED>
+__device__ __forceinline__ void find_border(CutShared<SRC, THREADS, LISTED>& sh, const SampleRows& r, int ns, int bits,
+                                            const SegRec* rec, const CutPlan& plan, int listing, const u64* lists,
+                                            u64 ahead, RowCut* cuts, DrawRec* draws, double* mass, float u,
+                                            long long* tokens) {
+  constexpr int kThreads = THREADS, kWaves = THREADS / kWave;
   const int slot = blockIdx.x, b = slot / (r.K + 1), i = slot % (r.K + 1);
   const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
-  if (i >= r.count(b)) return;
-  const CutPlan plan = plans[slot];
-  const float u = tokens ? uniforms[b] : 0.0f;
-  // (under way with the plan; what is not listed is not used)
-  const u64 ahead = t < most ? lists[(long long)slot * most + t] : 0;
   const Packed<SRC> packed(r.V);
   u64 border = 0;  // packed; 0: no cut
   double kept = plan.kept;
@@ -386,14 +402,11 @@ __global__ void __launch_bounds__(kCutThreads, 4)
     const Scale scale = make_scale(plan.top, r.temp(b));
     const float bins = bin_scale(scale);
     const double unit = (double)(1ULL << bits);
-    const auto put = [&](int at, u64 order) {
-      list[at] = packed.pack(order);
-      weight[at] = fixed_weight(sample_weight(order_logit(order), scale), unit);
-    };
-    fits = plan.listed <= most;
-    listed = fits ? plan.listed : 0;
-    if (t < listed) put(t, ahead);
-    for (int j = t + kCutThreads; j < listed; j += kCutThreads) put(j, lists[(long long)slot * most + j]);
+    const auto put = [&](int at, u64 order) { sh.put(at, order, packed, scale, unit); };
+    fits = listing <= LISTED;
+    listed = fits ? listing : 0;
+    if (lists && t < listed) put(t, ahead);
+    for (int j = t + kThreads; lists && j < listed; j += kThreads) put(j, lists[j]);
     kept = plan.total;
 #pragma unroll 1
     for (int turn = 0; turn < 2; ++turn) {
@@ -418,37 +431,37 @@ __global__ void __launch_bounds__(kCutThreads, 4)
       };
       // The step with the border, by the counts and sums of all of them.
       const auto narrow = [&](int shift) {
-        const uint32_t c0 = sub_count[2 * t], c1 = sub_count[2 * t + 1];
-        const u64 w0 = sub_sum[2 * t], w1 = sub_sum[2 * t + 1];
+        const uint32_t c0 = sh.sub_count[2 * t], c1 = sh.sub_count[2 * t + 1];
+        const u64 w0 = sh.sub_sum[2 * t], w1 = sh.sub_sum[2 * t + 1];
         const uint32_t pc = wave_prefix(c0 + c1);
         const u64 pw = wave_prefix(w0 + w1);
         if (lane == 63) {
-          wave_count[wave] = pc;
-          wave_fixed[wave] = pw;
+          sh.wave_count[wave] = pc;
+          sh.wave_fixed[wave] = pw;
         }
         __syncthreads();
         uint32_t c = before_count + pc - (c0 + c1);
         u64 w = before_fixed + pw - (w0 + w1), all = 0;
-        for (int v = 0; v < kCutWaves; ++v) {
+        for (int v = 0; v < kWaves; ++v) {
           if (v < wave) {
-            c += wave_count[v];
-            w += wave_fixed[v];
+            c += sh.wave_count[v];
+            w += sh.wave_fixed[v];
           }
-          all += wave_fixed[v];
+          all += sh.wave_fixed[v];
         }
         if (!have_goal) set_goal(all);
         const bool in0 = by_count ? c < k && c + c0 >= k : w < fixed_goal && w + w0 >= fixed_goal;
         const bool in1 = by_count ? c + c0 < k && c + c0 + c1 >= k : w + w0 < fixed_goal && w + w0 + w1 >= fixed_goal;
         if (in0 || in1) {  // (one thread: the interval has the border)
-          s_bin = 2 * t + (in0 ? 0 : 1);
-          s_count = in0 ? c0 : c1;
-          s_before_count = in0 ? c : c + c0;
-          s_before_fixed = in0 ? w : w + w0;
+          sh.bin_ = 2 * t + (in0 ? 0 : 1);
+          sh.count_ = in0 ? c0 : c1;
+          sh.before_count_ = in0 ? c : c + c0;
+          sh.before_fixed_ = in0 ? w : w + w0;
         }
         __syncthreads();
-        before_count = s_before_count;
-        before_fixed = s_before_fixed;
-        const u64 top = high - ((u64)s_bin << shift), span = (1ULL << shift) - 1;
+        before_count = sh.before_count_;
+        before_fixed = sh.before_fixed_;
+        const u64 top = high - ((u64)sh.bin_ << shift), span = (1ULL << shift) - 1;
         low = top - low > span ? top - span : low;
         high = top;
       };
@@ -457,36 +470,36 @@ __global__ void __launch_bounds__(kCutThreads, 4)
         // The list does not hold these bins' tokens (logits that lie closer
         // together than a bin is wide): passes over the row narrow their order
         // values by 10 bits each until what is left fits it.
-        int shift = max(0, packed.bits() - kSubBits);
+        int shift = max(0, packed.bits() - sh.kSubBits);
 #pragma unroll 1
         while (true) {
           __syncthreads();
-          for (int j = t; j < kSub; j += kCutThreads) {
-            sub_count[j] = 0;
-            sub_sum[j] = 0;
+          for (int j = t; j < sh.kSub; j += kThreads) {
+            sh.sub_count[j] = 0;
+            sh.sub_sum[j] = 0;
           }
-          if (t == 0) s_fill = 0;
+          if (t == 0) sh.fill_ = 0;
           __syncthreads();
 #pragma unroll 1
-          for (int e = t; e < V; e += kCutThreads) {
+          for (int e = t; e < V; e += kThreads) {
             const float l = L::value(row[e]);
             if (!range.holds(l * bins) || !(l > -INFINITY)) continue;
             const u64 order = order_value(l, e), o = packed.pack(order);
             if (o < low || o > high) continue;
             if (shift < 0) {
-              put(atomicAdd(&s_fill, 1), order);  // (there are as many as the last pass counted)
+              put(atomicAdd(&sh.fill_, 1), order);  // (there are as many as the last pass counted)
             } else {
-              atomicAdd(&sub_count[(high - o) >> shift], 1u);
-              atomicAdd(&sub_sum[(high - o) >> shift], fixed_weight(sample_weight(l, scale), unit));
+              atomicAdd(&sh.sub_count[(high - o) >> shift], 1u);
+              atomicAdd(&sh.sub_sum[(high - o) >> shift], fixed_weight(sample_weight(l, scale), unit));
             }
           }
           __syncthreads();
           if (shift < 0) break;
           narrow(shift);
           if (lost) break;
-          shift = s_count <= (uint32_t)kListed ? -1 : max(0, 64 - __clzll(high - low) - kSubBits);
+          shift = sh.count_ <= (uint32_t)LISTED ? -1 : max(0, 64 - __clzll(high - low) - sh.kSubBits);
         }
-        listed = lost ? 0 : s_fill;
+        listed = lost ? 0 : sh.fill_;
       }
 
       // Narrow the listed tokens of the bins that are within low .. high.  (A
@@ -498,11 +511,11 @@ __global__ void __launch_bounds__(kCutThreads, 4)
         // How many there are, what they weigh, and the interval that they take.
         u64 a = ~0ULL, z = 0, sum = 0;
         uint32_t count = 0;
-        for (int j = t; j < listed; j += kCutThreads) {
-          const u64 o = list[j];
+        for (int j = t; j < listed; j += kThreads) {
+          const u64 o = sh.list[j];
           if (o >= low && o <= high && (!first_look || range.holds(packed.logit(o) * bins))) {
             ++count;
-            if (!have_goal) sum += weight[j];
+            if (!have_goal) sum += sh.weight[j];
             a = min(a, o);
             z = max(z, o);
           }
@@ -512,36 +525,36 @@ __global__ void __launch_bounds__(kCutThreads, 4)
         a = wave_min(a, ~0ULL);
         z = wave_max(z, 0ULL);
         if (lane == 0) {
-          wave_count[wave] = count;
-          wave_fixed[wave] = sum;
-          wave_low[wave] = a;
-          wave_high[wave] = z;
+          sh.wave_count[wave] = count;
+          sh.wave_fixed[wave] = sum;
+          sh.wave_low[wave] = a;
+          sh.wave_high[wave] = z;
         }
-        for (int j = t; j < kSub; j += kCutThreads) {
-          sub_count[j] = 0;
-          sub_sum[j] = 0;
+        for (int j = t; j < sh.kSub; j += kThreads) {
+          sh.sub_count[j] = 0;
+          sh.sub_sum[j] = 0;
         }
-        if (t < kFew) few[t] = make_ulonglong2(0, 0);
-        if (t == 0) s_fill = 0;
+        if (t < kFew) sh.few[t] = make_ulonglong2(0, 0);
+        if (t == 0) sh.fill_ = 0;
         __syncthreads();
         n = 0;
         sum = 0;
-        for (int v = 0; v < kCutWaves; ++v) {
-          n += wave_count[v];
-          sum += wave_fixed[v];
-          a = min(a, wave_low[v]);
-          z = max(z, wave_high[v]);
+        for (int v = 0; v < kWaves; ++v) {
+          n += sh.wave_count[v];
+          sum += sh.wave_fixed[v];
+          a = min(a, sh.wave_low[v]);
+          z = max(z, sh.wave_high[v]);
         }
         if (!have_goal) set_goal(sum);
         low = a;
         high = z;
         if (n <= (uint32_t)kFew || lost) break;
-        const int shift = max(0, 64 - __clzll(high - low) - kSubBits);  // (high - low) >> shift is below kSub
-        for (int j = t; j < listed; j += kCutThreads) {
-          const u64 o = list[j];
+        const int shift = max(0, 64 - __clzll(high - low) - sh.kSubBits);  // (high - low) >> shift is below kSub
+        for (int j = t; j < listed; j += kThreads) {
+          const u64 o = sh.list[j];
           if (o >= low && o <= high) {
-            atomicAdd(&sub_count[(high - o) >> shift], 1u);
-            atomicAdd(&sub_sum[(high - o) >> shift], weight[j]);
+            atomicAdd(&sh.sub_count[(high - o) >> shift], 1u);
+            atomicAdd(&sh.sub_sum[(high - o) >> shift], sh.weight[j]);
           }
         }
         __syncthreads();
@@ -552,25 +565,25 @@ __global__ void __launch_bounds__(kCutThreads, 4)
       // part of the others.  (One wavefront with all of them took 3.8 us for 50;
       // 128 instead of 64 take 1 us longer where they are not needed and save as
       // much where they are.)
-      for (int j = t; j < listed; j += kCutThreads) {
-        const u64 o = list[j];
+      for (int j = t; j < listed; j += kThreads) {
+        const u64 o = sh.list[j];
         if (o >= low && o <= high) {
-          const int f = atomicAdd(&s_fill, 1);
-          few[f] = make_ulonglong2(o, weight[j]);
+          const int f = atomicAdd(&sh.fill_, 1);
+          sh.few[f] = make_ulonglong2(o, sh.weight[j]);
         }
       }
       __syncthreads();
-      constexpr int kEach = kFew * kFew / kCutThreads;
+      constexpr int kEach = kFew * kFew / kThreads;
       const int mine = t % kFew, others = t / kFew * kEach;
       if (others < (int)n) {
-        const u64 o = few[mine].x;
+        const u64 o = sh.few[mine].x;
         uint32_t c = 0;
         u64 w = 0;
 #pragma unroll 1
         for (int j = 0; j < kEach; j += 8) {
           ulonglong2 other[8];  // (0 behind the last one)
 #pragma unroll
-          for (int e = 0; e < 8; ++e) other[e] = few[others + j + e];
+          for (int e = 0; e < 8; ++e) other[e] = sh.few[others + j + e];
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             c += other[e].x > o ? 1 : 0;
@@ -578,23 +591,23 @@ __global__ void __launch_bounds__(kCutThreads, 4)
           }
         }
         if (c != 0) {
-          atomicAdd(&sub_count[mine], c);
-          atomicAdd(&sub_sum[mine], w);
+          atomicAdd(&sh.sub_count[mine], c);
+          atomicAdd(&sh.sub_sum[mine], w);
         }
       }
       __syncthreads();
       if (t < (int)n) {
-        const uint32_t c = before_count + sub_count[t];
-        const u64 up_to = before_fixed + sub_sum[t], w = few[t].y;
+        const uint32_t c = before_count + sh.sub_count[t];
+        const u64 up_to = before_fixed + sh.sub_sum[t], w = sh.few[t].y;
         if (by_count ? c + 1 == k : up_to < fixed_goal && up_to + w >= fixed_goal) {  // (one of them)
-          s_border = few[t].x;
-          s_before_fixed = up_to + w;
+          sh.border_ = sh.few[t].x;
+          sh.before_fixed_ = up_to + w;
         }
       }
       __syncthreads();
-      border = s_border;
+      border = sh.border_;
       of_p = !by_count;
-      kept = before + (double)s_before_fixed / unit;
+      kept = before + (double)sh.before_fixed_ / unit;
       __syncthreads();
     }
     if (border == 0) kept = plan.kept;
@@ -625,19 +638,19 @@ __global__ void __launch_bounds__(kCutThreads, 4)
   const double unit = (double)(1ULL << bits);
   // What the second launch summed is right where the cut is in the bins that it
   // listed; the segments are summed here otherwise.
-  const bool summed = plan.filters && cut != 0 && fits && (plan.all_listed || of_p == (plan.by_p != 0));
+  const bool summed = lists && plan.filters && cut != 0 && fits && (plan.all_listed || of_p == (plan.by_p != 0));
   if (summed) {
-    for (int j = t; j < ns; j += kCutThreads) sub_sum[j] = 0;
+    for (int j = t; j < ns; j += kThreads) sh.sub_sum[j] = 0;
     __syncthreads();
     const BinRange range(plan.by_p ? plan.p_last : plan.k_last, plan.by_p ? plan.p_first : plan.k_first);
     const float bins = bin_scale(scale);
-    for (int j = t; j < listed; j += kCutThreads) {
-      const u64 o = list[j];
+    for (int j = t; j < listed; j += kThreads) {
+      const u64 o = sh.list[j];
       if (o >= border && (plan.all_listed || range.holds(packed.logit(o) * bins)))
-        atomicAdd(&sub_sum[packed.index(o) / kSegment], weight[j]);
+        atomicAdd(&sh.sub_sum[packed.index(o) / kSegment], sh.weight[j]);
     }
   } else if (cut != 0) {
-    for (int seg = wave; seg < ns; seg += kCutWaves) {
+    for (int seg = wave; seg < ns; seg += kWaves) {
       float x[kSamplePer];
       load_segment<SRC>(row, seg, r.V, x);
       constexpr int kVec = Logit<SRC>::kVec;
@@ -655,36 +668,129 @@ __global__ void __launch_bounds__(kCutThreads, 4)
   }
   __syncthreads();
   const SegRec* recs = rec + (long long)slot * ns;
-  pick_token<SRC, kCutWaves>(pick, row, r.V, ns, w, scale, nullptr, false, fmin(fmax((double)u, 0.0), 1.0),
+  pick_token<SRC, kWaves>(sh.pick, row, r.V, ns, w, scale, nullptr, false, fmin(fmax((double)u, 0.0), 1.0),
                              [&](int j) {
                                if (cut == 0) return segment_sum(recs[j], scale);
                                if (!summed) return masses[j];
-                               return (plan.all_listed ? 0.0 : masses[j]) + (double)sub_sum[j] / unit;
+                               return (plan.all_listed ? 0.0 : masses[j]) + (double)sh.sub_sum[j] / unit;
                              },
                              tokens + b);
 }
 
+// One workgroup per row.  (128 registers, so that a compute unit has two rows.)
 template <int SRC>
-void launch(const SampleRows& r, int bits, const SegRec* rec, const Histogram* hist, CutPlan* plans, u64* lists,
+__global__ void __launch_bounds__(kCutThreads, 4)
+    sample_border_kernel(SampleRows r, int ns, int bits, const SegRec* rec, const CutPlan* plans, const u64* lists,
+                         RowCut* cuts, DrawRec* draws, double* mass, const float* uniforms, long long* tokens) {
+  __shared__ CutShared<SRC, kCutThreads, kListed> sh;
+  const int slot = blockIdx.x, b = slot / (r.K + 1), t = threadIdx.x;
+  if (slot % (r.K + 1) >= r.count(b)) return;
+  const CutPlan plan = plans[slot];
+  const float u = tokens ? uniforms[b] : 0.0f;
+  const u64* list = lists + (long long)slot * kListed;
+  // (under way with the plan; what is not listed is not used)
+  const u64 ahead = list[t];
+  find_border(sh, r, ns, bits, rec, plan, plan.listed, list, ahead, cuts, draws, mass, u, tokens);
+}
+
+// All of it for rows of one part, whose logits stay in registers until they are
+// listed: one launch instead of four.  (Drafts of 952 rows of 1325, top_k 1000,
+// 73.6 us in four, 46.3 so; of 1773 rows of 2722 with top_p 88.7 and 51.9; draws
+// from 300 rows of 8192 39.3 and 24.9, from one 27.3 and 21.5.)
+template <int SRC>
+__global__ void __launch_bounds__(kSampleThreads, 4)
+    sample_short_kernel(SampleRows r, int ns, int bits, SegRec* rec, RowCut* cuts, DrawRec* draws, double* mass,
+                        const float* uniforms, long long* tokens) {
+  __shared__ union {
+    struct {
+      Histogram hist;
+      double bin_sum[kBins];
+    } bins;
+    CutShared<SRC, kSampleThreads, kShortListed> cut;
+  } both;  // (40 KB, so that a compute unit has four rows)
+  auto& sh = both.cut;
+  Histogram& h = both.bins.hist;
+  double* const bin_sum = both.bins.bin_sum;
+  __shared__ float tops[4];
+  __shared__ SegRec part[4];
+  __shared__ CutPlan s_plan;
+  __shared__ int listing;
+  const int slot = blockIdx.x, b = slot / (r.K + 1), i = slot % (r.K + 1);
+  const int t = threadIdx.x, seg = t >> 6, lane = t & 63;
+  if (i >= r.count(b)) return;
+  for (int j = t; j < kBins; j += kSampleThreads) {
+    h.sum[j] = 0;
+    h.count[j] = 0;
+  }
+  if (t == 0) listing = 0;
+  constexpr int kVec = Logit<SRC>::kVec;
+  const auto* row = row_at<SRC>(r, r.first(b) + i);
+  const float u = tokens ? uniforms[b] : 0.0f;
+  float x[kSamplePer];
+  load_segment<SRC>(row, seg, r.V, x);
+  const float temp = r.temp(b);
+  bool by_k, by_p;
+  const bool filters = row_filters(r, b, temp, by_k, by_p);
+  const SegRec g = part_sums<SRC>(x, seg, temp, filters, by_k, tops, h);
+  if (lane == 0) {
+    part[seg] = g;
+    if (seg < ns) rec[(long long)slot * ns + seg] = g;
+  }
+  __syncthreads();
+  for (int j = t; j < kBins; j += kSampleThreads) bin_sum[j] = (double)h.sum[j] * (1.0 / (double)(1ULL << kBinBits));
+  __syncthreads();
+  if (t < kWave) {
+    CutPlan plan{};
+    Scale scale;
+    combine_segments(part, ns, temp, plan.top, plan.arg, scale, plan.kept);
+    if (filters && plan.arg == -2)
+      plan_cut(plan, BinScan(h.count, bin_sum), r, b, bin_of(plan.top, bin_scale(scale)), by_k, by_p);
+    if (lane == 0) s_plan = plan;
+  }
+  __syncthreads();
+  const CutPlan plan = s_plan;
+  if (plan.filters) {
+    const Scale scale = make_scale(plan.top, temp);
+    const float bins = bin_scale(scale);
+    const double unit = (double)(1ULL << bits);
+    const Packed<SRC> packed(r.V);
+    uint32_t hits = plan_hits(plan, x, bins);
+    int at = hits ? atomicAdd(&listing, __popc(hits)) : 0;
+#pragma unroll 1
+    for (; hits; hits &= hits - 1, ++at) {  // (read again: registers have no index)
+      const int bit = __ffs(hits) - 1, e = segment_element<SRC>(seg, bit / kVec) + bit % kVec;
+      if (at < kShortListed) sh.put(at, order_value(Logit<SRC>::value(row[e]), e), packed, scale, unit);
+    }
+  }
+  __syncthreads();
+  find_border(sh, r, ns, bits, rec, plan, listing, (const u64*)nullptr, 0, cuts, draws, mass, u, tokens);
+}
+
+template <int SRC>
+void launch(const SampleRows& r, int bits, SegRec* rec, const Histogram* hist, CutPlan* plans, u64* lists,
             RowCut* cuts, DrawRec* draws, double* mass, const float* uniforms, long long* tokens, hipStream_t st) {
   const int blocks = (r.V + kSampleBlock - 1) / kSampleBlock;
   const long long slots = (long long)r.B * (r.K + 1);
-  const int most = std::min(kListed, r.V);
+  if (blocks == 1) {
+    hipLaunchKernelGGL((sample_short_kernel<SRC>), dim3((unsigned)slots), dim3(kSampleThreads), 0, st, r, r.segments(),
+                       bits, rec, cuts, draws, mass, uniforms, tokens);
+    return;
+  }
   hipLaunchKernelGGL(sample_bins_kernel, dim3((unsigned)slots), dim3(kCutThreads), 0, st, r, r.segments(), blocks, rec,
                      hist, plans);
   if (tokens)
     hipLaunchKernelGGL((sample_collect_kernel<SRC, true>), dim3((unsigned)(slots * blocks)), dim3(kSampleThreads), 0, st,
-                       r, r.segments(), blocks, plans, lists, most, mass);
+                       r, r.segments(), blocks, plans, lists, mass);
   else
     hipLaunchKernelGGL((sample_collect_kernel<SRC, false>), dim3((unsigned)(slots * blocks)), dim3(kSampleThreads), 0,
-                       st, r, r.segments(), blocks, plans, lists, most, nullptr);
+                       st, r, r.segments(), blocks, plans, lists, nullptr);
   hipLaunchKernelGGL((sample_border_kernel<SRC>), dim3((unsigned)slots), dim3(kCutThreads), 0, st, r, r.segments(), bits,
-                     rec, plans, lists, most, cuts, draws, mass, uniforms, tokens);
+                     rec, plans, lists, cuts, draws, mass, uniforms, tokens);
 }
 
 }  // namespace
 
-int launch_sample_cut(const SampleRows& r, int dtype, const SegRec* rec, const Histogram* hist, CutPlan* plans,
+int launch_sample_cut(const SampleRows& r, int dtype, SegRec* rec, const Histogram* hist, CutPlan* plans,
                       u64* lists, RowCut* cuts, DrawRec* draws, double* mass, const float* uniforms, long long* tokens,
                       hipStream_t st) {
   int bits = 45;
