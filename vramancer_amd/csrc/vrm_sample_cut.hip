@@ -9,6 +9,8 @@
 //   sample_collect_kernel  lists those bins' tokens (a wavefront per segment)
 //   sample_border_kernel   narrows the list down by bins of order values until
 //                          64 tokens are left, which it compares with each other
+// Rows of up to 8192 logits (one part) go through all of it, their histogram
+// included, in one launch: sample_short_kernel.
 // A draw that needs nothing else comes out of the same launches: the second one
 // adds up what the segments hold above the border's bins, the third adds the
 // listed tokens that stay and picks.
@@ -32,9 +34,9 @@ namespace vrm {
 namespace {
 
 constexpr int kCutThreads = 512;  // = kBins
-constexpr int kFew = 64;            // tokens that are compared with each other
+constexpr int kFew = 64;           // tokens that are compared with each other
 constexpr int kPartsAhead = 24;
-constexpr int kShortListed = 2048;   // tokens of a short row's list
+constexpr int kShortListed = 2048;  // tokens of a short row's list
 static_assert(2 * kCutThreads >= kDrawSegments, "a sum for each segment");
 
 using u64 = unsigned long long;
@@ -361,7 +363,6 @@ template <int SRC, int THREADS, int LISTED>
 struct CutShared {
   static constexpr int kThreads = THREADS, kWaves = THREADS / kWave;
   static constexpr int kSub = 2 * THREADS, kSubBits = 31 - __builtin_clz(kSub);  // steps of order values
-  u64 list[LISTED], weight[LISTED];  // packed order values, weights as integers
   u64 sub_sum[kSub];
   uint32_t sub_count[kSub];
   ulonglong2 few[kFew];  // (order, weight)
@@ -371,6 +372,9 @@ struct CutShared {
   uint32_t before_count_, count_;
   int bin_, fill_;
   PickShared<SRC> pick;
+  // Packed order values, weights as integers; last, so that the others are within
+  // the 16 bits of an LDS instruction's offset.
+  u64 list[LISTED], weight[LISTED];
 
   __device__ __forceinline__ void put(int at, u64 order, const Packed<SRC>& packed, const Scale& scale, double unit) {
     list[at] = packed.pack(order);
@@ -379,10 +383,10 @@ struct CutShared {
 };
 
 // The borders of a row, and where tokens are asked for the draw, by a workgroup.
-// `listing` tokens are those of the plan's bins: in `lists` (thread t has one of
-// them, ahead), or where that is NULL in sh.list already; more than LISTED are
-// in neither.  With lists, mass has the sums of sample_collect_kernel.
-template <int SRC, int THREADS, int LISTED>
+// `listing` tokens are those of the plan's bins: with LISTS in `lists` (thread t
+// has one of them, ahead), otherwise in sh.list already; more than LISTED are in
+// neither.  With LISTS mass has the sums of sample_collect_kernel.
+template <bool LISTS, int SRC, int THREADS, int LISTED>
 __device__ __forceinline__ void find_border(CutShared<SRC, THREADS, LISTED>& sh, const SampleRows& r, int ns, int bits,
                                             const SegRec* rec, const CutPlan& plan, int listing, const u64* lists,
                                             u64 ahead, RowCut* cuts, DrawRec* draws, double* mass, float u,
@@ -405,8 +409,10 @@ __device__ __forceinline__ void find_border(CutShared<SRC, THREADS, LISTED>& sh,
     const auto put = [&](int at, u64 order) { sh.put(at, order, packed, scale, unit); };
     fits = listing <= LISTED;
     listed = fits ? listing : 0;
-    if (lists && t < listed) put(t, ahead);
-    for (int j = t + kThreads; lists && j < listed; j += kThreads) put(j, lists[j]);
+    if constexpr (LISTS) {
+      if (t < listed) put(t, ahead);
+      for (int j = t + kThreads; j < listed; j += kThreads) put(j, lists[j]);
+    }
     kept = plan.total;
 #pragma unroll 1
     for (int turn = 0; turn < 2; ++turn) {
@@ -638,7 +644,7 @@ __device__ __forceinline__ void find_border(CutShared<SRC, THREADS, LISTED>& sh,
   const double unit = (double)(1ULL << bits);
   // What the second launch summed is right where the cut is in the bins that it
   // listed; the segments are summed here otherwise.
-  const bool summed = lists && plan.filters && cut != 0 && fits && (plan.all_listed || of_p == (plan.by_p != 0));
+  const bool summed = LISTS && plan.filters && cut != 0 && fits && (plan.all_listed || of_p == (plan.by_p != 0));
   if (summed) {
     for (int j = t; j < ns; j += kThreads) sh.sub_sum[j] = 0;
     __syncthreads();
@@ -690,7 +696,7 @@ __global__ void __launch_bounds__(kCutThreads, 4)
   const u64* list = lists + (long long)slot * kListed;
   // (under way with the plan; what is not listed is not used)
   const u64 ahead = list[t];
-  find_border(sh, r, ns, bits, rec, plan, plan.listed, list, ahead, cuts, draws, mass, u, tokens);
+  find_border<true>(sh, r, ns, bits, rec, plan, plan.listed, list, ahead, cuts, draws, mass, u, tokens);
 }
 
 // All of it for rows of one part, whose logits stay in registers until they are
@@ -763,7 +769,7 @@ __global__ void __launch_bounds__(kSampleThreads, 4)
     }
   }
   __syncthreads();
-  find_border(sh, r, ns, bits, rec, plan, listing, (const u64*)nullptr, 0, cuts, draws, mass, u, tokens);
+  find_border<false>(sh, r, ns, bits, rec, plan, listing, nullptr, 0, cuts, draws, mass, u, tokens);
 }
 
 template <int SRC>
