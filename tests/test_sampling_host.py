@@ -115,6 +115,14 @@ def test_workspaces_grow_with_the_call(lib):
     assert sample(4, (1 << 24) + 1, 1, 1) == 0 and ver(-1, 2, 10, 0) == 0
 
 
+@pytest.mark.parametrize("B,K,V", [(5000, 3, 8000), (9000, 3, 1000), (1 << 20, 1, 17), (3, 4, 8192), (3, 4, 8193),
+                                   (300, 1, 150000)])
+def test_a_workspace_with_filters_is_enough_without(lib, B, K, V):
+    sample, ver = lib.vrm_sample_workspace_bytes, lib.vrm_verify_workspace_bytes
+    assert ver(B, K, V, 1) >= ver(B, K, V, 0) >= ver(B, K, V - 1, 0) and ver(B, K, V, 1) >= ver(B, K, V - 1, 1)
+    assert sample(B, V, 1, 1) >= max(sample(B, V, 0, 1), sample(B, V, 1, 0), sample(B, V - 1, 1, 1))
+
+
 def test_python_refusals():
     x, u = torch.zeros((2, 5)), torch.zeros(2)
     with pytest.raises(RuntimeError, match="run on the GPU"):

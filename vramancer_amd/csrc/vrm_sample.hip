@@ -19,6 +19,8 @@
 // that decides (sample_rough_*).
 // A draw without top_k and top_p is 1 and 5, one with them 1 and 2 (which picks
 // too), and 1, 2, 4 and 5 where its distribution is asked for.
+#include <algorithm>
+
 #include "vrm_sample.h"
 
 namespace vrm {
@@ -739,7 +741,9 @@ extern "C" int vrm_sample_tokens(const void* logits, int dtype, long long row_st
 
 extern "C" size_t vrm_verify_workspace_bytes(int B, int K, int V, int filtered) {
   if (check_sizes(B, K, V, VRM_SRC_F32, 0, "vrm_verify_workspace_bytes")) return 0;
-  return plan_of(B, K, V, filtered != 0, true, false).bytes;
+  // (of a large batch of short rows the calls without top_k and top_p need more)
+  const size_t plain = plan_of(B, K, V, false, true, false).bytes;
+  return filtered ? std::max(plan_of(B, K, V, true, true, false).bytes, plain) : plain;
 }
 
 extern "C" int vrm_verify_drafts(const void* logits, int dtype, long long row_stride, const int32_t* cu_seqlens,
