@@ -156,6 +156,7 @@ class PageTableEntry:
     num_tokens: int = 0
     created_at: float = field(default_factory=time.time)
     reserved: bool = False  # may hold pages that no token is in yet (``reserve``)
+    handed_out: int = 0  # how often others have got pages and token count of it (``reserve``)
 
 
 @dataclass
@@ -172,7 +173,8 @@ class ChunkBatch:
     places: List[Tuple[int, int]]  # (page, slot) of every new token, in row order
     expected_context: Optional[int] = None  # mean context of the new tokens
     # where it is from: its manager, that manager's epoch when the batch was last
-    # found good, and each request's entry, token count and pages added to it
+    # found good, and each request's entry, token count, pages added to it and
+    # the entry's handed_out
     owner: Any = field(default=None, repr=False, compare=False)
     epoch: int = field(default=0, repr=False, compare=False)
     states: List[tuple] = field(default_factory=list, repr=False, compare=False)
@@ -425,7 +427,7 @@ class PagedKVCacheManager:
                 e.num_tokens += n
             self._peak_usage = max(self._peak_usage, self.config.max_pages - len(self._free_pages))
             self._epoch += 1
-            epoch, states = self._epoch, [(e, e.num_tokens, m) for e, m in zip(entries, more)]
+            epoch, states = self._epoch, [(e, e.num_tokens, m, e.handed_out) for e, m in zip(entries, more)]
             width = max([1] + [len(e.pages) for e in entries])
             B = len(ids)
             host = np.full(B * (width + 2) + 1, -1, dtype=np.int32)  # table, lengths, offsets: one upload
@@ -454,13 +456,15 @@ class PagedKVCacheManager:
             self._check_states_locked(chunk, what)
             chunk.epoch = self._epoch
 
-    def _check_states_locked(self, chunk: ChunkBatch, what: str, pages: bool = False) -> None:
-        # With ``pages``, for callers that take the batch's last pages back: they
-        # are not the last ones any more where ``reserve`` has added some.
-        PS = self.config.page_size
-        for rid, (entry, n, added) in zip(chunk.request_ids, chunk.states):
+    def _check_states_locked(self, chunk: ChunkBatch, what: str, kept: Optional[Sequence[int]] = None) -> None:
+        # With ``kept``, for callers that take the other tokens back: what has
+        # been handed out since (a table on the device and the length it goes on
+        # from) names these tokens and their pages, whether or not pages were
+        # added for it.
+        kept = chunk.counts if kept is None else kept
+        for rid, (entry, n, _, handed_out), had, keeps in zip(chunk.request_ids, chunk.states, chunk.counts, kept):
             if (self._page_tables.get(rid) is not entry or entry.num_tokens != n
-                    or (pages and added and len(entry.pages) != -(-n // PS))):
+                    or (keeps < had and entry.handed_out != handed_out)):
                 raise RuntimeError(f"{what}: request {rid!r} has changed since append_chunk made this batch")
 
     def _take_back(self, chunk: ChunkBatch) -> None:
@@ -469,10 +473,10 @@ class PagedKVCacheManager:
         list is as it was) and their rows in the compression queue.  What they
         wrote lies behind the requests' last tokens; an fp8 page's scale keeps
         what they raised it to.  Raises, and changes nothing, where a request
-        has changed since."""
+        has changed or was reserved for since."""
         with self._lock:
-            self._check_states_locked(chunk, "_take_back", pages=True)
-            for (entry, n, added), count in reversed(list(zip(chunk.states, chunk.counts))):
+            self._check_states_locked(chunk, "_take_back", [0] * len(chunk.counts))
+            for (entry, n, added, _), count in reversed(list(zip(chunk.states, chunk.counts))):
                 entry.num_tokens = n - count
                 for _ in range(added):
                     self._release_locked(entry.pages.pop())
@@ -487,7 +491,8 @@ class PagedKVCacheManager:
         tokens that were refused.  What those wrote lies behind the requests'
         last tokens; an fp8 page's scale keeps what they raised it to.  The
         batch is spent unless all of it is kept.  Raises, and changes nothing,
-        where a request has changed since append_chunk."""
+        where a request has changed since append_chunk, or where tokens would be
+        taken back from one that has been reserved for since."""
         counts = [int(n) for n in counts]
         if len(counts) != len(chunk.counts) or any(not 0 <= n <= had for n, had in zip(counts, chunk.counts)):
             raise RuntimeError(f"keep_chunk takes a number of tokens for each request, at most {chunk.counts}, "
@@ -499,8 +504,8 @@ class PagedKVCacheManager:
             return
         PS = self.config.page_size
         with self._lock:
-            self._check_states_locked(chunk, "keep_chunk", pages=True)
-            for (entry, n, added), had, kept in reversed(list(zip(chunk.states, chunk.counts, counts))):
+            self._check_states_locked(chunk, "keep_chunk", counts)
+            for (entry, n, added, _), had, kept in reversed(list(zip(chunk.states, chunk.counts, counts))):
                 entry.num_tokens = n - had + kept
                 for _ in range(added):
                     if (len(entry.pages) - 1) * PS < entry.num_tokens:
@@ -559,6 +564,7 @@ class PagedKVCacheManager:
                 raise RuntimeError("requests that share the page their next token goes to (forks) cannot be reserved "
                                    "for together")
             for e, m in zip(entries, more):
+                e.handed_out += 1
                 if m:
                     e.pages.extend(self._alloc_page() for _ in range(m))
                     e.reserved = True
