@@ -68,3 +68,78 @@ def test_a_reservation_that_is_refused_changes_nothing():
         _refused(m, lambda: m.reserve(ids, counts), match=".")
     m.keep_chunk(chunk, [1, 3])
     assert list(m.token_counts(["a", "b"])) == [1, 3] and len(m._page_tables["a"].pages) == 1
+
+
+@pytest.mark.parametrize("had", [0, 2])
+@pytest.mark.parametrize("kept", [0, 1, 3])
+def test_tokens_that_a_fork_has_stay(kept, had):
+    """A fork has the batch's tokens and shares their page: the request's next
+    token must not go over them."""
+    m = _mgr()
+    m.allocate("a", had), m.allocate("b")
+    chunk = m.append_chunk(["a", "b"], [4, 4])
+    m.fork("a", "f")
+    page = m._page_tables["a"].pages[0]
+    if kept + had == 0:  # (all tokens of a page that came with them: it is the fork's alone then)
+        m.keep_chunk(chunk, [kept, 4])
+        assert m._page_tables["a"].pages == [] and m._page_tables["f"].pages == [page]
+        assert m.append_token("a")[0] != page
+        return
+    _refused(m, lambda: m.keep_chunk(chunk, [kept, 4]))
+    if had:
+        _refused(m, lambda: m._take_back(chunk))
+    m.keep_chunk(chunk, [4, kept])
+    assert list(m.token_counts(["a", "b", "f"])) == [had + 4, kept, had + 4]
+    assert m.append_token("a") == (page, had + 4)  # behind the fork's last token
+
+
+@pytest.mark.parametrize("kept,fits", [(16, True), (9, False), (8, True), (3, False), (0, True)])
+def test_tokens_of_whole_pages_go(kept, fits):
+    m = _mgr()
+    m.allocate("a", 16)
+    chunk = m.append_chunk(["a"], [20])  # three pages of its own
+    m.fork("a", "f")
+    if not fits:
+        _refused(m, lambda: m.keep_chunk(chunk, [kept]))
+        return
+    held = list(m._page_tables["a"].pages)
+    m.keep_chunk(chunk, [kept])
+    assert m._page_tables["a"].pages == held[:2 + kept // 8] and m._page_tables["f"].pages == held
+    assert m.append_token("a")[0] not in held and len(m._free_pages) == 2
+
+
+def test_pages_that_were_there_before_the_tokens():
+    """Reserved pages stay the request's when their tokens are taken back, so
+    that a fork must not have those."""
+    m = _mgr()
+    m.allocate("a")
+    m.reserve(["a"], [16])
+    chunk = m.append_chunk(["a"], [16])
+    m.fork("a", "f")
+    _refused(m, lambda: m.keep_chunk(chunk, [8]), lambda: m.keep_chunk(chunk, [0]), lambda: m._take_back(chunk))
+    m.free("f")
+    m.keep_chunk(chunk, [8])  # (nobody else has them any more)
+    assert list(m.token_counts(["a"])) == [8] and len(m._page_tables["a"].pages) == 2
+
+
+def test_forks_made_before():
+    m = _mgr()
+    m.allocate("a", 8)
+    m.fork("a", "f")
+    chunk = m.append_chunk(["a", "f"], [3, 4])  # (a page of its own for each)
+    m.keep_chunk(chunk, [1, 2])
+    assert list(m.token_counts(["a", "f"])) == [9, 10]
+    chunk = m.append_chunk(["f"], [2])
+    m.fork("f", "g")
+    _refused(m, lambda: m.keep_chunk(chunk, [1]))
+    assert m.fork("missing", "h") is None
+
+
+def test_a_fork_of_pages_that_are_taken_back_whole():
+    m = _mgr(PS=16, max_pages=12)
+    m.allocate("a")
+    chunk = m.append_chunk(["a"], [5])
+    m.fork("a", "c")
+    m._take_back(chunk)
+    assert list(m.token_counts(["a", "c"])) == [0, 5] and len(m._free_pages) == 11
+    assert m.append_chunk(["a"], [1]).places[0][0] != m._page_tables["c"].pages[0]

@@ -157,6 +157,7 @@ class PageTableEntry:
     created_at: float = field(default_factory=time.time)
     reserved: bool = False  # may hold pages that no token is in yet (``reserve``)
     handed_out: int = 0  # how often others have got pages and token count of it (``reserve``)
+    forks: int = 0       # how often it has been forked
 
 
 @dataclass
@@ -174,7 +175,7 @@ class ChunkBatch:
     expected_context: Optional[int] = None  # mean context of the new tokens
     # where it is from: its manager, that manager's epoch when the batch was last
     # found good, and each request's entry, token count, pages added to it and
-    # the entry's handed_out
+    # the entry's handed_out and forks
     owner: Any = field(default=None, repr=False, compare=False)
     epoch: int = field(default=0, repr=False, compare=False)
     states: List[tuple] = field(default_factory=list, repr=False, compare=False)
@@ -427,7 +428,7 @@ class PagedKVCacheManager:
                 e.num_tokens += n
             self._peak_usage = max(self._peak_usage, self.config.max_pages - len(self._free_pages))
             self._epoch += 1
-            epoch, states = self._epoch, [(e, e.num_tokens, m, e.handed_out) for e, m in zip(entries, more)]
+            epoch, states = self._epoch, [(e, e.num_tokens, m, e.handed_out, e.forks) for e, m in zip(entries, more)]
             width = max([1] + [len(e.pages) for e in entries])
             B = len(ids)
             host = np.full(B * (width + 2) + 1, -1, dtype=np.int32)  # table, lengths, offsets: one upload
@@ -457,14 +458,23 @@ class PagedKVCacheManager:
             chunk.epoch = self._epoch
 
     def _check_states_locked(self, chunk: ChunkBatch, what: str, kept: Optional[Sequence[int]] = None) -> None:
-        # With ``kept``, for callers that take the other tokens back: what has
-        # been handed out since (a table on the device and the length it goes on
+        # With ``kept``, for callers that take the other tokens back: a
+        # reservation since (a table on the device and the length it goes on
         # from) names these tokens and their pages, whether or not pages were
-        # added for it.
+        # added for it; and a fork since has these tokens, so that none of the
+        # pages they are in may stay the request's to write to.
+        PS = self.config.page_size
         kept = chunk.counts if kept is None else kept
-        for rid, (entry, n, _, handed_out), had, keeps in zip(chunk.request_ids, chunk.states, chunk.counts, kept):
-            if (self._page_tables.get(rid) is not entry or entry.num_tokens != n
-                    or (keeps < had and entry.handed_out != handed_out)):
+        for rid, (entry, n, added, handed_out, forks), had, keeps in zip(chunk.request_ids, chunk.states, chunk.counts,
+                                                                         kept):
+            changed = self._page_tables.get(rid) is not entry or entry.num_tokens != n
+            if not changed and keeps < had:
+                changed = entry.handed_out != handed_out
+                if entry.forks != forks:
+                    left = n - had + keeps
+                    pages = entry.pages[:max(len(entry.pages) - added, -(-left // PS))]  # (those that stay)
+                    changed |= any(self._pages[p].ref_count > 1 for p in pages[left // PS:])
+            if changed:
                 raise RuntimeError(f"{what}: request {rid!r} has changed since append_chunk made this batch")
 
     def _take_back(self, chunk: ChunkBatch) -> None:
@@ -473,10 +483,11 @@ class PagedKVCacheManager:
         list is as it was) and their rows in the compression queue.  What they
         wrote lies behind the requests' last tokens; an fp8 page's scale keeps
         what they raised it to.  Raises, and changes nothing, where a request
-        has changed or was reserved for since."""
+        has changed or was reserved for since, or a fork made since has these
+        tokens in pages that were there before."""
         with self._lock:
             self._check_states_locked(chunk, "_take_back", [0] * len(chunk.counts))
-            for (entry, n, added, _), count in reversed(list(zip(chunk.states, chunk.counts))):
+            for (entry, n, added, _, _), count in reversed(list(zip(chunk.states, chunk.counts))):
                 entry.num_tokens = n - count
                 for _ in range(added):
                     self._release_locked(entry.pages.pop())
@@ -492,7 +503,8 @@ class PagedKVCacheManager:
         last tokens; an fp8 page's scale keeps what they raised it to.  The
         batch is spent unless all of it is kept.  Raises, and changes nothing,
         where a request has changed since append_chunk, or where tokens would be
-        taken back from one that has been reserved for since."""
+        taken back from one that has been reserved for since, or out of a page
+        that a fork made since has them in."""
         counts = [int(n) for n in counts]
         if len(counts) != len(chunk.counts) or any(not 0 <= n <= had for n, had in zip(counts, chunk.counts)):
             raise RuntimeError(f"keep_chunk takes a number of tokens for each request, at most {chunk.counts}, "
@@ -505,7 +517,7 @@ class PagedKVCacheManager:
         PS = self.config.page_size
         with self._lock:
             self._check_states_locked(chunk, "keep_chunk", counts)
-            for (entry, n, added, _), had, kept in reversed(list(zip(chunk.states, chunk.counts, counts))):
+            for (entry, n, added, _, _), had, kept in reversed(list(zip(chunk.states, chunk.counts, counts))):
                 entry.num_tokens = n - had + kept
                 for _ in range(added):
                     if (len(entry.pages) - 1) * PS < entry.num_tokens:
@@ -662,6 +674,7 @@ class PagedKVCacheManager:
             entry = PageTableEntry(request_id=dst_request_id, pages=list(src.pages), num_tokens=src.num_tokens)
             if src.reserved:  # (the pages of tokens to come are the source's own)
                 del entry.pages[-(-src.num_tokens // self.config.page_size):]
+            src.forks += 1
             for page_id in entry.pages:
                 self._pages[page_id].ref_count += 1
             self._page_tables[dst_request_id] = entry
