@@ -143,3 +143,14 @@ def test_a_fork_of_pages_that_are_taken_back_whole():
     m._take_back(chunk)
     assert list(m.token_counts(["a", "c"])) == [0, 5] and len(m._free_pages) == 11
     assert m.append_chunk(["a"], [1]).places[0][0] != m._page_tables["c"].pages[0]
+
+
+def test_no_reservations_with_compression():
+    """What steps over reserved pages store does not enter the compression
+    queue: refused before there are such pages, not when they are counted."""
+    m = _mgr(kv_compression="turboquant")
+    m.allocate("a")
+    for n in (0, 3, 9):
+        _refused(m, lambda: m.reserve(["a"], [n]), match="kv_compression")
+    _refused(m, lambda: m.commit(["a"], [1]), match="kv_compression")
+    assert m.append_chunk(["a"], [9]).places[0][1] == 0

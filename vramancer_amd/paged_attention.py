@@ -549,10 +549,14 @@ class PagedKVCacheManager:
         All or nothing: an unknown id raises ``KeyError``; an id given twice, a
         negative count, too few free pages, or requests (forks) that share a
         page their next tokens go to raise ``RuntimeError``, and nothing has
-        changed."""
+        changed.  Not with ``kv_compression``, whose queue such steps do not
+        feed."""
         import torch
 
         self._require_pool("reserve")
+        if self._kv_compressor is not None:
+            raise RuntimeError("tokens stored on the device alone do not enter the compression queue: reserve is for "
+                               "managers without kv_compression")
         ids, counts = list(request_ids), [int(n) for n in counts]
         if len(counts) != len(ids):
             raise RuntimeError(f"{len(ids)} request ids but {len(counts)} counts")
