@@ -154,3 +154,39 @@ def test_no_reservations_with_compression():
         _refused(m, lambda: m.reserve(["a"], [n]), match="kv_compression")
     _refused(m, lambda: m.commit(["a"], [1]), match="kv_compression")
     assert m.append_chunk(["a"], [9]).places[0][1] == 0
+
+
+def test_prefixes_once_no_reserved_page_is_left():
+    """A prefix can follow when the reserved pages hold tokens, however those
+    came; until then it is refused, and a fork does not get the empty ones."""
+    m = _mgr()
+    m.allocate("a")
+    m.reserve(["a"], [8])
+    _refused(m, lambda: m.try_prefix_cache("a", list(range(8))), match="reserved pages")
+    assert m.fork("a", "f").pages == []
+    chunk = m.append_chunk(["a"], [8])
+    m.keep_chunk(chunk, [0])
+    _refused(m, lambda: m.try_prefix_cache("a", list(range(8))), match="reserved pages")
+    m.commit(["a"], [0])
+    assert m.fork("a", "g").pages == []
+    m.append_chunk(["a"], [5])
+    assert m.fork("a", "h").pages == m._page_tables["a"].pages
+    assert m.try_prefix_cache("a", list(range(8))) == 0 and list(m.token_counts(["a"])) == [16]
+    for _ in range(2):
+        m.allocate("b")
+        m.reserve(["b"], [8])
+        for t in range(8):
+            m.append_token("b")
+        assert m.try_prefix_cache("b", list(range(8))) == 8  # (a's page)
+        m.free("b")
+
+
+def test_commit_leaves_reserved_pages_reserved_while_tokens_can_be_taken_back():
+    m = _mgr()
+    m.allocate("a")
+    m.reserve(["a"], [8])
+    chunk = m.append_chunk(["a"], [8])
+    m.commit(["a"], [0])  # (no reserved page is left at the moment)
+    m.keep_chunk(chunk, [0])
+    assert m.fork("a", "f").pages == []
+    _refused(m, lambda: m.try_prefix_cache("a", list(range(8))), match="reserved pages")

@@ -155,7 +155,7 @@ class PageTableEntry:
     pages: List[int] = field(default_factory=list)
     num_tokens: int = 0
     created_at: float = field(default_factory=time.time)
-    reserved: bool = False  # may hold pages that no token is in yet (``reserve``)
+    reserved: bool = False  # pages that no token is in yet, if it has any, are from ``reserve``
     handed_out: int = 0  # how often others have got pages and token count of it (``reserve``)
     forks: int = 0       # how often it has been forked
 
@@ -596,6 +596,11 @@ class PagedKVCacheManager:
         dev = torch.from_numpy(host).to(self._gpu_pool.device)
         return dev[:B * width].view(B, width), dev[B * width:]
 
+    def _tokens_to_come_locked(self, entry: PageTableEntry) -> bool:
+        """Whether a request has reserved pages that no token is in (yet, or
+        any more)."""
+        return entry.reserved and len(entry.pages) > -(-entry.num_tokens // self.config.page_size)
+
     def commit(self, request_ids: Sequence[str], counts: Sequence[int]) -> None:
         """Counts ``counts[i]`` tokens that steps over reserved pages have
         stored for ``request_ids[i]``.  All or nothing: an unknown id raises
@@ -624,7 +629,6 @@ class PagedKVCacheManager:
                 for page in e.pages[e.num_tokens // PS:-(-(e.num_tokens + n) // PS)] if n else []:
                     self._pages[page].last_access = now
                 e.num_tokens += n
-                e.reserved = len(e.pages) * PS - e.num_tokens >= PS
             self._epoch += 1
 
     @property
@@ -676,7 +680,7 @@ class PagedKVCacheManager:
             if src is None:
                 return None
             entry = PageTableEntry(request_id=dst_request_id, pages=list(src.pages), num_tokens=src.num_tokens)
-            if src.reserved:  # (the pages of tokens to come are the source's own)
+            if self._tokens_to_come_locked(src):  # (the pages of tokens to come are the source's own)
                 del entry.pages[-(-src.num_tokens // self.config.page_size):]
             src.forks += 1
             for page_id in entry.pages:
@@ -699,7 +703,7 @@ class PagedKVCacheManager:
         PS = self.config.page_size
         with self._lock:
             entry = self._page_tables.get(request_id)
-            if entry is not None and entry.reserved:
+            if entry is not None and self._tokens_to_come_locked(entry):
                 raise RuntimeError(f"request {request_id!r} has reserved pages: a prefix comes before them")
             if entry is None:
                 entry = self._page_tables[request_id] = PageTableEntry(request_id=request_id)
