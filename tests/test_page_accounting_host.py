@@ -190,3 +190,17 @@ def test_commit_leaves_reserved_pages_reserved_while_tokens_can_be_taken_back():
     m.keep_chunk(chunk, [0])
     assert m.fork("a", "f").pages == []
     _refused(m, lambda: m.try_prefix_cache("a", list(range(8))), match="reserved pages")
+
+
+@pytest.mark.parametrize("tokens,pages", [(1, 1), (8, 1), (9, 2), (24, 3)])
+def test_turbo_attention_compresses_pages_with_tokens_only(tokens, pages, monkeypatch):
+    """Pages behind a request's last token hold nothing to compress: codes made
+    of them would stay when rows are stored there."""
+    m = _mgr(kv_compression="turboquant")
+    held = list(m.allocate("a", 24).pages)
+    m._page_tables["a"].num_tokens = tokens
+    seen = []
+    monkeypatch.setattr(m, "_ensure_compressed", lambda ids, layer: seen.append(("made", list(ids), layer)))
+    monkeypatch.setattr(m, "_turbo_decode", lambda q, lists, n, layer, scale: seen.append((lists, n)) or [q[0]])
+    m.compute_attention_turbo(torch.zeros((4, 64)), "a", 1)
+    assert seen == [("made", held[:pages], 1), ([held[:pages]], [tokens])]

@@ -1121,7 +1121,8 @@ class PagedKVCacheManager:
             entry = self._page_tables.get(request_id)
             if entry is None or not entry.pages:
                 return None
-            page_ids, num_tokens = list(entry.pages), entry.num_tokens
+            num_tokens = entry.num_tokens
+            page_ids = entry.pages[:math.ceil(num_tokens / self.config.page_size)]
         if num_tokens <= 0:
             return None
         self._require_pool("compute_attention_turbo")
