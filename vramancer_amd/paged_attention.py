@@ -355,6 +355,11 @@ class PagedKVCacheManager:
         requests sharing the page their token goes to, raise
         ``RuntimeError``.  An fp8 append rescales its page, so one launch may
         write a page once only."""
+        return self._append_tokens(request_ids, strict)
+
+    def _append_tokens(self, request_ids: Sequence[str], strict: bool, undo: Optional[list] = None) -> Tuple[Any, Any]:
+        """``append_tokens``; ``undo`` takes the batch that ``_take_back`` undoes
+        it with."""
         import torch
 
         self._require_pool("append_tokens")
@@ -375,10 +380,18 @@ class PagedKVCacheManager:
                     if len(set(tails)) < len(tails):
                         raise RuntimeError("requests of an fp8 pool that share the page their next token goes to "
                                            "(forks) cannot append in one launch")
+            if undo is not None:
+                had = {rid: (e, e.num_tokens, len(e.pages)) for rid in request_ids
+                       if (e := self._page_tables.get(rid)) is not None}
             for i, rid in enumerate(request_ids):
                 got = self._append_locked(rid)
                 if got is not None:
                     out[0, i], out[1, i] = got
+            if undo is not None:
+                undo.append(ChunkBatch(
+                    list(had), [e.num_tokens - n for e, n, _ in had.values()], None, None, None, [], owner=self,
+                    epoch=self._epoch, states=[(e, e.num_tokens, len(e.pages) - pages, e.handed_out, e.forks)
+                                               for e, _, pages in had.values()]))
         dev = torch.from_numpy(out).to(self._gpu_pool.device)
         return dev[0], dev[1]
 
@@ -477,10 +490,11 @@ class PagedKVCacheManager:
             if changed:
                 raise RuntimeError(f"{what}: request {rid!r} has changed since append_chunk made this batch")
 
-    def _take_back(self, chunk: ChunkBatch) -> None:
+    def _take_back(self, chunk: ChunkBatch, page_ids: Any = None) -> None:
         """Undoes the append_chunk that made a batch, for a step that failed:
         its tokens, their new pages (in the order they came, so that the free
-        list is as it was) and their rows in the compression queue.  What they
+        list is as it was) and their rows in the compression queue (those of
+        ``write_chunk``, or that ``write_kv_batch`` got ``page_ids`` for).  What they
         wrote lies behind the requests' last tokens; an fp8 page's scale keeps
         what they raised it to.  Raises, and changes nothing, where a request
         has changed or was reserved for since, or a fork made since has these
@@ -491,7 +505,8 @@ class PagedKVCacheManager:
                 entry.num_tokens = n - count
                 for _ in range(added):
                     self._release_locked(entry.pages.pop())
-            self._pending_compress = [item for item in self._pending_compress if item[5] is not chunk.places]
+            self._pending_compress = [item for item in self._pending_compress
+                                      if item[5] is not chunk.places and (page_ids is None or item[1] is not page_ids)]
             self._table_cache = None  # (its patches take page lists to grow only)
             self._epoch += 1
 

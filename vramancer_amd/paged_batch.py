@@ -57,7 +57,8 @@ from transformers.cache_utils import Cache, CacheLayerMixin
 from .paged_attention import ChunkBatch, PagedKVCacheManager
 
 __all__ = ["PagedBatchCache", "PagedBatchLayer", "PagedChunkCache", "PagedChunkLayer", "decode_step", "chunk_step",
-           "sample_step", "speculative_step", "prefill", "prefill_chunked", "paged_attention_forward", "enable_paged_attention", "ATTENTION_NAME"]
+           "sample_step", "speculative_step", "prefill", "prefill_chunked", "paged_attention_forward",
+           "enable_paged_attention", "ATTENTION_NAME"]
 
 ATTENTION_NAME = "vramancer_paged"
 
@@ -125,6 +126,7 @@ class PagedBatchCache(Cache):
         self.manager = manager
         self.request_ids = list(request_ids)
         self._slots: Optional[Tuple[torch.Tensor, torch.Tensor]] = None
+        self._undo: Optional[list] = None  # of the running step, where it is taken back if it fails
         super().__init__(layers=[PagedBatchLayer(self, i) for i in range(manager.config.num_layers)])
 
     def token_counts(self) -> np.ndarray:
@@ -132,7 +134,22 @@ class PagedBatchCache(Cache):
         return self.manager.token_counts(self.request_ids)
 
     def _begin_step(self) -> None:
-        self._slots = self.manager.append_tokens(self.request_ids, strict=True)
+        self._slots = self.manager._append_tokens(self.request_ids, True, self._undo)
+
+    def _watch_step(self) -> None:
+        """The next step is one that ``_undo_step`` takes back."""
+        self._undo = []
+
+    def _undo_step(self) -> bool:
+        """Takes the tokens of a step that failed back; False where a request
+        has changed in the meantime, whose tokens stay then."""
+        undo, self._undo = self._undo, None
+        try:
+            for step in undo or []:
+                self.manager._take_back(step, self._slots and self._slots[0])
+        except RuntimeError:
+            return False
+        return True
 
     def _step_slots(self) -> Tuple[torch.Tensor, torch.Tensor]:
         if self._slots is None:
@@ -187,9 +204,10 @@ class PagedChunkCache(PagedBatchCache):
     def _begin_chunk(self, q: int) -> None:
         self._chunk = self.manager.append_chunk(self.request_ids, [q] * len(self.request_ids))
 
+    def _watch_step(self) -> None:
+        self._chunk = None  # (the step before is no concern of the next one)
+
     def _undo_step(self) -> bool:
-        """Takes the tokens of a step that failed back; False where a request
-        has changed in the meantime, whose tokens stay then."""
         chunk, self._chunk = self._chunk, None
         try:
             if chunk is not None:
@@ -277,7 +295,7 @@ def chunk_step(model, manager: PagedKVCacheManager, request_ids: Sequence[str], 
     ids = input_ids.reshape(len(request_ids), -1)
     pos = torch.from_numpy(cache.token_counts()).to(ids.device).reshape(-1, 1)
     pos = pos + torch.arange(ids.shape[1], device=ids.device)
-    cache._chunk = None  # (the step before is no concern of this one)
+    cache._watch_step()
     try:
         out = model(ids, position_ids=pos, past_key_values=cache, use_cache=True)
     except BaseException:
@@ -290,11 +308,21 @@ def sample_step(model, manager: PagedKVCacheManager, request_ids: Sequence[str],
                 uniforms: torch.Tensor, temperature: Any = None, top_k: Any = None, top_p: Any = None,
                 probs: Any = None, cache: Optional[PagedBatchCache] = None) -> torch.Tensor:
     """``decode_step`` and a token for each request, int64 [B], drawn from its
-    logits with ``uniforms`` [B] (``sampling.sample_tokens``)."""
+    logits with ``uniforms`` [B] (``sampling.sample_tokens``).  A step that
+    raises leaves the requests as they were."""
     from .sampling import sample_tokens
 
-    logits = decode_step(model, manager, request_ids, input_ids, cache)
-    return sample_tokens(logits, uniforms, temperature=temperature, top_k=top_k, top_p=top_p, probs=probs)
+    if cache is None or cache.manager is not manager or cache.request_ids != list(request_ids):
+        cache = PagedBatchCache(manager, request_ids)
+    cache._watch_step()
+    try:
+        logits = decode_step(model, manager, request_ids, input_ids, cache)
+        tokens = sample_tokens(logits, uniforms, temperature=temperature, top_k=top_k, top_p=top_p, probs=probs)
+    except BaseException:
+        cache._undo_step()
+        raise
+    cache._undo = None
+    return tokens
 
 
 def speculative_step(model, manager: PagedKVCacheManager, request_ids: Sequence[str], input_ids: torch.Tensor,
