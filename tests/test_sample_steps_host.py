@@ -100,3 +100,31 @@ def test_a_request_twice_in_a_step():
     with pytest.raises(RuntimeError, match="run on the GPU"):
         sample_step(model, m, ["a", "b", "a"], torch.arange(3), torch.zeros(3))
     assert _state(m) == before
+
+
+def test_requests_without_a_token_do_not_reach_the_embeddings(monkeypatch):
+    """A row of nothing but -inf or NaN gives token -1, which the loop hands to
+    the next step: an index outside the embeddings ends a GPU process."""
+    m, model = _mgr(), Model()
+    none = torch.full((3,), -1, dtype=torch.int64)
+    monkeypatch.setattr(sampling, "sample_tokens", lambda logits, u, **kw: none)
+    pending = torch.tensor([4, -1, 0])
+    pending = sample_step(model, m, ["a", "b", "c"], pending, torch.zeros(3))
+    sample_step(model, m, ["a", "b", "c"], pending, torch.zeros(3))
+    assert [x.flatten().tolist() for x in model.seen] == [[4, 0, 0], [0, 0, 0]]
+
+    asked = []
+
+    def verify(logits, drafts, *args, **kw):
+        asked.append(drafts.tolist())
+        return torch.full((3, 3), -1, dtype=torch.int64), torch.zeros(3, dtype=torch.int32)
+
+    monkeypatch.setattr(sampling, "verify_drafts", verify)
+    drafts = torch.tensor([[1, V], [-1, 2], [3, 1 << 40]])
+    for dtype in (torch.int64, torch.int32):
+        tokens, accepted = speculative_step(model, m, ["a", "b", "c"], torch.tensor([-1, 7, -1], dtype=dtype), drafts, None,
+                                            None)
+        pending = tokens.gather(1, accepted.long()[:, None])[:, 0]
+        assert pending.tolist() == [-1] * 3
+        assert model.seen[-1].tolist() == [[0, 1, V - 1], [7, 0, 2], [0, 3, V - 1]] and model.seen[-1].dtype == dtype
+    assert asked == [drafts.tolist()] * 2

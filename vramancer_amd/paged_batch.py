@@ -309,14 +309,17 @@ def sample_step(model, manager: PagedKVCacheManager, request_ids: Sequence[str],
                 probs: Any = None, cache: Optional[PagedBatchCache] = None) -> torch.Tensor:
     """``decode_step`` and a token for each request, int64 [B], drawn from its
     logits with ``uniforms`` [B] (``sampling.sample_tokens``).  A step that
-    raises leaves the requests as they were."""
+    raises leaves the requests as they were.
+
+    A row of logits without a token gives -1.  Such a request is the caller's to
+    end; where its -1 is an input again, the model gets token 0 for it."""
     from .sampling import sample_tokens
 
     if cache is None or cache.manager is not manager or cache.request_ids != list(request_ids):
         cache = PagedBatchCache(manager, request_ids)
     cache._watch_step()
     try:
-        logits = decode_step(model, manager, request_ids, input_ids, cache)
+        logits = decode_step(model, manager, request_ids, input_ids.clamp(min=0), cache)
         tokens = sample_tokens(logits, uniforms, temperature=temperature, top_k=top_k, top_p=top_p, probs=probs)
     except BaseException:
         cache._undo_step()
@@ -335,8 +338,10 @@ def speculative_step(model, manager: PagedKVCacheManager, request_ids: Sequence[
 
     Afterwards a request has its pending token and the accepted drafts in its
     pages; the token after them, ``tokens[b, accepted[b]]``, is its next
-    pending one.  Reads ``accepted`` back, since the pages are the host's.  A
-    step that raises leaves the requests as they were."""
+    pending one (-1 where a row of logits has no token: such a request is the
+    caller's to end, and the model gets token 0 for a pending -1).  Reads
+    ``accepted`` back, since the pages are the host's.  A step that raises leaves
+    the requests as they were."""
     from .sampling import verify_drafts
 
     B = len(request_ids)
@@ -347,7 +352,8 @@ def speculative_step(model, manager: PagedKVCacheManager, request_ids: Sequence[
     # (a draft outside the vocabulary ends the list: the model gets some token there)
     vocab = model.get_input_embeddings().weight.shape[0]
     known = drafts.clamp(0, vocab - 1).to(input_ids.dtype)
-    logits = chunk_step(model, manager, request_ids, torch.cat([input_ids.reshape(B, 1), known], 1), cache)
+    logits = chunk_step(model, manager, request_ids, torch.cat([input_ids.reshape(B, 1).clamp(min=0), known], 1),
+                        cache)
     try:
         tokens, accepted = verify_drafts(logits, drafts, accept_uniforms, draw_uniforms, draft_probs=draft_probs,
                                          temperature=temperature, top_k=top_k, top_p=top_p)
