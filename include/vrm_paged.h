@@ -759,9 +759,9 @@ int vrm_chunk_tables(const int32_t* block_table, long long row_stride, int R, in
  *
  * Weights, their sums and every comparison with them are 64-bit floats, weights
  * to 2.2e-12 of themselves, or decided as with those (under top_k and top_p a
- * border is found in sums of weights rounded to multiples of 2^-S of the
- * largest, S = min(45, 62 - ceil(log2 V)); tokens below 2^-50 of the largest may
- * count for nothing there).  Results are the same from call to call.  The
+ * border of top_p is found in sums of weights rounded to multiples of 2^-S of the
+ * largest, S = min(45, 62 - ceil(log2 V)); tokens below 2^-49 of the largest may
+ * count for nothing in them).  Results are the same from call to call.  The
  * workspace is 16-byte aligned and written before it is read.  Outputs and the
  * workspace must not overlap inputs (VRM_ERR_ARG).
  * -------------------------------------------------------------------------- */

@@ -176,18 +176,21 @@ template <>
 struct Logit<VRM_SRC_F32> {
   using Raw = uint32_t;
   static constexpr int kVec = 4, kZeros = 0;  // (last bits that are 0 in every value as float32)
+  static constexpr Raw kMinus = 0xff800000u;  // -inf
   static __device__ __forceinline__ float value(uint32_t u) { return __uint_as_float(u); }
 };
 template <>
 struct Logit<VRM_SRC_F16> {
   using Raw = uint16_t;
   static constexpr int kVec = 8, kZeros = 13;
+  static constexpr Raw kMinus = 0xfc00;  // -inf
   static __device__ __forceinline__ float value(uint16_t u) { return f16_bits_to_f32(u); }
 };
 template <>
 struct Logit<VRM_SRC_BF16> {
   using Raw = uint16_t;
   static constexpr int kVec = 8, kZeros = 16;
+  static constexpr Raw kMinus = 0xff80;  // -inf
   static __device__ __forceinline__ float value(uint16_t u) { return bf16_bits_to_f32(u); }
 };
 
@@ -633,6 +636,8 @@ __device__ __forceinline__ SegRec part_sums(const float* x, int seg, float t, bo
 // What a row's cut looks for (vrm_sample_cut.hip).  Bins are absolute; first is
 // the one of the larger logits.
 constexpr int kListed = 4096;  // tokens that a row's list holds
+constexpr int kBelow = 1;      // the bins to list have k tokens or more
+constexpr int kWhole = 2;      // they have all tokens that weigh anything
 
 struct CutPlan {
   double kept;                // the sum of the row's weights, all of them
@@ -647,6 +652,7 @@ struct CutPlan {
   int k_first, k_last, p_first, p_last;
   int list_first, list_last, also, also_first, also_last;  // bins to list
   int all_listed;             // every token that can stay is in them
+  int deep;                   // top_k's border lies past the bins: kBelow or kWhole
   int listed;                 // how many tokens they have
 };
 

@@ -22,8 +22,9 @@
 // Counts and sums do not depend on the order in which tokens are listed: the
 // parts' sums are integers, added in 64-bit floats part by part; among listed
 // tokens weights are integers in units of 2^-S, S such that V of them stay below
-// 2^62 (S = 45 for V up to 2^17).  Tokens below 2^-50 of the row's largest may
-// count and weigh nothing here: a border among them may lie further down.
+// 2^62 (S = 45 for V up to 2^17).  Tokens below 2^-49 of the row's largest may
+// count and weigh nothing in the histograms: top_p's sums leave them out, and a
+// top_k that reaches them has its border found among all tokens by their order.
 //
 // A workgroup of the first and the last kernel runs each part of its code a few
 // times at most, so that fetching it is what short code saves (170 KB, with a
@@ -38,6 +39,12 @@ constexpr int kFew = 64;           // tokens that are compared with each other
 constexpr int kPartsAhead = 24;
 constexpr int kShortListed = 2048;  // tokens of a short row's list
 static_assert(2 * kCutThreads >= kDrawSegments, "a sum for each segment");
+// Down to here every token is counted in its bin, since it is at least one as an
+// integer of its part's histogram: 488 tenths and one for the roundings of two
+// products are 2^-49 of the row's largest, kBinBits being 49.
+constexpr int kSureBins = 488;
+constexpr int kNoBins = 1 << 30;  // the shift of a part that weighs nothing
+constexpr int kLeastBits = 1100;  // a factor of 2^-1100 of the row's largest is 0
 
 using u64 = unsigned long long;
 
@@ -77,6 +84,7 @@ struct BinScan {
     sum = lane_move<0x138, 0xf>(up_to, 0.0);  // wave_shr 1: what is before the lane
     total = lane_value(up_to, 63);
   }
+  __device__ __forceinline__ uint32_t all() const { return lane_value(count + lane_count, kWave - 1); }
   __device__ __forceinline__ int find(bool by_count, uint32_t k, double goal, uint32_t& before_count,
                                       double& before_sum, uint32_t& bin_count, double& bin_sum) const {
     const u64 here = __ballot(by_count ? count + lane_count >= k : up_to >= goal);
@@ -113,8 +121,19 @@ __device__ __forceinline__ void plan_cut(CutPlan& plan, const BinScan& scan, con
     uint32_t n_before, n_bin;
     double s_before, s_bin;
     const int at = scan.find(true, (uint32_t)plan.k, 0.0, n_before, s_before, n_bin, s_bin);
-    if (at == kBins) {
-      plan.k = 0;  // (all that weighs anything stays)
+    if (at >= kSureBins) {
+      // The k-th token weighs so little that some before it may not be counted.
+      // A top_p ends before it; without one all tokens down to a bin that has the
+      // border at the latest are listed (those that weigh anything, unless the
+      // caller finds one), and the border found by order alone.
+      if (by_p) {
+        plan.k = 0;
+      } else {
+        plan.deep = at < kBins ? kBelow : kWhole;
+        plan.all_listed = 1;
+        plan.k_first = plan.list_first = top_bin;
+        plan.k_last = plan.list_last = top_bin - (at < kBins ? at : 10 * kLeastBits + 2);
+      }
     } else {
       plan.k_first = plan.k_last = top_bin - at;
       plan.k_count = n_before;
@@ -214,7 +233,7 @@ __global__ void __launch_bounds__(kCutThreads)
       const SegRec one{1.0 / (double)(1ULL << kBinBits), top, 0};
       const double factor = segment_sum(one, scale);
       part_factor[t] = factor;
-      part_shift[t] = factor > 0.0 ? top_bin - bin_of(top, bins) : kBins;  // (weighs nothing: no bins)
+      part_shift[t] = factor > 0.0 ? top_bin - bin_of(top, bins) : kNoBins;
     }
     __syncthreads();
     const int n = min(parts - p0, kCutThreads);
@@ -244,8 +263,48 @@ __global__ void __launch_bounds__(kCutThreads)
   bin_count[t] = count;
   __syncthreads();
   if (t >= kWave) return;
-  plan_cut(plan, BinScan(bin_count, bin_sum), r, b, top_bin, by_k, by_p);
+  const BinScan scan(bin_count, bin_sum);
+  plan_cut(plan, scan, r, b, top_bin, by_k, by_p);
   if (lane == 0) plans[slot] = plan;
+  if (plan.deep != kWhole || parts > kCutThreads) return;
+  // The border of top_k lies past these bins (a few tokens far above the others,
+  // a low temperature).  A part's histogram counts from its own maximum on, so
+  // that the parts without those tokens still tell a bin down to which there are
+  // k tokens at least: what is listed down to it has the border.  Counts of
+  // further bins, 512 at a time, from where there are any.  (The draw of a row of
+  // 152000 with top_k 50 and a token 50 bits above the others: 49 us; 104 with
+  // everything listed, which overflows the list.)
+  uint32_t counted = scan.all();
+#pragma unroll 1
+  for (int from = kBins;; from += kBins) {
+    int next = kNoBins;
+    for (int p = lane; p < parts; p += kWave)
+      if (part_shift[p] + kBins > from) next = min(next, max(part_shift[p], from));
+    from = wave_min(next, kNoBins);
+    if (from >= 10 * kLeastBits) return;
+    uint32_t c[BinScan::kPer] = {};
+#pragma unroll 2
+    for (int p = 0; p < parts; ++p) {
+      const int at = from + lane * BinScan::kPer - part_shift[p];
+      const uint32_t* counts = hist[(long long)slot * parts + p].count;
+#pragma unroll
+      for (int j = 0; j < BinScan::kPer; ++j)
+        if (at + j >= 0 && at + j < kBins) c[j] += counts[at + j];
+    }
+#pragma unroll
+    for (int j = 0; j < BinScan::kPer; ++j) bin_count[lane * BinScan::kPer + j] = c[j];
+    const BinScan more(bin_count, bin_sum);
+    uint32_t before, in_bin;
+    double unused;
+    const int at = more.find(true, (uint32_t)plan.k - counted, 0.0, before, unused, in_bin, unused);
+    if (at < kBins) {
+      plan.deep = kBelow;
+      plan.k_last = plan.list_last = top_bin - from - at;
+      if (lane == 0) plans[slot] = plan;
+      return;
+    }
+    counted += more.all();
+  }
 }
 
 // Which of a lane's logits are in the bins to list.
@@ -304,9 +363,9 @@ __global__ void __launch_bounds__(kSampleThreads, 5)
     // (A lane has three at most, mostly: their logits are read again, since
     // registers have no index.)
 #pragma unroll 1
-    for (; hits; hits &= hits - 1, ++at) {
+    for (; hits && at < kListed; hits &= hits - 1, ++at) {
       const int bit = __ffs(hits) - 1, e = segment_element<SRC>(seg, bit / kVec) + bit % kVec;
-      if (at < kListed) list[at] = order_value(Logit<SRC>::value(row[e]), e);
+      list[at] = order_value(Logit<SRC>::value(row[e]), e);
     }
   }
   if constexpr (!MASS) return;
@@ -418,9 +477,11 @@ __device__ __forceinline__ void find_border(CutShared<SRC, THREADS, LISTED>& sh,
     for (int turn = 0; turn < 2; ++turn) {
       const bool by_count = turn == 0;
       if (!(by_count ? plan.k > 0 : plan.by_p != 0)) continue;
+      if (plan.deep == kWhole && listing <= plan.k) continue;  // (all that weighs anything stays)
       const uint32_t k = (uint32_t)plan.k;
       const int first = by_count ? plan.k_first : plan.p_first, last = by_count ? plan.k_last : plan.p_last;
-      const BinRange range(last, first);
+      BinRange range(last, first);
+      float steps = bins;  // what range's bins are of
       const double before = by_count ? plan.k_before : plan.p_before;
       const double goal = fmin(fmax((double)r.nucleus(b) * kept, 0x1p-200), kept);
       uint32_t before_count = by_count ? plan.k_count : 0;
@@ -436,7 +497,8 @@ __device__ __forceinline__ void find_border(CutShared<SRC, THREADS, LISTED>& sh,
         lost = all == 0;
       };
       // The step with the border, by the counts and sums of all of them.
-      const auto narrow = [&](int shift) {
+      // orders: steps are of order values, of which low .. high are left then.
+      const auto narrow = [&](int shift, bool orders) {
         const uint32_t c0 = sh.sub_count[2 * t], c1 = sh.sub_count[2 * t + 1];
         const u64 w0 = sh.sub_sum[2 * t], w1 = sh.sub_sum[2 * t + 1];
         const uint32_t pc = wave_prefix(c0 + c1);
@@ -467,6 +529,7 @@ __device__ __forceinline__ void find_border(CutShared<SRC, THREADS, LISTED>& sh,
         __syncthreads();
         before_count = sh.before_count_;
         before_fixed = sh.before_fixed_;
+        if (!orders) return;
         const u64 top = high - ((u64)sh.bin_ << shift), span = (1ULL << shift) - 1;
         low = top - low > span ? top - span : low;
         high = top;
@@ -475,8 +538,24 @@ __device__ __forceinline__ void find_border(CutShared<SRC, THREADS, LISTED>& sh,
       if (!fits) {
         // The list does not hold these bins' tokens (logits that lie closer
         // together than a bin is wide): passes over the row narrow their order
-        // values by 10 bits each until what is left fits it.
+        // values by 10 bits each until what is left fits it.  Where the border
+        // lies past the bins (and the row is long) the first pass counts by wider
+        // ones, which reach down to weights of 0: a border behind those cuts
+        // nothing.
         int shift = max(0, packed.bits() - sh.kSubBits);
+        const float wide = bins * ((sh.kSub - 4) / (10.0f * kLeastBits));
+        const int wide_top = bin_of(plan.top, wide);
+        bool by_steps = LISTS && by_count && plan.deep != 0;
+        const auto take = [&](int e, float l) {
+          const u64 order = order_value(l, e), o = packed.pack(order);
+          if (o < low || o > high) return;
+          if (shift < 0) {
+            put(atomicAdd(&sh.fill_, 1), order);  // (there are as many as the last pass counted)
+          } else {
+            atomicAdd(&sh.sub_count[(high - o) >> shift], 1u);
+            atomicAdd(&sh.sub_sum[(high - o) >> shift], fixed_weight(sample_weight(l, scale), unit));
+          }
+        };
 #pragma unroll 1
         while (true) {
           __syncthreads();
@@ -486,24 +565,64 @@ __device__ __forceinline__ void find_border(CutShared<SRC, THREADS, LISTED>& sh,
           }
           if (t == 0) sh.fill_ = 0;
           __syncthreads();
+          if constexpr (LISTS) {
+            // (Two vectors of a lane at once, and the few logits that are in the
+            // bins read again, as sample_collect_kernel does.)
+            constexpr int kAhead = 2, kChunk = kAhead * kWave * L::kVec;
 #pragma unroll 1
-          for (int e = t; e < V; e += kThreads) {
-            const float l = L::value(row[e]);
-            if (!range.holds(l * bins) || !(l > -INFINITY)) continue;
-            const u64 order = order_value(l, e), o = packed.pack(order);
-            if (o < low || o > high) continue;
-            if (shift < 0) {
-              put(atomicAdd(&sh.fill_, 1), order);  // (there are as many as the last pass counted)
-            } else {
-              atomicAdd(&sh.sub_count[(high - o) >> shift], 1u);
-              atomicAdd(&sh.sub_sum[(high - o) >> shift], fixed_weight(sample_weight(l, scale), unit));
+            for (int c0 = wave * kChunk; c0 < V; c0 += kWaves * kChunk) {
+              const int e0 = c0 + lane * L::kVec;
+              Unaligned16<typename L::Raw> raw[kAhead];
+#pragma unroll
+              for (int i = 0; i < kAhead; ++i) {
+                const int at = e0 + i * kWave * L::kVec;
+                if (at + L::kVec <= V) {
+                  raw[i] = *reinterpret_cast<const Unaligned16<typename L::Raw>*>(row + at);
+                } else {
+#pragma unroll
+                  for (int j = 0; j < L::kVec; ++j) raw[i].v[j] = at + j < V ? row[at + j] : L::kMinus;
+                }
+              }
+              uint32_t hits = 0;
+#pragma unroll
+              for (int i = 0; i < kAhead; ++i) {
+#pragma unroll
+                for (int j = 0; j < L::kVec; ++j) {
+                  const float l = L::value(raw[i].v[j]);
+                  if (!(l > -INFINITY)) continue;
+                  if (by_steps) {
+                    atomicAdd(&sh.sub_count[min(wide_top - bin_of(l, wide), sh.kSub - 1)], 1u);
+                  } else if (range.holds(l * steps)) {
+                    hits |= 1u << (i * L::kVec + j);
+                  }
+                }
+              }
+#pragma unroll 1
+              for (; hits; hits &= hits - 1) {
+                const int bit = __ffs(hits) - 1, e = e0 + bit / L::kVec * kWave * L::kVec + bit % L::kVec;
+                take(e, L::value(row[e]));
+              }
+            }
+          } else {  // (a short row: one logit a lane, no registers for more)
+#pragma unroll 1
+            for (int e = t; e < V; e += kThreads) {
+              const float l = L::value(row[e]);
+              if (range.holds(l * steps) && l > -INFINITY) take(e, l);
             }
           }
           __syncthreads();
           if (shift < 0) break;
-          narrow(shift);
+          narrow(shift, !by_steps);
+          if (by_steps) {
+            by_steps = false;
+            lost = sh.bin_ == sh.kSub - 1;
+            steps = wide;
+            range = BinRange(wide_top - sh.bin_, wide_top - sh.bin_);
+            if (sh.count_ <= (uint32_t)LISTED) shift = -1;
+          } else {
+            shift = sh.count_ <= (uint32_t)LISTED ? -1 : max(0, 64 - __clzll(high - low) - sh.kSubBits);
+          }
           if (lost) break;
-          shift = sh.count_ <= (uint32_t)LISTED ? -1 : max(0, 64 - __clzll(high - low) - sh.kSubBits);
         }
         listed = lost ? 0 : sh.fill_;
       }
@@ -519,7 +638,7 @@ __device__ __forceinline__ void find_border(CutShared<SRC, THREADS, LISTED>& sh,
         uint32_t count = 0;
         for (int j = t; j < listed; j += kThreads) {
           const u64 o = sh.list[j];
-          if (o >= low && o <= high && (!first_look || range.holds(packed.logit(o) * bins))) {
+          if (o >= low && o <= high && (!first_look || range.holds(packed.logit(o) * steps))) {
             ++count;
             if (!have_goal) sum += sh.weight[j];
             a = min(a, o);
@@ -564,7 +683,7 @@ __device__ __forceinline__ void find_border(CutShared<SRC, THREADS, LISTED>& sh,
           }
         }
         __syncthreads();
-        narrow(shift);
+        narrow(shift, true);
       }
       if (lost || n == 0) continue;  // (the same for every thread)
       // The few that are left, each against the others: a thread has one and a
@@ -613,7 +732,7 @@ __device__ __forceinline__ void find_border(CutShared<SRC, THREADS, LISTED>& sh,
       __syncthreads();
       border = sh.border_;
       of_p = !by_count;
-      kept = before + (double)sh.before_fixed_ / unit;
+      kept = plan.deep ? plan.total : before + (double)sh.before_fixed_ / unit;
       __syncthreads();
     }
     if (border == 0) kept = plan.kept;
@@ -643,8 +762,10 @@ __device__ __forceinline__ void find_border(CutShared<SRC, THREADS, LISTED>& sh,
   double* masses = mass + (long long)slot * ns;
   const double unit = (double)(1ULL << bits);
   // What the second launch summed is right where the cut is in the bins that it
-  // listed; the segments are summed here otherwise.
-  const bool summed = LISTS && plan.filters && cut != 0 && fits && (plan.all_listed || of_p == (plan.by_p != 0));
+  // listed; the segments are summed here otherwise.  (Tokens that stay and are
+  // nothing as integers matter to random numbers of 0 and 1 alone.)
+  bool summed = LISTS && plan.filters && cut != 0 && fits && (plan.all_listed || of_p == (plan.by_p != 0));
+  if (summed && !(u > 0.0f && u < 1.0f)) summed = fixed_weight(sample_weight(order_logit(cut), scale), unit) != 0;
   if (summed) {
     for (int j = t; j < ns; j += kThreads) sh.sub_sum[j] = 0;
     __syncthreads();
@@ -763,9 +884,9 @@ __global__ void __launch_bounds__(kSampleThreads, 4)
     uint32_t hits = plan_hits(plan, x, bins);
     int at = hits ? atomicAdd(&listing, __popc(hits)) : 0;
 #pragma unroll 1
-    for (; hits; hits &= hits - 1, ++at) {  // (read again: registers have no index)
+    for (; hits && at < kShortListed; hits &= hits - 1, ++at) {  // (read again: registers have no index)
       const int bit = __ffs(hits) - 1, e = segment_element<SRC>(seg, bit / kVec) + bit % kVec;
-      if (at < kShortListed) sh.put(at, order_value(Logit<SRC>::value(row[e]), e), packed, scale, unit);
+      sh.put(at, order_value(Logit<SRC>::value(row[e]), e), packed, scale, unit);
     }
   }
   __syncthreads();
