@@ -755,7 +755,7 @@ int vrm_chunk_tables(const int32_t* block_table, long long row_stride, int R, in
  *
  * temperature, top_k and top_p are device arrays with a value per sequence, or
  * NULL: temperature_all, top_k_all, top_p_all hold for every one.  V is at most
- * VRM_SAMPLE_MAX_V.  Random numbers are taken into [0, 1].
+ * VRM_SAMPLE_MAX_V.  Random numbers are taken into [0, 1], NaN as 0.
  *
  * Weights, their sums and every comparison with them are 64-bit floats, weights
  * to 2.2e-12 of themselves, or decided as with those (under top_k and top_p a

@@ -215,7 +215,7 @@ __device__ __forceinline__ DrawRec choose(const SampleRows& r, const Drafts& d, 
     const bool draft = i < n - 1;
     const long long x = draft ? d.id(at) : -1;
     const bool known = x >= 0 && x < r.V;
-    const float u = draft ? fmaxf(d.accept[at], 0.0f) : 0.0f;
+    const float u = draft ? fminf(fmaxf(d.accept[at], 0.0f), 1.0f) : 0.0f;
     const float l = known ? Logit<SRC>::value(row_at<SRC>(r, first + i)[x]) : 0.0f;
     const float qx = known && d.probs ? d.probs[b * d.seq_stride + i * d.draft_stride + x] : 1.0f;
     Scale at_row;

@@ -7,8 +7,8 @@ the logits of a chunk whose tokens after the first are drafts, accepts as many
 of them as the target's distribution allows and draws the token that follows.
 Random numbers are inputs, so that a program owns its generators, a captured
 graph draws anew from numbers written into the same tensor, and every call can
-be repeated.  Weights and sums are float64.  The reference draws on the host
-from its batcher's logits.
+be repeated; numbers outside [0, 1] are taken into it, NaN as 0.  Weights and
+sums are float64.  The reference draws on the host from its batcher's logits.
 
 Rows of logits are float32, float16 or bfloat16; a row's token i has the weight
 exp((l_i - max l) / temperature).  ``top_k`` keeps the k first in the order
