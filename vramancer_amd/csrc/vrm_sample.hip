@@ -97,7 +97,11 @@ __global__ void __launch_bounds__(kSampleThreads, 5)
 // exact ones: a term errs by 3 2^-24 |y| ln 2 + 2^-23 of itself (the difference,
 // the scale and their product, and the exponential's last place), which is
 // 4.1e-6 for |y| <= 32; what lies below weighs V 2^-32 of the largest at most;
-// 32 terms of a lane, added in pairs, add 5 2^-24: 4.4e-6 in all.
+// 32 terms of a lane, added in pairs, add 5 2^-24: 4.4e-6 in all.  Differences
+// are taken in halves where whole ones could overflow, and times 2^64 where the
+// scale could (temperatures below 1e-38 tell subnormal logits apart; logits
+// above 1e18 then differ by nothing or by everything).  A subnormal scale errs by
+// more, and is of |y| < 3.
 constexpr double kRough = 5e-6;
 
 template <int SRC>
@@ -115,10 +119,11 @@ __global__ void __launch_bounds__(kSampleThreads) sample_rough_kernel(SampleRows
   SegRec g{0.0, m, -1};
   if (m > -INFINITY) {
     if (t > 0.0f) {
-      const float c = fminf((float)(1.4426950408889634074 / (double)t), 3e38f);
+      const float unit = m > 1e30f ? 0.5f : t < 1e-38f && fabsf(m) < 1e18f ? 0x1p64f : 1.0f;
+      const float c = fminf((float)(1.4426950408889634074 / ((double)t * unit)), 3e38f), top = -m * unit;
 #pragma unroll
       for (int e = 0; e < kSamplePer; ++e) {
-        const float y = fmaxf((x[e] - m) * c, -200.0f);  // (a NaN is the lower bound, which underflows)
+        const float y = fmaxf(fmaf(x[e], unit, top) * c, -200.0f);  // (a NaN is the lower bound, which underflows)
         x[e] = m == INFINITY ? (x[e] == m ? 1.0f : 0.0f) : __builtin_amdgcn_exp2f(y);
       }
 #pragma unroll
