@@ -263,6 +263,8 @@ def _ints(name: str, t, n: Optional[int]):
     if t.dtype != torch.int32:
         if t.dtype not in (torch.int64, torch.int16, torch.int8, torch.uint8):
             raise RuntimeError(f"{name} must be integers, got {t.dtype}")
+        if t.dtype == torch.int64:  # (the nearest value of 32 bits)
+            t = t.clamp(-0x80000000, 0x7fffffff)
         t = t.to(torch.int32)
     return t.contiguous()
 
