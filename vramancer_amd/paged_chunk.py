@@ -301,6 +301,9 @@ def chunk_tables(
     if N < 0 or PS < 1 or max_pp < 0:
         raise RuntimeError(f"num_rows and max_pages must not be negative and page_size positive, got {N}, {max_pp}, "
                            f"{PS}")
+    if max(R, W, N, PS, max_pp) > 0x7fffffff:
+        raise RuntimeError(f"sizes must be below 2^31, got {R} rows of {W} pages, num_rows {N}, page_size {PS} and "
+                           f"max_pages {max_pp}")
     if block_table.stride(1) != 1 and W > 1:
         block_table = block_table.contiguous()
     past_lens = _ints("past_lens", past_lens, R)

@@ -104,6 +104,11 @@ def _workspace(workspace, need: int, device):
     return workspace
 
 
+def _check_sizes(*sizes) -> None:
+    if max(sizes) > 0x7fffffff:
+        raise RuntimeError(f"rows, drafts and vocabulary must be below 2^31, got {sizes}")
+
+
 def sample_tokens(
     logits: Any,    # [N, V] float32 / float16 / bfloat16
     uniforms: Any,  # [N] float32 in [0, 1)
@@ -129,6 +134,7 @@ def sample_tokens(
         raise RuntimeError(f"logits must be [N, V], got shape {tuple(logits.shape)}")
     code = src_code(logits.dtype)
     N, V = logits.shape
+    _check_sizes(N, V)
     if V < 1:
         raise RuntimeError("logits must have at least one token")
     if logits.stride(1) != 1 and V > 1:
@@ -200,6 +206,7 @@ def verify_drafts(
             raise RuntimeError(f"cu_seqlens must be int32 or int64 [B + 1 = {B + 1}], got {cu_seqlens.dtype} "
                                f"{tuple(cu_seqlens.shape)}")
         cu_seqlens = cu_seqlens.to(torch.int32).contiguous()
+    _check_sizes(logits.shape[0], B, K, V)
     if V < 1:
         raise RuntimeError("logits must have at least one token")
     if logits.stride(1) != 1 and V > 1:
