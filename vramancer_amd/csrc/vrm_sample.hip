@@ -62,8 +62,12 @@ __global__ void __launch_bounds__(kSampleThreads) sample_segment_kernel(SampleRo
 }
 
 // The same with the histogram of the workgroup's four segments, whose common
-// maximum gives the scale.  (Five wavefronts a SIMD, at the price of three
-// registers that spill: 64 rows of 152000 are 4.75 of them, one round.)
+// maximum gives the scale.  (Five wavefronts a SIMD here and in
+// sample_collect_kernel, at the price of three registers that spill: more loads
+// are under way where there are wavefronts for it.  Calls with five and with four:
+// 52.9 and 56.1 us for 64 rows of 152000, 59.8 and 60.8 for 96 of 131072, 124 and
+// 134 for 300 of 128256; 40.5 and 40.3 for 20 of 100003, 43.4 and 43.1 for 128 of
+// 50000.)
 template <int SRC>
 __global__ void __launch_bounds__(kSampleThreads, 5)
     sample_histogram_kernel(SampleRows r, int ns, int blocks, SegRec* rec, Histogram* hist) {
@@ -596,7 +600,9 @@ Plan plan_of(long long B, int K, int V, bool filtered, bool drafts, bool probs) 
 // sequence's masses tests its drafts (for a few drafts): 9.7 us against 5.2 + 7.0
 // in two launches for 8 sequences of 3 drafts and 32000 logits (32 workgroups),
 // 15.6 against 7.0 + 10.7 for 37 of 7 and 100003 (481); 23.5 against 6.0 + 15.8
-// for 64 of 4 and 152000 (1216).
+// for 64 of 4 and 152000 (1216).  Of many drafts each workgroup repeats as many
+// tests: 23.7 us a call against 25.3 for 8 sequences of 9 and 32000, 24.6 and 25.0
+// for 12, 26.4 and 25.8 for 16, 30.6 and 28.4 for 24.
 constexpr int kChooseBlocks = 768, kChooseDrafts = 12;
 
 // A launch counts its threads in 32 bits.
