@@ -133,10 +133,12 @@ def test_cuts_between_groups_far_from_each_other(where, dtype):
             check(x, u, temperature=t, top_k=k)
 
 
-def test_a_very_long_row_cut_far_below_its_largest():
-    V = 2_200_003
+@pytest.mark.parametrize("V", [2_200_003, 4_500_001])  # (549 parts: more than one workgroup's threads)
+def test_a_very_long_row_cut_far_below_its_largest(V):
     x, u = peaked(2, V, torch.float16, 3, 40.0)
-    check(x, u, temperature=0.7, top_k=70)
+    for kw in (dict(temperature=0.7, top_k=70), dict(temperature=0.7, top_k=5000), dict(top_p=0.3, temperature=20.0),
+               dict(top_k=40, temperature=20.0)):
+        check(x, u, **kw)
 
 
 @pytest.mark.parametrize("V", [900, 20001])

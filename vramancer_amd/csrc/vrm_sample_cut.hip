@@ -549,8 +549,9 @@ __device__ __forceinline__ void find_border(CutShared<SRC, THREADS, LISTED>& sh,
         const auto take = [&](int e, float l) {
           const u64 order = order_value(l, e), o = packed.pack(order);
           if (o < low || o > high) return;
-          if (shift < 0) {
-            put(atomicAdd(&sh.fill_, 1), order);  // (there are as many as the last pass counted)
+          if (shift < 0) {  // (there are as many as the last pass counted, which fit)
+            const int at = atomicAdd(&sh.fill_, 1);
+            if (at < LISTED) put(at, order);
           } else {
             atomicAdd(&sh.sub_count[(high - o) >> shift], 1u);
             atomicAdd(&sh.sub_sum[(high - o) >> shift], fixed_weight(sample_weight(l, scale), unit));
@@ -624,7 +625,7 @@ __device__ __forceinline__ void find_border(CutShared<SRC, THREADS, LISTED>& sh,
           }
           if (lost) break;
         }
-        listed = lost ? 0 : sh.fill_;
+        listed = lost ? 0 : min(sh.fill_, LISTED);
       }
 
       // Narrow the listed tokens of the bins that are within low .. high.  (A
