@@ -758,10 +758,11 @@ int vrm_chunk_tables(const int32_t* block_table, long long row_stride, int R, in
  * VRM_SAMPLE_MAX_V.  Random numbers are taken into [0, 1], NaN as 0.
  *
  * Weights, their sums and every comparison with them are 64-bit floats, weights
- * to 2.2e-12 of themselves, or decided as with those (under top_k and top_p a
- * border of top_p is found in sums of weights rounded to multiples of 2^-S of the
- * largest, S = min(45, 62 - ceil(log2 V)); tokens below 2^-49 of the largest may
- * count for nothing in them).  Results are the same from call to call.  The
+ * to 2.2e-12 of themselves, or decided as with those (under top_k and top_p
+ * the border of top_p, and a draw by a random number above 2^-16, may be found in
+ * sums of weights rounded to multiples of 2^-S of the largest, S = min(45,
+ * 62 - ceil(log2 V)); tokens below 2^-49 of the largest may count for nothing in
+ * them).  Results are the same from call to call.  The
  * workspace is 16-byte aligned and written before it is read.  Outputs and the
  * workspace must not overlap inputs (VRM_ERR_ARG).
  * -------------------------------------------------------------------------- */

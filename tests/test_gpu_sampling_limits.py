@@ -114,6 +114,21 @@ def test_cuts_far_from_zero(V, shift, t):
         check(x, u, temperature=t, top_k=k)
 
 
+def test_random_numbers_next_to_nothing():
+    # few tokens that weigh anything to speak of, behind many that hardly do
+    V = 30001
+    g = torch.Generator().manual_seed(8)
+    x = torch.randn((60, V), generator=g) - 30.0
+    x[:, V // 2:] += 30.0
+    x[::2, :V // 2] += 8.0
+    u = torch.rand(60, generator=g) * 2.0 ** -torch.arange(0, 60).float()
+    check(x.to(DEV), u.to(DEV), top_k=V - 10)
+    check(x.to(DEV), u.to(DEV), top_k=V // 2 + 2000)
+    check(x.to(DEV), u.to(DEV), top_p=1.0 - 2.0 ** -20)
+    x[:, V // 2 + 30:] = -60.0
+    check(x.to(DEV), u.to(DEV), top_k=3000)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("where", ["apart", "everywhere"])
 def test_cuts_between_groups_far_from_each_other(where, dtype):

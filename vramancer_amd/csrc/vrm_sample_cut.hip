@@ -763,10 +763,11 @@ __device__ __forceinline__ void find_border(CutShared<SRC, THREADS, LISTED>& sh,
   double* masses = mass + (long long)slot * ns;
   const double unit = (double)(1ULL << bits);
   // What the second launch summed is right where the cut is in the bins that it
-  // listed; the segments are summed here otherwise.  (Tokens that stay and are
-  // nothing as integers matter to random numbers of 0 and 1 alone.)
-  bool summed = LISTS && plan.filters && cut != 0 && fits && (plan.all_listed || of_p == (plan.by_p != 0));
-  if (summed && !(u > 0.0f && u < 1.0f)) summed = fixed_weight(sample_weight(order_logit(cut), scale), unit) != 0;
+  // listed; the segments are summed here otherwise, and for random numbers next
+  // to 0 and of 1 (one draw in 65536), for which tokens count that are little or
+  // nothing as integers.
+  const bool summed = LISTS && plan.filters && cut != 0 && fits && u > 0x1p-16f && u < 1.0f &&
+                      (plan.all_listed || of_p == (plan.by_p != 0));
   if (summed) {
     for (int j = t; j < ns; j += kThreads) sh.sub_sum[j] = 0;
     __syncthreads();
